@@ -610,6 +610,91 @@ int mogt_split_ce_bwd(const void* A, int64_t lda, int64_t plane_a, int pieces_a,
                       int64_t N, int64_t K, int64_t ignore_index, const float* scale, void* grad,
                       int64_t ld_grad, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Selective state space scan: per channel d and state n
+ *   dt_t = delta_t[d] + delta_bias[d], softplus of it where `softplus` is set
+ *   h_t  = exp(dt_t A[d,n]) h_{t-1} + dt_t x_t[d] B_t[n],  h_{-1} = initial_state
+ *   y_t[d] = sum_n C_t[n] h_t + D[d] x_t[d],   out_t = y_t silu(z_t) (y_t without z)
+ * with fp32 arithmetic and state; out is rounded once.  x, delta, z (io_dtype)
+ * are [batch, length, channels] with unit channel stride and the given row and
+ * batch strides in elements; B, C (bc_dtype, fp32 or io_dtype) are rows of
+ * groups x states, group-major, a group shared by channels / groups consecutive
+ * channels; bf16 rows need 4-byte alignment and an even state count.  A
+ * [channels, states], D and delta_bias [channels], initial_state and
+ * final_state [batch, channels, states] are contiguous fp32; z, D, delta_bias,
+ * initial_state and lengths may be null.  lengths [batch] (4- or 8-byte
+ * integers, clamped to [0, length]): steps past a sequence's length are not
+ * read, leave the state as it is and write zero.
+ *
+ * `segment` (a multiple of 8): steps of one wave; sequences of several segments
+ * take a scratch workspace of mogt_ssm_scan_workspace_bytes (no initial
+ * content, free again once the call's work has run).
+ * mogt_ssm_scan_fwd: `final_state` may be null; `carries` (may be null)
+ *   [batch, segments, states, channels] receives the state entering each
+ *   segment, which the backward takes.
+ * mogt_ssm_scan_bwd: from the same problem, the forward's carries, dout
+ *   (io_dtype, contiguous [batch, length, channels]) and
+ *   dfinal_state (may be null) the gradients, each of which may be null: dx, ddelta, dz (io_dtype,
+ *   contiguous), dB, dC (bc_dtype, contiguous [batch, length, groups, states]),
+ *   dA, dD, ddelta_bias and dinitial_state (fp32, their tensors' layouts).
+ *   Sums run in a fixed order: results do not change from run to run.
+ * mogt_ssm_step: one token per sequence (length 1; rows are addressed by the
+ *   batch strides), `state` [batch, channels, states] updated in place.
+ * No counterpart in the reference.                                          */
+#define MOGT_SSM_MAX_STATES 128
+typedef struct mogt_ssm_problem {
+    int64_t batch, length, channels, states, groups, segment;
+    int io_dtype, bc_dtype, softplus, lengths_bytes;
+    const void *x, *delta, *z, *B, *C;
+    const float *A, *D, *delta_bias, *initial_state;
+    const void* lengths;
+    int64_t x_row, x_batch, delta_row, delta_batch, z_row, z_batch;
+    int64_t B_row, B_batch, C_row, C_batch;
+} mogt_ssm_problem;
+typedef struct mogt_ssm_gradients {
+    void *dx, *ddelta, *dz, *dB, *dC;
+    float *dA, *dD, *ddelta_bias, *dinitial_state;
+} mogt_ssm_gradients;
+size_t mogt_ssm_scan_workspace_bytes(int64_t batch, int64_t length, int64_t channels, int64_t states,
+                                     int64_t segment);
+int mogt_ssm_scan_fwd(const mogt_ssm_problem* problem, void* out, float* final_state, float* carries,
+                      void* workspace, size_t workspace_bytes, void* stream);
+size_t mogt_ssm_scan_bwd_workspace_bytes(int64_t batch, int64_t length, int64_t channels, int64_t states,
+                                         int64_t groups, int64_t segment);
+int mogt_ssm_scan_bwd(const mogt_ssm_problem* problem, const void* dout, const float* dfinal_state,
+                      const float* carries, const mogt_ssm_gradients* gradients, void* workspace,
+                      size_t workspace_bytes, void* stream);
+int mogt_ssm_step(const mogt_ssm_problem* problem, float* state, void* out, void* stream);
+
+/* Short causal depthwise convolution, the usual companion of the scan above:
+ *   s_t[d] = bias[d] + sum_k weight[d,k] x_{t-K+1+k}[d],  y_t = s_t or silu(s_t)
+ * with K = `taps` in 1 .. 8, fp32 arithmetic, y rounded once.  x [batch, length,
+ * channels] (io_dtype, unit channel stride, row and batch strides in elements);
+ * weight [channels, taps] and bias [channels] (may be null) contiguous fp32.
+ * The K - 1 inputs before the first step are initial_state [batch, K-1,
+ * channels] (io_dtype, contiguous; zero if null); final_state (may be null,
+ * same layout) receives the last K - 1 inputs of each sequence.  lengths as
+ * above.  mogt_short_conv_bwd: gradients of dy (contiguous) and
+ *   dfinal_state (may be null) with respect to x (contiguous, io_dtype),
+ *   weight, bias (fp32) and initial_state (io_dtype), each of which may be
+ *   null; scratch workspace of mogt_short_conv_bwd_workspace_bytes.
+ * mogt_short_conv_step: one token per sequence; `state` is shifted in place.
+ * No counterpart in the reference.                                          */
+typedef struct mogt_short_conv_problem {
+    int64_t batch, length, channels, taps;
+    int io_dtype, silu, lengths_bytes;
+    const void* x;
+    const float *weight, *bias;
+    const void *initial_state, *lengths;
+    int64_t x_row, x_batch;
+} mogt_short_conv_problem;
+int mogt_short_conv_fwd(const mogt_short_conv_problem* problem, void* y, void* final_state, void* stream);
+size_t mogt_short_conv_bwd_workspace_bytes(int64_t batch, int64_t length, int64_t channels, int64_t taps);
+int mogt_short_conv_bwd(const mogt_short_conv_problem* problem, const void* dy, const void* dfinal_state, void* dx,
+                        float* dweight, float* dbias, void* dinitial_state, void* workspace,
+                        size_t workspace_bytes, void* stream);
+int mogt_short_conv_step(const mogt_short_conv_problem* problem, void* state, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

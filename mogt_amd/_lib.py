@@ -26,6 +26,32 @@ _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
 _c_float = ctypes.c_float
 
+
+
+class SsmProblem(ctypes.Structure):
+    """``mogt_ssm_problem`` of include/mogt_scan.h."""
+    _fields_ = ([(n, _c_i64) for n in ("batch", "length", "channels", "states", "groups", "segment")]
+                + [(n, _c_int) for n in ("io_dtype", "bc_dtype", "softplus", "lengths_bytes")]
+                + [(n, _c_void_p) for n in ("x", "delta", "z", "B", "C", "A", "D", "delta_bias", "initial_state",
+                                            "lengths")]
+                + [(n, _c_i64) for n in ("x_row", "x_batch", "delta_row", "delta_batch", "z_row", "z_batch", "B_row",
+                                         "B_batch", "C_row", "C_batch")])
+
+
+class SsmGradients(ctypes.Structure):
+    """``mogt_ssm_gradients`` of include/mogt_scan.h."""
+    _fields_ = [(n, _c_void_p) for n in ("dx", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias",
+                                         "dinitial_state")]
+
+
+class ShortConvProblem(ctypes.Structure):
+    """``mogt_short_conv_problem`` of include/mogt_scan.h."""
+    _fields_ = ([(n, _c_i64) for n in ("batch", "length", "channels", "taps")]
+                + [(n, _c_int) for n in ("io_dtype", "silu", "lengths_bytes")]
+                + [(n, _c_void_p) for n in ("x", "weight", "bias", "initial_state", "lengths")]
+                + [(n, _c_i64) for n in ("x_row", "x_batch")])
+
+
 # name -> (restype, argtypes); must match include/mogt_scan.h
 SIGNATURES: dict[str, tuple] = {
     "mogt_last_error": (ctypes.c_char_p, []),
@@ -208,6 +234,20 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_i64, _c_i64,
          _c_int, _c_int, _c_int, _c_void_p, _c_size, _c_int, _c_void_p]),
     "mogt_rank1_check_ranges": (_c_int, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "mogt_ssm_scan_workspace_bytes": (_c_size, [_c_i64] * 5),
+    "mogt_ssm_scan_fwd": (
+        _c_int, [ctypes.POINTER(SsmProblem), _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
+    "mogt_ssm_scan_bwd_workspace_bytes": (_c_size, [_c_i64] * 6),
+    "mogt_ssm_scan_bwd": (
+        _c_int, [ctypes.POINTER(SsmProblem), _c_void_p, _c_void_p, _c_void_p, ctypes.POINTER(SsmGradients), _c_void_p,
+                 _c_size, _c_void_p]),
+    "mogt_ssm_step": (_c_int, [ctypes.POINTER(SsmProblem), _c_void_p, _c_void_p, _c_void_p]),
+    "mogt_short_conv_fwd": (_c_int, [ctypes.POINTER(ShortConvProblem), _c_void_p, _c_void_p, _c_void_p]),
+    "mogt_short_conv_bwd_workspace_bytes": (_c_size, [_c_i64] * 4),
+    "mogt_short_conv_bwd": (
+        _c_int, [ctypes.POINTER(ShortConvProblem), _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                 _c_void_p, _c_size, _c_void_p]),
+    "mogt_short_conv_step": (_c_int, [ctypes.POINTER(ShortConvProblem), _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

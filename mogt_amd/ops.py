@@ -2438,3 +2438,468 @@ def split_head_grad_pieces(a: torch.Tensor, b: torch.Tensor, k: int, labels: tor
     if scale.numel() != 1 or scale.dtype != torch.float32 or scale.device != a.device:
         raise ValueError("split_head_grad_pieces: scale must be a one-element float32 tensor on the operands' device")
     return _split_head_grad_pieces_op(a, b, int(k), labels, lse, scale.reshape(1).contiguous(), int(ignore_index))
+
+
+# ---------------------------------------------------------------------------
+# selective state space scan and its short causal convolution
+# ---------------------------------------------------------------------------
+SSM_MAX_STATES = 128
+CONV_MAX_TAPS = 8
+
+
+def _on_device(device: torch.device):
+    """The device context of a launch (nothing to enter on the current one)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_RANGE
+    return torch.cuda.device(device)
+
+
+def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    require_cuda(what, first)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {t.device} and {first.device}; one device expected")
+
+
+def _check_shape(what: str, name: str, t: torch.Tensor | None, shape: tuple) -> None:
+    if t is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} must have shape {list(shape)}, got {list(t.shape)}")
+
+
+def _check_lengths(what: str, lengths: torch.Tensor | None, B: int) -> None:
+    if lengths is None:
+        return
+    _check_shape(what, "lengths", lengths, (B,))
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: lengths must be int32 or int64, got {lengths.dtype}")
+
+
+def _float32(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.dtype == torch.float32 else t.float()
+
+
+def _unit_channels(t: torch.Tensor | None) -> torch.Tensor | None:
+    """Rows with unit channel stride, at whatever row and batch strides."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _short_conv_problem(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
+                        initial_state: torch.Tensor | None, lengths: torch.Tensor | None, silu: bool):
+    """The C problem and the tensors it points into."""
+    x = _unit_channels(x)
+    weight = weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    initial_state = None if initial_state is None else initial_state.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    B, L, D = x.shape
+    p = _lib.ShortConvProblem(B, L, D, weight.shape[1], dtype_code(x.dtype, "short_conv"), int(silu),
+                              0 if lengths is None else lengths.element_size(), x.data_ptr(), weight.data_ptr(),
+                              _ptr(bias), _ptr(initial_state), _ptr(lengths), x.stride(1), x.stride(0))
+    return p, (x, weight, bias, initial_state, lengths)
+
+
+@_op("mogt::short_conv")
+def _short_conv_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
+                   initial_state: torch.Tensor | None, lengths: torch.Tensor | None, silu: bool,
+                   want_state: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    B, L, D = x.shape
+    y = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
+    last = torch.empty((B, weight.shape[1] - 1, D) if want_state else (0,), dtype=x.dtype, device=x.device)
+    p, held = _short_conv_problem(x, weight, bias, initial_state, lengths, silu)
+    with _on_device(x.device):
+        rc = _lib.load().mogt_short_conv_fwd(ctypes.byref(p), y.data_ptr(), last.data_ptr() if want_state else None,
+                                             _stream_handle(x.device))
+    _lib.check(rc, "mogt_short_conv_fwd")
+    return y, last
+
+
+@_short_conv_op.register_fake
+def _(x, weight, bias, initial_state, lengths, silu, want_state):
+    B, L, D = x.shape
+    return x.new_empty((B, L, D)), x.new_empty((B, weight.shape[1] - 1, D) if want_state else (0,))
+
+
+@_op("mogt::short_conv_grad")
+def _short_conv_grad_op(dy: torch.Tensor, dlast: torch.Tensor | None, x: torch.Tensor, weight: torch.Tensor,
+                        bias: torch.Tensor | None, initial_state: torch.Tensor | None, lengths: torch.Tensor | None,
+                        silu: bool, need_x: bool, need_state: bool
+                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias, dinitial_state); dx and dinitial_state are empty
+    where not needed."""
+    lib = _lib.load()
+    B, L, D = x.shape
+    K = weight.shape[1]
+    dy = dy.to(x.dtype).contiguous()
+    dlast = None if dlast is None else dlast.to(x.dtype).contiguous()
+    dx = torch.empty((B, L, D) if need_x else (0,), dtype=x.dtype, device=x.device)
+    dinit = torch.empty((B, K - 1, D) if need_state else (0,), dtype=x.dtype, device=x.device)
+    some = B > 0 and D > 0
+    dw = (torch.empty if some else torch.zeros)((D, K), dtype=torch.float32, device=x.device)
+    db = (torch.empty if some else torch.zeros)((D,), dtype=torch.float32, device=x.device)
+    p, held = _short_conv_problem(x, weight, bias, initial_state, lengths, silu)
+    ws = scratch(lib.mogt_short_conv_bwd_workspace_bytes(B, L, D, K), x.device)
+    with _on_device(x.device):
+        rc = lib.mogt_short_conv_bwd(ctypes.byref(p), dy.data_ptr(), _ptr(dlast), dx.data_ptr() if need_x else None,
+                                     dw.data_ptr(), db.data_ptr(), dinit.data_ptr() if need_state else None,
+                                     ws.data_ptr(), ws.numel(), _stream_handle(x.device))
+    _lib.check(rc, "mogt_short_conv_bwd")
+    return dx, dw, db, dinit
+
+
+@_short_conv_grad_op.register_fake
+def _(dy, dlast, x, weight, bias, initial_state, lengths, silu, need_x, need_state):
+    B, L, D = x.shape
+    return (x.new_empty((B, L, D) if need_x else (0,)), weight.new_empty(weight.shape),
+            weight.new_empty((D,)), x.new_empty((B, weight.shape[1] - 1, D) if need_state else (0,)))
+
+
+def _short_conv_setup(ctx, inputs, output):
+    x, weight, bias, initial_state, lengths, silu, want_state = inputs
+    ctx.save_for_backward(x, weight, bias, initial_state, lengths)
+    ctx.silu = silu
+    ctx.want_state = want_state
+    ctx.set_materialize_grads(False)
+
+
+def _short_conv_backward(ctx, dy, dlast):
+    x, weight, bias, initial_state, lengths = ctx.saved_tensors
+    if not ctx.want_state:
+        dlast = None
+    if dy is None and dlast is None:
+        return (None,) * 7
+    if dy is None:
+        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+    need = ctx.needs_input_grad
+    dx, dw, db, dinit = _short_conv_grad_op(dy, dlast, x, weight, bias, initial_state, lengths, ctx.silu, need[0],
+                                            need[3])
+    return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dinit if need[3] else None,
+            None, None, None)
+
+
+_short_conv_op.register_autograd(_short_conv_backward, _short_conv_setup)
+
+
+def _check_conv(what: str, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
+                state: torch.Tensor | None, activation: str | None) -> None:
+    _same_device(what, x, weight, bias, state)
+    dtype_code(x.dtype, what)
+    D = x.shape[-1]
+    if weight.ndim != 2 or weight.shape[0] != D:
+        raise ValueError(f"{what}: weight must be [{D}, taps], got {list(weight.shape)}")
+    if not 1 <= weight.shape[1] <= CONV_MAX_TAPS:
+        raise ValueError(f"{what}: {weight.shape[1]} taps not supported (1 to {CONV_MAX_TAPS})")
+    _check_shape(what, "bias", bias, (D,))
+    if activation not in (None, "silu"):
+        raise ValueError(f"{what}: activation {activation!r} not supported (None or 'silu')")
+    if state is not None:
+        _check_shape(what, "state", state, (x.shape[0], weight.shape[1] - 1, D))
+        if state.dtype != x.dtype:
+            raise ValueError(f"{what}: the state must have x's dtype {x.dtype}, got {state.dtype}")
+
+
+def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+               activation: str | None = None, initial_state: torch.Tensor | None = None,
+               lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Short causal depthwise convolution over channels-last rows.
+
+    ``y_t = act(bias + sum_k weight[:, k] * x_{t-K+1+k})`` for ``x [B, L, D]``
+    (float32 or bfloat16, any row and batch strides), ``weight [D, K]`` with K
+    up to 8, ``activation`` None or "silu"; fp32 arithmetic, ``y`` in x's dtype.
+    ``initial_state [B, K-1, D]`` (x's dtype) holds the inputs before the first
+    step (zero without it).  ``lengths [B]`` (int32 or int64 on the GPU, taken
+    within [0, L]) marks the padding of a ragged batch: rows past a length are
+    not read, their outputs and gradients are zero.  With ``return_state`` also
+    returns the last K-1 inputs of each sequence, which ``short_conv`` and
+    ``short_conv_step`` continue from.  Differentiable in x, weight, bias and
+    initial_state, through both outputs."""
+    if x.ndim != 3:
+        raise ValueError("short_conv: x must be [B, L, D]")
+    _check_conv("short_conv", x, weight, bias, initial_state, activation)
+    _same_device("short_conv", x, lengths)
+    _check_lengths("short_conv", lengths, x.shape[0])
+    y, last = _short_conv_op(x, _float32(weight), _float32(bias), initial_state, lengths, activation == "silu",
+                             bool(return_state))
+    return (y, last) if return_state else y
+
+
+@_op("mogt::short_conv_step_", mutates=("state",))
+def _short_conv_step_op(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
+                        silu: bool) -> torch.Tensor:
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    p, held = _short_conv_problem(x.unsqueeze(1), weight, bias, None, None, silu)
+    with _on_device(x.device):
+        rc = _lib.load().mogt_short_conv_step(ctypes.byref(p), state.data_ptr(), y.data_ptr(),
+                                              _stream_handle(x.device))
+    _lib.check(rc, "mogt_short_conv_step")
+    return y
+
+
+@_short_conv_step_op.register_fake
+def _(x, state, weight, bias, silu):
+    return x.new_empty(x.shape)
+
+
+def _check_step_state(what: str, state: torch.Tensor) -> None:
+    if not state.is_contiguous():
+        raise ValueError(f"{what}: the state is updated in place and must be contiguous")
+
+
+def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                    activation: str | None = None) -> torch.Tensor:
+    """One token of ``short_conv``: ``x [B, D]``; ``state [B, K-1, D]``, the last
+    K-1 inputs (x's dtype, contiguous), is shifted in place.  No autograd."""
+    if x.ndim != 2:
+        raise ValueError("short_conv_step: x must be [B, D]")
+    _check_conv("short_conv_step", x, weight, bias, state, activation)
+    _check_step_state("short_conv_step", state)
+    return _short_conv_step_op(x, state, _float32(weight), _float32(bias), activation == "silu")
+
+
+# One wave scans a segment of a sequence for 64 channels and 16 states.  The
+# segments that make about two waves per SIMD (256 CUs x 4) keep the vector
+# units busy; more would repeat the exponentials of the sums pass without need.
+SSM_WAVES = 2048
+SSM_MIN_SEGMENT = 16
+
+
+def _ssm_segment(B: int, L: int, D: int, N: int, G: int) -> int:
+    """Steps of a segment (a multiple of 8)."""
+    waves = max(1, B * G * -(-(D // G) // 64) * (-(-N // 16) if N > 16 else 1))
+    return max(SSM_MIN_SEGMENT, 8 * -(-L // (8 * max(1, SSM_WAVES // waves))))
+
+
+def _ssm_rows(m: torch.Tensor) -> torch.Tensor:
+    """B or C with its groups' states contiguous in a row."""
+    G, N = m.shape[-2:]
+    return m if (m.stride(-1) == 1 or N == 1) and (m.stride(-2) == N or G == 1) else m.contiguous()
+
+
+def _ssm_problem(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                 D: torch.Tensor | None, z: torch.Tensor | None, delta_bias: torch.Tensor | None,
+                 initial_state: torch.Tensor | None, lengths: torch.Tensor | None, softplus: bool, segment: int):
+    """The C problem and the tensors it points into."""
+    x, delta, z = _unit_channels(x), _unit_channels(delta), _unit_channels(z)
+    B, C = _ssm_rows(B), _ssm_rows(C)
+    if B.dtype == torch.bfloat16 and segment:
+        # the scan reads bf16 rows as 32-bit words
+        odd = B.shape[-1] | B.stride(0) | B.stride(1) | C.stride(0) | C.stride(1)
+        if odd & 1 or (B.data_ptr() | C.data_ptr()) & 3:
+            B, C = B.float().contiguous(), C.float().contiguous()
+    f32 = [None if t is None else t.contiguous() for t in (A, D, delta_bias, initial_state)]
+    lengths = None if lengths is None else lengths.contiguous()
+    b, L, ch = x.shape
+    p = _lib.SsmProblem(b, L, ch, A.shape[1], B.shape[2], segment, dtype_code(x.dtype, "ssm_scan"),
+                        dtype_code(B.dtype, "ssm_scan"), int(softplus),
+                        0 if lengths is None else lengths.element_size(), x.data_ptr(), delta.data_ptr(), _ptr(z),
+                        B.data_ptr(), C.data_ptr(), *[_ptr(t) for t in f32], _ptr(lengths), x.stride(1), x.stride(0),
+                        delta.stride(1), delta.stride(0), 0 if z is None else z.stride(1),
+                        0 if z is None else z.stride(0), B.stride(1), B.stride(0), C.stride(1), C.stride(0))
+    return p, (x, delta, z, B, C, f32, lengths)
+
+
+@_op("mogt::ssm_scan")
+def _ssm_scan_op(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                 D: torch.Tensor | None, z: torch.Tensor | None, delta_bias: torch.Tensor | None,
+                 initial_state: torch.Tensor | None, lengths: torch.Tensor | None, softplus: bool, want_state: bool,
+                 want_carries: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    lib = _lib.load()
+    b, L, ch = x.shape
+    N = A.shape[1]
+    segment = _ssm_segment(b, L, ch, N, B.shape[2])
+    f32 = dict(dtype=torch.float32, device=x.device)
+    out = torch.empty((b, L, ch), dtype=x.dtype, device=x.device)
+    state = torch.empty((b, ch, N) if want_state else (0,), **f32)
+    carries = torch.empty((b, max(1, -(-L // segment)), N, ch) if want_carries else (0,), **f32)
+    p, held = _ssm_problem(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, softplus, segment)
+    nbytes = lib.mogt_ssm_scan_workspace_bytes(b, L, ch, N, segment)
+    ws = scratch(nbytes, x.device) if nbytes else None
+    with _on_device(x.device):
+        rc = lib.mogt_ssm_scan_fwd(ctypes.byref(p), out.data_ptr(), state.data_ptr() if want_state else None,
+                                   carries.data_ptr() if want_carries else None, _ptr(ws), nbytes,
+                                   _stream_handle(x.device))
+    _lib.check(rc, "mogt_ssm_scan_fwd")
+    return out, state, carries
+
+
+@_ssm_scan_op.register_fake
+def _(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, softplus, want_state, want_carries):
+    b, L, ch = x.shape
+    N = A.shape[1]
+    segment = _ssm_segment(b, L, ch, N, B.shape[2])
+    return (x.new_empty((b, L, ch)), A.new_empty((b, ch, N) if want_state else (0,)),
+            A.new_empty((b, max(1, -(-L // segment)), N, ch) if want_carries else (0,)))
+
+
+@_op("mogt::ssm_scan_grad")
+def _ssm_scan_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, x: torch.Tensor, delta: torch.Tensor,
+                      A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: torch.Tensor | None,
+                      z: torch.Tensor | None, delta_bias: torch.Tensor | None, lengths: torch.Tensor | None,
+                      carries: torch.Tensor, softplus: bool, need: list[bool]) -> list[torch.Tensor]:
+    """Gradients of (x, delta, A, B, C, D, z, delta_bias, initial_state); empty
+    where ``need`` is false."""
+    lib = _lib.load()
+    b, L, ch = x.shape
+    N, G = A.shape[1], B.shape[2]
+    segment = _ssm_segment(b, L, ch, N, G)
+    dout = dout.to(x.dtype).contiguous()
+    dfinal = None if dfinal is None else dfinal.to(torch.float32).contiguous()
+    p, held = _ssm_problem(x, delta, A, B, C, D, z, delta_bias, None, lengths, softplus, segment)
+    bc_dtype = held[3].dtype   # what the kernel reads and writes; B's and C's, or fp32
+    rows, f32 = (b, L, ch), torch.float32
+    shapes = [(rows, x.dtype), (rows, x.dtype), ((ch, N), f32), ((b, L, G, N), bc_dtype), ((b, L, G, N), bc_dtype),
+              ((ch,), f32), (rows, x.dtype), ((ch,), f32), ((b, ch, N), f32)]
+    make = torch.empty if b > 0 and ch > 0 else torch.zeros
+    grads = [make(s if n else (0,), dtype=t, device=x.device) for (s, t), n in zip(shapes, need)]
+    dx, ddelta, dA, dB, dC, dD, dz, dbias, dinit = [_ptr(g) if n else None for g, n in zip(grads, need)]
+    ws = scratch(lib.mogt_ssm_scan_bwd_workspace_bytes(b, L, ch, N, G, segment), x.device)
+    out = _lib.SsmGradients(dx, ddelta, dz, dB, dC, dA, dD, dbias, dinit)
+    with _on_device(x.device):
+        rc = lib.mogt_ssm_scan_bwd(ctypes.byref(p), dout.data_ptr(), _ptr(dfinal), carries.data_ptr(),
+                                   ctypes.byref(out), ws.data_ptr(), ws.numel(), _stream_handle(x.device))
+    _lib.check(rc, "mogt_ssm_scan_bwd")
+    if bc_dtype != B.dtype:
+        grads[3], grads[4] = grads[3].to(B.dtype), grads[4].to(B.dtype)
+    return grads
+
+
+@_ssm_scan_grad_op.register_fake
+def _(dout, dfinal, x, delta, A, B, C, D, z, delta_bias, lengths, carries, softplus, need):
+    b, L, ch = x.shape
+    N, G = A.shape[1], B.shape[2]
+    rows = (b, L, ch)
+    shapes = [(rows, x), (rows, x), ((ch, N), A), ((b, L, G, N), B), ((b, L, G, N), B), ((ch,), A), (rows, x),
+              ((ch,), A), ((b, ch, N), A)]
+    return [t.new_empty(s if n else (0,)) for (s, t), n in zip(shapes, need)]
+
+
+def _ssm_scan_setup(ctx, inputs, output):
+    x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, softplus, want_state, want_carries = inputs
+    ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, lengths, output[2])
+    ctx.softplus = softplus
+    ctx.want_state = want_state
+    ctx.want_carries = want_carries
+    # the carries are saved for the backward, not differentiated
+    ctx.set_materialize_grads(False)
+
+
+def _ssm_scan_backward(ctx, dout, dfinal, dcarries):
+    x, delta, A, B, C, D, z, delta_bias, lengths, carries = ctx.saved_tensors
+    if not ctx.want_state:
+        dfinal = None
+    if dout is None and dfinal is None:
+        return (None,) * 13
+    if not ctx.want_carries:
+        raise RuntimeError("ssm_scan: the forward kept no carries for this backward")
+    if dout is None:
+        dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+    need = list(ctx.needs_input_grad[:9])
+    grads = _ssm_scan_grad_op(dout, dfinal, x, delta, A, B, C, D, z, delta_bias, lengths, carries, ctx.softplus, need)
+    return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 4
+
+
+_ssm_scan_op.register_autograd(_ssm_scan_backward, _ssm_scan_setup)
+
+
+def _check_ssm(what: str, x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+               D: torch.Tensor | None, z: torch.Tensor | None, delta_bias: torch.Tensor | None,
+               state: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Argument checks of the scan and its step; returns B and C as [..., G, N]."""
+    _same_device(what, x, delta, A, B, C, D, z, delta_bias, state)
+    dtype_code(x.dtype, what)
+    rows, ch = tuple(x.shape[:-1]), x.shape[-1]
+    if A.ndim != 2 or A.shape[0] != ch:
+        raise ValueError(f"{what}: A must be [{ch}, states], got {list(A.shape)}")
+    N = A.shape[1]
+    if not 1 <= N <= SSM_MAX_STATES:
+        raise ValueError(f"{what}: {N} states not supported (1 to {SSM_MAX_STATES})")
+    _check_shape(what, "delta", delta, tuple(x.shape))
+    _check_shape(what, "z", z, tuple(x.shape))
+    for name, t in (("delta", delta), ("z", z)):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f"{what}: {name} must have x's dtype {x.dtype}, got {t.dtype}")
+    _check_shape(what, "D", D, (ch,))
+    _check_shape(what, "delta_bias", delta_bias, (ch,))
+    if state is not None:
+        _check_shape(what, "state", state, (rows[0], ch, N))
+        if state.dtype != torch.float32:
+            raise ValueError(f"{what}: the state must be float32, got {state.dtype}")
+    if B.shape != C.shape:
+        raise ValueError(f"{what}: B {list(B.shape)} and C {list(C.shape)} must have the same shape")
+    if B.ndim == len(rows) + 1:
+        B, C = B.unsqueeze(-2), C.unsqueeze(-2)
+    if B.ndim != len(rows) + 2 or tuple(B.shape[:-2]) != rows or B.shape[-1] != N or B.shape[-2] < 1:
+        raise ValueError(f"{what}: B and C must be {list(rows)} + [{N}] or [groups, {N}], got {list(C.shape)}")
+    if ch % B.shape[-2] != 0:
+        raise ValueError(f"{what}: {ch} channels do not divide into {B.shape[-2]} groups")
+    if B.dtype != C.dtype or B.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{what}: B and C must both have dtype {x.dtype} or float32, got {B.dtype} and {C.dtype}")
+    return B, C
+
+
+def ssm_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+             D: torch.Tensor | None = None, z: torch.Tensor | None = None, delta_bias: torch.Tensor | None = None,
+             delta_softplus: bool = False, initial_state: torch.Tensor | None = None,
+             lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Selective state space scan: N states per channel, with a step size, an
+    input row and a readout row per token.
+
+    ``dt = delta + delta_bias`` (``softplus`` of it with ``delta_softplus``),
+    ``h_t[d, n] = exp(dt_t[d] A[d, n]) h_{t-1}[d, n] + dt_t[d] x_t[d] B_t[n]``,
+    ``y_t[d] = sum_n C_t[n] h_t[d, n] + D[d] x_t[d]``, returned times ``silu(z)``
+    where ``z`` is given.  ``x``, ``delta``, ``z`` are ``[B, L, D]`` of one dtype
+    (float32 or bfloat16, any row and batch strides), ``A [D, N]`` with N up to
+    128, ``B`` and ``C`` ``[B, L, N]`` or ``[B, L, G, N]`` (each group shared by
+    D/G consecutive channels; x's dtype or float32).  fp32 state and arithmetic,
+    the output in x's dtype.  ``initial_state [B, D, N]`` (float32, zero without
+    it); ``return_state`` also returns the final one, from which ``ssm_scan`` and
+    ``ssm_step`` continue.  ``lengths [B]`` (int32 or int64 on the GPU, taken
+    within [0, L]) marks the padding of a ragged batch: steps past a length are
+    not read and leave the state as it is; their outputs and gradients are zero.
+    Differentiable in every tensor but ``lengths``, through both outputs; the
+    gradients do not change from run to run."""
+    if x.ndim != 3:
+        raise ValueError("ssm_scan: x must be [B, L, D]")
+    B, C = _check_ssm("ssm_scan", x, delta, A, B, C, D, z, delta_bias, initial_state)
+    _same_device("ssm_scan", x, lengths)
+    _check_lengths("ssm_scan", lengths, x.shape[0])
+    want_carries = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, delta, A, B, C, D, z, delta_bias, initial_state))
+    out, state, _ = _ssm_scan_op(x, delta, _float32(A), B, C, _float32(D), z, _float32(delta_bias), initial_state,
+                                 lengths, bool(delta_softplus), bool(return_state), want_carries)
+    return (out, state) if return_state else out
+
+
+@_op("mogt::ssm_step_", mutates=("state",))
+def _ssm_step_op(x: torch.Tensor, state: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+                 C: torch.Tensor, D: torch.Tensor | None, z: torch.Tensor | None, delta_bias: torch.Tensor | None,
+                 softplus: bool) -> torch.Tensor:
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    p, held = _ssm_problem(x.unsqueeze(1), delta.unsqueeze(1), A, B.unsqueeze(1), C.unsqueeze(1), D,
+                           None if z is None else z.unsqueeze(1), delta_bias, None, None, softplus, 0)
+    with _on_device(x.device):
+        rc = _lib.load().mogt_ssm_step(ctypes.byref(p), state.data_ptr(), out.data_ptr(), _stream_handle(x.device))
+    _lib.check(rc, "mogt_ssm_step")
+    return out
+
+
+@_ssm_step_op.register_fake
+def _(x, state, delta, A, B, C, D, z, delta_bias, softplus):
+    return x.new_empty(x.shape)
+
+
+def ssm_step(x: torch.Tensor, state: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+             C: torch.Tensor, *, D: torch.Tensor | None = None, z: torch.Tensor | None = None,
+             delta_bias: torch.Tensor | None = None, delta_softplus: bool = False) -> torch.Tensor:
+    """One token of ``ssm_scan`` for every sequence: ``x``, ``delta``, ``z``
+    ``[B, D]``, ``B`` and ``C`` ``[B, N]`` or ``[B, G, N]``; ``state [B, D, N]``
+    (float32, contiguous) is updated in place.  No autograd."""
+    if x.ndim != 2:
+        raise ValueError("ssm_step: x must be [B, D]")
+    B, C = _check_ssm("ssm_step", x, delta, A, B, C, D, z, delta_bias, state)
+    _check_step_state("ssm_step", state)
+    return _ssm_step_op(x, state, delta, _float32(A), B, C, _float32(D), z, _float32(delta_bias),
+                        bool(delta_softplus))

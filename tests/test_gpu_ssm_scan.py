@@ -1,0 +1,372 @@
+"""Selective state space scan and its step (``ops.ssm_scan``, ``ops.ssm_step``)
+against the float64 loops of ``oracle/ssm_oracle.py``.
+
+Tolerances, derived: every result is a sum of products, and its error is
+measured against the same sum with absolute values (the oracle's ``mag``), S.
+One rounding is 2^-24 of what it rounds.  The step size carries up to 24 of
+them (its argument's, |raw| < 8 in the softplus's exponent, and the
+exponential's, logarithm's and reciprocal's one or two ulp each); a decay takes
+2 more and the product of t decays the sum of what they carry, at most
+24 |A| sum(dt) exp(-|A| sum(dt)) < 9 for the step size's part plus 2 t <= 2 L.
+The sums add at most one rounding per term in fp32: N states, L steps (dA, dD,
+bias), D channels (dB, dC).  Each test's bound is (64 + 4 (L + N + D)) 2^-24 S.
+With positive or no decay (A >= 0) the step size's part is not damped: 26 |A|
+sum(dt) more.  bf16 outputs add half a step, 2^-8 of the value."""
+import pytest
+import torch
+
+from conftest import announce
+from oracle import ssm_oracle as so
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+NAMES = ("x", "delta", "A", "B", "C", "D", "z", "delta_bias", "initial_state")
+
+
+def make(B, L, D, N, G=1, dtype=torch.float32, z=True, softplus=True, skip=True, bias=True, init=True, lengths=None,
+         seed=0, device="cuda"):
+    g = torch.Generator(device=device).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=device)  # noqa: E731
+    t = dict(x=r(B, L, D).to(dtype), delta=(0.7 * r(B, L, D)).to(dtype) if softplus else
+             (0.1 * r(B, L, D).abs()).to(dtype), A=-torch.rand(D, N, generator=g, device=device) * 4,
+             B=r(B, L, G, N).to(dtype), C=r(B, L, G, N).to(dtype))
+    t["D"] = r(D) if skip else None
+    t["z"] = r(B, L, D).to(dtype) if z else None
+    t["delta_bias"] = (r(D) - 2 if softplus else 0.05 * r(D).abs()) if bias else None
+    t["initial_state"] = r(B, D, N) if init else None
+    kw = dict(delta_softplus=softplus, lengths=None if lengths is None else
+              torch.tensor(lengths, device=device, dtype=torch.int32))
+    return t, kw
+
+
+def call(t, kw, **more):
+    from mogt_amd import ops
+    return ops.ssm_scan(t["x"], t["delta"], t["A"], t["B"], t["C"], D=t["D"], z=t["z"], delta_bias=t["delta_bias"],
+                        initial_state=t["initial_state"], **kw, **more)
+
+
+def bound(t, extra=0.0):
+    B, L, D = t["x"].shape
+    return (64 + 4 * (L + t["A"].shape[1] + D) + extra) * U
+
+
+def check(name, got, want, mag, tol):
+    got = got.detach()
+    half = torch.finfo(got.dtype).eps / 2 if got.dtype != torch.float32 else 0.0
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    err = (got.double().cpu() - want).abs()
+    lim = tol * mag + half * (want.abs() + tol * mag) + 1e-30
+    assert bool((err <= lim).all()), f"{name}: {float((err / lim).max()):.3g} of the bound"
+
+
+def oracle(t, kw, **more):
+    args = [t[k] for k in ("x", "delta", "A", "B", "C")]
+    opt = {k: t[k] for k in ("D", "z", "delta_bias", "initial_state")}
+    return [so.ssm_scan(*args, **opt, **kw, **more, mag=m) for m in (False, True)]
+
+
+def run_both(t, kw, seed=1, tol=None):
+    """Forward and all gradients, through both outputs, against the oracle."""
+    B, L, D = t["x"].shape
+    N = t["A"].shape[1]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    dout = torch.randn(B, L, D, generator=g, device="cuda").to(t["x"].dtype)
+    dstate = torch.randn(B, D, N, generator=g, device="cuda")
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None}
+    out, state = call({**{k: None for k in NAMES}, **leaves}, kw, return_state=True)
+    grads = dict(zip(leaves, torch.autograd.grad([out, state], list(leaves.values()), [dout, dstate])))
+    want, mag = oracle(t, kw, dout=dout, dstate=dstate)
+    tol = bound(t) if tol is None else tol
+    check("out", out, want["out"], mag["out"], tol)
+    check("state", state, want["state"], mag["state"], tol)
+    for k, v in grads.items():
+        assert v.dtype == t[k].dtype
+        check("d" + k, v, want["d" + k], mag["d" + k], tol)
+    return out, state, grads
+
+
+F32, BF16 = torch.float32, torch.bfloat16
+SHAPES = [  # B, L, D, N, G, dtype: single tokens, edges of the 8-step blocks and of the segments, odd sizes
+    (1, 1, 1, 1, 1, F32), (2, 1, 64, 16, 1, BF16), (1, 7, 65, 16, 1, F32), (1, 8, 64, 16, 1, BF16),
+    (2, 9, 63, 3, 1, F32), (1, 16, 128, 16, 2, F32), (1, 17, 70, 8, 7, BF16), (3, 31, 130, 15, 1, BF16),
+    (1, 33, 40, 16, 4, BF16), (1, 100, 64, 17, 1, F32), (2, 25, 66, 24, 2, BF16), (1, 40, 64, 64, 1, BF16),
+    (1, 19, 65, 128, 1, F32), (1, 18, 10, 127, 5, BF16), (1, 300, 64, 16, 1, BF16), (2, 129, 192, 4, 3, F32),
+]
+
+
+@pytest.mark.parametrize("B,L,D,N,G,dtype", SHAPES)
+def test_forward_and_gradients(gpu, B, L, D, N, G, dtype):
+    announce(f"ssm_scan B={B} L={L} D={D} N={N} G={G} {dtype}")
+    run_both(*make(B, L, D, N, G, dtype, seed=L))
+
+
+@pytest.mark.parametrize("opt", [dict(z=False), dict(softplus=False), dict(skip=False), dict(bias=False),
+                                 dict(init=False), dict(z=False, softplus=False, skip=False, bias=False, init=False)])
+@pytest.mark.parametrize("dtype,N", [(F32, 16), (BF16, 40)])
+def test_options(gpu, opt, dtype, N):
+    announce(f"ssm_scan options {opt} {dtype}")
+    run_both(*make(2, 37, 72, N, 1, dtype, seed=4, **opt))
+
+
+@pytest.mark.parametrize("lengths", [[50, 0, 1, 49], [0, 0, 0, 0], [16, 17, 8, 9], [60, -3, 50, 32]])
+@pytest.mark.parametrize("N", [16, 20])
+def test_lengths(gpu, lengths, N):
+    """Empty and single-token sequences, lengths at the edges of blocks and
+    segments, and lengths outside the batch, which count as its ends."""
+    announce(f"ssm_scan lengths {lengths} N={N}")
+    t, kw = make(4, 50, 64, N, 2, F32, lengths=lengths, seed=2)
+    out, state, grads = run_both(t, kw)
+    for i, n in enumerate(lengths):
+        n = min(max(n, 0), 50)
+        for v in (out, grads["x"], grads["delta"], grads["z"], grads["B"], grads["C"]):
+            assert not v[i, n:].any()
+        if n == 0:
+            assert torch.equal(state[i], t["initial_state"][i])
+
+
+def test_padding_is_not_read(gpu):
+    """NaN and infinities in the padded rows reach nothing."""
+    t, kw = make(3, 40, 64, 16, 1, F32, lengths=[40, 13, 0], seed=3)
+    clean = [o.clone() for o in call(t, kw, return_state=True)]
+    bad = {k: v if v is None else v.clone() for k, v in t.items()}
+    for k, v in (("x", float("nan")), ("delta", float("inf")), ("B", float("nan")), ("C", float("-inf")),
+                 ("z", float("nan"))):
+        bad[k][1, 13:] = v
+        bad[k][2] = v
+    for a, b in zip(call(bad, kw, return_state=True), clean):
+        assert torch.equal(a, b)
+    _, _, want = run_both(t, kw)
+    leaves = {k: v.requires_grad_(True) for k, v in bad.items()}
+    g = torch.Generator(device="cuda").manual_seed(1)
+    dout = torch.randn(3, 40, 64, generator=g, device="cuda")
+    dstate = torch.randn(3, 64, 16, generator=g, device="cuda")
+    dout[1, 13:] = float("nan")
+    got = torch.autograd.grad(list(call(leaves, kw, return_state=True)), list(leaves.values()), [dout, dstate])
+    for k, v in zip(leaves, got):
+        assert torch.equal(v, want[k]), k
+
+
+def test_decays_of_zero_one_and_above(gpu):
+    """A of 0 keeps the state for good, a large step size clears it, a positive A
+    grows it."""
+    t, kw = make(1, 60, 64, 16, seed=6)
+    t["A"][:, 0] = 0.0
+    t["A"][:, 1] = 0.05
+    t["A"][:, 2] = -200.0
+    t["delta"][0, 20] = 30.0
+    run_both(t, kw, tol=bound(t, 26 * 0.05 * 40 + 26 * 4))
+
+
+def test_long_sequence_in_many_segments(gpu):
+    announce("ssm_scan 3000 steps")
+    run_both(*make(1, 3000, 16, 16, 1, F32, seed=8))
+
+
+def test_strided_rows(gpu):
+    """Inputs as slices of wider projections, broadcast batches, transposed rows."""
+    t, kw = make(2, 21, 64, 16, 2, BF16, seed=5)
+    want = call(t, kw)
+    proj = torch.zeros(2, 21, 3 * 64 + 2, dtype=BF16, device="cuda")
+    proj[..., 1:65], proj[..., 66:130], proj[..., 130:194] = t["x"], t["z"], t["delta"]
+    bc = torch.zeros(2, 21, 2 * 32 + 3, dtype=BF16, device="cuda")
+    bc[..., 1:33], bc[..., 33:65] = t["B"].flatten(2), t["C"].flatten(2)
+    s = {**t, "x": proj[..., 1:65], "z": proj[..., 66:130], "delta": proj[..., 130:194],
+         "B": bc[..., 1:33].unflatten(-1, (2, 16)), "C": bc[..., 33:65].unflatten(-1, (2, 16))}
+    assert torch.equal(call(s, kw), want)
+    time_first = {k: v.transpose(0, 1).contiguous().transpose(0, 1) if k in ("x", "z", "delta", "B", "C") else v
+                  for k, v in t.items()}
+    assert torch.equal(call(time_first, kw), want)
+    channel_slow = {**t, "x": t["x"].transpose(1, 2).contiguous().transpose(1, 2)}
+    assert torch.equal(call(channel_slow, kw), want)
+    one = {**t, "x": t["x"][:1].expand(2, -1, -1), "B": t["B"][:, :1].expand(-1, 21, -1, -1)}
+    same = {k: v if v is None else v.contiguous() for k, v in one.items()}
+    assert torch.equal(call(one, kw), call(same, kw))
+
+
+def test_shared_rows_and_dtypes(gpu):
+    """B and C without a group dimension, in fp32 beside bf16 rows, parameters in bf16."""
+    from mogt_amd import ops
+    t, kw = make(2, 30, 64, 16, 1, BF16, seed=7)
+    want = call(t, kw)
+    flat = {**t, "B": t["B"].squeeze(2), "C": t["C"].squeeze(2)}
+    assert torch.equal(call(flat, kw), want)
+    wide = {**t, "B": t["B"].float(), "C": t["C"].float()}
+    assert torch.equal(call(wide, kw), want)
+    half = {k: t[k].bfloat16() for k in ("A", "D", "delta_bias")}
+    assert torch.equal(call({**t, **half}, kw), call({**t, **{k: v.float() for k, v in half.items()}}, kw))
+    with torch.enable_grad():
+        leaf = half["A"].requires_grad_(True)
+        flat["B"] = flat["B"].requires_grad_(True)
+        dA, dB = torch.autograd.grad(call({**flat, "A": leaf}, kw).float().sum(), [leaf, flat["B"]])
+    assert dA.dtype == BF16 and dA.shape == leaf.shape and dB.shape == flat["B"].shape
+    assert ops.ssm_scan(t["x"][:, :0], t["delta"][:, :0], t["A"], t["B"][:, :0], t["C"][:, :0]).shape == (2, 0, 64)
+
+
+@pytest.mark.parametrize("shape", [(0, 5, 8), (2, 0, 8), (2, 5, 0)])
+def test_empty(gpu, shape):
+    t, kw = make(*shape, 4, seed=1)
+    leaves = {k: v.requires_grad_(True) for k, v in t.items()}
+    out, state = call(leaves, kw, return_state=True)
+    assert out.shape == shape and state.shape == (shape[0], shape[2], 4)
+    if shape[1] == 0:
+        assert torch.equal(state, t["initial_state"])
+    grads = torch.autograd.grad([out, state], list(leaves.values()), [torch.ones_like(out), torch.ones_like(state)])
+    for (k, v), g in zip(leaves.items(), grads):
+        assert g.shape == v.shape
+        assert bool((g == (1.0 if k == "initial_state" and shape[1] == 0 else 0.0)).all()) or g.numel() == 0
+
+
+def test_gradient_is_the_difference_quotient(gpu):
+    """Along a random direction of all inputs.  The quotient's own error: the
+    rounding of two fp32 results, (bound S) / eps with eps = 2^-6, beside the
+    eps^2 of the third derivative; measured against the sum of the gradient's
+    magnitudes along the direction."""
+    t, kw = make(1, 24, 32, 16, seed=12)
+    leaves = {k: v.double().float().requires_grad_(True) for k, v in t.items()}
+    g = torch.Generator(device="cuda").manual_seed(3)
+    way = {k: torch.randn(v.shape, generator=g, device="cuda") for k, v in t.items()}
+    dout = torch.randn(1, 24, 32, generator=g, device="cuda")
+    grads = torch.autograd.grad(call(leaves, kw), list(leaves.values()), dout)
+    along = sum(float((v.double() * way[k].double()).sum()) for k, v in zip(leaves, grads))
+    eps = 2.0 ** -6
+
+    def loss(s):
+        return float((call({k: v + s * way[k] for k, v in t.items()}, kw).double() * dout.double()).sum())
+
+    # four-point quotient: its error is eps^4 of the fifth derivative
+    quotient = (8 * (loss(eps) - loss(-eps)) - (loss(2 * eps) - loss(-2 * eps))) / (12 * eps)
+    size = sum(float((v.double() * way[k].double()).abs().sum()) for k, v in zip(leaves, grads))
+    assert abs(quotient - along) <= 1e-3 * size
+
+
+def test_pieces_and_steps_continue_one_another(gpu):
+    """A prompt in one call, in pieces, and token by token: the same outputs and
+    state up to the order of their roundings."""
+    from mogt_amd import ops
+    t, kw = make(2, 45, 96, 16, 1, F32, seed=10)
+    want, wstate = call(t, kw, return_state=True)
+    _, mag = oracle(t, kw)
+    outs, state = [], t["initial_state"]
+    rows = ("x", "delta", "B", "C", "z")
+    for lo, hi in ((0, 20), (20, 21), (21, 40)):
+        piece = {**t, **{k: t[k][:, lo:hi] for k in rows}, "initial_state": state}
+        o, state = call(piece, kw, return_state=True)
+        outs.append(o)
+    for i in range(40, 45):
+        s = {k: t[k][:, i] for k in rows}
+        outs.append(ops.ssm_step(s["x"], state, s["delta"], t["A"], s["B"], s["C"], D=t["D"], z=s["z"],
+                                 delta_bias=t["delta_bias"], delta_softplus=True)[:, None])
+    check("out", torch.cat(outs, 1), want.double().cpu(), mag["out"], 2 * bound(t))
+    check("state", state, wstate.double().cpu(), mag["state"], 2 * bound(t))
+
+
+@pytest.mark.parametrize("B,D,N,G,dtype", [(1, 1, 1, 1, F32), (3, 65, 16, 1, BF16), (2, 130, 17, 2, F32),
+                                           (5, 64, 128, 1, BF16), (2, 96, 6, 3, BF16), (300, 64, 16, 1, BF16)])
+@pytest.mark.parametrize("plain", [False, True])
+def test_step(gpu, B, D, N, G, dtype, plain):
+    from mogt_amd import ops
+    announce(f"ssm_step B={B} D={D} N={N} G={G} {dtype}")
+    opt = dict(z=False, skip=False, bias=False, softplus=False) if plain else {}
+    t, kw = make(B, 1, D, N, G, dtype, seed=N, **opt)
+    state = t["initial_state"].clone()
+    version = state._version
+    one = {k: v if v is None or k not in ("x", "delta", "B", "C", "z") else v[:, 0] for k, v in t.items()}
+    out = ops.ssm_step(one["x"], state, one["delta"], t["A"], one["B"], one["C"], D=t["D"], z=one["z"],
+                       delta_bias=t["delta_bias"], delta_softplus=kw["delta_softplus"])
+    assert state._version > version
+    want, mag = oracle(t, kw)
+    check("out", out[:, None], want["out"], mag["out"], bound(t))
+    check("state", state, want["state"], mag["state"], bound(t))
+
+
+def test_runs_repeat_bit_for_bit(gpu):
+    t, kw = make(2, 500, 128, 16, 2, BF16, seed=11)
+    first = [v for v in run_once_all(t, kw)]
+    for a, b in zip(first, run_once_all(t, kw)):
+        assert torch.equal(a, b)
+
+
+def run_once_all(t, kw):
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    out, state = call(leaves, kw, return_state=True)
+    return [out, state, *torch.autograd.grad([out, state], list(leaves.values()),
+                                             [torch.ones_like(out), torch.ones_like(state)])]
+
+
+def test_other_stream_and_two_calls_at_once(gpu):
+    """Calls on two streams at a time, each with memory of its own."""
+    t, kw = make(1, 400, 64, 16, 1, F32, seed=13)
+    u, _ = make(1, 400, 64, 16, 1, F32, seed=14)
+    want = call(t, kw), call(u, kw)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call((t, u)[i], kw))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            assert torch.equal(o, want[i])
+
+
+def test_captured_graphs(gpu):
+    """Forward, backward and steps in two captured graphs, replayed in turn with
+    eager calls between; every replay equals the eager result."""
+    from mogt_amd import ops
+    sets = [make(1, 200, 64, 16, 1, F32, seed=s) for s in (20, 21)]
+    wants = [[v.clone() for v in run_once_all(*s)] for s in sets]
+    step_state = sets[0][0]["initial_state"].clone()
+
+    def step():
+        t = sets[0][0]
+        return ops.ssm_step(t["x"][:, 0], step_state, t["delta"][:, 0], t["A"], t["B"][:, 0], t["C"][:, 0])
+
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in sets:
+            run_once_all(*s)
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = run_once_all(*s)
+            if s is sets[0]:
+                o = o + [step()]
+        graphs.append(g)
+        outs.append(o)
+    fresh = sets[0][0]["initial_state"].clone()
+    for turn in range(4):
+        step_state.copy_(fresh)
+        eager = fresh.clone()
+        t = sets[0][0]
+        want_step = ops.ssm_step(t["x"][:, 0], eager, t["delta"][:, 0], t["A"], t["B"][:, 0], t["C"][:, 0])
+        for i in (0, 1) if turn % 2 else (1, 0):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            for k, (a, b) in enumerate(zip(outs[i], wants[i])):
+                assert torch.equal(a, b), (turn, i, k)
+        assert torch.equal(outs[0][-1], want_step) and torch.equal(step_state, eager)
+        assert torch.equal(call(*sets[1]), wants[1][0])
+
+
+def test_partial_gradients_and_second_derivatives(gpu):
+    """Only what is asked for is formed; a second derivative is refused."""
+    t, kw = make(1, 20, 64, 16, seed=15)
+    full = dict(zip(NAMES, run_once_all(t, kw)[2:]))
+    assert list(t) == ["x", "delta", "A", "B", "C", "D", "z", "delta_bias", "initial_state"]
+    for k in NAMES:
+        leaf = {**t, k: t[k].detach().requires_grad_(True)}
+        out, state = call(leaf, kw, return_state=True)
+        (g,) = torch.autograd.grad([out, state], [leaf[k]], [torch.ones_like(out), torch.ones_like(state)])
+        assert torch.equal(g, full[k]), k
+    x = t["x"].detach().requires_grad_(True)
+    (g,) = torch.autograd.grad(call({**t, "x": x}, kw).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

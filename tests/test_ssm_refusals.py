@@ -1,0 +1,198 @@
+"""What the selective scan, the short convolution and their steps refuse: the
+public functions on fake GPU tensors, the C entries before any device call
+(CPU); and the public functions traced into one graph."""
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from mogt_amd import _lib, ops
+
+
+def scan_args(**change):
+    dev = change.pop("device", "cuda")
+    e = lambda *s, dtype=torch.float32: torch.empty(*s, device=dev, dtype=dtype)  # noqa: E731
+    a = dict(x=e(2, 5, 8), delta=e(2, 5, 8), A=e(8, 4), B=e(2, 5, 2, 4), C=e(2, 5, 2, 4), D=e(8), z=e(2, 5, 8),
+             delta_bias=e(8), initial_state=e(2, 8, 4), lengths=e(2, dtype=torch.int32))
+    a.update({k: v(e) for k, v in change.items()})
+    return a
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(x=lambda e: e(5, 8)), r"\[B, L, D\]"),
+    (dict(x=lambda e: e(2, 5, 8, dtype=torch.float16)), "dtype"),
+    (dict(delta=lambda e: e(2, 5, 7)), "delta"),
+    (dict(delta=lambda e: e(2, 5, 8, dtype=torch.bfloat16)), "delta"),
+    (dict(z=lambda e: e(2, 4, 8)), "z must"),
+    (dict(A=lambda e: e(7, 4)), "A must"),
+    (dict(A=lambda e: e(8, 129)), "129 states"),
+    (dict(A=lambda e: e(8, 0)), "0 states"),
+    (dict(B=lambda e: e(2, 5, 4, 4)), "same shape"),
+    (dict(B=lambda e: e(2, 5, 2, 3), C=lambda e: e(2, 5, 2, 3)), "B and C"),
+    (dict(B=lambda e: e(2, 5, 3, 4), C=lambda e: e(2, 5, 3, 4)), "groups"),
+    (dict(B=lambda e: e(2, 5, 0, 4), C=lambda e: e(2, 5, 0, 4)), "B and C"),
+    (dict(B=lambda e: e(2, 5, 2, 4, dtype=torch.float64), C=lambda e: e(2, 5, 2, 4, dtype=torch.float64)), "dtype"),
+    (dict(C=lambda e: e(2, 5, 2, 4, dtype=torch.bfloat16)), "dtype"),
+    (dict(D=lambda e: e(9)), "D must"),
+    (dict(delta_bias=lambda e: e(1)), "delta_bias"),
+    (dict(initial_state=lambda e: e(2, 4, 8)), "state"),
+    (dict(initial_state=lambda e: e(2, 8, 4, dtype=torch.bfloat16)), "float32"),
+    (dict(lengths=lambda e: e(3, dtype=torch.int32)), "lengths"),
+    (dict(lengths=lambda e: e(2)), "lengths"),
+    (dict(A=lambda e: torch.empty(8, 4)), "one device"),
+    (dict(lengths=lambda e: torch.empty(2, dtype=torch.int32)), "one device"),
+    (dict(device="cpu"), "CUDA"),
+])
+def test_scan_refuses(change, word):
+    with FakeTensorMode():
+        a = scan_args(**change)
+        args = [a.pop(k) for k in ("x", "delta", "A", "B", "C")]
+        with pytest.raises(ValueError, match=word):
+            ops.ssm_scan(*args, **a)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(x=lambda e: e(2, 1, 8)), r"\[B, D\]"),
+    (dict(state=lambda e: e(3, 8, 4)), "state"),
+    (dict(state=lambda e: e(2, 8, 4, dtype=torch.bfloat16)), "float32"),
+    (dict(state=lambda e: e(2, 4, 8).transpose(1, 2)), "contiguous"),
+    (dict(B=lambda e: e(2, 5), C=lambda e: e(2, 5)), "B and C"),
+])
+def test_step_refuses(change, word):
+    with FakeTensorMode():
+        e = lambda *s, dtype=torch.float32: torch.empty(*s, device="cuda", dtype=dtype)  # noqa: E731
+        a = dict(x=e(2, 8), state=e(2, 8, 4), delta=e(2, 8), A=e(8, 4), B=e(2, 4), C=e(2, 4))
+        a.update({k: v(e) for k, v in change.items()})
+        with pytest.raises(ValueError, match=word):
+            ops.ssm_step(**a)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(x=lambda e: e(5, 8)), r"\[B, L, D\]"),
+    (dict(x=lambda e: e(2, 5, 8, dtype=torch.float16)), "dtype"),
+    (dict(weight=lambda e: e(7, 4)), "weight"),
+    (dict(weight=lambda e: e(8, 9)), "9 taps"),
+    (dict(weight=lambda e: e(8, 0)), "0 taps"),
+    (dict(bias=lambda e: e(7)), "bias"),
+    (dict(activation=lambda e: "gelu"), "gelu"),
+    (dict(initial_state=lambda e: e(2, 4, 8)), "state"),
+    (dict(initial_state=lambda e: e(2, 3, 8, dtype=torch.bfloat16)), "dtype"),
+    (dict(lengths=lambda e: e(1, dtype=torch.int64)), "lengths"),
+    (dict(lengths=lambda e: e(2, dtype=torch.int16)), "lengths"),
+    (dict(weight=lambda e: torch.empty(8, 4)), "one device"),
+])
+def test_conv_refuses(change, word):
+    with FakeTensorMode():
+        e = lambda *s, dtype=torch.float32: torch.empty(*s, device="cuda", dtype=dtype)  # noqa: E731
+        a = dict(x=e(2, 5, 8), weight=e(8, 4), bias=e(8), activation="silu", initial_state=e(2, 3, 8), lengths=None)
+        a.update({k: v(e) for k, v in change.items()})
+        args = [a.pop(k) for k in ("x", "weight", "bias")]
+        with pytest.raises(ValueError, match=word):
+            ops.short_conv(*args, **a)
+        with pytest.raises(ValueError, match="contiguous"):
+            ops.short_conv_step(e(2, 8), e(2, 8, 3).transpose(1, 2), e(8, 4))
+
+
+class _Traced(Exception):
+    pass
+
+
+def test_traced_into_one_graph():
+    """The public functions under a compiler: one graph, the ops in it; and
+    the gradients' shapes on fake tensors."""
+    with FakeTensorMode():
+        a = scan_args()
+        args = [a.pop(k).requires_grad_(True) for k in ("x", "delta", "A", "B", "C")]
+        w = torch.empty(8, 4, device="cuda", requires_grad=True)
+
+    def layer(x, delta, A, B, C, w):
+        u = ops.short_conv(x, w, activation="silu")
+        out, state = ops.ssm_scan(u, delta, A, B, C, **a, return_state=True)
+        return out.sum() + state.sum()
+
+    graphs = []
+
+    def backend(gm, inputs):
+        graphs.append(gm)
+
+        def run(*_):
+            raise _Traced
+
+        return run
+
+    torch._dynamo.reset()
+    with pytest.raises(_Traced):
+        torch.compile(layer, fullgraph=True, backend=backend)(*args, w)
+    code = "".join(m.code for m in graphs[0].modules() if isinstance(m, torch.fx.GraphModule))
+    assert len(graphs) == 1 and "mogt.ssm_scan" in code and "mogt.short_conv" in code
+    with args[0].fake_mode, torch.no_grad():
+        inputs = [*args, a["D"], a["z"], a["delta_bias"], a["initial_state"]]
+        carries = torch.empty(2, 1, 4, 8, device="cuda")
+        grads = ops._ssm_scan_grad_op(a["z"], None, *inputs[:8], a["lengths"], carries, True, [True] * 9)
+        assert [tuple(g.shape) for g in grads] == [tuple(t.shape) for t in inputs]
+        dx, dw, db, dinit = ops._short_conv_grad_op(a["z"], None, args[0], w, None, None, None, True, True, False)
+        assert dx.shape == args[0].shape and dw.shape == w.shape and dinit.shape == (0,)
+
+
+def scan_problem(**change):
+    p = _lib.SsmProblem(1, 8, 8, 4, 1, 16, 0, 0, 0, 0, *[64] * 5, 64, None, None, None, None, 8, 64, 8, 64, 8, 64, 4,
+                        32, 4, 32)
+    for k, v in change.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("change,rc,word", [
+    (dict(states=0), -1, b"sizes"), (dict(states=129), -1, b"states"), (dict(batch=-1), -1, b"sizes"),
+    (dict(groups=3), -1, b"groups"), (dict(io_dtype=2), -1, b"dtype"), (dict(bc_dtype=1), -1, b"dtype"),
+    (dict(segment=12), -1, b"segment"), (dict(segment=0), -1, b"segment"), (dict(batch=65536), -1, b"batch"),
+    (dict(length=1 << 31), -1, b"length"), (dict(x=None), -1, b"null"), (dict(lengths=64, lengths_bytes=2), -1, b"lengths"),
+    (dict(io_dtype=1, bc_dtype=1, states=3), -1, b"even"), (dict(io_dtype=1, bc_dtype=1, B=66), -1, b"alignment"),
+    (dict(io_dtype=1, bc_dtype=1, C_row=5), -1, b"even"), (dict(length=20), -2, b"workspace"),
+    (dict(length=8 * 65536 * 2, segment=8), -1, b"segments"), (dict(batch=0), 0, b""),
+])
+def test_scan_entry_refuses(change, rc, word):
+    lib = _lib.load()
+    p = scan_problem(**change)
+    assert lib.mogt_ssm_scan_fwd(ctypes.byref(p), 64, None, None, None, 0, None) == rc
+    assert word in lib.mogt_last_error()
+
+
+def test_entries_refuse_null_and_small():
+    lib = _lib.load()
+    p, g = scan_problem(), _lib.SsmGradients()
+    assert lib.mogt_ssm_scan_fwd(None, 64, None, None, None, 0, None) == -1
+    assert lib.mogt_ssm_scan_fwd(ctypes.byref(p), None, None, None, None, 0, None) == -1
+    n = lib.mogt_ssm_scan_bwd_workspace_bytes(1, 8, 8, 4, 1, 16)
+    assert n > 0 and lib.mogt_ssm_scan_bwd_workspace_bytes(1, 8, 8, 4, 3, 16) == 0
+    assert lib.mogt_ssm_scan_bwd(ctypes.byref(p), 64, None, 64, None, 64, n, None) == -1
+    assert lib.mogt_ssm_scan_bwd(ctypes.byref(p), 64, None, None, ctypes.byref(g), 64, n, None) == -1
+    assert lib.mogt_ssm_scan_bwd(ctypes.byref(p), 64, None, 64, ctypes.byref(g), 64, n - 1, None) == -2
+    g.dz, p.z = 64, None
+    assert lib.mogt_ssm_scan_bwd(ctypes.byref(p), 64, None, 64, ctypes.byref(g), 64, n, None) == -1
+    assert lib.mogt_ssm_step(ctypes.byref(p), 64, 64, None) == -1   # length 8
+    assert lib.mogt_ssm_scan_workspace_bytes(1, 16, 8, 4, 16) == 0
+    assert lib.mogt_ssm_scan_workspace_bytes(1, 17, 8, 4, 16) == 2 * 8 * 5 * 4
+
+    c = _lib.ShortConvProblem(1, 8, 8, 4, 0, 1, 0, 64, 64, None, None, None, 8, 64)
+    for k, v, word in (("taps", 9, b"taps"), ("taps", 0, b"taps"), ("io_dtype", 2, b"dtype"), ("length", -1, b"sizes"),
+                       ("length", 1 << 27, b"length"), ("weight", None, b"null"), ("batch", 1 << 17, b"batch")):
+        old = getattr(c, k)
+        setattr(c, k, v)
+        assert lib.mogt_short_conv_fwd(ctypes.byref(c), 64, None, None) == -1 and word in lib.mogt_last_error(), k
+        setattr(c, k, old)
+    assert lib.mogt_short_conv_fwd(ctypes.byref(c), None, None, None) == -1
+    n = lib.mogt_short_conv_bwd_workspace_bytes(1, 8, 8, 4)
+    assert lib.mogt_short_conv_bwd(ctypes.byref(c), 64, None, 64, 64, 64, None, 64, n - 1, None) == -2
+    assert lib.mogt_short_conv_bwd(ctypes.byref(c), None, None, 64, 64, 64, None, 64, n, None) == -1
+    assert lib.mogt_short_conv_step(ctypes.byref(c), 64, 64, None) == -1
+    c.length = 1
+    assert lib.mogt_short_conv_step(ctypes.byref(c), None, 64, None) == -1
+
+
+@pytest.mark.parametrize("B,L,D,N,G", [(1, 1, 1, 1, 1), (1, 200, 1280, 16, 1), (1, 32768, 2048, 16, 1),
+                                       (256, 4096, 2048, 64, 2), (3, 1001, 333, 24, 1), (1, 1 << 20, 64, 128, 1)])
+def test_segments_are_whole_blocks_within_the_grid(B, L, D, N, G):
+    s = ops._ssm_segment(B, L, D, N, G)
+    assert s % 8 == 0 and s >= 16 and -(-L // s) <= max(1, ops.SSM_WAVES)
