@@ -16,7 +16,8 @@
 
 namespace mogt {
 
-int column_sums(const float* part, float* out, int64_t rows, int64_t D, int64_t N, hipStream_t st);
+int column_sums(const float* part, float* a, float* b, float* c, int64_t rows, int64_t K, int64_t D, int64_t N,
+                hipStream_t st);
 
 constexpr int CONV_U = 8;   // steps whose rows are loaded together
 
@@ -30,7 +31,7 @@ struct ConvArgs {
     void *y, *last;                       // forward outputs
     const void *dy, *dlast;               // backward inputs
     void *dx, *dinit;
-    float *part_w, *part_b;               // [B nchunk][K][D], [B nchunk][D]
+    float* part;                          // [B nchunk][K + 1][D]: gradients of the taps, of the bias
 };
 
 __device__ __forceinline__ int conv_length(const ConvArgs& p, int b) {
@@ -256,12 +257,8 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p) {
     const int64_t row = static_cast<int64_t>(b) * p.nchunk + chunk;
 #pragma unroll
     for (int k = 0; k < KM; ++k)
-        if (k < K) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) p.part_w[(row * K + k) * p.D + c + e] = dw[k][e];
-        }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) p.part_b[row * p.D + c + e] = db[e];
+        if (k < K) store_vec<float, VEC>(p.part + (row * (K + 1) + k) * p.D + c, dw[k]);
+    store_vec<float, VEC>(p.part + (row * (K + 1) + K) * p.D + c, db);
 }
 
 // One token: a thread per channel; the state moves up by one row.
@@ -407,19 +404,15 @@ extern "C" int mogt_short_conv_bwd(const mogt_short_conv_problem* q, const void*
     a.steps = CONV_BWD_STEPS;
     a.nchunk = a.L > 0 ? (a.L + a.steps - 1) / a.steps : 1;
     const int64_t rows = q->batch * a.nchunk;
-    a.part_w = static_cast<float*>(workspace);
-    a.part_b = a.part_w + rows * q->taps * q->channels;
+    a.part = static_cast<float*>(workspace);
     const bool vec = conv_vectors(q, {dy, dfinal_state, dx, dinitial_state});
     const int batch = static_cast<int>(q->batch);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int rc = q->io_dtype == MOGT_F32 ? (vec ? conv_bwd<float, 4>(a, batch, st) : conv_bwd<float, 1>(a, batch, st))
                                            : (vec ? conv_bwd<bf16_t, 8>(a, batch, st) : conv_bwd<bf16_t, 1>(a, batch, st));
     if (rc) return rc;
-    if (dweight)
-        if (const int r = column_sums(a.part_w, dweight, rows, q->channels, q->taps, st)) return r;
-    if (dbias)
-        if (const int r = column_sums(a.part_b, dbias, rows, q->channels, 1, st)) return r;
-    return MOGT_OK;
+    if (!dweight && !dbias) return MOGT_OK;
+    return column_sums(a.part, dweight, dbias, nullptr, rows, q->taps + 1, q->channels, q->taps, st);
 }
 
 extern "C" int mogt_short_conv_step(const mogt_short_conv_problem* q, void* state, void* y, void* stream) {

@@ -12,6 +12,8 @@
 // loads and feed the vector instructions as scalar operands.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace mogt {
@@ -37,50 +39,163 @@ __device__ __forceinline__ int ssm_length(const SsmArgs& p, int b) {
     return __builtin_amdgcn_readfirstlane(static_cast<int>(n));
 }
 
-// NS consecutive values of a B or C row from state n0, the same for every
-// lane; states past N read as zero.  Rows are in constant memory for the
-// launch, so the loads are scalar.  bf16 rows are 4-byte aligned and N is even
-// (checked on the host): a 32-bit word holds two states.
-template <typename TB, int NS>
-__device__ __forceinline__ void ssm_row(const TB* row, int n0, int N, float (&v)[NS]) {
-    if constexpr (sizeof(TB) == 4) {
-        typedef const __attribute__((address_space(4))) float* cptr;
-        const cptr q = (cptr)reinterpret_cast<uintptr_t>(row + n0);
-        if (N - n0 >= NS) {
-#pragma unroll
-            for (int i = 0; i < NS; ++i) v[i] = q[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < NS; ++i) v[i] = n0 + i < N ? q[i] : 0.0f;
-        }
+// States of a wave.  16 keep the vector unit busy for about 16 issues per
+// memory instruction and fit four waves on a SIMD; 8 where that leaves no state
+// idle, or fewer.  WHOLE: every wave holds NS states of the N; otherwise the
+// last one's idle states read zeros.
+constexpr int ssm_states_per_wave(int N) { return N % 16 == 0 || N > 64 || (N > 32 && N % 8 != 0) ? 16 : 8; }
+inline int ssm_waves(int N) { return (N + ssm_states_per_wave(N) - 1) / ssm_states_per_wave(N); }
+
+// Calls f with (NS, SPLIT, WHOLE) as integral constants for N states.
+template <typename F>
+void ssm_with_states(int N, F&& f) {
+    using std::bool_constant;
+    using std::integral_constant;
+    const int ns = ssm_states_per_wave(N);
+    if (ns == 16 && N % 16 == 0) {
+        if (N == 16)
+            f(integral_constant<int, 16>(), std::false_type(), std::true_type());
+        else
+            f(integral_constant<int, 16>(), std::true_type(), std::true_type());
+    } else if (ns == 16) {
+        f(integral_constant<int, 16>(), std::true_type(), std::false_type());
+    } else if (N % 8 == 0) {
+        if (N == 8)
+            f(integral_constant<int, 8>(), std::false_type(), std::true_type());
+        else
+            f(integral_constant<int, 8>(), std::true_type(), std::true_type());
     } else {
-        typedef const __attribute__((address_space(4))) uint32_t* cptr;
-        const cptr q = (cptr)reinterpret_cast<uintptr_t>(row + n0);
-        uint32_t w[NS / 2];
-        if (N - n0 >= NS) {
-#pragma unroll
-            for (int i = 0; i < NS / 2; ++i) w[i] = q[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < NS / 2; ++i) w[i] = n0 + 2 * i < N ? q[i] : 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < NS / 2; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        f(integral_constant<int, 8>(), std::true_type(), std::false_type());
     }
 }
 
-// softplus(v) = log(1 + e^v), v itself past 20 (there the two agree in fp32).
-// log(1 + e) / e for the rounded u = 1 + e is log(u) / (u - 1) to fp32
-// accuracy, which keeps the small step sizes (e of 2^-10 and below) exact to a
-// few ulp.
+// The B (and C) values of U steps, the same for every channel of a wave: each
+// lane loads E of them into registers (while the steps before are computed),
+// then the wave lays them out in LDS as [U][VALS] floats, from where every lane
+// reads them all.  A vector instruction with a scalar operand runs at little
+// more than half the rate of one with registers alone (4.3 against 2.5 cycles
+// measured, and 2.4 for every scalar instruction that unpacks one), so the rows
+// do not come through the scalar unit.  States from `left` on (not WHOLE) and
+// steps past cnt (not FULL) are zero.
+template <typename TB, int NS, int U, bool WITH_C, bool WHOLE>
+struct SsmRows {
+    static constexpr int VALS = WITH_C ? 2 * NS : NS;
+    static constexpr int ALL = U * VALS, E = ALL < 64 ? 1 : ALL / 64;   // lanes past ALL repeat the first ones
+    static_assert((ALL % 64 == 0 || 64 % ALL == 0) && NS % E == 0, "a lane's values lie in one row of B or of C");
+    const TB* p;
+    int64_t stride;
+    int step, first, left;
+
+    __device__ __forceinline__ SsmRows(const TB* B, int64_t Bs, const TB* C, int64_t Cs, int lane, int left_) {
+        const int e = lane * E % ALL, k = e % VALS;
+        step = e / VALS;
+        first = k % NS;
+        left = left_;
+        stride = WITH_C && k >= NS ? Cs : Bs;
+        p = (WITH_C && k >= NS ? C : B) + first + step * stride;
+    }
+    template <bool FULL>
+    __device__ __forceinline__ void load(int64_t t, int cnt, float (&v)[E]) const {   // of the steps from row t on
+        const TB* q = p + (t + (FULL ? 0 : min(cnt - 1 - step, 0))) * stride;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            v[i] = IO<TB>::ld(q[WHOLE ? i : min(i, max(left - 1 - first, -first))]);
+            if ((!WHOLE && first + i >= left) || (!FULL && step >= cnt)) v[i] = 0.0f;
+        }
+    }
+    static __device__ __forceinline__ void store(float* s, int lane, const float (&v)[E]) {
+        Pack<float, E> pk;
+#pragma unroll
+        for (int i = 0; i < E; ++i) pk.v[i] = v[i];
+        *reinterpret_cast<Pack<float, E>*>(s + lane * E % ALL) = pk;
+    }
+};
+
+// Four values from LDS.
+__device__ __forceinline__ void ssm_lds4(const float* s, float (&v)[4]) {
+    const Pack<float, 4> q = *reinterpret_cast<const Pack<float, 4>*>(s);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = q.v[k];
+}
+
+// LDS accesses of one wave run in order; the compiler has to keep them so.
+__device__ __forceinline__ void ssm_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Element at a byte offset from a pointer that is the same for the whole wave:
+// the scalar base and the 32-bit offset go into the memory instruction as they
+// are (an index would be added up in 64-bit vector arithmetic first).
+template <typename T>
+__device__ __forceinline__ T ssm_ld(const T* base, uint32_t off) {
+    return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off);
+}
+template <typename T>
+__device__ __forceinline__ void ssm_st(T* base, uint32_t off, T v) {
+    *reinterpret_cast<T*>(reinterpret_cast<char*>(base) + off) = v;
+}
+
+// Keeps an offset out of the loop's address arithmetic: the compiler would carry
+// base + offset from step to step as one 64-bit vector address per tensor.
+__device__ __forceinline__ void ssm_offset(uint32_t& off) { asm volatile("" : "+v"(off)); }
+
+// A lane's channel (byte offset) of the next U rows (of the first cnt where not
+// FULL, the last of them again past it); the row pointer moves on by U rows.
+template <typename T, int U, bool FULL>
+__device__ __forceinline__ void ssm_load_rows(const T*& p, int64_t stride, uint32_t& off, int cnt, T (&v)[U]) {
+    const T* q = p;
+    ssm_offset(off);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        v[i] = ssm_ld(q, off);
+        if (FULL || i + 1 < cnt) q += stride;
+    }
+    p += U * stride;
+}
+
+// Zero past the first cnt of U steps.
+template <int U>
+__device__ __forceinline__ void ssm_mask(int cnt, float (&v)[U]) {
+    if (cnt < U) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i >= cnt) v[i] = 0.0f;
+    }
+}
+
+// The compiler finishes these before it goes on, and starts no LDS read earlier.
+// Left to itself it reads the rows of all steps of a block first and forms the
+// decays of all states ahead, which takes the registers of several waves.
+__device__ __forceinline__ void ssm_done(float& a) { asm volatile("" : "+v"(a) :: "memory"); }
+template <int N>
+__device__ __forceinline__ void ssm_done4(float (&v)[N], int n) {
+    asm volatile("" : "+v"(v[n]), "+v"(v[n + 1]), "+v"(v[n + 2]), "+v"(v[n + 3]) :: "memory");
+}
+
+typedef float ssm_f4 __attribute__((ext_vector_type(4)));
+
+// softplus(v) = max(v, 0) + log(1 + e) with e = exp(-|v|) <= 1: for the rounded
+// u = 1 + e the part that u lost, e - (u - 1), is added to log(u), which keeps
+// small results (v far below zero) exact to a few ulp.  No selects: infinities
+// and NaN pass as in the definition.
 __device__ __forceinline__ float ssm_softplus(float v) {
-    const float e = __builtin_amdgcn_exp2f(v * SSM_LOG2E);
-    const float u = 1.0f + e, d = u - 1.0f;
-    const float s = __builtin_amdgcn_logf(u) * SSM_LN2 * e * __builtin_amdgcn_rcpf(d);
-    return v > 20.0f ? v : d == 0.0f ? e : s;
+    const float e = __builtin_amdgcn_exp2f(fabsf(v) * -SSM_LOG2E);
+    const float u = 1.0f + e;
+    return fmaxf(v, 0.0f) + fmaf(__builtin_amdgcn_logf(u), SSM_LN2, e - (u - 1.0f));
+}
+
+// Step sizes of U steps; zero past the first cnt: such a step leaves the state
+// as it is.
+template <typename T, int U>
+__device__ __forceinline__ void ssm_steps(const T (&raw)[U], float bias, int softplus, int cnt, float (&dt)[U]) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) dt[i] = IO<T>::ld(raw[i]) + bias;
+    if (softplus) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) dt[i] = ssm_softplus(dt[i]);
+    }
+    ssm_mask<U>(cnt, dt);
 }
 
 __device__ __forceinline__ float ssm_exp2(float v) { return __builtin_amdgcn_exp2f(v); }

@@ -10,10 +10,11 @@
 //   marks   scans each segment forward from its start state, leaves the state
 //           entering every SSM_R steps and, in the same sweep, the segment's
 //           share of the gradient of its start state: sum_t (prod_{s<=t} a_s) C_t dy_t.
-//   grad    folds those shares of the segments after its own (last first) into
-//           the gradient arriving at its end, then walks its blocks of SSM_R
-//           steps backwards: the states of a block are formed again from its
-//           mark and stay in registers while g runs through it.
+//   carry   folds those shares, the last segment first, into the gradient
+//           arriving at each segment's end.
+//   grad    walks a segment's blocks of SSM_R steps backwards: the states of a
+//           block are formed again from its mark and stay in registers while g
+//           runs through it.
 //   sums    over the 64-channel blocks of a group (dB, dC) and over segments
 //           and sequences (dA, dD, bias), in a fixed order.
 // The sum of 2 NS products over the 64 channels of a wave is a halving
@@ -27,7 +28,7 @@ namespace mogt {
 
 int ssm_args(const mogt_ssm_problem* q, bool step, SsmArgs& a);
 
-constexpr int SSM_R = 8;   // steps between marks
+constexpr int SSM_R = 4;   // steps between marks
 
 struct SsmBwd {
     SsmArgs a;
@@ -36,13 +37,11 @@ struct SsmBwd {
     const float* carries;      // [B, nseg, N, D]
     void *dx, *ddelta, *dz;    // [B, L, D], each may be null
     float* dh0;                // [B, D, N] or null
-    float* marks;              // [B, ceil(L / SSM_R), N, D]
+    float* marks;              // [B, ceil(L / SSM_R), G nbk, N, 64]: of a 64-channel block, idle lanes too
     float* part_g;             // [B, nseg, N, D]
     float* part_s;             // [B, nseg, D]
-    float* part_bc;            // [2][G nbk][B][L][N]: dB, dC of a 64-channel block
-    float* part_a;             // [B nseg][N][D]
-    float* part_d;             // [waves][B nseg][D]
-    float* part_bias;          // [waves][B nseg][D]
+    float* part_bc;            // [G nbk][B][L][2][N]: dB, dC of a 64-channel block
+    float* part_a;             // [B nseg][N + 2][D]: dA, dD, gradient of the bias
     int batch, nblk;
 };
 
@@ -88,15 +87,43 @@ __device__ __forceinline__ void wave_sums(float (&v)[M]) {
     }
 }
 
-template <typename T, typename TB, int NS, bool Z, bool SPLIT>
+// Sum of each of 4 values over the lanes with the same lane % Q (4 or 8); a lane
+// gets value 2 * (lane / 32) + (lane / 16) % 2.
+template <int Q>
+__device__ __forceinline__ float wave_sums4(const float (&u)[4]) {
+    float v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(u[i]), __float_as_uint(u[i + 2]), false, false);
+        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[0]), __float_as_uint(v[1]), false, false);
+    float r = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    r += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(r), 0x128, 0xf, 0xf, false));   // row_ror:8
+    if constexpr (Q == 4)
+        r += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(r), 0x124, 0xf, 0xf, false));   // row_ror:4
+    return r;
+}
+
+// Whether the grad kernel sums dB and dC through LDS: work-groups of many waves
+// of 16 states have no room for it.
+constexpr bool grad_via_lds(int NS, int OWN) { return NS == 8 || OWN > 1; }
+constexpr int grad_row(int NS) { return 2 * NS + 4; }
+
+template <typename T, typename TB, int NS, bool Z, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
+    constexpr int U = SSM_R;
+    typedef SsmRows<TB, NS, U, true, WHOLE> Rows;
+    __shared__ __align__(16) float s_rows[(SPLIT ? 8 : 1) * Rows::ALL];
     const SsmArgs& p = f.a;
     const int lane = threadIdx.x & 63;
-    const int n0 = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * NS : 0;
+    const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    const int n0 = nb * NS, left = p.N - n0;
     const int g = blockIdx.x / p.nbk;
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
     const bool valid = ci < p.per;
     const int c = g * p.per + (valid ? ci : p.per - 1);
+    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T));
     const int seg = blockIdx.y, b = blockIdx.z;
     const int t0 = seg * p.seg;
     const int te = min(t0 + p.seg, ssm_length(p, b));
@@ -105,339 +132,563 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
     float A[NS], h[NS], P[NS], G[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        const bool in = n0 + n < p.N;
+        const bool in = WHOLE || n < left;
         A[n] = in ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
         h[n] = in ? f.carries[(row * p.N + n0 + n) * p.D + c] : 0.0f;
         P[n] = 1.0f;
         G[n] = 0.0f;
     }
     const float bias = p.bias ? p.bias[c] : 0.0f;
-    const T* px = static_cast<const T*>(p.x) + b * p.xb;
-    const T* pd = static_cast<const T*>(p.delta) + b * p.db;
-    const T* pz = static_cast<const T*>(p.z) + b * p.zb;
-    const T* pg = static_cast<const T*>(f.dout) + static_cast<int64_t>(b) * p.L * p.D;
-    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N;
-    const TB* pC = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N;
-    float S = 0.0f;
-    for (int t = t0; t < te; t += SSM_R) {
-        T xr[SSM_R], dr[SSM_R], zr[SSM_R], gr[SSM_R];
-#pragma unroll
-        for (int i = 0; i < SSM_R; ++i) {
-            const int64_t tt = min(t + i, te - 1);
-            xr[i] = (px + tt * p.xs)[c];
-            dr[i] = (pd + tt * p.ds)[c];
-            gr[i] = (pg + tt * p.D)[c];
-            if constexpr (Z) zr[i] = (pz + tt * p.zs)[c];
+    const T* px = static_cast<const T*>(p.x) + b * p.xb + t0 * p.xs;
+    const T* pd = static_cast<const T*>(p.delta) + b * p.db + t0 * p.ds;
+    const T* pz = static_cast<const T*>(p.z) + b * p.zb + t0 * p.zs;
+    const T* pg = static_cast<const T*>(f.dout) + (static_cast<int64_t>(b) * p.L + t0) * p.D;
+    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0;
+    const TB* pC = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N + n0;
+    const Rows rows(pB, p.Bs, pC, p.Cs, lane, left);
+    const int64_t block_marks = static_cast<int64_t>(gridDim.x) * p.N * 64;
+    float* pm = f.marks + (static_cast<int64_t>(b) * f.nblk + t0 / SSM_R) * block_marks +
+                (static_cast<int64_t>(blockIdx.x) * p.N + n0) * 64;
+    float* lds = s_rows + nb * Rows::ALL;
+    uint32_t lane4 = lane * 4u;
+    T xr[U], dr[U], zr[U], gr[U];
+    float rv[Rows::E], S = 0.0f;
+    auto load = [&](int t) {   // the rows of the block at t
+        const int cnt = te - t;
+        if (cnt >= U) {
+            ssm_load_rows<T, U, true>(px, p.xs, off, U, xr);
+            ssm_load_rows<T, U, true>(pd, p.ds, off, U, dr);
+            ssm_load_rows<T, U, true>(pg, p.D, off, U, gr);
+            if constexpr (Z) ssm_load_rows<T, U, true>(pz, p.zs, off, U, zr);
+            rows.template load<true>(t, U, rv);
+        } else if (cnt > 0) {
+            ssm_load_rows<T, U, false>(px, p.xs, off, cnt, xr);
+            ssm_load_rows<T, U, false>(pd, p.ds, off, cnt, dr);
+            ssm_load_rows<T, U, false>(pg, p.D, off, cnt, gr);
+            if constexpr (Z) ssm_load_rows<T, U, false>(pz, p.zs, off, cnt, zr);
+            rows.template load<false>(t, cnt, rv);
         }
-        if (valid) {
-            float* m = f.marks + ((static_cast<int64_t>(b) * f.nblk + t / SSM_R) * p.N + n0) * p.D + c;
+    };
+    load(t0);
+    for (int t = t0; t < te; t += U) {
+        const int cnt = te - t;
+        float dt[U], w[U], dy[U];
+        ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-                if (n0 + n < p.N) m[static_cast<int64_t>(n) * p.D] = h[n];
-        }
-#pragma unroll
-        for (int i = 0; i < SSM_R; ++i) {
-            if (t + i >= te) break;
-            float Bv[NS], Cv[NS];
-            ssm_row<TB, NS>(pB + (t + i) * p.Bs, n0, p.N, Bv);
-            ssm_row<TB, NS>(pC + (t + i) * p.Cs, n0, p.N, Cv);
-            float dt = IO<T>::ld(dr[i]) + bias;
-            if (p.softplus) dt = ssm_softplus(dt);
-            const float w = dt * IO<T>::ld(xr[i]);
-            float dy = IO<T>::ld(gr[i]);
+        for (int i = 0; i < U; ++i) {
+            w[i] = dt[i] * IO<T>::ld(xr[i]);
+            dy[i] = IO<T>::ld(gr[i]);
             if constexpr (Z) {
                 const float z = IO<T>::ld(zr[i]);
-                dy *= z * sigmoid_hw(z);
+                dy[i] *= z * sigmoid_hw(z);
             }
-            S += dt;
+            S += dt[i];
+        }
+        ssm_mask<U>(cnt, w);
+        ssm_mask<U>(cnt, dy);
+        Rows::store(lds, lane, rv);
+        ssm_wave_sync();
+        load(t + U);
+        ssm_offset(lane4);
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const float a = ssm_exp2(dt * A[n]);
-                h[n] = fmaf(a, h[n], w * Bv[n]);
-                P[n] *= a;
-                G[n] = fmaf(P[n], Cv[n] * dy, G[n]);
+        for (int n = 0; n < NS; ++n)
+            if (WHOLE || n < left) ssm_st<float>(pm + n * 64, lane4, h[n]);
+        pm += block_marks;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+#pragma unroll
+            for (int m = 0; m < NS; m += 4) {
+                float Bv[4], Cv[4];
+                ssm_lds4(lds + i * Rows::VALS + m, Bv);
+                ssm_lds4(lds + i * Rows::VALS + NS + m, Cv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = m + e;
+                    const float a = ssm_exp2(dt[i] * A[n]);
+                    h[n] = fmaf(a, h[n], w[i] * Bv[e]);
+                    P[n] *= a;
+                    G[n] = fmaf(P[n], Cv[e] * dy[i], G[n]);
+                }
+                ssm_done4(h, m);
+                ssm_done4(G, m);
             }
         }
+        ssm_wave_sync();
     }
     if (!valid) return;
     if (n0 == 0) f.part_s[row * p.D + c] = S;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-        if (n0 + n < p.N) f.part_g[(row * p.N + n0 + n) * p.D + c] = G[n];
+        if (WHOLE || n < left) f.part_g[(row * p.N + n0 + n) * p.D + c] = G[n];
 }
 
-template <typename T, typename TB, int NS, bool Z, bool SPLIT>
-__global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_grad_kernel(SsmBwd f) {
-    extern __shared__ float s_part[];   // SPLIT: [waves][3][SSM_R][64] parts of y, dw and sum q A
+// The gradient arriving at each segment's end from the segments' shares, in
+// place, the last segment first.
+__global__ __launch_bounds__(256) void ssm_carry_back_kernel(SsmBwd f) {
+    const SsmArgs& p = f.a;
+    const int c = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y, b = blockIdx.z;
+    if (c >= p.D) return;
+    const float A = p.A[static_cast<int64_t>(c) * p.N + n] * SSM_LOG2E;
+    float g = f.dfinal ? f.dfinal[(static_cast<int64_t>(b) * p.D + c) * p.N + n] : 0.0f;
+    const int64_t row0 = static_cast<int64_t>(b) * p.nseg;
+    const float* ps = f.part_s + row0 * p.D + c;
+    float* pg = f.part_g + (row0 * p.N + n) * p.D + c;
+    const int64_t gs = static_cast<int64_t>(p.N) * p.D;
+    constexpr int U = 16;   // segments whose shares are loaded together
+    for (int j = p.nseg - 1; j >= 0; j -= U) {
+        float S[U], e[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int k = max(j - i, 0);
+            S[i] = ps[static_cast<int64_t>(k) * p.D];
+            e[i] = pg[k * gs];
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (j - i < 0) break;
+            pg[(j - i) * gs] = g;
+            g = fmaf(ssm_exp2(S[i] * A), g, e[i]);
+        }
+    }
+}
+
+// One work-group: 64 channels, a wave for NS of their states.  With several waves
+// (SPLIT) what a step needs of its channel (step size, written value, gradient of
+// y) is formed by one of them and shared through LDS; each adds its part of y, dw
+// and sum q A there, and the step's owner finishes its outputs.  OWN: steps of a
+// block that a wave owns.
+//
+// dB and dC are summed over the 64 channels through LDS: each lane leaves its 2 NS
+// products in a row (padded to 16-byte accesses without bank conflicts) and adds 4
+// values of NS / 2 rows, which leaves 4 values instead of 2 NS to exchange between
+// lanes.  KEEP: the decays of a block stay in registers beside its states; 16
+// states leave no room for them, and form them again on the way back.
+template <typename T, typename TB, int NS, int OWN, bool Z, bool SPLIT, bool WHOLE>
+__global__ __launch_bounds__(SPLIT ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2)))
+void ssm_grad_kernel(SsmBwd f) {
+    constexpr int R = SSM_R;
+    constexpr bool KEEP = NS == 8, VIA_LDS = grad_via_lds(NS, OWN);
+    constexpr int ROW = grad_row(NS), QUADS = NS / 2;   // quads of products in a row
+    typedef SsmRows<TB, NS, R, true, WHOLE> Rows;
+    extern __shared__ __align__(16) float smem[];
     const SsmArgs& p = f.a;
     const int lane = threadIdx.x & 63;
     const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     const int NB = SPLIT ? __builtin_amdgcn_readfirstlane(blockDim.x >> 6) : 1;
-    const int n0 = nb * NS;
+    const int n0 = nb * NS, left = p.N - n0;
+    // SPLIT: [2][R][3][64] dt, w, dy and each wave's parts [R][3][64]; per wave
+    // its rows and its products
+    float* s_chan = smem;
+    float* s_part = s_chan + 2 * R * 3 * 64;
+    float* s_rows = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + nb * Rows::ALL;
+    float* s_prod = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + NB * Rows::ALL + nb * (64 * ROW);
     const int g = blockIdx.x / p.nbk;
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
     const bool valid = ci < p.per;
     const int c = g * p.per + (valid ? ci : p.per - 1);
+    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)), lane4 = lane * 4u;
     const int seg = blockIdx.y, b = blockIdx.z;
     const int len = ssm_length(p, b);
     const int t0 = seg * p.seg, t1 = min(t0 + p.seg, p.L);
     const int te = min(t1, len);
-    const int64_t row0 = static_cast<int64_t>(b) * p.nseg;
+    const int64_t row = static_cast<int64_t>(b) * p.nseg + seg;
 
-    // gradient arriving at the segment's end; idle lanes hold zeros throughout
+    // gradient arriving at the segment's end.  Idle lanes repeat the last
+    // channel's step sizes and states on inputs and gradients of zero, so they add
+    // nothing to the sums over channels.
     float A[NS], gc[NS], dA[NS];
     const int64_t cn = (static_cast<int64_t>(b) * p.D + c) * p.N + n0;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        const bool in = n0 + n < p.N;
+        const bool in = WHOLE || n < left;
         A[n] = in ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
-        gc[n] = in && valid && f.dfinal ? f.dfinal[cn + n] : 0.0f;
+        gc[n] = in && valid ? f.part_g[(row * p.N + n0 + n) * p.D + c] : 0.0f;
         dA[n] = 0.0f;
-    }
-    for (int j = (len - 1) / p.seg; j > seg && len > 0; --j) {
-        const float S = f.part_s[(row0 + j) * p.D + c];
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            const float e = n0 + n < p.N ? f.part_g[((row0 + j) * p.N + n0 + n) * p.D + c] : 0.0f;
-            gc[n] = valid ? fmaf(ssm_exp2(S * A[n]), gc[n], e) : 0.0f;
-        }
     }
     const float bias = p.bias ? p.bias[c] : 0.0f;
     const float skip = p.skip ? p.skip[c] : 0.0f;
     float d_skip = 0.0f, d_bias = 0.0f;
     const int64_t bl = static_cast<int64_t>(b) * p.L;
-    const T* px = static_cast<const T*>(p.x) + b * p.xb;
-    const T* pd = static_cast<const T*>(p.delta) + b * p.db;
-    const T* pz = static_cast<const T*>(p.z) + b * p.zb;
-    const T* pg = static_cast<const T*>(f.dout) + bl * p.D;
-    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N;
-    const TB* pC = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N;
-    T* ox = static_cast<T*>(f.dx) + bl * p.D;
-    T* od = static_cast<T*>(f.ddelta) + bl * p.D;
-    T* oz = static_cast<T*>(f.dz) + bl * p.D;
-    // dB, dC rows of this 64-channel block
-    const int64_t plane = static_cast<int64_t>(gridDim.x) * f.batch * p.L * p.N;
-    float* pbc = f.part_bc + (static_cast<int64_t>(blockIdx.x) * f.batch * p.L + bl) * p.N + n0;
+    // the last block's first step, and the rows at it of the inputs and outputs
+    int t = te > t0 ? t0 + (te - 1 - t0) / R * R : t0 - R;
+    const T* px = static_cast<const T*>(p.x) + b * p.xb + t * p.xs;
+    const T* pd = static_cast<const T*>(p.delta) + b * p.db + t * p.ds;
+    const T* pz = static_cast<const T*>(p.z) + b * p.zb + t * p.zs;
+    int64_t pg = (bl + t) * p.D;   // of dx, ddelta and dz
+    const T* pdo = static_cast<const T*>(f.dout) + pg;
+    const float* pm = f.marks + (((static_cast<int64_t>(b) * f.nblk + t / R) * gridDim.x + blockIdx.x) * p.N + n0) * 64;
+    const Rows rows(static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0, p.Bs,
+                    static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N + n0, p.Cs, lane, left);
+    // dB, dC rows of this 64-channel block: a lane ends with value `mine` of
+    // them, of step `slot` of every GROUP among the lanes with the same one
+    constexpr int GROUP = 32 / NS;
+    const int mine = VIA_LDS ? 4 * (lane & (QUADS - 1)) + 2 * (lane >> 5) + ((lane >> 4) & 1)
+                             : NS / 8 * (lane >> 2) + (NS == 16 ? lane & 1 : 0);
+    const int slot = (lane / QUADS) & (GROUP - 1);
+    const bool held = f.part_bc && (WHOLE || mine % NS < left) && (VIA_LDS || (lane & (NS == 16 ? 2 : 3)) == 0);
+    uint32_t bc_off = ((mine >= NS ? p.N : 0) + n0 + mine % NS) * 4u;
 
-    auto block = [&](int t, auto full) {
+    // inputs of the next block: the rows of the steps this wave owns, B and C,
+    // the state it starts from
+    T xr[OWN], dr[OWN], gr[OWN], zr[OWN];
+    float rv[Rows::E], hm[NS];
+    auto load_as = [&](auto full, int t) {   // the block at t; pointers move to the one before it
         constexpr bool FULL = decltype(full)::value;
-        float x[SSM_R], raw[SSM_R], z[SSM_R], go[SSM_R];
+        const int cnt = te - t;
+        ssm_offset(off);
+        ssm_offset(lane4);
 #pragma unroll
-        for (int i = 0; i < SSM_R; ++i) {
-            const int64_t tt = FULL ? t + i : min(t + i, te - 1);
-            const bool on = valid && (FULL || t + i < te);
-            x[i] = IO<T>::ld((px + tt * p.xs)[c]);
-            raw[i] = IO<T>::ld((pd + tt * p.ds)[c]) + bias;
-            go[i] = IO<T>::ld((pg + tt * p.D)[c]);
-            z[i] = 0.0f;
-            if constexpr (Z) z[i] = IO<T>::ld((pz + tt * p.zs)[c]);
-            if (!on) x[i] = raw[i] = go[i] = z[i] = 0.0f;
+        for (int k = 0; k < OWN; ++k) {
+            const int i = nb + k * NB, at = FULL && !SPLIT ? i : min(i, min(cnt, R) - 1);
+            xr[k] = ssm_ld(px + at * p.xs, off);
+            dr[k] = ssm_ld(pd + at * p.ds, off);
+            gr[k] = ssm_ld(pdo + static_cast<int64_t>(at) * p.D, off);
+            if constexpr (Z) zr[k] = ssm_ld(pz + at * p.zs, off);
         }
-        float h0[NS], hs[SSM_R][NS], dt[SSM_R], y[SSM_R];
-        const float* m = f.marks + ((static_cast<int64_t>(b) * f.nblk + t / SSM_R) * p.N + n0) * p.D + c;
+        rows.template load<FULL>(t, cnt, rv);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) h0[n] = valid && n0 + n < p.N ? m[static_cast<int64_t>(n) * p.D] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < SSM_R; ++i) {
-            if (!FULL && t + i >= te) break;
-            float Bv[NS], Cv[NS];
-            ssm_row<TB, NS>(pB + (t + i) * p.Bs, n0, p.N, Bv);
-            if constexpr (Z) ssm_row<TB, NS>(pC + (t + i) * p.Cs, n0, p.N, Cv);
-            dt[i] = p.softplus ? ssm_softplus(raw[i]) : raw[i];
-            const float w = dt[i] * x[i];
-            y[i] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                hs[i][n] = fmaf(ssm_exp2(dt[i] * A[n]), i > 0 ? hs[i > 0 ? i - 1 : 0][n] : h0[n], w * Bv[n]);
-                if constexpr (Z) y[i] = fmaf(Cv[n], hs[i][n], y[i]);
-            }
-        }
-        auto finish = [&](int i, float yi, float dw, float qA) {
-            float dy = go[i];
-            const int64_t at = static_cast<int64_t>(t + i) * p.D;
-            if constexpr (Z) {
-                const float s = sigmoid_hw(z[i]);
-                dy *= z[i] * s;
-                if (f.dz && valid)
-                    (oz + at)[c] = IO<T>::st(go[i] * fmaf(skip, x[i], yi) * (s * fmaf(z[i], 1.0f - s, 1.0f)));
-            }
-            float dd = fmaf(dw, x[i], qA * SSM_LN2);
-            if (p.softplus) dd *= sigmoid_hw(raw[i]);
-            d_skip = fmaf(dy, x[i], d_skip);
-            d_bias += dd;
-            if (valid) {
-                if (f.dx) (ox + at)[c] = IO<T>::st(fmaf(dw, dt[i], skip * dy));
-                if (f.ddelta) (od + at)[c] = IO<T>::st(dd);
-            }
+        for (int n = 0; n < NS; ++n) hm[n] = WHOLE || n < left ? ssm_ld(pm + n * 64, lane4) : 0.0f;
+        px -= R * p.xs;
+        pd -= R * p.ds;
+        pz -= R * p.zs;
+        pdo -= static_cast<int64_t>(R) * p.D;
+        pm -= static_cast<int64_t>(gridDim.x) * p.N * 64;
+    };
+    auto load = [&](int t) {
+        if (te - t >= R)
+            load_as(std::true_type(), t);
+        else
+            load_as(std::false_type(), t);
+    };
+    const float on = valid ? 1.0f : 0.0f;
+    const int64_t bc_row = static_cast<int64_t>(blockIdx.x) * f.batch * p.L + bl;
+    float* pbc = f.part_bc + (bc_row + t) * 2 * p.N;
+    uint32_t bc_mine = bc_off + (VIA_LDS ? slot * 2 * p.N * 4u : 0u);
+    if (t >= t0) load(t);
+    for (int buf = 0; t >= t0; t -= R, buf ^= 1) {
+        const int cnt = te - t;
+        float* chan = s_chan + buf * R * 3 * 64 + lane;
+        // of the owned steps: x, gradient of the output, raw step size, the gate
+        float x[OWN], go[OWN], raw[OWN], z[OWN], dt_own[OWN];
+        // gradient of y, and the gate's sigmoid
+        auto grad_y = [&](int k, float& sig) {
+            sig = Z ? sigmoid_hw(z[k]) : 0.0f;
+            return Z ? go[k] * (z[k] * sig) : go[k];
         };
 #pragma unroll
-        for (int i = SSM_R - 1; i >= 0; --i) {
-            if (!FULL && t + i >= te) continue;
-            float Bv[NS], Cv[NS], v[2 * NS];
-            ssm_row<TB, NS>(pB + (t + i) * p.Bs, n0, p.N, Bv);
-            ssm_row<TB, NS>(pC + (t + i) * p.Cs, n0, p.N, Cv);
-            const float w = dt[i] * x[i];
-            const float dy = Z ? go[i] * z[i] * sigmoid_hw(z[i]) : go[i];
-            float dw = 0.0f, qA = 0.0f;
+        for (int k = 0; k < OWN; ++k) {
+            const int i = nb + k * NB;
+            x[k] = IO<T>::ld(xr[k]) * on;
+            go[k] = IO<T>::ld(gr[k]) * on;
+            raw[k] = IO<T>::ld(dr[k]) + bias;
+            dt_own[k] = p.softplus ? ssm_softplus(raw[k]) : raw[k];
+            z[k] = Z ? IO<T>::ld(zr[k]) : 0.0f;
+            if (cnt < R && i >= cnt) x[k] = go[k] = dt_own[k] = z[k] = 0.0f;
+            if (SPLIT && i < R) {
+                float sig;
+                chan[(i * 3 + 0) * 64] = dt_own[k];
+                chan[(i * 3 + 1) * 64] = dt_own[k] * x[k];
+                chan[(i * 3 + 2) * 64] = grad_y(k, sig);
+            }
+        }
+        Rows::store(s_rows, lane, rv);
+        float h0[NS], hs[R][NS], a[KEEP ? R : 1][NS], dt[R];
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const float gn = fmaf(Cv[n], dy, gc[n]);
-                v[n] = gn * w;
-                v[NS + n] = dy * hs[i][n];
-                dw = fmaf(gn, Bv[n], dw);
-                gc[n] = gn * ssm_exp2(dt[i] * A[n]);
-                const float q = gc[n] * (i > 0 ? hs[i > 0 ? i - 1 : 0][n] : h0[n]);
-                qA = fmaf(q, A[n], qA);
-                dA[n] = fmaf(q, dt[i], dA[n]);
+        for (int n = 0; n < NS; ++n) h0[n] = hm[n];
+        if constexpr (SPLIT)
+            __syncthreads();
+        else
+            ssm_wave_sync();
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            dt[i] = SPLIT ? chan[(i * 3 + 0) * 64] : dt_own[SPLIT ? 0 : i];
+            const float w = SPLIT ? chan[(i * 3 + 1) * 64] : dt[i] * x[SPLIT ? 0 : i];
+#pragma unroll
+            for (int m = 0; m < NS; m += 4) {
+                float Bv[4];
+                ssm_lds4(s_rows + i * Rows::VALS + m, Bv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = m + e;
+                    const float d = ssm_exp2(dt[i] * A[n]);
+                    if constexpr (KEEP) a[KEEP ? i : 0][n] = d;
+                    hs[i][n] = fmaf(d, i > 0 ? hs[i > 0 ? i - 1 : 0][n] : h0[n], w * Bv[e]);
+                }
+                ssm_done4(hs[i], m);
+            }
+        }
+        auto finish = [&](int k, float dy, float sig, float y, float dw, float qA) {   // outputs of an owned step
+            const int64_t at = pg + static_cast<int64_t>(nb + k * NB) * p.D;
+            float dd = fmaf(dw, x[k], qA * SSM_LN2);
+            if (p.softplus) dd *= sigmoid_hw(raw[k]);
+            d_skip = fmaf(dy, x[k], d_skip);
+            d_bias += dd;
+            if (!valid) return;
+            if constexpr (Z) {
+                if (f.dz)
+                    ssm_st<T>(static_cast<T*>(f.dz) + at, off,
+                              IO<T>::st(go[k] * fmaf(skip, x[k], y) * (sig * fmaf(z[k], 1.0f - sig, 1.0f))));
+            }
+            if (f.dx) ssm_st<T>(static_cast<T*>(f.dx) + at, off, IO<T>::st(fmaf(dw, dt_own[k], skip * dy)));
+            if (f.ddelta) ssm_st<T>(static_cast<T*>(f.ddelta) + at, off, IO<T>::st(dd));
+        };
+        float kept = 0.0f;   // of dB, dC
+#pragma unroll
+        for (int i = R - 1; i >= 0; --i) {
+            float v[2 * NS];
+            float sig = 0.0f;
+            const float dy = SPLIT ? chan[(i * 3 + 2) * 64] : grad_y(SPLIT ? 0 : i, sig);
+            const float w = SPLIT ? chan[(i * 3 + 1) * 64] : dt[i] * x[SPLIT ? 0 : i];
+            if constexpr (!KEEP) asm volatile("" : "+v"(dt[i]));   // no decays kept from the way there
+            float y = 0.0f, dw = 0.0f, qA = 0.0f;
+#pragma unroll
+            for (int m = 0; m < NS; m += 4) {   // four states at a time
+                float Bv[4], Cv[4];
+                ssm_f4 qb, qc;   // products of dB and dC
+                ssm_lds4(s_rows + i * Rows::VALS + m, Bv);
+                ssm_lds4(s_rows + i * Rows::VALS + NS + m, Cv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = m + e;
+                    if constexpr (Z) y = fmaf(Cv[e], hs[i][n], y);
+                    const float gn = fmaf(Cv[e], dy, gc[n]);
+                    qb[e] = gn * w;
+                    qc[e] = dy * hs[i][n];
+                    dw = fmaf(gn, Bv[e], dw);
+                    gc[n] = gn * (KEEP ? a[KEEP ? i : 0][n] : ssm_exp2(dt[i] * A[n]));
+                    const float q = gc[n] * (i > 0 ? hs[i > 0 ? i - 1 : 0][n] : h0[n]);
+                    qA = fmaf(q, A[n], qA);
+                    dA[n] = fmaf(q, dt[i], dA[n]);
+                }
+                if constexpr (VIA_LDS) {
+                    *reinterpret_cast<ssm_f4*>(s_prod + lane * ROW + m) = qb;
+                    *reinterpret_cast<ssm_f4*>(s_prod + lane * ROW + NS + m) = qc;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[m + e] = qb[e];
+                        v[NS + m + e] = qc[e];
+                    }
+                }
+                ssm_done4(gc, m);
+                ssm_done4(dA, m);
+                ssm_done(qA);
+                ssm_done(dw);
+                if constexpr (Z) ssm_done(y);
             }
             if (f.part_bc) {
-                wave_sums<2 * NS>(v);
-                constexpr int R = NS / 8;
-                const int j = lane & 3, k = R * (lane >> 2) + j, n = k % NS;
-                if (j < R && n0 + n < p.N)
-                    pbc[(k >= NS ? plane : 0) + static_cast<int64_t>(t + i) * p.N + n] = R == 2 && j == 1 ? v[R - 1] : v[0];
+                if constexpr (VIA_LDS) {
+                    ssm_wave_sync();
+                    const float* q = s_prod + (lane / QUADS) * QUADS * ROW + (lane & (QUADS - 1)) * 4;
+                    float u[4];
+                    ssm_lds4(q, u);
+#pragma unroll
+                    for (int k = 1; k < QUADS; ++k) {
+                        float r[4];
+                        ssm_lds4(q + k * ROW, r);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[e] += r[e];
+                    }
+                    ssm_wave_sync();
+                    const float s = wave_sums4<QUADS>(u);
+                    kept = slot == i % GROUP ? s : kept;
+                    if (i % GROUP == 0 && held && i + slot < cnt) ssm_st<float>(pbc + i * 2 * p.N, bc_mine, kept);
+                } else {
+                    wave_sums<2 * NS>(v);
+                    const float s = NS == 16 && (lane & 1) ? v[NS / 8 - 1] : v[0];
+                    if (held && i < cnt) ssm_st<float>(pbc + i * 2 * p.N, bc_mine, s);
+                }
             }
             if constexpr (SPLIT) {
-                float* s = s_part + (nb * 3 * SSM_R + i) * 64 + lane;
-                s[0] = y[i];
-                s[SSM_R * 64] = dw;
-                s[2 * SSM_R * 64] = qA;
-            } else {
-                finish(i, y[i], dw, qA);
+                float* part = s_part + (nb * R + i) * 3 * 64 + lane;
+                part[0] = y;
+                part[64] = dw;
+                part[128] = qA;
+            } else if (i < cnt) {
+                finish(SPLIT ? 0 : i, dy, sig, y, dw, qA);
             }
+            // the next block's inputs take the registers of the states passed
+            if (i == R - 2 && t - R >= t0) load(t - R);
         }
         if constexpr (SPLIT) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < SSM_R; ++i) {
-                if (!FULL && t + i >= te) break;
-                if (i % NB != nb) continue;
-                float yi = 0.0f, dw = 0.0f, qA = 0.0f;
-                for (int k = 0; k < NB; ++k) {
-                    const float* s = s_part + (k * 3 * SSM_R + i) * 64 + lane;
-                    yi += s[0];
-                    dw += s[SSM_R * 64];
-                    qA += s[2 * SSM_R * 64];
+            for (int k = 0; k < OWN; ++k) {
+                const int i = nb + k * NB;
+                if (i >= R || i >= cnt) continue;
+                float y = 0.0f, dw = 0.0f, qA = 0.0f;
+                for (int m = 0; m < NB; ++m) {
+                    const float* part = s_part + (m * R + i) * 3 * 64 + lane;
+                    y += part[0];
+                    dw += part[64];
+                    qA += part[128];
                 }
-                finish(i, yi, dw, qA);
+                float sig;
+                const float dy = grad_y(k, sig);
+                finish(k, dy, sig, y, dw, qA);
             }
-            __syncthreads();
         }
-    };
-    if (te > t0) {
-        int t = t0 + (te - 1 - t0) / SSM_R * SSM_R;
-        if (t + SSM_R > te) {
-            block(t, std::integral_constant<bool, false>());
-            t -= SSM_R;
-        }
-        for (; t >= t0; t -= SSM_R) block(t, std::integral_constant<bool, true>());
+        pg -= static_cast<int64_t>(R) * p.D;
+        pbc -= R * 2 * p.N;
+        ssm_offset(bc_mine);
     }
     // rows past the sequence's length
-    for (int t = max(t0, te); t < t1; ++t) {
-        const int64_t at = static_cast<int64_t>(t) * p.D;
+    for (t = max(t0, te); t < t1; ++t) {
+        const int64_t at = (bl + t) * p.D;
         if (nb == 0 && valid) {
-            if (f.dx) (ox + at)[c] = IO<T>::st(0.0f);
-            if (f.ddelta) (od + at)[c] = IO<T>::st(0.0f);
-            if (Z && f.dz) (oz + at)[c] = IO<T>::st(0.0f);
+            if (f.dx) (static_cast<T*>(f.dx) + at)[c] = IO<T>::st(0.0f);
+            if (f.ddelta) (static_cast<T*>(f.ddelta) + at)[c] = IO<T>::st(0.0f);
+            if (Z && f.dz) (static_cast<T*>(f.dz) + at)[c] = IO<T>::st(0.0f);
         }
-        if (f.part_bc && lane < 2 * NS && n0 + lane % NS < p.N)
-            pbc[(lane >= NS ? plane : 0) + static_cast<int64_t>(t) * p.N + lane % NS] = 0.0f;
+        if (held) ssm_st<float>(f.part_bc + (bc_row + t) * 2 * p.N, bc_off, 0.0f);
+    }
+    if constexpr (SPLIT) {   // the first wave adds up the owned steps' sums
+        __syncthreads();
+        s_part[(nb * 2 + 0) * 64 + lane] = d_skip;
+        s_part[(nb * 2 + 1) * 64 + lane] = d_bias;
+        __syncthreads();
+        d_skip = d_bias = 0.0f;
+        for (int m = 0; m < NB; ++m) {
+            d_skip += s_part[(m * 2 + 0) * 64 + lane];
+            d_bias += s_part[(m * 2 + 1) * 64 + lane];
+        }
     }
     if (!valid) return;
-    const int64_t row = row0 + seg;
+    float* pa = f.part_a + row * (p.N + 2) * p.D + c;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-        if (n0 + n < p.N) {
-            f.part_a[(row * p.N + n0 + n) * p.D + c] = dA[n];
+        if (WHOLE || n < left) {
+            pa[static_cast<int64_t>(n0 + n) * p.D] = dA[n];
             if (f.dh0 && seg == 0) f.dh0[cn + n] = gc[n];
         }
-    const int64_t rows = static_cast<int64_t>(f.batch) * p.nseg;
-    f.part_d[(nb * rows + row) * p.D + c] = d_skip;
-    f.part_bias[(nb * rows + row) * p.D + c] = d_bias;
+    if (nb == 0) {
+        pa[static_cast<int64_t>(p.N) * p.D] = d_skip;
+        pa[static_cast<int64_t>(p.N + 1) * p.D] = d_bias;
+    }
 }
 
 // dB, dC [B, L, G, N]: the sums over the 64-channel blocks of a group, in order.
 template <typename TB>
 __global__ __launch_bounds__(256) void ssm_bc_kernel(const float* part, TB* dB, TB* dC, int64_t rows, int G, int nbk,
                                                      int N) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;   // (row, n) of one group
-    if (i >= rows * N) return;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;   // (row, dB or dC, n) of one group
+    const int64_t all = rows * 2 * N;
+    if (i >= all) return;
     const int g = blockIdx.y;
-    TB* out = blockIdx.z ? dC : dB;
+    const int64_t r = i / (2 * N);
+    const int k = static_cast<int>(i - r * (2 * N));
+    TB* out = k < N ? dB : dC;
     if (!out) return;
-    const float* q = part + (static_cast<int64_t>(blockIdx.z) * G + g) * nbk * rows * N + i;
+    const float* q = part + static_cast<int64_t>(g) * nbk * all + i;
     float s = 0.0f;
-    for (int k = 0; k < nbk; ++k) s += q[static_cast<int64_t>(k) * rows * N];
-    const int64_t r = i / N;
-    out[(r * G + g) * N + (i - r * N)] = IO<TB>::st(s);
+    for (int m = 0; m < nbk; ++m) s += q[m * all];
+    out[(r * G + g) * N + (k < N ? k : k - N)] = IO<TB>::st(s);
 }
 
-// Column sums over rows of [rows][cols], in a fixed order: a work-group takes
-// 64 columns, its 16 waves every 16th row each.  Column k goes to out[(k % D) *
-// N + k / D] (state-major to channel-major).
-__global__ __launch_bounds__(1024) void column_sums_kernel(const float* part, float* out, int64_t rows, int64_t cols,
-                                                           int64_t D, int64_t N) {
+// Column sums over rows of [rows][K][D], in a fixed order: a work-group takes 64
+// columns, its 16 waves every 16th row each.  Column (k, d) goes to a[d N + k]
+// for k < N, then to b[d] and c[d]; each may be null.
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* part, float* a, float* b, float* c, int64_t rows,
+                                                           int64_t cols, int64_t D, int64_t N) {
     __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t k = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + lane;
     float v = 0.0f;
-    if (k < cols)
-        for (int64_t r = w; r < rows; r += 16) v += part[r * cols + k];
+    if (i < cols)
+        for (int64_t r = w; r < rows; r += 16) v += part[r * cols + i];
     s[w][lane] = v;
     __syncthreads();
-    if (w != 0 || k >= cols) return;
+    if (w != 0 || i >= cols) return;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += s[i][lane];
-    out[(k % D) * N + k / D] = v;
+    for (int m = 1; m < 16; ++m) v += s[m][lane];
+    const int64_t k = i / D, d = i - k * D;
+    if (k < N) {
+        if (a) a[d * N + k] = v;
+    } else if (k == N) {
+        if (b) b[d] = v;
+    } else if (c) {
+        c[d] = v;
+    }
 }
 
-int column_sums(const float* part, float* out, int64_t rows, int64_t D, int64_t N, hipStream_t st) {
-    const int64_t cols = D * N;
-    column_sums_kernel<<<static_cast<unsigned>((cols + 63) / 64), 1024, 0, st>>>(part, out, rows, cols, D, N);
+int column_sums(const float* part, float* a, float* b, float* c, int64_t rows, int64_t K, int64_t D, int64_t N,
+                hipStream_t st) {
+    const int64_t cols = K * D;
+    column_sums_kernel<<<static_cast<unsigned>((cols + 63) / 64), 1024, 0, st>>>(part, a, b, c, rows, cols, D, N);
     return check_launch("column sums");
 }
 
 namespace {
 
-template <typename T, typename TB, int NS, bool SPLIT>
-void grad_launch(const SsmBwd& f, hipStream_t st) {
+// States of a wave of the grad kernel.
+constexpr int grad_states_per_wave(int64_t N) { return N > 8 && (N <= 16 || N > 64 || N % 16 == 0) ? 16 : 8; }
+inline int grad_waves(int64_t N) {
+    const int ns = grad_states_per_wave(N);
+    return static_cast<int>((N + ns - 1) / ns);
+}
+
+template <typename T, typename TB, int NS, int OWN, bool SPLIT>
+void grad_launch_as(const SsmBwd& f, hipStream_t st) {
     const SsmArgs& a = f.a;
-    const int waves = SPLIT ? (a.N + NS - 1) / NS : 1;
+    const int waves = grad_waves(a.N);
     const dim3 grid(a.D / a.per * a.nbk, a.nseg, f.batch);
-    const size_t lds = SPLIT ? sizeof(float) * 3 * waves * SSM_R * 64 : 0;
-    if (a.z) {
-        ssm_marks_kernel<T, TB, NS, true, SPLIT><<<grid, 64 * waves, 0, st>>>(f);
-        ssm_grad_kernel<T, TB, NS, true, SPLIT><<<grid, 64 * waves, lds, st>>>(f);
-    } else {
-        ssm_marks_kernel<T, TB, NS, false, SPLIT><<<grid, 64 * waves, 0, st>>>(f);
-        ssm_grad_kernel<T, TB, NS, false, SPLIT><<<grid, 64 * waves, lds, st>>>(f);
-    }
+    const size_t lds = sizeof(float) * ((SPLIT ? (2 + waves) * SSM_R * 3 * 64 : 0) + waves * SSM_R * 2 * NS +
+                                        (grad_via_lds(NS, OWN) ? waves * 64 * grad_row(NS) : 0));
+    const bool whole = a.N % NS == 0;
+    if (a.z && whole)
+        ssm_grad_kernel<T, TB, NS, OWN, true, SPLIT, true><<<grid, 64 * waves, lds, st>>>(f);
+    else if (a.z)
+        ssm_grad_kernel<T, TB, NS, OWN, true, SPLIT, false><<<grid, 64 * waves, lds, st>>>(f);
+    else if (whole)
+        ssm_grad_kernel<T, TB, NS, OWN, false, SPLIT, true><<<grid, 64 * waves, lds, st>>>(f);
+    else
+        ssm_grad_kernel<T, TB, NS, OWN, false, SPLIT, false><<<grid, 64 * waves, lds, st>>>(f);
 }
 
 template <typename T, typename TB>
-void grad_states(const SsmBwd& f, hipStream_t st) {
-    if (f.a.N <= 8)
-        grad_launch<T, TB, 8, false>(f, st);
-    else if (f.a.N <= 16)
-        grad_launch<T, TB, 16, false>(f, st);
-    else
-        grad_launch<T, TB, 16, true>(f, st);
+void grad_launch(const SsmBwd& f, hipStream_t st) {
+    const SsmArgs& a = f.a;
+    const dim3 grid(a.D / a.per * a.nbk, a.nseg, f.batch);
+    ssm_with_states(a.N, [&](auto ns, auto split, auto whole) {
+        constexpr int NS = decltype(ns)::value;
+        constexpr bool SPLIT = decltype(split)::value, WHOLE = decltype(whole)::value;
+        if (a.z)
+            ssm_marks_kernel<T, TB, NS, true, SPLIT, WHOLE><<<grid, 64 * ssm_waves(a.N), 0, st>>>(f);
+        else
+            ssm_marks_kernel<T, TB, NS, false, SPLIT, WHOLE><<<grid, 64 * ssm_waves(a.N), 0, st>>>(f);
+    });
+    ssm_carry_back_kernel<<<dim3((a.D + 255) / 256, a.N, f.batch), 256, 0, st>>>(f);
+    const int waves = grad_waves(a.N);
+    if (grad_states_per_wave(a.N) == 8) {
+        if (waves == 1)
+            grad_launch_as<T, TB, 8, 4, false>(f, st);
+        else if (waves < 4)
+            grad_launch_as<T, TB, 8, 2, true>(f, st);
+        else
+            grad_launch_as<T, TB, 8, 1, true>(f, st);
+    } else if (waves == 1) {
+        grad_launch_as<T, TB, 16, 4, false>(f, st);
+    } else if (waves < 4) {
+        grad_launch_as<T, TB, 16, 2, true>(f, st);
+    } else {
+        grad_launch_as<T, TB, 16, 1, true>(f, st);
+    }
 }
 
 struct BwdSizes {
-    size_t marks, seg, s, bc, d;   // floats of each part
-    size_t total() const { return marks + 2 * seg + s + bc + 2 * d; }
+    size_t marks, g, s, bc, a;   // floats of each part
+    size_t total() const { return marks + g + s + bc + a; }
 };
 
 BwdSizes bwd_sizes(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G, int64_t segment) {
     const int64_t nseg = L > 0 ? (L + segment - 1) / segment : 1;
-    const int64_t ncb = G * ((D / G + 63) / 64), waves = N <= 16 ? 1 : (N + 15) / 16;
     BwdSizes z;
-    z.marks = static_cast<size_t>(B * ((L + SSM_R - 1) / SSM_R) * N * D);
-    z.seg = static_cast<size_t>(B * nseg * N * D);
+    const int64_t ncb = G * ((D / G + 63) / 64);
+    z.marks = static_cast<size_t>(B * ((L + SSM_R - 1) / SSM_R) * N * ncb * 64);
+    z.g = static_cast<size_t>(B * nseg * N * D);
     z.s = static_cast<size_t>(B * nseg * D);
     z.bc = static_cast<size_t>(2 * ncb * B * L * N);
-    z.d = static_cast<size_t>(waves * B * nseg * D);
+    z.a = static_cast<size_t>(B * nseg * (N + 2) * D);
     return z;
 }
 
@@ -465,8 +716,8 @@ extern "C" int mogt_ssm_scan_bwd(const mogt_ssm_problem* q, const void* dout, co
     if (!carries || !q->A || (q->length > 0 && !dout)) return set_error(MOGT_E_INVALID, "null input pointer");
     if (out->dz && !q->z) return set_error(MOGT_E_INVALID, "a gradient of z without z");
     // one-dimensional grids of the sums
-    if (q->batch * q->length * q->states >= (1ll << 32) || q->channels * q->states >= (1ll << 28))
-        return set_error(MOGT_E_INVALID, "batch x length x states below 2^32 and channels x states below 2^28 expected");
+    if (q->batch * q->length * q->states >= (1ll << 31) || q->channels * q->states >= (1ll << 28))
+        return set_error(MOGT_E_INVALID, "batch x length x states below 2^31 and channels x states below 2^28 expected");
     const BwdSizes n = bwd_sizes(q->batch, q->length, q->channels, q->states, q->groups, q->segment);
     if (!workspace || workspace_bytes < n.total() * sizeof(float))
         return set_error(MOGT_E_WORKSPACE, "workspace of %zu bytes expected, got %zu", n.total() * sizeof(float),
@@ -482,23 +733,21 @@ extern "C" int mogt_ssm_scan_bwd(const mogt_ssm_problem* q, const void* dout, co
     f.nblk = (f.a.L + SSM_R - 1) / SSM_R;
     f.marks = static_cast<float*>(workspace);
     f.part_g = f.marks + n.marks;
-    f.part_a = f.part_g + n.seg;
-    f.part_s = f.part_a + n.seg;
-    float* bc = f.part_s + n.s;
+    f.part_s = f.part_g + n.g;
+    f.part_a = f.part_s + n.s;
+    float* bc = f.part_a + n.a;
     f.part_bc = out->dB || out->dC ? bc : nullptr;
-    f.part_d = bc + n.bc;
-    f.part_bias = f.part_d + n.d;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (q->io_dtype == MOGT_F32)
-        grad_states<float, float>(f, st);
+        grad_launch<float, float>(f, st);
     else if (q->bc_dtype == MOGT_F32)
-        grad_states<bf16_t, float>(f, st);
+        grad_launch<bf16_t, float>(f, st);
     else
-        grad_states<bf16_t, bf16_t>(f, st);
+        grad_launch<bf16_t, bf16_t>(f, st);
     if (const int rc = check_launch("mogt_ssm_scan_bwd")) return rc;
     const int64_t rows = q->batch * q->length;
     if (f.part_bc && rows > 0) {
-        const dim3 grid(static_cast<unsigned>((rows * q->states + 255) / 256), static_cast<unsigned>(q->groups), 2);
+        const dim3 grid(static_cast<unsigned>((rows * 2 * q->states + 255) / 256), static_cast<unsigned>(q->groups));
         if (q->bc_dtype == MOGT_F32)
             ssm_bc_kernel<float><<<grid, 256, 0, st>>>(bc, static_cast<float*>(out->dB), static_cast<float*>(out->dC),
                                                        rows, static_cast<int>(q->groups), f.a.nbk, f.a.N);
@@ -508,12 +757,7 @@ extern "C" int mogt_ssm_scan_bwd(const mogt_ssm_problem* q, const void* dout, co
                                                         static_cast<int>(q->groups), f.a.nbk, f.a.N);
         if (const int rc = check_launch("mogt_ssm_scan_bwd")) return rc;
     }
-    const int64_t parts = q->batch * f.a.nseg, waves = f.a.N <= 16 ? 1 : (f.a.N + 15) / 16;
-    if (out->dA)
-        if (const int rc = column_sums(f.part_a, out->dA, parts, q->channels, q->states, st)) return rc;
-    if (out->dD)
-        if (const int rc = column_sums(f.part_d, out->dD, waves * parts, q->channels, 1, st)) return rc;
-    if (out->ddelta_bias)
-        if (const int rc = column_sums(f.part_bias, out->ddelta_bias, waves * parts, q->channels, 1, st)) return rc;
-    return MOGT_OK;
+    if (!out->dA && !out->dD && !out->ddelta_bias) return MOGT_OK;
+    return column_sums(f.part_a, out->dA, out->dD, out->ddelta_bias, q->batch * f.a.nseg, q->states + 2, q->channels,
+                       q->states, st);
 }

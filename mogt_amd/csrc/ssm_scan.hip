@@ -6,10 +6,11 @@
 //   sums    each segment but the last scans from a zero state and leaves its
 //           end state and its sum of step sizes: the segment's decay is
 //           exp(A sum dt), one exponential per state and segment.
-//   out     each segment folds the sums of the segments before it (in order,
-//           so results do not depend on timing) into its start state, scans
-//           again and writes the outputs.
-// With one segment only the second launch runs.  More than 16 states: the
+//   carry   the segments' start states, in order, one thread per channel and
+//           state;
+//   out     each segment scans again from its start state and writes the
+//           outputs.
+// With one segment only the last launch runs.  More than 16 states: the
 // waves of a work-group take 16 each and add their parts of y through LDS.
 //
 // Bound: the vector unit.  A state and step take one exponential and about
@@ -28,20 +29,25 @@ struct SsmFwd {
     SsmArgs a;
     void* out;          // [B, L, D]
     float* state;       // [B, D, N] or null
-    float* carries;     // [B, nseg, N, D] or null: the state entering each segment
+    float* carries;     // [B, nseg, N, D]: the state entering each segment; null if not wanted and nseg == 1
     float* part_h;      // [B, nseg, N, D]
     float* part_s;      // [B, nseg, D]
 };
 
-template <typename T, typename TB, int NS, bool SPLIT>
+template <typename T, typename TB, int NS, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_sums_kernel(SsmFwd f) {
+    constexpr int U = SSM_U;
+    typedef SsmRows<TB, NS, U, false, WHOLE> Rows;
+    __shared__ __align__(16) float s_rows[(SPLIT ? 8 : 1) * Rows::ALL];
     const SsmArgs& p = f.a;
     const int lane = threadIdx.x & 63;
-    const int n0 = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * NS : 0;
+    const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    const int n0 = nb * NS, left = p.N - n0;
     const int g = blockIdx.x / p.nbk;
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
     const bool valid = ci < p.per;
     const int c = g * p.per + (valid ? ci : p.per - 1);
+    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T));
     const int seg = blockIdx.y, b = blockIdx.z;
     const int t0 = seg * p.seg;
     const int te = min(t0 + p.seg, ssm_length(p, b));
@@ -49,150 +55,240 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_sums_kernel(SsmFwd f) {
     float A[NS], h[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        A[n] = n0 + n < p.N ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
+        A[n] = WHOLE || n < left ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
         h[n] = 0.0f;
     }
     const float bias = p.bias ? p.bias[c] : 0.0f;
-    const T* px = static_cast<const T*>(p.x) + b * p.xb;
-    const T* pd = static_cast<const T*>(p.delta) + b * p.db;
-    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N;
-    float S = 0.0f;
-    for (int t = t0; t < te; t += SSM_U) {
-        T xr[SSM_U], dr[SSM_U];
-#pragma unroll
-        for (int i = 0; i < SSM_U; ++i) {
-            const int64_t tt = min(t + i, te - 1);
-            xr[i] = (px + tt * p.xs)[c];
-            dr[i] = (pd + tt * p.ds)[c];
+    const T* px = static_cast<const T*>(p.x) + b * p.xb + t0 * p.xs;
+    const T* pd = static_cast<const T*>(p.delta) + b * p.db + t0 * p.ds;
+    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0;
+    const Rows rows(pB, p.Bs, pB, p.Bs, lane, left);
+    float* lds = s_rows + nb * Rows::ALL;
+    T xr[U], dr[U];
+    float rv[Rows::E], S = 0.0f;
+    auto load = [&](int t) {   // the rows of the block at t
+        const int cnt = te - t;
+        if (cnt >= U) {
+            ssm_load_rows<T, U, true>(px, p.xs, off, U, xr);
+            ssm_load_rows<T, U, true>(pd, p.ds, off, U, dr);
+            rows.template load<true>(t, U, rv);
+        } else if (cnt > 0) {
+            ssm_load_rows<T, U, false>(px, p.xs, off, cnt, xr);
+            ssm_load_rows<T, U, false>(pd, p.ds, off, cnt, dr);
+            rows.template load<false>(t, cnt, rv);
         }
+    };
+    load(t0);
+    for (int t = t0; t < te; t += U) {
+        const int cnt = te - t;
+        float dt[U], w[U];
+        ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
 #pragma unroll
-        for (int i = 0; i < SSM_U; ++i) {
-            if (t + i >= te) break;
-            float Bv[NS];
-            ssm_row<TB, NS>(pB + (t + i) * p.Bs, n0, p.N, Bv);
-            float dt = IO<T>::ld(dr[i]) + bias;
-            if (p.softplus) dt = ssm_softplus(dt);
-            const float w = dt * IO<T>::ld(xr[i]);
-            S += dt;
-#pragma unroll
-            for (int n = 0; n < NS; ++n) h[n] = fmaf(ssm_exp2(dt * A[n]), h[n], w * Bv[n]);
+        for (int i = 0; i < U; ++i) {
+            w[i] = dt[i] * IO<T>::ld(xr[i]);
+            S += dt[i];
         }
+        ssm_mask<U>(cnt, w);
+        Rows::store(lds, lane, rv);
+        ssm_wave_sync();
+        load(t + U);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+#pragma unroll
+            for (int m = 0; m < NS; m += 4) {
+                float Bv[4];
+                ssm_lds4(lds + i * Rows::VALS + m, Bv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
+                ssm_done4(h, m);
+            }
+        }
+        ssm_wave_sync();
     }
     if (!valid) return;
     const int64_t row = static_cast<int64_t>(b) * p.nseg + seg;
     if (n0 == 0) f.part_s[row * p.D + c] = S;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-        if (n0 + n < p.N) f.part_h[(row * p.N + n0 + n) * p.D + c] = h[n];
+        if (WHOLE || n < left) f.part_h[(row * p.N + n0 + n) * p.D + c] = h[n];
 }
 
-template <typename T, typename TB, int NS, bool Z, bool SPLIT>
+// The state entering each segment from the segments' sums, one thread per
+// channel and state; `carries` may be part_h itself.
+__global__ __launch_bounds__(256) void ssm_carry_kernel(SsmFwd f) {
+    const SsmArgs& p = f.a;
+    const int c = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y, b = blockIdx.z;
+    if (c >= p.D) return;
+    const float A = p.A[static_cast<int64_t>(c) * p.N + n] * SSM_LOG2E;
+    float h = p.h0 ? p.h0[(static_cast<int64_t>(b) * p.D + c) * p.N + n] : 0.0f;
+    const int64_t row0 = static_cast<int64_t>(b) * p.nseg;
+    const float* ps = f.part_s + row0 * p.D + c;
+    const float* ph = f.part_h + (row0 * p.N + n) * p.D + c;
+    float* out = f.carries + (row0 * p.N + n) * p.D + c;
+    const int64_t hs = static_cast<int64_t>(p.N) * p.D;
+    const int last = p.nseg - 1;   // its sums are not formed
+    constexpr int U = 16;   // segments whose sums are loaded together
+    for (int j = 0; j < p.nseg; j += U) {
+        float S[U], e[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int k = min(j + i, last > 0 ? last - 1 : 0);
+            S[i] = ps[static_cast<int64_t>(k) * p.D];
+            e[i] = ph[k * hs];
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (j + i > last) break;
+            out[(j + i) * hs] = h;
+            h = fmaf(ssm_exp2(S[i] * A), h, e[i]);
+        }
+    }
+}
+
+template <typename T, typename TB, int NS, bool Z, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_out_kernel(SsmFwd f) {
-    extern __shared__ float s_y[];   // SPLIT: [2][waves][SSM_U][64]
+    constexpr int U = SSM_U;
+    typedef SsmRows<TB, NS, U, true, WHOLE> Rows;
+    __shared__ __align__(16) float s_rows[(SPLIT ? 8 : 1) * Rows::ALL];
+    __shared__ float s_y[SPLIT ? 2 * 8 * U * 64 : 1];   // [2][waves][U][64]
     const SsmArgs& p = f.a;
     const int lane = threadIdx.x & 63;
     const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     const int NB = SPLIT ? __builtin_amdgcn_readfirstlane(blockDim.x >> 6) : 1;
-    const int n0 = nb * NS;
+    const int n0 = nb * NS, left = p.N - n0;
     const int g = blockIdx.x / p.nbk;
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
     const bool valid = ci < p.per;
     const int c = g * p.per + (valid ? ci : p.per - 1);
+    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T));
     const int seg = blockIdx.y, b = blockIdx.z;
     const int len = ssm_length(p, b);
     const int t0 = seg * p.seg, t1 = min(t0 + p.seg, p.L);
     const int te = min(t1, len);
 
     float A[NS], h[NS];
+    const int64_t sn = ((static_cast<int64_t>(b) * p.nseg + seg) * p.N + n0) * p.D + c;
     const int64_t cn = (static_cast<int64_t>(b) * p.D + c) * p.N + n0;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        const bool in = n0 + n < p.N;
+        const bool in = WHOLE || n < left;
         A[n] = in ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
-        h[n] = in && p.h0 ? p.h0[cn + n] : 0.0f;
-    }
-    // the segments before this one; those past the sequence's end hold no step
-    const int64_t row0 = static_cast<int64_t>(b) * p.nseg;
-    for (int j = 0; j < seg && j * p.seg < len; ++j) {
-        const float S = f.part_s[(row0 + j) * p.D + c];
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            const float e = n0 + n < p.N ? f.part_h[((row0 + j) * p.N + n0 + n) * p.D + c] : 0.0f;
-            h[n] = fmaf(ssm_exp2(S * A[n]), h[n], e);
-        }
-    }
-    if (f.carries && valid) {
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-            if (n0 + n < p.N) f.carries[((row0 + seg) * p.N + n0 + n) * p.D + c] = h[n];
+        h[n] = 0.0f;
+        if (p.nseg > 1)
+            h[n] = in ? f.carries[sn + static_cast<int64_t>(n) * p.D] : 0.0f;
+        else if (p.h0 && in)
+            h[n] = p.h0[cn + n];
+        if (p.nseg == 1 && f.carries && valid && in) f.carries[sn + static_cast<int64_t>(n) * p.D] = h[n];
     }
     const float bias = p.bias ? p.bias[c] : 0.0f;
     const float skip = p.skip ? p.skip[c] : 0.0f;
-    const T* px = static_cast<const T*>(p.x) + b * p.xb;
-    const T* pd = static_cast<const T*>(p.delta) + b * p.db;
-    const T* pz = static_cast<const T*>(p.z) + b * p.zb;
-    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N;
-    const TB* pC = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N;
-    T* po = static_cast<T*>(f.out) + static_cast<int64_t>(b) * p.L * p.D;
-    int buf = 0;
-    for (int t = t0; t < te; t += SSM_U) {
-        T xr[SSM_U], dr[SSM_U], zr[SSM_U];
-#pragma unroll
-        for (int i = 0; i < SSM_U; ++i) {
-            const int64_t tt = min(t + i, te - 1);
-            xr[i] = (px + tt * p.xs)[c];
-            dr[i] = (pd + tt * p.ds)[c];
-            if constexpr (Z) zr[i] = (pz + tt * p.zs)[c];
+    const T* px = static_cast<const T*>(p.x) + b * p.xb + t0 * p.xs;
+    const T* pd = static_cast<const T*>(p.delta) + b * p.db + t0 * p.ds;
+    const T* pz = static_cast<const T*>(p.z) + b * p.zb + t0 * p.zs;
+    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0;
+    const TB* pC = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N + n0;
+    const Rows rows(pB, p.Bs, pC, p.Cs, lane, left);
+    T* po = static_cast<T*>(f.out) + (static_cast<int64_t>(b) * p.L + t0) * p.D;
+    float* lds = s_rows + nb * Rows::ALL;
+    T xr[U], dr[U], zr[U];
+    float rv[Rows::E];
+    auto load = [&](int t) {   // the rows of the block at t
+        const int cnt = te - t;
+        if (cnt >= U) {
+            ssm_load_rows<T, U, true>(px, p.xs, off, U, xr);
+            ssm_load_rows<T, U, true>(pd, p.ds, off, U, dr);
+            if constexpr (Z) ssm_load_rows<T, U, true>(pz, p.zs, off, U, zr);
+            rows.template load<true>(t, U, rv);
+        } else if (cnt > 0) {
+            ssm_load_rows<T, U, false>(px, p.xs, off, cnt, xr);
+            ssm_load_rows<T, U, false>(pd, p.ds, off, cnt, dr);
+            if constexpr (Z) ssm_load_rows<T, U, false>(pz, p.zs, off, cnt, zr);
+            rows.template load<false>(t, cnt, rv);
         }
-        auto finish = [&](int i, float y) {
-            y = fmaf(skip, IO<T>::ld(xr[i]), y);
+    };
+    int buf = 0;
+    load(t0);
+    for (int t = t0; t < te; t += U, po += static_cast<int64_t>(U) * p.D) {
+        const int cnt = te - t;
+        // what a step needs of its channel: step size, written value, and the
+        // factors of the output, out = gate y + gx
+        float dt[U], w[U], gate[U], gx[U];
+        ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const float x = IO<T>::ld(xr[i]);
+            w[i] = dt[i] * x;
+            gate[i] = 1.0f;
+            gx[i] = skip * x;
             if constexpr (Z) {
                 const float z = IO<T>::ld(zr[i]);
-                y *= z * sigmoid_hw(z);
+                gate[i] = z * sigmoid_hw(z);
+                gx[i] *= gate[i];
             }
-            if (valid) (po + static_cast<int64_t>(t + i) * p.D)[c] = IO<T>::st(y);
-        };
+        }
+        ssm_mask<U>(cnt, w);
+        Rows::store(lds, lane, rv);
+        ssm_wave_sync();
+        load(t + U);
 #pragma unroll
-        for (int i = 0; i < SSM_U; ++i) {
-            if (t + i >= te) break;
-            float Bv[NS], Cv[NS];
-            ssm_row<TB, NS>(pB + (t + i) * p.Bs, n0, p.N, Bv);
-            ssm_row<TB, NS>(pC + (t + i) * p.Cs, n0, p.N, Cv);
-            float dt = IO<T>::ld(dr[i]) + bias;
-            if (p.softplus) dt = ssm_softplus(dt);
-            const float w = dt * IO<T>::ld(xr[i]);
+        for (int i = 0; i < U; ++i) {
             float y = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                h[n] = fmaf(ssm_exp2(dt * A[n]), h[n], w * Bv[n]);
-                y = fmaf(Cv[n], h[n], y);
+            for (int m = 0; m < NS; m += 4) {
+                float Bv[4], Cv[4];
+                ssm_lds4(lds + i * Rows::VALS + m, Bv);
+                ssm_lds4(lds + i * Rows::VALS + NS + m, Cv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
+                    y = fmaf(Cv[e], h[m + e], y);
+                }
+                ssm_done4(h, m);
+                ssm_done(y);
             }
             if constexpr (SPLIT)
-                s_y[((buf * NB + nb) * SSM_U + i) * 64 + lane] = y;
+                s_y[((buf * 8 + nb) * U + i) * 64 + lane] = y;
             else
-                finish(i, y);
+                gx[i] = fmaf(gate[i], y, gx[i]);
         }
         if constexpr (SPLIT) {
             // two buffers: a wave writes one again only past the next barrier,
             // which every wave reaches after its reads of it
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < SSM_U; ++i) {
-                if (t + i >= te) break;
-                if (i % NB != nb) continue;
+            for (int i = 0; i < U; ++i) {
+                if (i % NB != nb || i >= cnt) continue;
                 float y = 0.0f;
-                for (int k = 0; k < NB; ++k) y += s_y[((buf * NB + k) * SSM_U + i) * 64 + lane];
-                finish(i, y);
+                for (int m = 0; m < NB; ++m) y += s_y[((buf * 8 + m) * U + i) * 64 + lane];
+                if (valid) ssm_st<T>(po + static_cast<int64_t>(i) * p.D, off, IO<T>::st(fmaf(gate[i], y, gx[i])));
             }
             buf ^= 1;
+        } else {
+            ssm_wave_sync();
+            if (valid) {
+                T* q = po;
+                ssm_offset(off);
+                if (cnt >= U) {
+#pragma unroll
+                    for (int i = 0; i < U; ++i, q += p.D) ssm_st<T>(q, off, IO<T>::st(gx[i]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < U; ++i, q += p.D)
+                        if (i < cnt) ssm_st<T>(q, off, IO<T>::st(gx[i]));
+                }
+            }
         }
     }
-    if (nb == 0 && valid)   // rows past the sequence's length
-        for (int t = max(t0, te); t < t1; ++t) (po + static_cast<int64_t>(t) * p.D)[c] = IO<T>::st(0.0f);
-    if (f.state && seg == p.nseg - 1 && valid) {
+    if (!valid) return;
+    if (nb == 0) {   // rows past the sequence's length
+        T* pt = static_cast<T*>(f.out) + static_cast<int64_t>(b) * p.L * p.D + c;
+        for (int t = max(t0, te); t < t1; ++t) pt[static_cast<int64_t>(t) * p.D] = IO<T>::st(0.0f);
+    }
+    if (f.state && seg == p.nseg - 1) {
 #pragma unroll
         for (int n = 0; n < NS; ++n)
-            if (n0 + n < p.N) f.state[cn + n] = h[n];
+            if (WHOLE || n < left) f.state[cn + n] = h[n];
     }
 }
 
@@ -298,27 +394,24 @@ int ssm_args(const mogt_ssm_problem* q, bool step, SsmArgs& a) {
 
 namespace {
 
-template <typename T, typename TB, int NS, bool SPLIT>
+template <typename T, typename TB>
 int fwd_launch(const SsmFwd& f, int batch, hipStream_t st) {
     const SsmArgs& a = f.a;
-    const int waves = SPLIT ? (a.N + NS - 1) / NS : 1;
-    const int blocks = a.D / a.per * a.nbk;
-    if (a.nseg > 1)
-        ssm_sums_kernel<T, TB, NS, SPLIT><<<dim3(blocks, a.nseg - 1, batch), 64 * waves, 0, st>>>(f);
-    const size_t lds = SPLIT ? sizeof(float) * 2 * waves * SSM_U * 64 : 0;
-    const dim3 grid(blocks, a.nseg, batch);
-    if (a.z)
-        ssm_out_kernel<T, TB, NS, true, SPLIT><<<grid, 64 * waves, lds, st>>>(f);
-    else
-        ssm_out_kernel<T, TB, NS, false, SPLIT><<<grid, 64 * waves, lds, st>>>(f);
+    const int waves = ssm_waves(a.N), blocks = a.D / a.per * a.nbk;
+    ssm_with_states(a.N, [&](auto ns, auto split, auto whole) {
+        constexpr int NS = decltype(ns)::value;
+        constexpr bool SPLIT = decltype(split)::value, WHOLE = decltype(whole)::value;
+        if (a.nseg > 1) {
+            ssm_sums_kernel<T, TB, NS, SPLIT, WHOLE><<<dim3(blocks, a.nseg - 1, batch), 64 * waves, 0, st>>>(f);
+            ssm_carry_kernel<<<dim3((a.D + 255) / 256, a.N, batch), 256, 0, st>>>(f);
+        }
+        const dim3 grid(blocks, a.nseg, batch);
+        if (a.z)
+            ssm_out_kernel<T, TB, NS, true, SPLIT, WHOLE><<<grid, 64 * waves, 0, st>>>(f);
+        else
+            ssm_out_kernel<T, TB, NS, false, SPLIT, WHOLE><<<grid, 64 * waves, 0, st>>>(f);
+    });
     return check_launch("mogt_ssm_scan_fwd");
-}
-
-template <typename T, typename TB>
-int fwd_states(const SsmFwd& f, int batch, hipStream_t st) {
-    if (f.a.N <= 8) return fwd_launch<T, TB, 8, false>(f, batch, st);
-    if (f.a.N <= 16) return fwd_launch<T, TB, 16, false>(f, batch, st);
-    return fwd_launch<T, TB, 16, true>(f, batch, st);
 }
 
 }  // namespace
@@ -347,14 +440,14 @@ extern "C" int mogt_ssm_scan_fwd(const mogt_ssm_problem* q, void* out, float* fi
     if (!f.a.A) return set_error(MOGT_E_INVALID, "null input pointer");
     f.out = out;
     f.state = final_state;
-    f.carries = carries;
     f.part_h = static_cast<float*>(workspace);
+    f.carries = carries || f.a.nseg == 1 ? carries : f.part_h;
     f.part_s = f.part_h + q->batch * f.a.nseg * q->channels * q->states;
     const int batch = static_cast<int>(q->batch);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (q->io_dtype == MOGT_F32) return fwd_states<float, float>(f, batch, st);
-    if (q->bc_dtype == MOGT_F32) return fwd_states<bf16_t, float>(f, batch, st);
-    return fwd_states<bf16_t, bf16_t>(f, batch, st);
+    if (q->io_dtype == MOGT_F32) return fwd_launch<float, float>(f, batch, st);
+    if (q->bc_dtype == MOGT_F32) return fwd_launch<bf16_t, float>(f, batch, st);
+    return fwd_launch<bf16_t, bf16_t>(f, batch, st);
 }
 
 extern "C" int mogt_ssm_step(const mogt_ssm_problem* q, float* state, void* out, void* stream) {
