@@ -619,7 +619,7 @@ int mogt_split_ce_bwd(const void* A, int64_t lda, int64_t plane_a, int pieces_a,
  * are [batch, length, channels] with unit channel stride and the given row and
  * batch strides in elements; B, C (bc_dtype, fp32 or io_dtype) are rows of
  * groups x states, group-major, a group shared by channels / groups consecutive
- * channels; bf16 rows need 4-byte alignment and an even state count.  A
+ * channels.  A
  * [channels, states], D and delta_bias [channels], initial_state and
  * final_state [batch, channels, states] are contiguous fp32; z, D, delta_bias,
  * initial_state and lengths may be null.  lengths [batch] (4- or 8-byte

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -36,6 +37,13 @@ class SsmProblem(ctypes.Structure):
                                             "lengths")]
                 + [(n, _c_i64) for n in ("x_row", "x_batch", "delta_row", "delta_batch", "z_row", "z_batch", "B_row",
                                          "B_batch", "C_row", "C_batch")])
+
+
+# The same layouts for struct.pack, which fills one in a third of the time (a
+# problem goes by its bytes; the entry points only read it during the call).
+SSM_PROBLEM = struct.Struct("@6q4i10P10q")
+SSM_GRADIENTS = struct.Struct("@9P")
+SHORT_CONV_PROBLEM = struct.Struct("@4q3i5P2q")
 
 
 class SsmGradients(ctypes.Structure):
@@ -236,18 +244,17 @@ SIGNATURES: dict[str, tuple] = {
     "mogt_rank1_check_ranges": (_c_int, [_c_i64, _c_i64, _c_i64, _c_int]),
     "mogt_ssm_scan_workspace_bytes": (_c_size, [_c_i64] * 5),
     "mogt_ssm_scan_fwd": (
-        _c_int, [ctypes.POINTER(SsmProblem), _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
+        _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
     "mogt_ssm_scan_bwd_workspace_bytes": (_c_size, [_c_i64] * 6),
     "mogt_ssm_scan_bwd": (
-        _c_int, [ctypes.POINTER(SsmProblem), _c_void_p, _c_void_p, _c_void_p, ctypes.POINTER(SsmGradients), _c_void_p,
-                 _c_size, _c_void_p]),
-    "mogt_ssm_step": (_c_int, [ctypes.POINTER(SsmProblem), _c_void_p, _c_void_p, _c_void_p]),
-    "mogt_short_conv_fwd": (_c_int, [ctypes.POINTER(ShortConvProblem), _c_void_p, _c_void_p, _c_void_p]),
+        _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
+    "mogt_ssm_step": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "mogt_short_conv_fwd": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "mogt_short_conv_bwd_workspace_bytes": (_c_size, [_c_i64] * 4),
     "mogt_short_conv_bwd": (
-        _c_int, [ctypes.POINTER(ShortConvProblem), _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-                 _c_void_p, _c_size, _c_void_p]),
-    "mogt_short_conv_step": (_c_int, [ctypes.POINTER(ShortConvProblem), _c_void_p, _c_void_p, _c_void_p]),
+        _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size,
+                 _c_void_p]),
+    "mogt_short_conv_step": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -6,7 +6,8 @@
 //
 // Bound: HBM (one read and one write of the rows; the backward reads x and dy
 // and writes dx).  A lane owns VEC consecutive channels (16 bytes of a row
-// where the rows allow it) and walks a stretch of steps with the last K - 1
+// where the rows allow it, 8 bf16 ones in the backward, whose windows and sums
+// take the registers) and walks a stretch of steps with the last K - 1
 // rows in registers, so a row is read once per stretch plus K - 1 rows in
 // front of it (and behind it in the backward), which the neighbouring wave
 // has brought to the cache.  The backward forms s again instead of keeping it.
@@ -131,134 +132,160 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs p) {
     for (int t = max(t0, te); t < t1; ++t) store_vec<T, VEC>(py + static_cast<int64_t>(t) * p.D, zero);
 }
 
-// A step enters at the front of the window; the row K - 1 steps behind it has all
-// its terms then and leaves.
+// The gradient of s enters at step t, row t - (K - 1) then has all its terms and
+// leaves.  The four waves of a work-group take neighbouring stretches and add
+// their tap and bias sums, so one row of partial sums is written for all four.
+constexpr int CONV_BWD_STEPS = 32;   // steps of a wave
+constexpr int CONV_BWD_U = 4;        // rows loaded together, a block ahead
+
 template <typename T, int KM, int VEC>
 __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int chunk = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = (blockIdx.x * 64 + lane) * VEC;
+    constexpr int U = CONV_BWD_U;
+    __shared__ float s_sum[3][KM + 1][64 * VEC];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int chunk = blockIdx.y * 4 + wave;
+    const int ci = (blockIdx.x * 64 + lane) * VEC;
+    const bool valid = ci < p.D;
+    const int c = valid ? ci : 0;
     const int b = blockIdx.z;
-    if (chunk >= p.nchunk || c >= p.D) return;
     const int K = KM == 8 ? p.K : KM;
     const int len = conv_length(p, b);
-    const int t0 = chunk * p.steps, t1 = min(t0 + p.steps, p.L), te = min(t1, len);
+    const int t0 = chunk * CONV_BWD_STEPS, t1 = min(t0 + CONV_BWD_STEPS, p.L), te = min(t1, len);
     const T* px = static_cast<const T*>(p.x) + b * p.xb;
     const int64_t at = static_cast<int64_t>(b) * p.L * p.D + c;
     const T* pg = static_cast<const T*>(p.dy) + at;
     T* pdx = static_cast<T*>(p.dx) + at;
 
-    float w[KM][VEC], bias[VEC], dw[KM][VEC], db[VEC];
+    // taps with the last at KM - 1 (a window's rows end at the same place) and,
+    // for the way back, with the first at 0: the same array where K == KM
+    float w[KM][VEC], first[KM][VEC], bias[VEC], dw[KM][VEC], db[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         bias[e] = p.bias ? p.bias[c + e] : 0.0f;
         db[e] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KM; ++k) {
-            w[k][e] = k < K ? p.w[static_cast<int64_t>(c + e) * K + k] : 0.0f;
+            const int64_t q = static_cast<int64_t>(c + e) * K;
+            w[k][e] = k >= KM - K ? p.w[q + k - (KM - K)] : 0.0f;
+            first[k][e] = KM != 8 ? w[k][e] : k < K ? p.w[q + k] : 0.0f;
             dw[k][e] = 0.0f;
         }
     }
-    // win: rows t - K + 1 .. t at [0 .. K-1]; ds[j]: gradient of s at step
-    // tau + j, the K steps that row tau reaches
-    float win[KM][VEC], ds[KM][VEC];
+    // rows and gradients of s at steps t - (KM - 1) .. t + U - 1
+    float xe[KM - 1 + U][VEC], ds[KM - 1 + U][VEC];
 #pragma unroll
-    for (int k = 0; k < KM; ++k)
+    for (int k = 0; k < KM - 1; ++k) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) win[k][e] = ds[k][e] = 0.0f;
-    auto push = [&](int t) {   // step t enters: the window and ds move by one
+        for (int e = 0; e < VEC; ++e) xe[k][e] = ds[k][e] = 0.0f;
+        if (k >= KM - K && chunk < p.nchunk) conv_row<T, VEC>(p, px, b, t0 - (KM - 1) + k, c, xe[k]);
+    }
+    const bool open = chunk == 0 && p.dinit;   // rows of the initial state leave too
+    const int end = t0 < te || open ? te + K - 1 : t0;
+    Pack<T, VEC> xr[U], gr[U];
+    auto load = [&](int t) {
 #pragma unroll
-        for (int k = 0; k + 1 < KM; ++k)
+        for (int i = 0; i < U; ++i) {
+            const int64_t r = min(t + i, len - 1);
+            xr[i] = *reinterpret_cast<const Pack<T, VEC>*>(px + r * p.xs + c);
+            gr[i] = *reinterpret_cast<const Pack<T, VEC>*>(pg + r * p.D);
+        }
+    };
+    if (chunk < p.nchunk && t0 < end && len > 0) load(t0);
+    for (int t = t0; t < end && chunk < p.nchunk; t += U) {
+        float g[U][VEC];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                win[k][e] = win[k + 1][e];
-                ds[k][e] = ds[k + 1][e];
+                const bool on = t + i < len;   // past the end: nothing was read
+                xe[KM - 1 + i][e] = on ? IO<T>::ld(xr[i].v[e]) : 0.0f;
+                g[i][e] = on ? IO<T>::ld(gr[i].v[e]) : 0.0f;
             }
-        float x[VEC], g[VEC];
-        const bool on = t < len;
-        if (on) {
-            conv_row<T, VEC>(p, px, b, t, c, x);
-            load_vec<T, VEC>(pg + static_cast<int64_t>(t) * p.D, g);
-        }
+        if (t + U < end && len > 0) load(t + U);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
+        for (int i = 0; i < U; ++i) {
+            const bool on = t + i < len, own = t + i < te;
 #pragma unroll
-            for (int k = 0; k < KM; ++k)
-                if (k == K - 1) win[k][e] = on ? x[e] : 0.0f;
-            float s = bias[e];
-#pragma unroll
-            for (int k = 0; k < KM; ++k)
-                if (k < K) s = fmaf(w[k][e], win[k][e], s);
-            float d = on ? g[e] : 0.0f;
-            if (p.silu && on) {
-                const float sg = sigmoid_hw(s);
-                d *= sg * fmaf(s, 1.0f - sg, 1.0f);
-            }
-            if (t < te) {
-                db[e] += d;
-#pragma unroll
-                for (int k = 0; k < KM; ++k)
-                    if (k < K) dw[k][e] = fmaf(d, win[k][e], dw[k][e]);
-            }
-#pragma unroll
-            for (int k = 0; k < KM; ++k)
-                if (k == K - 1) ds[k][e] = d;
-        }
-    };
-    // gradient of row tau, ds[0] being step tau; the final state's added
-    auto row_grad = [&](int tau, float (&v)[VEC]) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            v[e] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < KM; ++j)
-                if (j < K && tau + j >= 0) {
+            for (int e = 0; e < VEC; ++e) {
+                float d = g[i][e];
+                if (p.silu) {
+                    float s = bias[e];
 #pragma unroll
                     for (int k = 0; k < KM; ++k)
-                        if (k == K - 1 - j) v[e] = fmaf(w[k][e], ds[j][e], v[e]);
+                        if (k >= KM - K) s = fmaf(w[k][e], xe[i + k][e], s);
+                    const float sg = sigmoid_hw(s);
+                    d *= sg * fmaf(s, 1.0f - sg, 1.0f);
                 }
-        }
-        if (p.dlast && tau >= len - (K - 1)) {
-            float g[VEC];
-            load_vec<T, VEC>(static_cast<const T*>(p.dlast) +
-                                 (static_cast<int64_t>(b) * (K - 1) + tau - len + K - 1) * p.D + c, g);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] += g[e];
-        }
-    };
-    const int first = chunk == 0 && p.dinit ? 1 - K : t0;   // rows of the initial state too
-    if (first < te || chunk == 0) {
-#pragma unroll
-        for (int k = 0; k < KM; ++k)
-            if (k > 0 && k < K) conv_row<T, VEC>(p, px, b, t0 - K + k, c, win[k]);
-        if (first < t0) {
-            for (int tau = first; tau < 0; ++tau) {
-                push(tau + K - 1);
-                float v[VEC];
-                row_grad(tau, v);
-                store_vec<T, VEC>(static_cast<T*>(p.dinit) +
-                                      (static_cast<int64_t>(b) * (K - 1) + K - 1 + tau) * p.D + c, v);
+                ds[KM - 1 + i][e] = on ? d : 0.0f;
             }
-        } else {
-            for (int t = t0; t < t0 + K - 1; ++t) push(t);
-        }
-        for (int tau = t0; tau < te; ++tau) {
-            push(tau + K - 1);
-            if (!p.dx) continue;
+            if (own) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float d = ds[KM - 1 + i][e];
+                    db[e] += d;
+#pragma unroll
+                    for (int k = 0; k < KM; ++k)
+                        if (k >= KM - K) dw[k][e] = fmaf(d, xe[i + k][e], dw[k][e]);
+                }
+            }
+            const int r = t + i - (K - 1);
+            if (r >= te || (r < t0 && !open)) continue;
             float v[VEC];
-            row_grad(tau, v);
-            store_vec<T, VEC>(pdx + static_cast<int64_t>(tau) * p.D, v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                v[e] = 0.0f;
+#pragma unroll
+                for (int m = 0; m < KM; ++m)
+                    if (m < K && t + i - m >= 0) v[e] = fmaf(first[m][e], ds[KM - 1 + i - m][e], v[e]);
+            }
+            if (p.dlast && r >= len - (K - 1)) {
+                float q[VEC];
+                load_vec<T, VEC>(static_cast<const T*>(p.dlast) +
+                                     (static_cast<int64_t>(b) * (K - 1) + r - len + K - 1) * p.D + c, q);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] += q[e];
+            }
+            if (!valid) continue;
+            if (r >= 0) {
+                if (p.dx) store_vec<T, VEC>(pdx + static_cast<int64_t>(r) * p.D, v);
+            } else {
+                store_vec<T, VEC>(static_cast<T*>(p.dinit) + (static_cast<int64_t>(b) * (K - 1) + K - 1 + r) * p.D + c,
+                                  v);
+            }
         }
+#pragma unroll
+        for (int k = 0; k < KM - 1; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                xe[k][e] = xe[U + k][e];
+                ds[k][e] = ds[U + k][e];
+            }
     }
-    if (p.dx) {
+    if (p.dx && valid) {
         const float zero[VEC] = {};
         for (int t = max(t0, te); t < t1; ++t) store_vec<T, VEC>(pdx + static_cast<int64_t>(t) * p.D, zero);
     }
-    const int64_t row = static_cast<int64_t>(b) * p.nchunk + chunk;
+    if (wave > 0) {
 #pragma unroll
-    for (int k = 0; k < KM; ++k)
-        if (k < K) store_vec<float, VEC>(p.part + (row * (K + 1) + k) * p.D + c, dw[k]);
-    store_vec<float, VEC>(p.part + (row * (K + 1) + K) * p.D + c, db);
+        for (int k = 0; k < KM; ++k) store_vec<float, VEC>(&s_sum[wave - 1][k][lane * VEC], dw[k]);
+        store_vec<float, VEC>(&s_sum[wave - 1][KM][lane * VEC], db);
+    }
+    __syncthreads();
+    if (wave > 0 || !valid) return;
+    const int64_t row = static_cast<int64_t>(b) * gridDim.y + blockIdx.y;
+    float* part = p.part + row * (K + 1) * p.D + c;
+#pragma unroll
+    for (int k = 0; k <= KM; ++k) {
+        if (k < KM - K) continue;
+        float v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            v[e] = k < KM ? dw[k < KM ? k : 0][e] : db[e];
+#pragma unroll
+            for (int m = 0; m < 3; ++m) v[e] += s_sum[m][k][lane * VEC + e];
+        }
+        store_vec<float, VEC>(part + static_cast<int64_t>(k - (KM - K)) * p.D, v);
+    }
 }
 
 // One token: a thread per channel; the state moves up by one row.
@@ -354,7 +381,8 @@ int conv_bwd(ConvArgs& a, int batch, hipStream_t st) {
     return check_launch("mogt_short_conv_bwd");
 }
 
-constexpr int CONV_BWD_STEPS = 32;
+// Work-groups along the sequence of the backward.
+int64_t conv_bwd_groups(int64_t L) { return L > 0 ? (L + 4 * CONV_BWD_STEPS - 1) / (4 * CONV_BWD_STEPS) : 1; }
 
 }  // namespace
 }  // namespace mogt
@@ -380,8 +408,7 @@ extern "C" int mogt_short_conv_fwd(const mogt_short_conv_problem* q, void* y, vo
 
 extern "C" size_t mogt_short_conv_bwd_workspace_bytes(int64_t batch, int64_t length, int64_t channels, int64_t taps) {
     if (batch <= 0 || channels <= 0 || taps <= 0 || length < 0) return 0;
-    const int64_t n = length > 0 ? (length + CONV_BWD_STEPS - 1) / CONV_BWD_STEPS : 1;
-    return static_cast<size_t>(batch * n * (taps + 1) * channels) * sizeof(float);
+    return static_cast<size_t>(batch * conv_bwd_groups(length) * (taps + 1) * channels) * sizeof(float);
 }
 
 extern "C" int mogt_short_conv_bwd(const mogt_short_conv_problem* q, const void* dy, const void* dfinal_state, void* dx,
@@ -401,15 +428,14 @@ extern "C" int mogt_short_conv_bwd(const mogt_short_conv_problem* q, const void*
     a.dlast = dfinal_state;
     a.dx = dx;
     a.dinit = dinitial_state;
-    a.steps = CONV_BWD_STEPS;
-    a.nchunk = a.L > 0 ? (a.L + a.steps - 1) / a.steps : 1;
-    const int64_t rows = q->batch * a.nchunk;
+    a.nchunk = a.L > 0 ? (a.L + CONV_BWD_STEPS - 1) / CONV_BWD_STEPS : 1;
+    const int64_t rows = q->batch * conv_bwd_groups(q->length);
     a.part = static_cast<float*>(workspace);
     const bool vec = conv_vectors(q, {dy, dfinal_state, dx, dinitial_state});
     const int batch = static_cast<int>(q->batch);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int rc = q->io_dtype == MOGT_F32 ? (vec ? conv_bwd<float, 4>(a, batch, st) : conv_bwd<float, 1>(a, batch, st))
-                                           : (vec ? conv_bwd<bf16_t, 8>(a, batch, st) : conv_bwd<bf16_t, 1>(a, batch, st));
+                                           : (vec ? conv_bwd<bf16_t, 4>(a, batch, st) : conv_bwd<bf16_t, 1>(a, batch, st));
     if (rc) return rc;
     if (!dweight && !dbias) return MOGT_OK;
     return column_sums(a.part, dweight, dbias, nullptr, rows, q->taps + 1, q->channels, q->taps, st);

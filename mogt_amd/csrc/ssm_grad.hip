@@ -194,13 +194,19 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
         for (int n = 0; n < NS; ++n)
             if (WHOLE || n < left) ssm_st<float>(pm + n * 64, lane4, h[n]);
         pm += block_marks;
+        float Bn[4], Cn[4];   // the next four values of B and C, read ahead
+        ssm_lds4(lds, Bn);
+        ssm_lds4(lds + NS, Cn);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
 #pragma unroll
             for (int m = 0; m < NS; m += 4) {
-                float Bv[4], Cv[4];
-                ssm_lds4(lds + i * Rows::VALS + m, Bv);
-                ssm_lds4(lds + i * Rows::VALS + NS + m, Cv);
+                const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]}, Cv[4] = {Cn[0], Cn[1], Cn[2], Cn[3]};
+                if (i * NS + m + 4 < U * NS) {
+                    const int at = m + 4 < NS ? i * Rows::VALS + m + 4 : (i + 1) * Rows::VALS;
+                    ssm_lds4(lds + at, Bn);
+                    ssm_lds4(lds + at + NS, Cn);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int n = m + e;
@@ -261,13 +267,15 @@ __global__ __launch_bounds__(256) void ssm_carry_back_kernel(SsmBwd f) {
 // dB and dC are summed over the 64 channels through LDS: each lane leaves its 2 NS
 // products in a row (padded to 16-byte accesses without bank conflicts) and adds 4
 // values of NS / 2 rows, which leaves 4 values instead of 2 NS to exchange between
-// lanes.  KEEP: the decays of a block stay in registers beside its states; 16
-// states leave no room for them, and form them again on the way back.
+// lanes.  KEEP: the decays of a block's last steps stay in registers beside its
+// states; 16 states leave room for two steps of them, the others form them again
+// on the way back.
 template <typename T, typename TB, int NS, int OWN, bool Z, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(SPLIT ? 512 : 64) __attribute__((amdgpu_waves_per_eu(2)))
 void ssm_grad_kernel(SsmBwd f) {
     constexpr int R = SSM_R;
-    constexpr bool KEEP = NS == 8, VIA_LDS = grad_via_lds(NS, OWN);
+    constexpr int KEEP = NS == 8 ? R : 2;   // of the last steps of a block
+    constexpr bool VIA_LDS = grad_via_lds(NS, OWN);
     constexpr int ROW = grad_row(NS), QUADS = NS / 2;   // quads of products in a row
     typedef SsmRows<TB, NS, R, true, WHOLE> Rows;
     extern __shared__ __align__(16) float smem[];
@@ -392,26 +400,32 @@ void ssm_grad_kernel(SsmBwd f) {
             }
         }
         Rows::store(s_rows, lane, rv);
-        float h0[NS], hs[R][NS], a[KEEP ? R : 1][NS], dt[R];
+        float h0[NS], hs[R][NS], a[KEEP][NS], dt[R];
 #pragma unroll
         for (int n = 0; n < NS; ++n) h0[n] = hm[n];
         if constexpr (SPLIT)
             __syncthreads();
         else
             ssm_wave_sync();
+        float Bn[4], Cn[4];   // the next four values of B and C, read ahead
+        ssm_lds4(s_rows, Bn);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             dt[i] = SPLIT ? chan[(i * 3 + 0) * 64] : dt_own[SPLIT ? 0 : i];
             const float w = SPLIT ? chan[(i * 3 + 1) * 64] : dt[i] * x[SPLIT ? 0 : i];
 #pragma unroll
             for (int m = 0; m < NS; m += 4) {
-                float Bv[4];
-                ssm_lds4(s_rows + i * Rows::VALS + m, Bv);
+                const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]};
+                if (m + 4 < NS)
+                    ssm_lds4(s_rows + i * Rows::VALS + m + 4, Bn);
+                else   // on the way back the last step comes first
+                    ssm_lds4(s_rows + min(i + 1, R - 1) * Rows::VALS, Bn);
+                if (i == R - 1 && m + 4 == NS) ssm_lds4(s_rows + i * Rows::VALS + NS, Cn);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int n = m + e;
                     const float d = ssm_exp2(dt[i] * A[n]);
-                    if constexpr (KEEP) a[KEEP ? i : 0][n] = d;
+                    if (i >= R - KEEP) a[i >= R - KEEP ? i - (R - KEEP) : 0][n] = d;
                     hs[i][n] = fmaf(d, i > 0 ? hs[i > 0 ? i - 1 : 0][n] : h0[n], w * Bv[e]);
                 }
                 ssm_done4(hs[i], m);
@@ -439,14 +453,17 @@ void ssm_grad_kernel(SsmBwd f) {
             float sig = 0.0f;
             const float dy = SPLIT ? chan[(i * 3 + 2) * 64] : grad_y(SPLIT ? 0 : i, sig);
             const float w = SPLIT ? chan[(i * 3 + 1) * 64] : dt[i] * x[SPLIT ? 0 : i];
-            if constexpr (!KEEP) asm volatile("" : "+v"(dt[i]));   // no decays kept from the way there
+            if (i < R - KEEP) asm volatile("" : "+v"(dt[i]));   // no decays kept from the way there
             float y = 0.0f, dw = 0.0f, qA = 0.0f;
 #pragma unroll
             for (int m = 0; m < NS; m += 4) {   // four states at a time
-                float Bv[4], Cv[4];
                 ssm_f4 qb, qc;   // products of dB and dC
-                ssm_lds4(s_rows + i * Rows::VALS + m, Bv);
-                ssm_lds4(s_rows + i * Rows::VALS + NS + m, Cv);
+                const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]}, Cv[4] = {Cn[0], Cn[1], Cn[2], Cn[3]};
+                if (i > 0 || m + 4 < NS) {
+                    const int at = m + 4 < NS ? i * Rows::VALS + m + 4 : (i - 1) * Rows::VALS;
+                    ssm_lds4(s_rows + at, Bn);
+                    ssm_lds4(s_rows + at + NS, Cn);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int n = m + e;
@@ -455,7 +472,7 @@ void ssm_grad_kernel(SsmBwd f) {
                     qb[e] = gn * w;
                     qc[e] = dy * hs[i][n];
                     dw = fmaf(gn, Bv[e], dw);
-                    gc[n] = gn * (KEEP ? a[KEEP ? i : 0][n] : ssm_exp2(dt[i] * A[n]));
+                    gc[n] = gn * (i >= R - KEEP ? a[i >= R - KEEP ? i - (R - KEEP) : 0][n] : ssm_exp2(dt[i] * A[n]));
                     const float q = gc[n] * (i > 0 ? hs[i > 0 ? i - 1 : 0][n] : h0[n]);
                     qA = fmaf(q, A[n], qA);
                     dA[n] = fmaf(q, dt[i], dA[n]);

@@ -92,12 +92,14 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_sums_kernel(SsmFwd f) {
         Rows::store(lds, lane, rv);
         ssm_wave_sync();
         load(t + U);
+        float Bn[4];   // the next four values of B, read ahead
+        ssm_lds4(lds, Bn);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
 #pragma unroll
             for (int m = 0; m < NS; m += 4) {
-                float Bv[4];
-                ssm_lds4(lds + i * Rows::VALS + m, Bv);
+                const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]};
+                if (i * NS + m + 4 < U * NS) ssm_lds4(lds + i * NS + m + 4, Bn);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
@@ -231,14 +233,20 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_out_kernel(SsmFwd f) {
         Rows::store(lds, lane, rv);
         ssm_wave_sync();
         load(t + U);
+        float Bn[4], Cn[4];   // the next four values of B and C, read ahead
+        ssm_lds4(lds, Bn);
+        ssm_lds4(lds + NS, Cn);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             float y = 0.0f;
 #pragma unroll
             for (int m = 0; m < NS; m += 4) {
-                float Bv[4], Cv[4];
-                ssm_lds4(lds + i * Rows::VALS + m, Bv);
-                ssm_lds4(lds + i * Rows::VALS + NS + m, Cv);
+                const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]}, Cv[4] = {Cn[0], Cn[1], Cn[2], Cn[3]};
+                if (i * NS + m + 4 < U * NS) {
+                    const int at = m + 4 < NS ? i * Rows::VALS + m + 4 : (i + 1) * Rows::VALS;
+                    ssm_lds4(lds + at, Bn);
+                    ssm_lds4(lds + at + NS, Cn);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
@@ -360,11 +368,6 @@ int ssm_args(const mogt_ssm_problem* q, bool step, SsmArgs& a) {
     if (q->batch == 0 || q->channels == 0) return MOGT_OK;
     if (q->length > 0) {
         if (!q->x || !q->delta || !q->A || !q->B || !q->C) return set_error(MOGT_E_INVALID, "null input pointer");
-        if (q->bc_dtype == MOGT_BF16 && !step) {
-            const uintptr_t at = reinterpret_cast<uintptr_t>(q->B) | reinterpret_cast<uintptr_t>(q->C);
-            if ((at & 3) || ((q->B_row | q->B_batch | q->C_row | q->C_batch | q->states) & 1))
-                return set_error(MOGT_E_INVALID, "bf16 B and C rows: 4-byte alignment and an even state count expected");
-        }
     }
     a.x = q->x; a.delta = q->delta; a.z = q->z; a.B = q->B; a.C = q->C;
     a.A = q->A; a.skip = q->D; a.bias = q->delta_bias; a.h0 = q->initial_state;

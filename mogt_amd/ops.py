@@ -178,8 +178,11 @@ def _plain(args: tuple) -> bool:
             or torch.autograd.forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None):
         return False
     for a in args:
-        if isinstance(a, torch.Tensor) and ((type(a) is not torch.Tensor and type(a) is not torch.nn.Parameter)
-                                            or a.is_neg()):
+        kind = type(a)
+        if kind is torch.Tensor or kind is torch.nn.Parameter:
+            if a.is_neg():
+                return False
+        elif isinstance(a, torch.Tensor):
             return False
     return True
 
@@ -2454,21 +2457,20 @@ def _on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
-def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+def _same_device(what: str, first: torch.Tensor, others: tuple) -> None:
     require_cuda(what, first)
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {t.device} and {first.device}; one device expected")
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {t.device} and {device}; one device expected")
 
 
 def _check_shape(what: str, name: str, t: torch.Tensor | None, shape: tuple) -> None:
-    if t is not None and tuple(t.shape) != shape:
+    if t is not None and t.shape != shape:
         raise ValueError(f"{what}: {name} must have shape {list(shape)}, got {list(t.shape)}")
 
 
-def _check_lengths(what: str, lengths: torch.Tensor | None, B: int) -> None:
-    if lengths is None:
-        return
+def _check_lengths(what: str, lengths: torch.Tensor, B: int) -> None:
     _check_shape(what, "lengths", lengths, (B,))
     if lengths.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: lengths must be int32 or int64, got {lengths.dtype}")
@@ -2483,22 +2485,25 @@ def _unit_channels(t: torch.Tensor | None) -> torch.Tensor | None:
     return t if t is None or t.stride(-1) == 1 else t.contiguous()
 
 
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _dense(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _short_conv_problem(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
                         initial_state: torch.Tensor | None, lengths: torch.Tensor | None, silu: bool):
-    """The C problem and the tensors it points into."""
-    x = _unit_channels(x)
-    weight = weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    initial_state = None if initial_state is None else initial_state.contiguous()
-    lengths = None if lengths is None else lengths.contiguous()
-    B, L, D = x.shape
-    p = _lib.ShortConvProblem(B, L, D, weight.shape[1], dtype_code(x.dtype, "short_conv"), int(silu),
-                              0 if lengths is None else lengths.element_size(), x.data_ptr(), weight.data_ptr(),
-                              _ptr(bias), _ptr(initial_state), _ptr(lengths), x.stride(1), x.stride(0))
+    """The C problem and the tensors it points into; ``x`` [B, L, D], or [B, D]
+    for a step."""
+    x, weight, bias, initial_state, lengths = (_unit_channels(x), _dense(weight), _dense(bias), _dense(initial_state),
+                                               _dense(lengths))
+    shape, stride = x.shape, x.stride()
+    p = _lib.SHORT_CONV_PROBLEM.pack(shape[0], shape[1] if len(shape) == 3 else 1, shape[-1], weight.shape[1],
+                                     _DTYPE_CODE[x.dtype], silu, 0 if lengths is None else lengths.element_size(),
+                                     x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(initial_state), _ptr(lengths),
+                                     stride[-2], stride[0])
     return p, (x, weight, bias, initial_state, lengths)
 
 
@@ -2511,7 +2516,7 @@ def _short_conv_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     last = torch.empty((B, weight.shape[1] - 1, D) if want_state else (0,), dtype=x.dtype, device=x.device)
     p, held = _short_conv_problem(x, weight, bias, initial_state, lengths, silu)
     with _on_device(x.device):
-        rc = _lib.load().mogt_short_conv_fwd(ctypes.byref(p), y.data_ptr(), last.data_ptr() if want_state else None,
+        rc = _lib.load().mogt_short_conv_fwd(p, y.data_ptr(), last.data_ptr() if want_state else None,
                                              _stream_handle(x.device))
     _lib.check(rc, "mogt_short_conv_fwd")
     return y, last
@@ -2543,7 +2548,7 @@ def _short_conv_grad_op(dy: torch.Tensor, dlast: torch.Tensor | None, x: torch.T
     p, held = _short_conv_problem(x, weight, bias, initial_state, lengths, silu)
     ws = scratch(lib.mogt_short_conv_bwd_workspace_bytes(B, L, D, K), x.device)
     with _on_device(x.device):
-        rc = lib.mogt_short_conv_bwd(ctypes.byref(p), dy.data_ptr(), _ptr(dlast), dx.data_ptr() if need_x else None,
+        rc = lib.mogt_short_conv_bwd(p, dy.data_ptr(), _ptr(dlast), dx.data_ptr() if need_x else None,
                                      dw.data_ptr(), db.data_ptr(), dinit.data_ptr() if need_state else None,
                                      ws.data_ptr(), ws.numel(), _stream_handle(x.device))
     _lib.check(rc, "mogt_short_conv_bwd")
@@ -2585,7 +2590,7 @@ _short_conv_op.register_autograd(_short_conv_backward, _short_conv_setup)
 
 def _check_conv(what: str, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
                 state: torch.Tensor | None, activation: str | None) -> None:
-    _same_device(what, x, weight, bias, state)
+    _same_device(what, x, (weight, bias, state))
     dtype_code(x.dtype, what)
     D = x.shape[-1]
     if weight.ndim != 2 or weight.shape[0] != D:
@@ -2619,8 +2624,9 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if x.ndim != 3:
         raise ValueError("short_conv: x must be [B, L, D]")
     _check_conv("short_conv", x, weight, bias, initial_state, activation)
-    _same_device("short_conv", x, lengths)
-    _check_lengths("short_conv", lengths, x.shape[0])
+    if lengths is not None:
+        _same_device("short_conv", x, (lengths,))
+        _check_lengths("short_conv", lengths, x.shape[0])
     y, last = _short_conv_op(x, _float32(weight), _float32(bias), initial_state, lengths, activation == "silu",
                              bool(return_state))
     return (y, last) if return_state else y
@@ -2630,9 +2636,9 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 def _short_conv_step_op(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
                         silu: bool) -> torch.Tensor:
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    p, held = _short_conv_problem(x.unsqueeze(1), weight, bias, None, None, silu)
+    p, held = _short_conv_problem(x, weight, bias, None, None, silu)
     with _on_device(x.device):
-        rc = _lib.load().mogt_short_conv_step(ctypes.byref(p), state.data_ptr(), y.data_ptr(),
+        rc = _lib.load().mogt_short_conv_step(p, state.data_ptr(), y.data_ptr(),
                                               _stream_handle(x.device))
     _lib.check(rc, "mogt_short_conv_step")
     return y
@@ -2662,7 +2668,7 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
 # One wave scans a segment of a sequence for 64 channels and 16 states.  The
 # segments that make about two waves per SIMD (256 CUs x 4) keep the vector
 # units busy; more would repeat the exponentials of the sums pass without need.
-SSM_WAVES = 2048
+SSM_WAVES = 6144
 SSM_MIN_SEGMENT = 16
 
 
@@ -2673,32 +2679,29 @@ def _ssm_segment(B: int, L: int, D: int, N: int, G: int) -> int:
 
 
 def _ssm_rows(m: torch.Tensor) -> torch.Tensor:
-    """B or C with its groups' states contiguous in a row."""
+    """B or C [..., G, N] with its groups' states contiguous in a row."""
     G, N = m.shape[-2:]
-    return m if (m.stride(-1) == 1 or N == 1) and (m.stride(-2) == N or G == 1) else m.contiguous()
+    stride = m.stride()
+    return m if (stride[-1] == 1 or N == 1) and (stride[-2] == N or G == 1) else m.contiguous()
 
 
 def _ssm_problem(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
                  D: torch.Tensor | None, z: torch.Tensor | None, delta_bias: torch.Tensor | None,
                  initial_state: torch.Tensor | None, lengths: torch.Tensor | None, softplus: bool, segment: int):
-    """The C problem and the tensors it points into."""
-    x, delta, z = _unit_channels(x), _unit_channels(delta), _unit_channels(z)
-    B, C = _ssm_rows(B), _ssm_rows(C)
-    if B.dtype == torch.bfloat16 and segment:
-        # the scan reads bf16 rows as 32-bit words
-        odd = B.shape[-1] | B.stride(0) | B.stride(1) | C.stride(0) | C.stride(1)
-        if odd & 1 or (B.data_ptr() | C.data_ptr()) & 3:
-            B, C = B.float().contiguous(), C.float().contiguous()
-    f32 = [None if t is None else t.contiguous() for t in (A, D, delta_bias, initial_state)]
-    lengths = None if lengths is None else lengths.contiguous()
-    b, L, ch = x.shape
-    p = _lib.SsmProblem(b, L, ch, A.shape[1], B.shape[2], segment, dtype_code(x.dtype, "ssm_scan"),
-                        dtype_code(B.dtype, "ssm_scan"), int(softplus),
-                        0 if lengths is None else lengths.element_size(), x.data_ptr(), delta.data_ptr(), _ptr(z),
-                        B.data_ptr(), C.data_ptr(), *[_ptr(t) for t in f32], _ptr(lengths), x.stride(1), x.stride(0),
-                        delta.stride(1), delta.stride(0), 0 if z is None else z.stride(1),
-                        0 if z is None else z.stride(0), B.stride(1), B.stride(0), C.stride(1), C.stride(0))
-    return p, (x, delta, z, B, C, f32, lengths)
+    """The C problem and the tensors it points into; ``x``, ``delta``, ``z``
+    [B, L, D] and ``B``, ``C`` [B, L, G, N], or without L for a step."""
+    x, delta, z, B, C = _unit_channels(x), _unit_channels(delta), _unit_channels(z), _ssm_rows(B), _ssm_rows(C)
+    A, D, delta_bias, initial_state, lengths = (_dense(A), _dense(D), _dense(delta_bias), _dense(initial_state),
+                                                _dense(lengths))
+    shape, xs, ds, Bs, Cs = x.shape, x.stride(), delta.stride(), B.stride(), C.stride()
+    zs = xs if z is None else z.stride()
+    p = _lib.SSM_PROBLEM.pack(shape[0], shape[1] if len(shape) == 3 else 1, shape[-1], A.shape[1], B.shape[-2],
+                              segment, _DTYPE_CODE[x.dtype], _DTYPE_CODE[B.dtype], softplus,
+                              0 if lengths is None else lengths.element_size(), x.data_ptr(), delta.data_ptr(),
+                              _ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _ptr(D), _ptr(delta_bias),
+                              _ptr(initial_state), _ptr(lengths), xs[-2], xs[0], ds[-2], ds[0], zs[-2], zs[0], Bs[-3],
+                              Bs[0], Cs[-3], Cs[0])
+    return p, (x, delta, z, B, C, A, D, delta_bias, initial_state, lengths)
 
 
 @_op("mogt::ssm_scan")
@@ -2718,7 +2721,7 @@ def _ssm_scan_op(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch
     nbytes = lib.mogt_ssm_scan_workspace_bytes(b, L, ch, N, segment)
     ws = scratch(nbytes, x.device) if nbytes else None
     with _on_device(x.device):
-        rc = lib.mogt_ssm_scan_fwd(ctypes.byref(p), out.data_ptr(), state.data_ptr() if want_state else None,
+        rc = lib.mogt_ssm_scan_fwd(p, out.data_ptr(), state.data_ptr() if want_state else None,
                                    carries.data_ptr() if want_carries else None, _ptr(ws), nbytes,
                                    _stream_handle(x.device))
     _lib.check(rc, "mogt_ssm_scan_fwd")
@@ -2748,21 +2751,17 @@ def _ssm_scan_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, x: torch.
     dout = dout.to(x.dtype).contiguous()
     dfinal = None if dfinal is None else dfinal.to(torch.float32).contiguous()
     p, held = _ssm_problem(x, delta, A, B, C, D, z, delta_bias, None, lengths, softplus, segment)
-    bc_dtype = held[3].dtype   # what the kernel reads and writes; B's and C's, or fp32
-    rows, f32 = (b, L, ch), torch.float32
-    shapes = [(rows, x.dtype), (rows, x.dtype), ((ch, N), f32), ((b, L, G, N), bc_dtype), ((b, L, G, N), bc_dtype),
-              ((ch,), f32), (rows, x.dtype), ((ch,), f32), ((b, ch, N), f32)]
+    rows, device, f32 = (b, L, ch), x.device, torch.float32
+    shapes = ((rows, x.dtype), (rows, x.dtype), ((ch, N), f32), ((b, L, G, N), B.dtype), ((b, L, G, N), B.dtype),
+              ((ch,), f32), (rows, x.dtype), ((ch,), f32), ((b, ch, N), f32))
     make = torch.empty if b > 0 and ch > 0 else torch.zeros
-    grads = [make(s if n else (0,), dtype=t, device=x.device) for (s, t), n in zip(shapes, need)]
-    dx, ddelta, dA, dB, dC, dD, dz, dbias, dinit = [_ptr(g) if n else None for g, n in zip(grads, need)]
+    grads = [make(s if n else (0,), dtype=t, device=device) for (s, t), n in zip(shapes, need)]
+    dx, ddelta, dA, dB, dC, dD, dz, dbias, dinit = [g.data_ptr() if n else 0 for g, n in zip(grads, need)]
     ws = scratch(lib.mogt_ssm_scan_bwd_workspace_bytes(b, L, ch, N, G, segment), x.device)
-    out = _lib.SsmGradients(dx, ddelta, dz, dB, dC, dA, dD, dbias, dinit)
+    out = _lib.SSM_GRADIENTS.pack(dx, ddelta, dz, dB, dC, dA, dD, dbias, dinit)
     with _on_device(x.device):
-        rc = lib.mogt_ssm_scan_bwd(ctypes.byref(p), dout.data_ptr(), _ptr(dfinal), carries.data_ptr(),
-                                   ctypes.byref(out), ws.data_ptr(), ws.numel(), _stream_handle(x.device))
+        rc = lib.mogt_ssm_scan_bwd(p, dout.data_ptr(), _ptr(dfinal), carries.data_ptr(), out, ws.data_ptr(), ws.numel(), _stream_handle(x.device))
     _lib.check(rc, "mogt_ssm_scan_bwd")
-    if bc_dtype != B.dtype:
-        grads[3], grads[4] = grads[3].to(B.dtype), grads[4].to(B.dtype)
     return grads
 
 
@@ -2808,19 +2807,20 @@ def _check_ssm(what: str, x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor,
                D: torch.Tensor | None, z: torch.Tensor | None, delta_bias: torch.Tensor | None,
                state: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
     """Argument checks of the scan and its step; returns B and C as [..., G, N]."""
-    _same_device(what, x, delta, A, B, C, D, z, delta_bias, state)
-    dtype_code(x.dtype, what)
-    rows, ch = tuple(x.shape[:-1]), x.shape[-1]
+    _same_device(what, x, (delta, A, B, C, D, z, delta_bias, state))
+    dtype, shape = x.dtype, x.shape
+    dtype_code(dtype, what)
+    rows, ch = shape[:-1], shape[-1]
     if A.ndim != 2 or A.shape[0] != ch:
         raise ValueError(f"{what}: A must be [{ch}, states], got {list(A.shape)}")
     N = A.shape[1]
     if not 1 <= N <= SSM_MAX_STATES:
         raise ValueError(f"{what}: {N} states not supported (1 to {SSM_MAX_STATES})")
-    _check_shape(what, "delta", delta, tuple(x.shape))
-    _check_shape(what, "z", z, tuple(x.shape))
     for name, t in (("delta", delta), ("z", z)):
-        if t is not None and t.dtype != x.dtype:
-            raise ValueError(f"{what}: {name} must have x's dtype {x.dtype}, got {t.dtype}")
+        if t is not None:
+            _check_shape(what, name, t, shape)
+            if t.dtype != dtype:
+                raise ValueError(f"{what}: {name} must have x's dtype {dtype}, got {t.dtype}")
     _check_shape(what, "D", D, (ch,))
     _check_shape(what, "delta_bias", delta_bias, (ch,))
     if state is not None:
@@ -2831,12 +2831,13 @@ def _check_ssm(what: str, x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor,
         raise ValueError(f"{what}: B {list(B.shape)} and C {list(C.shape)} must have the same shape")
     if B.ndim == len(rows) + 1:
         B, C = B.unsqueeze(-2), C.unsqueeze(-2)
-    if B.ndim != len(rows) + 2 or tuple(B.shape[:-2]) != rows or B.shape[-1] != N or B.shape[-2] < 1:
+    bc = B.shape
+    if len(bc) != len(rows) + 2 or bc[:-2] != rows or bc[-1] != N or bc[-2] < 1:
         raise ValueError(f"{what}: B and C must be {list(rows)} + [{N}] or [groups, {N}], got {list(C.shape)}")
-    if ch % B.shape[-2] != 0:
-        raise ValueError(f"{what}: {ch} channels do not divide into {B.shape[-2]} groups")
-    if B.dtype != C.dtype or B.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"{what}: B and C must both have dtype {x.dtype} or float32, got {B.dtype} and {C.dtype}")
+    if ch % bc[-2] != 0:
+        raise ValueError(f"{what}: {ch} channels do not divide into {bc[-2]} groups")
+    if B.dtype != C.dtype or B.dtype not in (dtype, torch.float32):
+        raise ValueError(f"{what}: B and C must both have dtype {dtype} or float32, got {B.dtype} and {C.dtype}")
     return B, C
 
 
@@ -2864,8 +2865,9 @@ def ssm_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
     if x.ndim != 3:
         raise ValueError("ssm_scan: x must be [B, L, D]")
     B, C = _check_ssm("ssm_scan", x, delta, A, B, C, D, z, delta_bias, initial_state)
-    _same_device("ssm_scan", x, lengths)
-    _check_lengths("ssm_scan", lengths, x.shape[0])
+    if lengths is not None:
+        _same_device("ssm_scan", x, (lengths,))
+        _check_lengths("ssm_scan", lengths, x.shape[0])
     want_carries = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, delta, A, B, C, D, z, delta_bias, initial_state))
     out, state, _ = _ssm_scan_op(x, delta, _float32(A), B, C, _float32(D), z, _float32(delta_bias), initial_state,
@@ -2878,10 +2880,9 @@ def _ssm_step_op(x: torch.Tensor, state: torch.Tensor, delta: torch.Tensor, A: t
                  C: torch.Tensor, D: torch.Tensor | None, z: torch.Tensor | None, delta_bias: torch.Tensor | None,
                  softplus: bool) -> torch.Tensor:
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    p, held = _ssm_problem(x.unsqueeze(1), delta.unsqueeze(1), A, B.unsqueeze(1), C.unsqueeze(1), D,
-                           None if z is None else z.unsqueeze(1), delta_bias, None, None, softplus, 0)
+    p, held = _ssm_problem(x, delta, A, B, C, D, z, delta_bias, None, None, softplus, 0)
     with _on_device(x.device):
-        rc = _lib.load().mogt_ssm_step(ctypes.byref(p), state.data_ptr(), out.data_ptr(), _stream_handle(x.device))
+        rc = _lib.load().mogt_ssm_step(p, state.data_ptr(), out.data_ptr(), _stream_handle(x.device))
     _lib.check(rc, "mogt_ssm_step")
     return out
 

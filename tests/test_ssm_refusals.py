@@ -135,6 +135,16 @@ def test_traced_into_one_graph():
         assert dx.shape == args[0].shape and dw.shape == w.shape and dinit.shape == (0,)
 
 
+def test_packed_layouts_are_the_structures():
+    assert _lib.SSM_PROBLEM.size == ctypes.sizeof(_lib.SsmProblem)
+    assert _lib.SSM_GRADIENTS.size == ctypes.sizeof(_lib.SsmGradients)
+    assert _lib.SHORT_CONV_PROBLEM.size == ctypes.sizeof(_lib.ShortConvProblem)
+    for packed, struct in ((_lib.SSM_PROBLEM, _lib.SsmProblem), (_lib.SHORT_CONV_PROBLEM, _lib.ShortConvProblem)):
+        values = list(range(1, len(struct._fields_) + 1))
+        read = struct.from_buffer_copy(packed.pack(*values))
+        assert [getattr(read, name) for name, _ in struct._fields_] == values
+
+
 def scan_problem(**change):
     p = _lib.SsmProblem(1, 8, 8, 4, 1, 16, 0, 0, 0, 0, *[64] * 5, 64, None, None, None, None, 8, 64, 8, 64, 8, 64, 4,
                         32, 4, 32)
@@ -148,8 +158,7 @@ def scan_problem(**change):
     (dict(groups=3), -1, b"groups"), (dict(io_dtype=2), -1, b"dtype"), (dict(bc_dtype=1), -1, b"dtype"),
     (dict(segment=12), -1, b"segment"), (dict(segment=0), -1, b"segment"), (dict(batch=65536), -1, b"batch"),
     (dict(length=1 << 31), -1, b"length"), (dict(x=None), -1, b"null"), (dict(lengths=64, lengths_bytes=2), -1, b"lengths"),
-    (dict(io_dtype=1, bc_dtype=1, states=3), -1, b"even"), (dict(io_dtype=1, bc_dtype=1, B=66), -1, b"alignment"),
-    (dict(io_dtype=1, bc_dtype=1, C_row=5), -1, b"even"), (dict(length=20), -2, b"workspace"),
+    (dict(io_dtype=0, bc_dtype=3), -1, b"dtype"), (dict(length=20), -2, b"workspace"),
     (dict(length=8 * 65536 * 2, segment=8), -1, b"segments"), (dict(batch=0), 0, b""),
 ])
 def test_scan_entry_refuses(change, rc, word):
