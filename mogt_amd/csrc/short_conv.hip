@@ -310,10 +310,10 @@ namespace {
 
 int conv_steps(int64_t B, int64_t L, int64_t D, int vec) {
     // steps a wave walks: at most 32 (rows in front are read again), fewer
-    // where the GPU would otherwise hold under 16 waves per CU
+    // where the GPU would otherwise hold under 8 waves per CU
     const int64_t waves = B * ((D + 64 * vec - 1) / (64 * vec));
     int64_t s = 32;
-    while (s > 8 && waves * ((L + s - 1) / s) < 4096) s /= 2;
+    while (s > 8 && waves * ((L + s - 1) / s) < 2048) s /= 2;
     return static_cast<int>(s);
 }
 

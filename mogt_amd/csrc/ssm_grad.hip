@@ -240,20 +240,30 @@ __global__ __launch_bounds__(256) void ssm_carry_back_kernel(SsmBwd f) {
     const float* ps = f.part_s + row0 * p.D + c;
     float* pg = f.part_g + (row0 * p.N + n) * p.D + c;
     const int64_t gs = static_cast<int64_t>(p.N) * p.D;
-    constexpr int U = 16;   // segments whose shares are loaded together
-    for (int j = p.nseg - 1; j >= 0; j -= U) {
-        float S[U], e[U];
+    constexpr int U = 16;   // segments whose shares are loaded together, a group ahead
+    float S[U], e[U];
+    auto load = [&](int j) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int k = max(j - i, 0);
             S[i] = ps[static_cast<int64_t>(k) * p.D];
             e[i] = pg[k * gs];
         }
+    };
+    load(p.nseg - 1);
+    for (int j = p.nseg - 1; j >= 0; j -= U) {
+        float a[U], v[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            a[i] = ssm_exp2(S[i] * A);
+            v[i] = e[i];
+        }
+        if (j >= U) load(j - U);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (j - i < 0) break;
             pg[(j - i) * gs] = g;
-            g = fmaf(ssm_exp2(S[i] * A), g, e[i]);
+            g = fmaf(a[i], g, v[i]);
         }
     }
 }

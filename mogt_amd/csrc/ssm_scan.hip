@@ -130,20 +130,30 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmFwd f) {
     float* out = f.carries + (row0 * p.N + n) * p.D + c;
     const int64_t hs = static_cast<int64_t>(p.N) * p.D;
     const int last = p.nseg - 1;   // its sums are not formed
-    constexpr int U = 16;   // segments whose sums are loaded together
-    for (int j = 0; j < p.nseg; j += U) {
-        float S[U], e[U];
+    constexpr int U = 16;   // segments whose sums are loaded together, a group ahead
+    float S[U], e[U];
+    auto load = [&](int j) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int k = min(j + i, last > 0 ? last - 1 : 0);
             S[i] = ps[static_cast<int64_t>(k) * p.D];
             e[i] = ph[k * hs];
         }
+    };
+    load(0);
+    for (int j = 0; j < p.nseg; j += U) {
+        float a[U], v[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            a[i] = ssm_exp2(S[i] * A);
+            v[i] = e[i];
+        }
+        if (j + U < p.nseg) load(j + U);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (j + i > last) break;
             out[(j + i) * hs] = h;
-            h = fmaf(ssm_exp2(S[i] * A), h, e[i]);
+            h = fmaf(a[i], h, v[i]);
         }
     }
 }
@@ -301,7 +311,11 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_out_kernel(SsmFwd f) {
 }
 
 // ---------------------------------------------------------------------------
-// single token: four lanes per channel, each every fourth state
+// single token: four lanes per channel, each four consecutive states of every
+// sixteen (VEC, states in whole aligned quads) or every fourth state.  Bound by
+// reading and writing the states (a server's batch) or by latency (one sequence):
+// a thread takes BT sequences, whose loads are in flight together and share the
+// channel's A, D and bias.
 // ---------------------------------------------------------------------------
 struct SsmStep {
     SsmArgs a;
@@ -310,37 +324,72 @@ struct SsmStep {
     int batch;
 };
 
-template <typename T, typename TB>
+template <typename T, typename TB, int BT, bool VEC>
 __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStep f) {
+    constexpr int V = VEC ? 4 : 1;
     const SsmArgs& p = f.a;
     const int q = threadIdx.x & 3;
-    const int ci = blockIdx.x * 64 + (threadIdx.x >> 2);
-    if (ci >= p.D) return;   // whole quads
-    const int b = blockIdx.y;
-    const int g = ci / p.per;
-    const float x = IO<T>::ld((static_cast<const T*>(p.x) + b * p.xb)[ci]);
-    float dt = IO<T>::ld((static_cast<const T*>(p.delta) + b * p.db)[ci]) + (p.bias ? p.bias[ci] : 0.0f);
-    if (p.softplus) dt = ssm_softplus(dt);
-    const float w = dt * x;
-    float* h = f.state + (static_cast<int64_t>(b) * p.D + ci) * p.N;
-    const float* A = p.A + static_cast<int64_t>(ci) * p.N;
-    const TB* B = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N;
-    const TB* C = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N;
-    float y = 0.0f;
-    for (int n = q; n < p.N; n += 4) {
-        const float v = fmaf(ssm_exp2(dt * A[n] * SSM_LOG2E), h[n], w * IO<TB>::ld(B[n]));
-        h[n] = v;
-        y = fmaf(IO<TB>::ld(C[n]), v, y);
+    const int c = blockIdx.x * 64 + (threadIdx.x >> 2);
+    if (c >= p.D) return;   // whole quads
+    const int b0 = blockIdx.y * BT;
+    const int g = c / p.per;
+    const float bias = p.bias ? p.bias[c] : 0.0f, skip = p.skip ? p.skip[c] : 0.0f;
+    float x[BT], dt[BT], y[BT];
+#pragma unroll
+    for (int k = 0; k < BT; ++k) {
+        const int64_t b = min(b0 + k, f.batch - 1);
+        x[k] = IO<T>::ld((static_cast<const T*>(p.x) + b * p.xb)[c]);
+        dt[k] = IO<T>::ld((static_cast<const T*>(p.delta) + b * p.db)[c]) + bias;
+        y[k] = 0.0f;
     }
-    y += __shfl_xor(y, 1, 64);
-    y += __shfl_xor(y, 2, 64);
-    if (q != 0) return;
-    y = fmaf(p.skip ? p.skip[ci] : 0.0f, x, y);
-    if (p.z) {
-        const float z = IO<T>::ld((static_cast<const T*>(p.z) + b * p.zb)[ci]);
-        y *= z * sigmoid_hw(z);
+    const float* A = p.A + static_cast<int64_t>(c) * p.N;
+    float* h = f.state + (static_cast<int64_t>(b0) * p.D + c) * p.N;
+    const TB* B = static_cast<const TB*>(p.B) + b0 * p.Bb + static_cast<int64_t>(g) * p.N;
+    const TB* C = static_cast<const TB*>(p.C) + b0 * p.Cb + static_cast<int64_t>(g) * p.N;
+    const int64_t hs = static_cast<int64_t>(p.D) * p.N;
+    bool first = true;
+    for (int n = q * V; n < p.N; n += 4 * V) {
+        Pack<float, V> a = *reinterpret_cast<const Pack<float, V>*>(A + n), v[BT];
+        float Bv[BT][V], Cv[BT][V];
+#pragma unroll
+        for (int k = 0; k < BT; ++k) {
+            if (b0 + k >= f.batch) break;
+            v[k] = *reinterpret_cast<const Pack<float, V>*>(h + k * hs + n);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                Bv[k][e] = IO<TB>::ld(B[k * p.Bb + n + e]);
+                Cv[k][e] = IO<TB>::ld(C[k * p.Cb + n + e]);
+            }
+        }
+        if (first && p.softplus) {   // after the loads have gone out
+#pragma unroll
+            for (int k = 0; k < BT; ++k) dt[k] = ssm_softplus(dt[k]);
+        }
+        first = false;
+#pragma unroll
+        for (int k = 0; k < BT; ++k) {
+            if (b0 + k >= f.batch) break;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[k].v[e] = fmaf(ssm_exp2(dt[k] * (a.v[e] * SSM_LOG2E)), v[k].v[e], dt[k] * x[k] * Bv[k][e]);
+                y[k] = fmaf(Cv[k][e], v[k].v[e], y[k]);
+            }
+            *reinterpret_cast<Pack<float, V>*>(h + k * hs + n) = v[k];
+        }
     }
-    (static_cast<T*>(f.out) + static_cast<int64_t>(b) * p.D)[ci] = IO<T>::st(y);
+#pragma unroll
+    for (int k = 0; k < BT; ++k) {
+        y[k] += __shfl_xor(y[k], 1, 64);
+        y[k] += __shfl_xor(y[k], 2, 64);
+        if (q != 0 || b0 + k >= f.batch) continue;
+        const int64_t b = b0 + k;
+        float o = fmaf(skip, x[k], y[k]);
+        if (p.z) {
+            const float z = IO<T>::ld((static_cast<const T*>(p.z) + b * p.zb)[c]);
+            o *= z * sigmoid_hw(z);
+        }
+        (static_cast<T*>(f.out) + b * p.D)[c] = IO<T>::st(o);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -417,6 +466,25 @@ int fwd_launch(const SsmFwd& f, int batch, hipStream_t st) {
     return check_launch("mogt_ssm_scan_fwd");
 }
 
+template <typename T, typename TB>
+int step_launch(const SsmStep& f, hipStream_t st) {
+    const SsmArgs& a = f.a;
+    const int blocks = (a.D + 63) / 64;
+    const bool vec = a.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(f.state) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
+    // four sequences a thread where that leaves the GPU 16 waves per CU
+    const bool many = static_cast<int64_t>(blocks) * 4 * f.batch >= 4 * 16 * 256;
+    const dim3 grid(blocks, many ? (f.batch + 3) / 4 : f.batch);
+    if (vec && many)
+        ssm_step_kernel<T, TB, 4, true><<<grid, 256, 0, st>>>(f);
+    else if (vec)
+        ssm_step_kernel<T, TB, 1, true><<<grid, 256, 0, st>>>(f);
+    else if (many)
+        ssm_step_kernel<T, TB, 4, false><<<grid, 256, 0, st>>>(f);
+    else
+        ssm_step_kernel<T, TB, 1, false><<<grid, 256, 0, st>>>(f);
+    return check_launch("mogt_ssm_step");
+}
+
 }  // namespace
 }  // namespace mogt
 
@@ -462,13 +530,11 @@ extern "C" int mogt_ssm_step(const mogt_ssm_problem* q, float* state, void* out,
     if (!state || !out) return set_error(MOGT_E_INVALID, "null state or output pointer");
     f.state = state;
     f.out = out;
-    const dim3 grid((f.a.D + 63) / 64, static_cast<unsigned>(q->batch));
+    f.batch = static_cast<int>(q->batch);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (q->io_dtype == MOGT_F32)
-        ssm_step_kernel<float, float><<<grid, 256, 0, st>>>(f);
-    else if (q->bc_dtype == MOGT_F32)
-        ssm_step_kernel<bf16_t, float><<<grid, 256, 0, st>>>(f);
-    else
-        ssm_step_kernel<bf16_t, bf16_t><<<grid, 256, 0, st>>>(f);
-    return check_launch("mogt_ssm_step");
+        return step_launch<float, float>(f, st);
+    if (q->bc_dtype == MOGT_F32)
+        return step_launch<bf16_t, float>(f, st);
+    return step_launch<bf16_t, bf16_t>(f, st);
 }
