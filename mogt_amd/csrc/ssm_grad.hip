@@ -240,7 +240,7 @@ __global__ __launch_bounds__(256) void ssm_carry_back_kernel(SsmBwd f) {
     const float* ps = f.part_s + row0 * p.D + c;
     float* pg = f.part_g + (row0 * p.N + n) * p.D + c;
     const int64_t gs = static_cast<int64_t>(p.N) * p.D;
-    constexpr int U = 16;   // segments whose shares are loaded together, a group ahead
+    constexpr int U = 32;   // segments whose shares are loaded together, a group ahead
     float S[U], e[U];
     auto load = [&](int j) {
 #pragma unroll
@@ -647,8 +647,9 @@ int column_sums(const float* part, float* a, float* b, float* c, int64_t rows, i
 
 namespace {
 
-// States of a wave of the grad kernel.
-constexpr int grad_states_per_wave(int64_t N) { return N > 8 && (N <= 16 || N > 64 || N % 16 == 0) ? 16 : 8; }
+// States of a wave of the grad kernel: 16 where that leaves none idle, 8 for the
+// rest up to 48 (more waves of 8 would not fit their products into 64 KB of LDS).
+constexpr int grad_states_per_wave(int64_t N) { return N > 8 && (N <= 16 || N > 48 || N % 16 == 0) ? 16 : 8; }
 inline int grad_waves(int64_t N) {
     const int ns = grad_states_per_wave(N);
     return static_cast<int>((N + ns - 1) / ns);

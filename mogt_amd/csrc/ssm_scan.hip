@@ -29,91 +29,247 @@ struct SsmFwd {
     SsmArgs a;
     void* out;          // [B, L, D]
     float* state;       // [B, D, N] or null
-    float* carries;     // [B, nseg, N, D]: the state entering each segment; null if not wanted and nseg == 1
+    float* carries;     // [B, nseg, N, D]: the state entering each segment; null if not wanted and not needed
     float* part_h;      // [B, nseg, N, D]
     float* part_s;      // [B, nseg, D]
 };
 
-template <typename T, typename TB, int NS, bool SPLIT, bool WHOLE>
-__global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_sums_kernel(SsmFwd f) {
-    constexpr int U = SSM_U;
-    typedef SsmRows<TB, NS, U, false, WHOLE> Rows;
-    __shared__ __align__(16) float s_rows[(SPLIT ? 8 : 1) * Rows::ALL];
-    const SsmArgs& p = f.a;
-    const int lane = threadIdx.x & 63;
-    const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-    const int n0 = nb * NS, left = p.N - n0;
-    const int g = blockIdx.x / p.nbk;
-    const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
-    const bool valid = ci < p.per;
-    const int c = g * p.per + (valid ? ci : p.per - 1);
-    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T));
-    const int seg = blockIdx.y, b = blockIdx.z;
-    const int t0 = seg * p.seg;
-    const int te = min(t0 + p.seg, ssm_length(p, b));
+// What a wave works on: its lane's channel, its states, its steps t0 .. te - 1 of
+// sequence b.  Idle lanes (valid false) repeat the group's last channel.
+template <typename T, typename TB, int NS, bool WHOLE>
+struct SsmWave {
+    const SsmArgs& p;
+    int lane, n0, left, g, c, b, t0, t1, te, len;
+    uint32_t off;
+    bool valid;
+    float A[NS], bias;
 
-    float A[NS], h[NS];
+    __device__ __forceinline__ SsmWave(const SsmArgs& p_, int n0_, int seg)
+        : p(p_), lane(threadIdx.x & 63), n0(n0_), left(p_.N - n0_), b(blockIdx.z) {
+        g = blockIdx.x / p.nbk;
+        const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
+        valid = ci < p.per;
+        c = g * p.per + (valid ? ci : p.per - 1);
+        off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T));
+        len = ssm_length(p, b);
+        t0 = seg * p.seg;
+        t1 = min(t0 + p.seg, p.L);
+        te = min(t1, len);
+        bias = p.bias ? p.bias[c] : 0.0f;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        A[n] = WHOLE || n < left ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
-        h[n] = 0.0f;
+        for (int n = 0; n < NS; ++n)
+            A[n] = WHOLE || n < left ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
     }
-    const float bias = p.bias ? p.bias[c] : 0.0f;
-    const T* px = static_cast<const T*>(p.x) + b * p.xb + t0 * p.xs;
-    const T* pd = static_cast<const T*>(p.delta) + b * p.db + t0 * p.ds;
-    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0;
-    const Rows rows(pB, p.Bs, pB, p.Bs, lane, left);
-    float* lds = s_rows + nb * Rows::ALL;
-    T xr[U], dr[U];
-    float rv[Rows::E], S = 0.0f;
-    auto load = [&](int t) {   // the rows of the block at t
-        const int cnt = te - t;
-        if (cnt >= U) {
-            ssm_load_rows<T, U, true>(px, p.xs, off, U, xr);
-            ssm_load_rows<T, U, true>(pd, p.ds, off, U, dr);
-            rows.template load<true>(t, U, rv);
-        } else if (cnt > 0) {
-            ssm_load_rows<T, U, false>(px, p.xs, off, cnt, xr);
-            ssm_load_rows<T, U, false>(pd, p.ds, off, cnt, dr);
-            rows.template load<false>(t, cnt, rv);
+    __device__ __forceinline__ const T* rows(const void* q, int64_t stride, int64_t batch) const {
+        return static_cast<const T*>(q) + b * batch + t0 * stride;
+    }
+    __device__ __forceinline__ const TB* states(const void* q, int64_t batch) const {
+        return static_cast<const TB*>(q) + b * batch + static_cast<int64_t>(g) * p.N + n0;
+    }
+
+    // h from the state it holds through the steps; returns the sum of step sizes.
+    // lds: SsmRows<.., false, ..>::ALL floats of the wave's own.
+    __device__ __forceinline__ float sums(float* lds, float (&h)[NS]) {
+        constexpr int U = SSM_U;
+        typedef SsmRows<TB, NS, U, false, WHOLE> Rows;
+        const T *px = rows(p.x, p.xs, p.xb), *pd = rows(p.delta, p.ds, p.db);
+        const TB* pB = states(p.B, p.Bb);
+        const Rows bc(pB, p.Bs, pB, p.Bs, lane, left);
+        T xr[U], dr[U];
+        float rv[Rows::E], S = 0.0f;
+        auto load = [&](int t) {   // the rows of the block at t
+            const int cnt = te - t;
+            if (cnt >= U) {
+                ssm_load_rows<T, U, true>(px, p.xs, off, U, xr);
+                ssm_load_rows<T, U, true>(pd, p.ds, off, U, dr);
+                bc.template load<true>(t, U, rv);
+            } else if (cnt > 0) {
+                ssm_load_rows<T, U, false>(px, p.xs, off, cnt, xr);
+                ssm_load_rows<T, U, false>(pd, p.ds, off, cnt, dr);
+                bc.template load<false>(t, cnt, rv);
+            }
+        };
+        load(t0);
+        for (int t = t0; t < te; t += U) {
+            const int cnt = te - t;
+            float dt[U], w[U];
+            ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                w[i] = dt[i] * IO<T>::ld(xr[i]);
+                S += dt[i];
+            }
+            ssm_mask<U>(cnt, w);
+            Rows::store(lds, lane, rv);
+            ssm_wave_sync();
+            load(t + U);
+            float Bn[4];   // the next four values of B, read ahead
+            ssm_lds4(lds, Bn);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+#pragma unroll
+                for (int m = 0; m < NS; m += 4) {
+                    const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]};
+                    if (i * NS + m + 4 < U * NS) ssm_lds4(lds + i * NS + m + 4, Bn);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
+                    ssm_done4(h, m);
+                }
+            }
+            ssm_wave_sync();
         }
-    };
-    load(t0);
-    for (int t = t0; t < te; t += U) {
-        const int cnt = te - t;
-        float dt[U], w[U];
-        ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
+        return S;
+    }
+
+    // h through the steps, their outputs written.  lds: SsmRows<.., true, ..>::ALL
+    // floats of the wave's own; SPLIT: s_y [2][8][U][64] of the work-group's, whose
+    // NB waves (this one the nb-th) hold the channel's other states.
+    template <bool Z, bool SPLIT>
+    __device__ __forceinline__ void outputs(void* out, float* lds, float* s_y, int nb, int NB, float (&h)[NS]) {
+        constexpr int U = SSM_U;
+        typedef SsmRows<TB, NS, U, true, WHOLE> Rows;
+        const float skip = p.skip ? p.skip[c] : 0.0f;
+        const T *px = rows(p.x, p.xs, p.xb), *pd = rows(p.delta, p.ds, p.db), *pz = rows(p.z, p.zs, p.zb);
+        const Rows bc(states(p.B, p.Bb), p.Bs, states(p.C, p.Cb), p.Cs, lane, left);
+        T* po = static_cast<T*>(out) + (static_cast<int64_t>(b) * p.L + t0) * p.D;
+        T xr[U], dr[U], zr[U];
+        float rv[Rows::E];
+        auto load = [&](int t) {   // the rows of the block at t
+            const int cnt = te - t;
+            if (cnt >= U) {
+                ssm_load_rows<T, U, true>(px, p.xs, off, U, xr);
+                ssm_load_rows<T, U, true>(pd, p.ds, off, U, dr);
+                if constexpr (Z) ssm_load_rows<T, U, true>(pz, p.zs, off, U, zr);
+                bc.template load<true>(t, U, rv);
+            } else if (cnt > 0) {
+                ssm_load_rows<T, U, false>(px, p.xs, off, cnt, xr);
+                ssm_load_rows<T, U, false>(pd, p.ds, off, cnt, dr);
+                if constexpr (Z) ssm_load_rows<T, U, false>(pz, p.zs, off, cnt, zr);
+                bc.template load<false>(t, cnt, rv);
+            }
+        };
+        int buf = 0;
+        load(t0);
+        for (int t = t0; t < te; t += U, po += static_cast<int64_t>(U) * p.D) {
+            const int cnt = te - t;
+            // what a step needs of its channel: step size, written value, and the
+            // factors of the output, out = gate y + gx
+            float dt[U], w[U], gate[U], gx[U];
+            ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            w[i] = dt[i] * IO<T>::ld(xr[i]);
-            S += dt[i];
-        }
-        ssm_mask<U>(cnt, w);
-        Rows::store(lds, lane, rv);
-        ssm_wave_sync();
-        load(t + U);
-        float Bn[4];   // the next four values of B, read ahead
-        ssm_lds4(lds, Bn);
+            for (int i = 0; i < U; ++i) {
+                const float x = IO<T>::ld(xr[i]);
+                w[i] = dt[i] * x;
+                gate[i] = 1.0f;
+                gx[i] = skip * x;
+                if constexpr (Z) {
+                    const float z = IO<T>::ld(zr[i]);
+                    gate[i] = z * sigmoid_hw(z);
+                    gx[i] *= gate[i];
+                }
+            }
+            ssm_mask<U>(cnt, w);
+            Rows::store(lds, lane, rv);
+            ssm_wave_sync();
+            load(t + U);
+            float Bn[4], Cn[4];   // the next four values of B and C, read ahead
+            ssm_lds4(lds, Bn);
+            ssm_lds4(lds + NS, Cn);
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
+            for (int i = 0; i < U; ++i) {
+                float y = 0.0f;
 #pragma unroll
-            for (int m = 0; m < NS; m += 4) {
-                const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]};
-                if (i * NS + m + 4 < U * NS) ssm_lds4(lds + i * NS + m + 4, Bn);
+                for (int m = 0; m < NS; m += 4) {
+                    const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]}, Cv[4] = {Cn[0], Cn[1], Cn[2], Cn[3]};
+                    if (i * NS + m + 4 < U * NS) {
+                        const int at = m + 4 < NS ? i * Rows::VALS + m + 4 : (i + 1) * Rows::VALS;
+                        ssm_lds4(lds + at, Bn);
+                        ssm_lds4(lds + at + NS, Cn);
+                    }
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
-                ssm_done4(h, m);
+                    for (int e = 0; e < 4; ++e) {
+                        h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
+                        y = fmaf(Cv[e], h[m + e], y);
+                    }
+                    ssm_done4(h, m);
+                    ssm_done(y);
+                }
+                if constexpr (SPLIT)
+                    s_y[((buf * 8 + nb) * U + i) * 64 + lane] = y;
+                else
+                    gx[i] = fmaf(gate[i], y, gx[i]);
+            }
+            if constexpr (SPLIT) {
+                // two buffers: a wave writes one again only past the next barrier,
+                // which every wave reaches after its reads of it
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    if (i % NB != nb || i >= cnt) continue;
+                    float y = 0.0f;
+                    for (int m = 0; m < NB; ++m) y += s_y[((buf * 8 + m) * U + i) * 64 + lane];
+                    if (valid) ssm_st<T>(po + static_cast<int64_t>(i) * p.D, off, IO<T>::st(fmaf(gate[i], y, gx[i])));
+                }
+                buf ^= 1;
+            } else {
+                ssm_wave_sync();
+                if (valid) {
+                    T* q = po;
+                    ssm_offset(off);
+                    if (cnt >= U) {
+#pragma unroll
+                        for (int i = 0; i < U; ++i, q += p.D) ssm_st<T>(q, off, IO<T>::st(gx[i]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < U; ++i, q += p.D)
+                            if (i < cnt) ssm_st<T>(q, off, IO<T>::st(gx[i]));
+                    }
+                }
             }
         }
-        ssm_wave_sync();
+        if (nb == 0 && valid) {   // rows past the sequence's length
+            T* pt = static_cast<T*>(out) + static_cast<int64_t>(b) * p.L * p.D + c;
+            for (int t = max(t0, te); t < t1; ++t) pt[static_cast<int64_t>(t) * p.D] = IO<T>::st(0.0f);
+        }
     }
-    if (!valid) return;
-    const int64_t row = static_cast<int64_t>(b) * p.nseg + seg;
-    if (n0 == 0) f.part_s[row * p.D + c] = S;
+
+    // The wave's states of a [B, D, N] tensor, and of segment seg of a
+    // [B, nseg, N, D] one.
+    __device__ __forceinline__ void read_state(const float* q, float (&h)[NS]) const {
+        const int64_t cn = (static_cast<int64_t>(b) * p.D + c) * p.N + n0;
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-        if (WHOLE || n < left) f.part_h[(row * p.N + n0 + n) * p.D + c] = h[n];
+        for (int n = 0; n < NS; ++n) h[n] = q && (WHOLE || n < left) ? q[cn + n] : 0.0f;
+    }
+    __device__ __forceinline__ void write_state(float* q, const float (&h)[NS]) const {
+        if (!q || !valid) return;
+        const int64_t cn = (static_cast<int64_t>(b) * p.D + c) * p.N + n0;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+            if (WHOLE || n < left) q[cn + n] = h[n];
+    }
+    __device__ __forceinline__ int64_t segment_at(int seg) const {
+        return ((static_cast<int64_t>(b) * p.nseg + seg) * p.N + n0) * p.D + c;
+    }
+    __device__ __forceinline__ void write_segment(float* q, int seg, const float (&h)[NS]) const {
+        if (!q || !valid) return;
+        q += segment_at(seg);
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+            if (WHOLE || n < left) q[static_cast<int64_t>(n) * p.D] = h[n];
+    }
+};
+
+template <typename T, typename TB, int NS, bool SPLIT, bool WHOLE>
+__global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_sums_kernel(SsmFwd f) {
+    constexpr int ALL = SsmRows<TB, NS, SSM_U, false, WHOLE>::ALL;
+    __shared__ __align__(16) float s_rows[(SPLIT ? 8 : 1) * ALL];
+    const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, seg = blockIdx.y;
+    SsmWave<T, TB, NS, WHOLE> w(f.a, nb * NS, seg);
+    float h[NS] = {};
+    const float S = w.sums(s_rows + nb * ALL, h);
+    if (w.valid && nb == 0) f.part_s[(static_cast<int64_t>(w.b) * f.a.nseg + seg) * f.a.D + w.c] = S;
+    w.write_segment(f.part_h, seg, h);
 }
 
 // The state entering each segment from the segments' sums, one thread per
@@ -130,7 +286,7 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmFwd f) {
     float* out = f.carries + (row0 * p.N + n) * p.D + c;
     const int64_t hs = static_cast<int64_t>(p.N) * p.D;
     const int last = p.nseg - 1;   // its sums are not formed
-    constexpr int U = 16;   // segments whose sums are loaded together, a group ahead
+    constexpr int U = 32;   // segments whose sums are loaded together, a group ahead
     float S[U], e[U];
     auto load = [&](int j) {
 #pragma unroll
@@ -160,154 +316,23 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmFwd f) {
 
 template <typename T, typename TB, int NS, bool Z, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_out_kernel(SsmFwd f) {
-    constexpr int U = SSM_U;
-    typedef SsmRows<TB, NS, U, true, WHOLE> Rows;
-    __shared__ __align__(16) float s_rows[(SPLIT ? 8 : 1) * Rows::ALL];
-    __shared__ float s_y[SPLIT ? 2 * 8 * U * 64 : 1];   // [2][waves][U][64]
-    const SsmArgs& p = f.a;
-    const int lane = threadIdx.x & 63;
-    const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    constexpr int ALL = SsmRows<TB, NS, SSM_U, true, WHOLE>::ALL;
+    __shared__ __align__(16) float s_rows[(SPLIT ? 8 : 1) * ALL];
+    __shared__ float s_y[SPLIT ? 2 * 8 * SSM_U * 64 : 1];
+    const int nb = SPLIT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, seg = blockIdx.y;
     const int NB = SPLIT ? __builtin_amdgcn_readfirstlane(blockDim.x >> 6) : 1;
-    const int n0 = nb * NS, left = p.N - n0;
-    const int g = blockIdx.x / p.nbk;
-    const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
-    const bool valid = ci < p.per;
-    const int c = g * p.per + (valid ? ci : p.per - 1);
-    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T));
-    const int seg = blockIdx.y, b = blockIdx.z;
-    const int len = ssm_length(p, b);
-    const int t0 = seg * p.seg, t1 = min(t0 + p.seg, p.L);
-    const int te = min(t1, len);
-
-    float A[NS], h[NS];
-    const int64_t sn = ((static_cast<int64_t>(b) * p.nseg + seg) * p.N + n0) * p.D + c;
-    const int64_t cn = (static_cast<int64_t>(b) * p.D + c) * p.N + n0;
+    SsmWave<T, TB, NS, WHOLE> w(f.a, nb * NS, seg);
+    float h[NS];
+    if (f.a.nseg > 1) {
+        const float* q = f.carries + w.segment_at(seg);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        const bool in = WHOLE || n < left;
-        A[n] = in ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
-        h[n] = 0.0f;
-        if (p.nseg > 1)
-            h[n] = in ? f.carries[sn + static_cast<int64_t>(n) * p.D] : 0.0f;
-        else if (p.h0 && in)
-            h[n] = p.h0[cn + n];
-        if (p.nseg == 1 && f.carries && valid && in) f.carries[sn + static_cast<int64_t>(n) * p.D] = h[n];
+        for (int n = 0; n < NS; ++n) h[n] = WHOLE || n < w.left ? q[static_cast<int64_t>(n) * f.a.D] : 0.0f;
+    } else {
+        w.read_state(f.a.h0, h);
+        w.write_segment(f.carries, 0, h);
     }
-    const float bias = p.bias ? p.bias[c] : 0.0f;
-    const float skip = p.skip ? p.skip[c] : 0.0f;
-    const T* px = static_cast<const T*>(p.x) + b * p.xb + t0 * p.xs;
-    const T* pd = static_cast<const T*>(p.delta) + b * p.db + t0 * p.ds;
-    const T* pz = static_cast<const T*>(p.z) + b * p.zb + t0 * p.zs;
-    const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0;
-    const TB* pC = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N + n0;
-    const Rows rows(pB, p.Bs, pC, p.Cs, lane, left);
-    T* po = static_cast<T*>(f.out) + (static_cast<int64_t>(b) * p.L + t0) * p.D;
-    float* lds = s_rows + nb * Rows::ALL;
-    T xr[U], dr[U], zr[U];
-    float rv[Rows::E];
-    auto load = [&](int t) {   // the rows of the block at t
-        const int cnt = te - t;
-        if (cnt >= U) {
-            ssm_load_rows<T, U, true>(px, p.xs, off, U, xr);
-            ssm_load_rows<T, U, true>(pd, p.ds, off, U, dr);
-            if constexpr (Z) ssm_load_rows<T, U, true>(pz, p.zs, off, U, zr);
-            rows.template load<true>(t, U, rv);
-        } else if (cnt > 0) {
-            ssm_load_rows<T, U, false>(px, p.xs, off, cnt, xr);
-            ssm_load_rows<T, U, false>(pd, p.ds, off, cnt, dr);
-            if constexpr (Z) ssm_load_rows<T, U, false>(pz, p.zs, off, cnt, zr);
-            rows.template load<false>(t, cnt, rv);
-        }
-    };
-    int buf = 0;
-    load(t0);
-    for (int t = t0; t < te; t += U, po += static_cast<int64_t>(U) * p.D) {
-        const int cnt = te - t;
-        // what a step needs of its channel: step size, written value, and the
-        // factors of the output, out = gate y + gx
-        float dt[U], w[U], gate[U], gx[U];
-        ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const float x = IO<T>::ld(xr[i]);
-            w[i] = dt[i] * x;
-            gate[i] = 1.0f;
-            gx[i] = skip * x;
-            if constexpr (Z) {
-                const float z = IO<T>::ld(zr[i]);
-                gate[i] = z * sigmoid_hw(z);
-                gx[i] *= gate[i];
-            }
-        }
-        ssm_mask<U>(cnt, w);
-        Rows::store(lds, lane, rv);
-        ssm_wave_sync();
-        load(t + U);
-        float Bn[4], Cn[4];   // the next four values of B and C, read ahead
-        ssm_lds4(lds, Bn);
-        ssm_lds4(lds + NS, Cn);
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            float y = 0.0f;
-#pragma unroll
-            for (int m = 0; m < NS; m += 4) {
-                const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]}, Cv[4] = {Cn[0], Cn[1], Cn[2], Cn[3]};
-                if (i * NS + m + 4 < U * NS) {
-                    const int at = m + 4 < NS ? i * Rows::VALS + m + 4 : (i + 1) * Rows::VALS;
-                    ssm_lds4(lds + at, Bn);
-                    ssm_lds4(lds + at + NS, Cn);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    h[m + e] = fmaf(ssm_exp2(dt[i] * A[m + e]), h[m + e], w[i] * Bv[e]);
-                    y = fmaf(Cv[e], h[m + e], y);
-                }
-                ssm_done4(h, m);
-                ssm_done(y);
-            }
-            if constexpr (SPLIT)
-                s_y[((buf * 8 + nb) * U + i) * 64 + lane] = y;
-            else
-                gx[i] = fmaf(gate[i], y, gx[i]);
-        }
-        if constexpr (SPLIT) {
-            // two buffers: a wave writes one again only past the next barrier,
-            // which every wave reaches after its reads of it
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (i % NB != nb || i >= cnt) continue;
-                float y = 0.0f;
-                for (int m = 0; m < NB; ++m) y += s_y[((buf * 8 + m) * U + i) * 64 + lane];
-                if (valid) ssm_st<T>(po + static_cast<int64_t>(i) * p.D, off, IO<T>::st(fmaf(gate[i], y, gx[i])));
-            }
-            buf ^= 1;
-        } else {
-            ssm_wave_sync();
-            if (valid) {
-                T* q = po;
-                ssm_offset(off);
-                if (cnt >= U) {
-#pragma unroll
-                    for (int i = 0; i < U; ++i, q += p.D) ssm_st<T>(q, off, IO<T>::st(gx[i]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < U; ++i, q += p.D)
-                        if (i < cnt) ssm_st<T>(q, off, IO<T>::st(gx[i]));
-                }
-            }
-        }
-    }
-    if (!valid) return;
-    if (nb == 0) {   // rows past the sequence's length
-        T* pt = static_cast<T*>(f.out) + static_cast<int64_t>(b) * p.L * p.D + c;
-        for (int t = max(t0, te); t < t1; ++t) pt[static_cast<int64_t>(t) * p.D] = IO<T>::st(0.0f);
-    }
-    if (f.state && seg == p.nseg - 1) {
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-            if (WHOLE || n < left) f.state[cn + n] = h[n];
-    }
+    w.template outputs<Z, SPLIT>(f.out, s_rows + nb * ALL, s_y, nb, NB, h);
+    if (seg == f.a.nseg - 1) w.write_state(f.state, h);
 }
 
 // ---------------------------------------------------------------------------
@@ -512,7 +537,7 @@ extern "C" int mogt_ssm_scan_fwd(const mogt_ssm_problem* q, void* out, float* fi
     f.out = out;
     f.state = final_state;
     f.part_h = static_cast<float*>(workspace);
-    f.carries = carries || f.a.nseg == 1 ? carries : f.part_h;
+    f.carries = carries || need == 0 ? carries : f.part_h;
     f.part_s = f.part_h + q->batch * f.a.nseg * q->channels * q->states;
     const int batch = static_cast<int>(q->batch);
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -90,7 +90,8 @@ SHAPES = [  # B, L, D, N, G, dtype: single tokens, edges of the 8-step blocks an
     (1, 1, 1, 1, 1, F32), (2, 1, 64, 16, 1, BF16), (1, 7, 65, 16, 1, F32), (1, 8, 64, 16, 1, BF16),
     (2, 9, 63, 3, 1, F32), (1, 16, 128, 16, 2, F32), (1, 17, 70, 8, 7, BF16), (3, 31, 130, 15, 1, BF16),
     (1, 33, 40, 16, 4, BF16), (1, 100, 64, 17, 1, F32), (2, 25, 66, 24, 2, BF16), (1, 40, 64, 64, 1, BF16),
-    (1, 19, 65, 128, 1, F32), (1, 18, 10, 127, 5, BF16), (1, 300, 64, 16, 1, BF16), (2, 129, 192, 4, 3, F32),
+    (1, 21, 64, 33, 1, F32), (1, 22, 33, 48, 1, BF16), (1, 26, 64, 56, 1, F32), (1, 13, 64, 60, 2, BF16),
+    (1, 12, 64, 72, 1, F32), (1, 19, 65, 128, 1, F32), (1, 18, 10, 127, 5, BF16), (1, 300, 64, 16, 1, BF16), (2, 129, 192, 4, 3, F32),
 ]
 
 
