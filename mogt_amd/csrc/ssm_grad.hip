@@ -45,11 +45,10 @@ struct SsmBwd {
     int batch, nblk;
 };
 
-// Sum of each of M values over the wave's lanes.  The halving steps leave
-// value R * (lane / 4) + j, R = M / 16, in v[j] of each lane.
-template <int M>
-__device__ __forceinline__ void wave_sums(float (&v)[M]) {
-    static_assert(M == 16 || M == 32, "16 or 32 values");
+// Sum of each of 32 values over the wave's lanes by halving steps; a lane gets
+// value 2 * (lane / 4) + lane % 2.
+__device__ __forceinline__ float wave_sums32(float (&v)[32], int lane) {
+    constexpr int M = 32;
 #pragma unroll
     for (int i = 0; i < M / 2; ++i) {   // lanes 32..63 keep the upper half of the values
         const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + M / 2]), false,
@@ -85,6 +84,8 @@ __device__ __forceinline__ void wave_sums(float (&v)[M]) {
         v[i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v[i]), 0xB1, 0xf, 0xf, false));
         v[i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v[i]), 0x4E, 0xf, 0xf, false));
     }
+    const float even = v[0], odd = v[1];   // (an index would put the array into memory)
+    return lane & 1 ? odd : even;
 }
 
 // Sum of each of 4 values over the lanes with the same lane % Q (4 or 8); a lane
@@ -300,6 +301,9 @@ void ssm_grad_kernel(SsmBwd f) {
     float* s_part = s_chan + 2 * R * 3 * 64;
     float* s_rows = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + nb * Rows::ALL;
     float* s_prod = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + NB * Rows::ALL + nb * (64 * ROW);
+    // a step's products are summed while the next ones are formed: two buffers, for
+    // which only a work-group of one wave has the room
+    constexpr bool BEHIND = VIA_LDS && !SPLIT;
     const int g = blockIdx.x / p.nbk;
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
     const bool valid = ci < p.per;
@@ -341,9 +345,10 @@ void ssm_grad_kernel(SsmBwd f) {
     // them, of step `slot` of every GROUP among the lanes with the same one
     constexpr int GROUP = 32 / NS;
     const int mine = VIA_LDS ? 4 * (lane & (QUADS - 1)) + 2 * (lane >> 5) + ((lane >> 4) & 1)
-                             : NS / 8 * (lane >> 2) + (NS == 16 ? lane & 1 : 0);
+                             : 2 * (lane >> 2) + (lane & 1);
     const int slot = (lane / QUADS) & (GROUP - 1);
-    const bool held = f.part_bc && (WHOLE || mine % NS < left) && (VIA_LDS || (lane & (NS == 16 ? 2 : 3)) == 0);
+    const float* s_mine = s_prod + (lane / QUADS) * QUADS * ROW + (lane & (QUADS - 1)) * 4;
+    const bool held = f.part_bc && (WHOLE || mine % NS < left) && (VIA_LDS || (lane & 2) == 0);
     uint32_t bc_off = ((mine >= NS ? p.N : 0) + n0 + mine % NS) * 4u;
 
     // inputs of the next block: the rows of the steps this wave owns, B and C,
@@ -456,7 +461,23 @@ void ssm_grad_kernel(SsmBwd f) {
             if (f.dx) ssm_st<T>(static_cast<T*>(f.dx) + at, off, IO<T>::st(fmaf(dw, dt_own[k], skip * dy)));
             if (f.ddelta) ssm_st<T>(static_cast<T*>(f.ddelta) + at, off, IO<T>::st(dd));
         };
-        float kept = 0.0f;   // of dB, dC
+        // this lane's part of a step's sums over the channels, from its products in
+        // LDS; BEHIND: while the step before it in time is computed
+        float kept = 0.0f, u[4];
+        auto read_rows = [&](int i, int k, float (&r0)[4], float (&r1)[4]) {   // k and k + 1 of step i
+            const float* q = s_mine + ((BEHIND ? i % 2 * 64 : 0) + k) * ROW;
+            ssm_lds4(q, r0);
+            ssm_lds4(q + ROW, r1);
+        };
+        auto add_rows = [&](int k, const float (&r0)[4], const float (&r1)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = (k > 0 ? u[e] + r0[e] : r0[e]) + r1[e];
+        };
+        auto put_sums = [&](int i) {
+            const float s = wave_sums4<QUADS>(u);
+            kept = slot == i % GROUP ? s : kept;
+            if (i % GROUP == 0 && held && i + slot < cnt) ssm_st<float>(pbc + i * 2 * p.N, bc_mine, kept);
+        };
 #pragma unroll
         for (int i = R - 1; i >= 0; --i) {
             float v[2 * NS];
@@ -469,6 +490,10 @@ void ssm_grad_kernel(SsmBwd f) {
             for (int m = 0; m < NS; m += 4) {   // four states at a time
                 ssm_f4 qb, qc;   // products of dB and dC
                 const float Bv[4] = {Bn[0], Bn[1], Bn[2], Bn[3]}, Cv[4] = {Cn[0], Cn[1], Cn[2], Cn[3]};
+                float r0[4], r1[4];   // of the step after
+                if constexpr (BEHIND) {
+                    if (i < R - 1) read_rows(i + 1, m / 2, r0, r1);
+                }
                 if (i > 0 || m + 4 < NS) {
                     const int at = m + 4 < NS ? i * Rows::VALS + m + 4 : (i - 1) * Rows::VALS;
                     ssm_lds4(s_rows + at, Bn);
@@ -488,8 +513,9 @@ void ssm_grad_kernel(SsmBwd f) {
                     dA[n] = fmaf(q, dt[i], dA[n]);
                 }
                 if constexpr (VIA_LDS) {
-                    *reinterpret_cast<ssm_f4*>(s_prod + lane * ROW + m) = qb;
-                    *reinterpret_cast<ssm_f4*>(s_prod + lane * ROW + NS + m) = qc;
+                    float* q = s_prod + ((BEHIND ? i % 2 * 64 : 0) + lane) * ROW + m;
+                    *reinterpret_cast<ssm_f4*>(q) = qb;
+                    *reinterpret_cast<ssm_f4*>(q + NS) = qc;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -502,27 +528,26 @@ void ssm_grad_kernel(SsmBwd f) {
                 ssm_done(qA);
                 ssm_done(dw);
                 if constexpr (Z) ssm_done(y);
+                if constexpr (BEHIND) {
+                    if (i < R - 1) add_rows(m / 2, r0, r1);
+                }
             }
             if (f.part_bc) {
                 if constexpr (VIA_LDS) {
                     ssm_wave_sync();
-                    const float* q = s_prod + (lane / QUADS) * QUADS * ROW + (lane & (QUADS - 1)) * 4;
-                    float u[4];
-                    ssm_lds4(q, u);
+                    if (BEHIND && i < R - 1) put_sums(i + 1);
+                    if (!BEHIND || i == 0) {
 #pragma unroll
-                    for (int k = 1; k < QUADS; ++k) {
-                        float r[4];
-                        ssm_lds4(q + k * ROW, r);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) u[e] += r[e];
+                        for (int k = 0; k < QUADS; k += 2) {
+                            float r0[4], r1[4];
+                            read_rows(i, k, r0, r1);
+                            add_rows(k, r0, r1);
+                        }
+                        ssm_wave_sync();
+                        put_sums(i);
                     }
-                    ssm_wave_sync();
-                    const float s = wave_sums4<QUADS>(u);
-                    kept = slot == i % GROUP ? s : kept;
-                    if (i % GROUP == 0 && held && i + slot < cnt) ssm_st<float>(pbc + i * 2 * p.N, bc_mine, kept);
                 } else {
-                    wave_sums<2 * NS>(v);
-                    const float s = NS == 16 && (lane & 1) ? v[NS / 8 - 1] : v[0];
+                    const float s = wave_sums32(v, lane);
                     if (held && i < cnt) ssm_st<float>(pbc + i * 2 * p.N, bc_mine, s);
                 }
             }
@@ -661,7 +686,7 @@ void grad_launch_as(const SsmBwd& f, hipStream_t st) {
     const int waves = grad_waves(a.N);
     const dim3 grid(a.D / a.per * a.nbk, a.nseg, f.batch);
     const size_t lds = sizeof(float) * ((SPLIT ? (2 + waves) * SSM_R * 3 * 64 : 0) + waves * SSM_R * 2 * NS +
-                                        (grad_via_lds(NS, OWN) ? waves * 64 * grad_row(NS) : 0));
+                                        (grad_via_lds(NS, OWN) ? (SPLIT ? waves : 2) * 64 * grad_row(NS) : 0));
     const bool whole = a.N % NS == 0;
     if (a.z && whole)
         ssm_grad_kernel<T, TB, NS, OWN, true, SPLIT, true><<<grid, 64 * waves, lds, st>>>(f);
