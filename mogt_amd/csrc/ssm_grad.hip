@@ -674,7 +674,7 @@ namespace {
 
 // States of a wave of the grad kernel: 16 where that leaves none idle, 8 for the
 // rest up to 48 (more waves of 8 would not fit their products into 64 KB of LDS).
-constexpr int grad_states_per_wave(int64_t N) { return N > 8 && (N <= 16 || N > 48 || N % 16 == 0) ? 16 : 8; }
+constexpr int grad_states_per_wave(int64_t N) { return N > 8 && (N <= 16 || N > 40) ? 16 : 8; }
 inline int grad_waves(int64_t N) {
     const int ns = grad_states_per_wave(N);
     return static_cast<int>((N + ns - 1) / ns);

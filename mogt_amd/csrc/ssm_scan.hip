@@ -163,7 +163,7 @@ struct SsmWave {
                 w[i] = dt[i] * x;
                 gate[i] = 1.0f;
                 gx[i] = skip * x;
-                if constexpr (Z) {
+                if (Z && (!SPLIT || i % NB == nb)) {
                     const float z = IO<T>::ld(zr[i]);
                     gate[i] = z * sigmoid_hw(z);
                     gx[i] *= gate[i];
@@ -337,84 +337,62 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_out_kernel(SsmFwd f) {
 
 // ---------------------------------------------------------------------------
 // single token: four lanes per channel, each four consecutive states of every
-// sixteen (VEC, states in whole aligned quads) or every fourth state.  Bound by
+// sixteen (VEC: states in whole aligned quads) or every fourth state.  Bound by
 // reading and writing the states (a server's batch) or by latency (one sequence):
-// a thread takes BT sequences, whose loads are in flight together and share the
-// channel's A, D and bias.
+// 256 sequences of 2048 channels with 16 states STEP256, one STEP1.  By single
+// states the 256 take 33.6 us.  Four sequences a thread, which share A, were no
+// faster at any batch (19.0 us for the 256, 5.1 against 3.7 for 16).
 // ---------------------------------------------------------------------------
 struct SsmStep {
     SsmArgs a;
     float* state;   // [B, D, N], updated
     void* out;      // [B, D]
-    int batch;
 };
 
-template <typename T, typename TB, int BT, bool VEC>
+template <typename T, typename TB, bool VEC>
 __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStep f) {
     constexpr int V = VEC ? 4 : 1;
     const SsmArgs& p = f.a;
     const int q = threadIdx.x & 3;
     const int c = blockIdx.x * 64 + (threadIdx.x >> 2);
     if (c >= p.D) return;   // whole quads
-    const int b0 = blockIdx.y * BT;
+    const int64_t b = blockIdx.y;
     const int g = c / p.per;
-    const float bias = p.bias ? p.bias[c] : 0.0f, skip = p.skip ? p.skip[c] : 0.0f;
-    float x[BT], dt[BT], y[BT];
-#pragma unroll
-    for (int k = 0; k < BT; ++k) {
-        const int64_t b = min(b0 + k, f.batch - 1);
-        x[k] = IO<T>::ld((static_cast<const T*>(p.x) + b * p.xb)[c]);
-        dt[k] = IO<T>::ld((static_cast<const T*>(p.delta) + b * p.db)[c]) + bias;
-        y[k] = 0.0f;
-    }
+    const float x = IO<T>::ld((static_cast<const T*>(p.x) + b * p.xb)[c]);
+    float dt = IO<T>::ld((static_cast<const T*>(p.delta) + b * p.db)[c]) + (p.bias ? p.bias[c] : 0.0f);
     const float* A = p.A + static_cast<int64_t>(c) * p.N;
-    float* h = f.state + (static_cast<int64_t>(b0) * p.D + c) * p.N;
-    const TB* B = static_cast<const TB*>(p.B) + b0 * p.Bb + static_cast<int64_t>(g) * p.N;
-    const TB* C = static_cast<const TB*>(p.C) + b0 * p.Cb + static_cast<int64_t>(g) * p.N;
-    const int64_t hs = static_cast<int64_t>(p.D) * p.N;
-    bool first = true;
+    float* h = f.state + (b * p.D + c) * p.N;
+    const TB* B = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N;
+    const TB* C = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N;
+    float y = 0.0f;
+    bool raw = p.softplus;
     for (int n = q * V; n < p.N; n += 4 * V) {
-        Pack<float, V> a = *reinterpret_cast<const Pack<float, V>*>(A + n), v[BT];
-        float Bv[BT][V], Cv[BT][V];
+        const Pack<float, V> a = *reinterpret_cast<const Pack<float, V>*>(A + n);
+        Pack<float, V> v = *reinterpret_cast<const Pack<float, V>*>(h + n);
+        float Bv[V], Cv[V];
 #pragma unroll
-        for (int k = 0; k < BT; ++k) {
-            if (b0 + k >= f.batch) break;
-            v[k] = *reinterpret_cast<const Pack<float, V>*>(h + k * hs + n);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                Bv[k][e] = IO<TB>::ld(B[k * p.Bb + n + e]);
-                Cv[k][e] = IO<TB>::ld(C[k * p.Cb + n + e]);
-            }
+        for (int e = 0; e < V; ++e) {
+            Bv[e] = IO<TB>::ld(B[n + e]);
+            Cv[e] = IO<TB>::ld(C[n + e]);
         }
-        if (first && p.softplus) {   // after the loads have gone out
+        if (raw) dt = ssm_softplus(dt);   // after the first loads have gone out
+        raw = false;
 #pragma unroll
-            for (int k = 0; k < BT; ++k) dt[k] = ssm_softplus(dt[k]);
+        for (int e = 0; e < V; ++e) {
+            v.v[e] = fmaf(ssm_exp2(dt * (a.v[e] * SSM_LOG2E)), v.v[e], dt * x * Bv[e]);
+            y = fmaf(Cv[e], v.v[e], y);
         }
-        first = false;
-#pragma unroll
-        for (int k = 0; k < BT; ++k) {
-            if (b0 + k >= f.batch) break;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                v[k].v[e] = fmaf(ssm_exp2(dt[k] * (a.v[e] * SSM_LOG2E)), v[k].v[e], dt[k] * x[k] * Bv[k][e]);
-                y[k] = fmaf(Cv[k][e], v[k].v[e], y[k]);
-            }
-            *reinterpret_cast<Pack<float, V>*>(h + k * hs + n) = v[k];
-        }
+        *reinterpret_cast<Pack<float, V>*>(h + n) = v;
     }
-#pragma unroll
-    for (int k = 0; k < BT; ++k) {
-        y[k] += __shfl_xor(y[k], 1, 64);
-        y[k] += __shfl_xor(y[k], 2, 64);
-        if (q != 0 || b0 + k >= f.batch) continue;
-        const int64_t b = b0 + k;
-        float o = fmaf(skip, x[k], y[k]);
-        if (p.z) {
-            const float z = IO<T>::ld((static_cast<const T*>(p.z) + b * p.zb)[c]);
-            o *= z * sigmoid_hw(z);
-        }
-        (static_cast<T*>(f.out) + b * p.D)[c] = IO<T>::st(o);
+    y += __shfl_xor(y, 1, 64);
+    y += __shfl_xor(y, 2, 64);
+    if (q != 0) return;
+    float o = fmaf(p.skip ? p.skip[c] : 0.0f, x, y);
+    if (p.z) {
+        const float z = IO<T>::ld((static_cast<const T*>(p.z) + b * p.zb)[c]);
+        o *= z * sigmoid_hw(z);
     }
+    (static_cast<T*>(f.out) + b * p.D)[c] = IO<T>::st(o);
 }
 
 // ---------------------------------------------------------------------------
@@ -492,21 +470,14 @@ int fwd_launch(const SsmFwd& f, int batch, hipStream_t st) {
 }
 
 template <typename T, typename TB>
-int step_launch(const SsmStep& f, hipStream_t st) {
+int step_launch(const SsmStep& f, int batch, hipStream_t st) {
     const SsmArgs& a = f.a;
-    const int blocks = (a.D + 63) / 64;
     const bool vec = a.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(f.state) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
-    // four sequences a thread where that leaves the GPU 16 waves per CU
-    const bool many = static_cast<int64_t>(blocks) * 4 * f.batch >= 4 * 16 * 256;
-    const dim3 grid(blocks, many ? (f.batch + 3) / 4 : f.batch);
-    if (vec && many)
-        ssm_step_kernel<T, TB, 4, true><<<grid, 256, 0, st>>>(f);
-    else if (vec)
-        ssm_step_kernel<T, TB, 1, true><<<grid, 256, 0, st>>>(f);
-    else if (many)
-        ssm_step_kernel<T, TB, 4, false><<<grid, 256, 0, st>>>(f);
+    const dim3 grid((a.D + 63) / 64, batch);
+    if (vec)
+        ssm_step_kernel<T, TB, true><<<grid, 256, 0, st>>>(f);
     else
-        ssm_step_kernel<T, TB, 1, false><<<grid, 256, 0, st>>>(f);
+        ssm_step_kernel<T, TB, false><<<grid, 256, 0, st>>>(f);
     return check_launch("mogt_ssm_step");
 }
 
@@ -555,11 +526,9 @@ extern "C" int mogt_ssm_step(const mogt_ssm_problem* q, float* state, void* out,
     if (!state || !out) return set_error(MOGT_E_INVALID, "null state or output pointer");
     f.state = state;
     f.out = out;
-    f.batch = static_cast<int>(q->batch);
+    const int batch = static_cast<int>(q->batch);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (q->io_dtype == MOGT_F32)
-        return step_launch<float, float>(f, st);
-    if (q->bc_dtype == MOGT_F32)
-        return step_launch<bf16_t, float>(f, st);
-    return step_launch<bf16_t, bf16_t>(f, st);
+    if (q->io_dtype == MOGT_F32) return step_launch<float, float>(f, batch, st);
+    if (q->bc_dtype == MOGT_F32) return step_launch<bf16_t, float>(f, batch, st);
+    return step_launch<bf16_t, bf16_t>(f, batch, st);
 }
