@@ -200,4 +200,66 @@ __device__ __forceinline__ void ssm_steps(const T (&raw)[U], float bias, int sof
 
 __device__ __forceinline__ float ssm_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 
+// What enters each segment, of one state of 64 channels: out[k] = h, then
+// h = exp2(A S[k]) h + part[k], over the segments in order (BACK: from the last
+// on); out may be part itself.  The first `formed` in that order have S and part.
+// The waves take 16 neighbouring segments each, fold them (one decay for the sum
+// of their S), and start from what the folds of the waves before them leave: a
+// chain over all segments in one thread waited for memory every 32 of them.
+constexpr int SSM_CARRY_U = 16, SSM_CARRY_WAVES = 16;
+inline int ssm_carry_threads(int nseg) {
+    const int waves = (nseg + SSM_CARRY_U - 1) / SSM_CARRY_U;
+    return 64 * (waves < 1 ? 1 : waves > SSM_CARRY_WAVES ? SSM_CARRY_WAVES : waves);
+}
+
+template <bool BACK>
+__device__ __forceinline__ void ssm_carry(float A, float h, const float* S, int64_t S_stride, const float* part,
+                                          float* out, int64_t stride, int nseg, int formed, bool valid) {
+    constexpr int U = SSM_CARRY_U;
+    __shared__ float s_fold[2][SSM_CARRY_WAVES][2][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int W = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
+    float Sv[U], e[U];
+    auto at = [&](int j) { return static_cast<int64_t>(BACK ? nseg - 1 - j : j); };
+    auto load = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) Sv[i] = e[i] = 0.0f;
+        if (j >= formed) return;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t k = at(min(j + i, formed - 1));
+            Sv[i] = S[k * S_stride];
+            e[i] = part[k * stride];
+        }
+    };
+    load(w * U);
+    for (int j0 = 0, buf = 0; j0 < nseg; j0 += W * U, buf ^= 1) {
+        const int j = j0 + w * U;
+        float a[U], v[U], sum = 0.0f, f = 0.0f;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            a[i] = ssm_exp2(Sv[i] * A);
+            v[i] = e[i];
+            sum += Sv[i];
+            f = fmaf(a[i], f, v[i]);
+        }
+        if (j0 + W * U < nseg) load(j + W * U);
+        s_fold[buf][w][0][lane] = ssm_exp2(sum * A);
+        s_fold[buf][w][1][lane] = f;
+        __syncthreads();   // a buffer is written again past the next one, when its readers are done
+        float g = h;
+        for (int m = 0; m < W; ++m) {
+            if (m == w) g = h;
+            h = fmaf(s_fold[buf][m][0][lane], h, s_fold[buf][m][1][lane]);
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (j + i >= nseg) break;
+            out[at(j + i) * stride] = g;
+            g = fmaf(a[i], g, v[i]);
+        }
+    }
+}
+
 }  // namespace mogt

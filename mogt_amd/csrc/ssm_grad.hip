@@ -231,42 +231,13 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
 
 // The gradient arriving at each segment's end from the segments' shares, in
 // place, the last segment first.
-__global__ __launch_bounds__(256) void ssm_carry_back_kernel(SsmBwd f) {
+__global__ __launch_bounds__(64 * SSM_CARRY_WAVES) void ssm_carry_back_kernel(SsmBwd f) {
     const SsmArgs& p = f.a;
-    const int c = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y, b = blockIdx.z;
-    if (c >= p.D) return;
-    const float A = p.A[static_cast<int64_t>(c) * p.N + n] * SSM_LOG2E;
-    float g = f.dfinal ? f.dfinal[(static_cast<int64_t>(b) * p.D + c) * p.N + n] : 0.0f;
-    const int64_t row0 = static_cast<int64_t>(b) * p.nseg;
-    const float* ps = f.part_s + row0 * p.D + c;
+    const int ci = blockIdx.x * 64 + (threadIdx.x & 63), c = min(ci, p.D - 1), n = blockIdx.y, b = blockIdx.z;
+    const int64_t cn = static_cast<int64_t>(c) * p.N + n, row0 = static_cast<int64_t>(b) * p.nseg;
     float* pg = f.part_g + (row0 * p.N + n) * p.D + c;
-    const int64_t gs = static_cast<int64_t>(p.N) * p.D;
-    constexpr int U = 32;   // segments whose shares are loaded together, a group ahead
-    float S[U], e[U];
-    auto load = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int k = max(j - i, 0);
-            S[i] = ps[static_cast<int64_t>(k) * p.D];
-            e[i] = pg[k * gs];
-        }
-    };
-    load(p.nseg - 1);
-    for (int j = p.nseg - 1; j >= 0; j -= U) {
-        float a[U], v[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            a[i] = ssm_exp2(S[i] * A);
-            v[i] = e[i];
-        }
-        if (j >= U) load(j - U);
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if (j - i < 0) break;
-            pg[(j - i) * gs] = g;
-            g = fmaf(a[i], g, v[i]);
-        }
-    }
+    ssm_carry<true>(p.A[cn] * SSM_LOG2E, f.dfinal ? f.dfinal[static_cast<int64_t>(b) * p.D * p.N + cn] : 0.0f,
+                    f.part_s + row0 * p.D + c, p.D, pg, pg, static_cast<int64_t>(p.N) * p.D, p.nseg, p.nseg, ci < p.D);
 }
 
 // One work-group: 64 channels, a wave for NS of their states.  With several waves
@@ -710,7 +681,7 @@ void grad_launch(const SsmBwd& f, hipStream_t st) {
         else
             ssm_marks_kernel<T, TB, NS, false, SPLIT, WHOLE><<<grid, 64 * ssm_waves(a.N), 0, st>>>(f);
     });
-    ssm_carry_back_kernel<<<dim3((a.D + 255) / 256, a.N, f.batch), 256, 0, st>>>(f);
+    ssm_carry_back_kernel<<<dim3((a.D + 63) / 64, a.N, f.batch), ssm_carry_threads(a.nseg), 0, st>>>(f);
     const int waves = grad_waves(a.N);
     if (grad_states_per_wave(a.N) == 8) {
         if (waves == 1)

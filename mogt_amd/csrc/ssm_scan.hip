@@ -272,46 +272,16 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_sums_kernel(SsmFwd f) {
     w.write_segment(f.part_h, seg, h);
 }
 
-// The state entering each segment from the segments' sums, one thread per
-// channel and state; `carries` may be part_h itself.
-__global__ __launch_bounds__(256) void ssm_carry_kernel(SsmFwd f) {
+// The state entering each segment from the segments' sums (the last one's are not
+// formed); `carries` may be part_h itself.
+__global__ __launch_bounds__(64 * SSM_CARRY_WAVES) void ssm_carry_kernel(SsmFwd f) {
     const SsmArgs& p = f.a;
-    const int c = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y, b = blockIdx.z;
-    if (c >= p.D) return;
-    const float A = p.A[static_cast<int64_t>(c) * p.N + n] * SSM_LOG2E;
-    float h = p.h0 ? p.h0[(static_cast<int64_t>(b) * p.D + c) * p.N + n] : 0.0f;
-    const int64_t row0 = static_cast<int64_t>(b) * p.nseg;
-    const float* ps = f.part_s + row0 * p.D + c;
-    const float* ph = f.part_h + (row0 * p.N + n) * p.D + c;
-    float* out = f.carries + (row0 * p.N + n) * p.D + c;
-    const int64_t hs = static_cast<int64_t>(p.N) * p.D;
-    const int last = p.nseg - 1;   // its sums are not formed
-    constexpr int U = 32;   // segments whose sums are loaded together, a group ahead
-    float S[U], e[U];
-    auto load = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int k = min(j + i, last > 0 ? last - 1 : 0);
-            S[i] = ps[static_cast<int64_t>(k) * p.D];
-            e[i] = ph[k * hs];
-        }
-    };
-    load(0);
-    for (int j = 0; j < p.nseg; j += U) {
-        float a[U], v[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            a[i] = ssm_exp2(S[i] * A);
-            v[i] = e[i];
-        }
-        if (j + U < p.nseg) load(j + U);
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if (j + i > last) break;
-            out[(j + i) * hs] = h;
-            h = fmaf(a[i], h, v[i]);
-        }
-    }
+    const int ci = blockIdx.x * 64 + (threadIdx.x & 63), c = min(ci, p.D - 1), n = blockIdx.y, b = blockIdx.z;
+    const int64_t cn = static_cast<int64_t>(c) * p.N + n, row0 = static_cast<int64_t>(b) * p.nseg;
+    const int64_t at = (row0 * p.N + n) * p.D + c;
+    ssm_carry<false>(p.A[cn] * SSM_LOG2E, p.h0 ? p.h0[static_cast<int64_t>(b) * p.D * p.N + cn] : 0.0f,
+                     f.part_s + row0 * p.D + c, p.D, f.part_h + at, f.carries + at, static_cast<int64_t>(p.N) * p.D,
+                     p.nseg, p.nseg - 1, ci < p.D);
 }
 
 template <typename T, typename TB, int NS, bool Z, bool SPLIT, bool WHOLE>
@@ -458,7 +428,7 @@ int fwd_launch(const SsmFwd& f, int batch, hipStream_t st) {
         constexpr bool SPLIT = decltype(split)::value, WHOLE = decltype(whole)::value;
         if (a.nseg > 1) {
             ssm_sums_kernel<T, TB, NS, SPLIT, WHOLE><<<dim3(blocks, a.nseg - 1, batch), 64 * waves, 0, st>>>(f);
-            ssm_carry_kernel<<<dim3((a.D + 255) / 256, a.N, batch), 256, 0, st>>>(f);
+            ssm_carry_kernel<<<dim3((a.D + 63) / 64, a.N, batch), ssm_carry_threads(a.nseg), 0, st>>>(f);
         }
         const dim3 grid(blocks, a.nseg, batch);
         if (a.z)
