@@ -371,3 +371,18 @@ def test_partial_gradients_and_second_derivatives(gpu):
     (g,) = torch.autograd.grad(call({**t, "x": x}, kw).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("lengths", [None, [4200, 4111]])
+def test_more_segments_than_are_folded_at_once(gpu, lengths):
+    """263 segments of 16 steps: the carries go round twice (256 a time), with a
+    channel block that is not full and a sequence that ends in the second round."""
+    announce(f"ssm_scan 4200 steps {lengths}")
+    run_both(*make(2, 4200, 70, 2, 1, F32, lengths=lengths, seed=16))
+
+
+@pytest.mark.parametrize("N", [9, 12, 20, 28, 32, 40, 41])
+def test_states_of_a_wave(gpu, N):
+    """State counts on both sides of each rule for how many a wave holds."""
+    announce(f"ssm_scan N={N}")
+    run_both(*make(1, 35, 66, N, 1, BF16, seed=N))
