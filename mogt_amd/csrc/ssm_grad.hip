@@ -17,9 +17,14 @@
 //           runs through it.
 //   sums    over the 64-channel blocks of a group (dB, dC) and over segments
 //           and sequences (dA, dD, bias), in a fixed order.
-// The sum of 2 NS products over the 64 channels of a wave is a halving
-// exchange: each step adds two lanes' values and halves the count, so it takes
-// about 2 instructions per product instead of 6.
+// 2 x 8192 steps of 1280 channels with 16 states, bf16: marks 124 us (4.1 TB/s:
+// near the 5.2 of a large copy), carry 16, grad 302 (2.2 TB/s), sums 12 and 10.
+// Bound of grad: the vector unit at two waves a SIMD, which is what a block's
+// states leave room for: 21 vector instructions per state and step, 14 of them the
+// formulas' and 3 the sums over channels.  Marks every 8 steps, 8 states a wave (85
+// instead of 62 us at 4096 x 1024) and three waves a SIMD with a part of the states
+// in scratch memory were slower; forming all decays twice to load the next block
+// earlier changed nothing.
 #include <type_traits>
 
 #include "ssm_common.h"
@@ -272,8 +277,8 @@ void ssm_grad_kernel(SsmBwd f) {
     float* s_part = s_chan + 2 * R * 3 * 64;
     float* s_rows = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + nb * Rows::ALL;
     float* s_prod = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + NB * Rows::ALL + nb * (64 * ROW);
-    // a step's products are summed while the next ones are formed: two buffers, for
-    // which only a work-group of one wave has the room
+    // a step's products are summed while the next ones are formed (331 us instead of
+    // 354, one card): two buffers, for which only a work-group of one wave has the room
     constexpr bool BEHIND = VIA_LDS && !SPLIT;
     const int g = blockIdx.x / p.nbk;
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
@@ -643,8 +648,11 @@ int column_sums(const float* part, float* a, float* b, float* c, int64_t rows, i
 
 namespace {
 
-// States of a wave of the grad kernel: 16 where that leaves none idle, 8 for the
-// rest up to 48 (more waves of 8 would not fit their products into 64 KB of LDS).
+// States of a wave of the grad kernel: 16 where one wave holds all, 8 from there
+// to 40, and 16 beyond (more waves of 8 would not fit their products into 64 KB of
+// LDS).  4096 steps of 1024 channels: 12 states in waves of 16 69 us and of 8 101,
+// 16 states 62 and 85, 24 states 147 both, 32 states 130 and 107, 40 states 250
+// both, 48 states 223 and 265.
 constexpr int grad_states_per_wave(int64_t N) { return N > 8 && (N <= 16 || N > 40) ? 16 : 8; }
 inline int grad_waves(int64_t N) {
     const int ns = grad_states_per_wave(N);

@@ -2665,11 +2665,15 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     return _short_conv_step_op(x, state, _float32(weight), _float32(bias), activation == "silu")
 
 
-# One wave scans a segment of a sequence for 64 channels and 16 states.  The
-# segments that make about two waves per SIMD (256 CUs x 4) keep the vector
-# units busy; more would repeat the exponentials of the sums pass without need.
+# One wave scans a segment of a sequence for 64 channels.  More segments fill the
+# GPU (1024 SIMDs) with more waves and end closer together, but leave more states
+# to carry: kernels over 32768 steps of 2048 channels with 16 states take 526, 438,
+# 437 and 428 us with segments for 2048, 4096, 6144 and 8192 waves, forward and
+# gradients of 2 x 8192 steps of 1280 channels 617, 599, 573 and 587.
 SSM_WAVES = 6144
-SSM_MIN_SEGMENT = 16
+# Shorter segments than that asks for where a call has few waves: 200 steps of
+# 1280 channels take 15.0 us in segments of 8, 18.9 of 16 and 28.4 of 32.
+SSM_MIN_SEGMENT = 8
 
 
 def _ssm_segment(B: int, L: int, D: int, N: int, G: int) -> int:
@@ -2760,7 +2764,8 @@ def _ssm_scan_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, x: torch.
     ws = scratch(lib.mogt_ssm_scan_bwd_workspace_bytes(b, L, ch, N, G, segment), x.device)
     out = _lib.SSM_GRADIENTS.pack(dx, ddelta, dz, dB, dC, dA, dD, dbias, dinit)
     with _on_device(x.device):
-        rc = lib.mogt_ssm_scan_bwd(p, dout.data_ptr(), _ptr(dfinal), carries.data_ptr(), out, ws.data_ptr(), ws.numel(), _stream_handle(x.device))
+        rc = lib.mogt_ssm_scan_bwd(p, dout.data_ptr(), _ptr(dfinal), carries.data_ptr(), out, ws.data_ptr(), ws.numel(),
+                                   _stream_handle(x.device))
     _lib.check(rc, "mogt_ssm_scan_bwd")
     return grads
 
@@ -2861,7 +2866,8 @@ def ssm_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
     within [0, L]) marks the padding of a ragged batch: steps past a length are
     not read and leave the state as it is; their outputs and gradients are zero.
     Differentiable in every tensor but ``lengths``, through both outputs; the
-    gradients do not change from run to run."""
+    gradients do not change from run to run.  ``A`` must be finite.  The backward's
+    workspace holds a state every 4 steps (B L D N bytes)."""
     if x.ndim != 3:
         raise ValueError("ssm_scan: x must be [B, L, D]")
     B, C = _check_ssm("ssm_scan", x, delta, A, B, C, D, z, delta_bias, initial_state)

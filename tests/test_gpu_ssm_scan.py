@@ -375,8 +375,8 @@ def test_partial_gradients_and_second_derivatives(gpu):
 
 @pytest.mark.parametrize("lengths", [None, [4200, 4111]])
 def test_more_segments_than_are_folded_at_once(gpu, lengths):
-    """263 segments of 16 steps: the carries go round twice (256 a time), with a
-    channel block that is not full and a sequence that ends in the second round."""
+    """525 segments of 8 steps: the carries go round three times (256 segments a
+    time), with a channel block that is not full and a sequence that ends early."""
     announce(f"ssm_scan 4200 steps {lengths}")
     run_both(*make(2, 4200, 70, 2, 1, F32, lengths=lengths, seed=16))
 

@@ -204,4 +204,4 @@ def test_entries_refuse_null_and_small():
                                        (256, 4096, 2048, 64, 2), (3, 1001, 333, 24, 1), (1, 1 << 20, 64, 128, 1)])
 def test_segments_are_whole_blocks_within_the_grid(B, L, D, N, G):
     s = ops._ssm_segment(B, L, D, N, G)
-    assert s % 8 == 0 and s >= 16 and -(-L // s) <= max(1, ops.SSM_WAVES)
+    assert s % 8 == 0 and s >= 8 and -(-L // s) <= max(1, ops.SSM_WAVES)
