@@ -386,3 +386,33 @@ def test_states_of_a_wave(gpu, N):
     """State counts on both sides of each rule for how many a wave holds."""
     announce(f"ssm_scan N={N}")
     run_both(*make(1, 35, 66, N, 1, BF16, seed=N))
+
+
+def test_rows_past_32_bit_offsets(gpu):
+    """Row strides that put x, delta and B beyond 2^31 elements."""
+    announce("ssm_scan rows past 2^31 elements")
+    t, kw = make(1, 20, 64, 16, 1, BF16, seed=17)
+    far = dict(t)
+    base = torch.zeros(2_500_000_000, dtype=BF16, device="cuda")
+    for i, k in enumerate(("x", "delta", "B")):
+        v = t[k]
+        view = base.as_strided(v.shape, (0, 130_000_000, *v.stride()[2:]), 1000 * i)
+        view.copy_(v)
+        far[k] = view
+    for a, b in zip(run_once_all(far, kw), run_once_all(t, kw)):
+        assert torch.equal(a, b)
+
+
+def test_one_tensor_in_several_places(gpu):
+    """x given as delta and as z too, B as C: the gradients add up."""
+    from mogt_amd import ops
+    t, _ = make(1, 30, 64, 16, 1, F32, seed=18)
+    x, B = t["x"].detach().requires_grad_(True), t["B"].detach().requires_grad_(True)
+    shared = torch.autograd.grad(ops.ssm_scan(x, x, t["A"], B, B, z=x, delta_softplus=True).sum(), (x, B))
+    own = [v.detach().clone().requires_grad_(True) for v in (x, x, x, B, B)]
+    out = ops.ssm_scan(own[0], own[1], t["A"], own[3], own[4], z=own[2], delta_softplus=True)
+    g = torch.autograd.grad(out.sum(), own)
+    # three terms in either order: two roundings of the sum of their magnitudes
+    for got, parts in ((shared[0], g[:3]), (shared[1], g[3:])):
+        want, mag = sum(p.double() for p in parts), sum(p.double().abs() for p in parts)
+        assert bool(((got.double() - want).abs() <= 2 * 2.0 ** -24 * mag + 1e-30).all())
