@@ -619,12 +619,12 @@ int mogt_split_ce_bwd(const void* A, int64_t lda, int64_t plane_a, int pieces_a,
  * are [batch, length, channels] with unit channel stride and the given row and
  * batch strides in elements; B, C (bc_dtype, fp32 or io_dtype) are rows of
  * groups x states, group-major, a group shared by channels / groups consecutive
- * channels.  A
- * [channels, states], D and delta_bias [channels], initial_state and
- * final_state [batch, channels, states] are contiguous fp32; z, D, delta_bias,
- * initial_state and lengths may be null.  lengths [batch] (4- or 8-byte
- * integers, clamped to [0, length]): steps past a sequence's length are not
- * read, leave the state as it is and write zero.
+ * channels.  A [channels, states] (finite), D and delta_bias [channels],
+ * initial_state and final_state [batch, channels, states] are contiguous fp32;
+ * z, D, delta_bias, initial_state and lengths may be null.  lengths [batch] (4- or
+ * 8-byte integers, clamped to [0, length]): steps past a sequence's length are not
+ * read, leave the state as it is and write zero.  Outputs and the workspace must
+ * not overlap each other or the inputs.
  *
  * `segment` (a multiple of 8): steps of one wave; sequences of several segments
  * take a scratch workspace of mogt_ssm_scan_workspace_bytes (no initial
@@ -632,12 +632,13 @@ int mogt_split_ce_bwd(const void* A, int64_t lda, int64_t plane_a, int pieces_a,
  * mogt_ssm_scan_fwd: `final_state` may be null; `carries` (may be null)
  *   [batch, segments, states, channels] receives the state entering each
  *   segment, which the backward takes.
- * mogt_ssm_scan_bwd: from the same problem, the forward's carries, dout
- *   (io_dtype, contiguous [batch, length, channels]) and
- *   dfinal_state (may be null) the gradients, each of which may be null: dx, ddelta, dz (io_dtype,
+ * mogt_ssm_scan_bwd: from the same problem (and segment), the forward's carries,
+ *   dout (io_dtype, contiguous [batch, length, channels]) and dfinal_state (may be
+ *   null) the gradients, each of which may be null: dx, ddelta, dz (io_dtype,
  *   contiguous), dB, dC (bc_dtype, contiguous [batch, length, groups, states]),
- *   dA, dD, ddelta_bias and dinitial_state (fp32, their tensors' layouts).
- *   Sums run in a fixed order: results do not change from run to run.
+ *   dA, dD, ddelta_bias and dinitial_state (fp32, their tensors' layouts).  Sums
+ *   run in a fixed order: results do not change from run to run.  Takes batch x
+ *   length x states below 2^31 and channels x states below 2^28.
  * mogt_ssm_step: one token per sequence (length 1; rows are addressed by the
  *   batch strides), `state` [batch, channels, states] updated in place.
  * No counterpart in the reference.                                          */
@@ -674,10 +675,11 @@ int mogt_ssm_step(const mogt_ssm_problem* problem, float* state, void* out, void
  * The K - 1 inputs before the first step are initial_state [batch, K-1,
  * channels] (io_dtype, contiguous; zero if null); final_state (may be null,
  * same layout) receives the last K - 1 inputs of each sequence.  lengths as
- * above.  mogt_short_conv_bwd: gradients of dy (contiguous) and
- *   dfinal_state (may be null) with respect to x (contiguous, io_dtype),
- *   weight, bias (fp32) and initial_state (io_dtype), each of which may be
- *   null; scratch workspace of mogt_short_conv_bwd_workspace_bytes.
+ * above.  Outputs must not overlap each other or the inputs.
+ * mogt_short_conv_bwd: gradients of dy (contiguous) and dfinal_state (may be
+ *   null) with respect to x (contiguous, io_dtype), weight, bias (fp32) and
+ *   initial_state (io_dtype), each of which may be null; scratch workspace of
+ *   mogt_short_conv_bwd_workspace_bytes.
  * mogt_short_conv_step: one token per sequence; `state` is shifted in place.
  * No counterpart in the reference.                                          */
 typedef struct mogt_short_conv_problem {

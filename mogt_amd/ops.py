@@ -2876,6 +2876,9 @@ def ssm_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
         _check_lengths("ssm_scan", lengths, x.shape[0])
     want_carries = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, delta, A, B, C, D, z, delta_bias, initial_state))
+    if want_carries and (x.shape[0] * x.shape[1] * A.shape[1] >= 1 << 31 or A.numel() >= 1 << 28):
+        raise ValueError("ssm_scan: a gradient takes batch x length x states below 2^31 and channels x states below "
+                         f"2^28, got x {list(x.shape)} with {A.shape[1]} states")
     out, state, _ = _ssm_scan_op(x, delta, _float32(A), B, C, _float32(D), z, _float32(delta_bias), initial_state,
                                  lengths, bool(delta_softplus), bool(return_state), want_carries)
     return (out, state) if return_state else out

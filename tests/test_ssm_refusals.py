@@ -205,3 +205,17 @@ def test_entries_refuse_null_and_small():
 def test_segments_are_whole_blocks_within_the_grid(B, L, D, N, G):
     s = ops._ssm_segment(B, L, D, N, G)
     assert s % 8 == 0 and s >= 8 and -(-L // s) <= max(1, ops.SSM_WAVES)
+
+
+@pytest.mark.parametrize("L,D,N,word", [(1 << 25, 1, 64, "below 2\\^31"), (1, 1 << 22, 64, "below 2\\^28")])
+def test_scan_refuses_what_its_backward_cannot_take(L, D, N, word):
+    """Before the forward runs, and only where a gradient is recorded."""
+    with FakeTensorMode():
+        e = lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
+        a = [e(1, L, D), e(1, L, D), e(D, N), e(1, L, N), e(1, L, N)]
+        assert ops.ssm_scan(*a).shape == (1, L, D)
+        a[0].requires_grad_(True)
+        with pytest.raises(ValueError, match=word):
+            ops.ssm_scan(*a)
+        with torch.no_grad():
+            assert ops.ssm_scan(*a).shape == (1, L, D)
