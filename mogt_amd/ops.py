@@ -216,6 +216,7 @@ class _Op:
             @staticmethod
             def forward(ctx, *args):
                 out = impl(*args)
+                ctx.plain = True
                 setup_context(ctx, args, out)
                 return out
 
@@ -235,6 +236,14 @@ class _Op:
             if not args[i].is_inference():
                 torch.autograd.graph.increment_version(args[i])
         return out
+
+
+    def in_backward(self, ctx, grad: torch.Tensor, *args):
+        """The op on an incoming gradient and what ``ctx`` saved: of a plain call
+        the arguments were looked at when it was recorded."""
+        if torch.is_grad_enabled() or not getattr(ctx, "plain", False) or not _plain((grad,)):
+            return self(grad, *args)
+        return self.impl(grad, *args)
 
 
 def _op(qualname: str, mutates: tuple = ()):
@@ -2452,7 +2461,7 @@ CONV_MAX_TAPS = 8
 
 def _on_device(device: torch.device):
     """The device context of a launch (nothing to enter on the current one)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == torch._C._cuda_getDevice():
         return _NO_RANGE
     return torch.cuda.device(device)
 
@@ -2538,7 +2547,7 @@ def _short_conv_grad_op(dy: torch.Tensor, dlast: torch.Tensor | None, x: torch.T
     lib = _lib.load()
     B, L, D = x.shape
     K = weight.shape[1]
-    dy = dy.to(x.dtype).contiguous()
+    dy = _dense(dy if dy.dtype == x.dtype else dy.to(x.dtype))
     dlast = None if dlast is None else dlast.to(x.dtype).contiguous()
     dx = torch.empty((B, L, D) if need_x else (0,), dtype=x.dtype, device=x.device)
     dinit = torch.empty((B, K - 1, D) if need_state else (0,), dtype=x.dtype, device=x.device)
@@ -2579,8 +2588,8 @@ def _short_conv_backward(ctx, dy, dlast):
     if dy is None:
         dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
     need = ctx.needs_input_grad
-    dx, dw, db, dinit = _short_conv_grad_op(dy, dlast, x, weight, bias, initial_state, lengths, ctx.silu, need[0],
-                                            need[3])
+    dx, dw, db, dinit = _short_conv_grad_op.in_backward(ctx, dy, dlast, x, weight, bias, initial_state, lengths,
+                                                        ctx.silu, need[0], need[3])
     return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dinit if need[3] else None,
             None, None, None)
 
@@ -2752,7 +2761,7 @@ def _ssm_scan_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, x: torch.
     b, L, ch = x.shape
     N, G = A.shape[1], B.shape[2]
     segment = _ssm_segment(b, L, ch, N, G)
-    dout = dout.to(x.dtype).contiguous()
+    dout = _dense(dout if dout.dtype == x.dtype else dout.to(x.dtype))
     dfinal = None if dfinal is None else dfinal.to(torch.float32).contiguous()
     p, held = _ssm_problem(x, delta, A, B, C, D, z, delta_bias, None, lengths, softplus, segment)
     rows, device, f32 = (b, L, ch), x.device, torch.float32
@@ -2801,7 +2810,8 @@ def _ssm_scan_backward(ctx, dout, dfinal, dcarries):
     if dout is None:
         dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
     need = list(ctx.needs_input_grad[:9])
-    grads = _ssm_scan_grad_op(dout, dfinal, x, delta, A, B, C, D, z, delta_bias, lengths, carries, ctx.softplus, need)
+    grads = _ssm_scan_grad_op.in_backward(ctx, dout, dfinal, x, delta, A, B, C, D, z, delta_bias, lengths, carries,
+                                          ctx.softplus, need)
     return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 4
 
 
