@@ -227,6 +227,57 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
         }
         ssm_wave_sync();
     }
+    // The products of a growing state's decays leave fp32 where the gradient that
+    // they carry need not (zero or small rows of it): such a share is formed again
+    // from the segment's end, step by step, which scales by one decay at a time.
+    bool beyond = false;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) beyond |= !(fabsf(P[n]) < INFINITY) || !(fabsf(G[n]) < INFINITY);
+    if (__any(beyond)) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) G[n] = 0.0f;
+        // the row pointers stand behind the last block
+        for (int t = t0 + (te - 1 - t0) / U * U; t >= t0; t -= U) {
+            const int cnt = te - t;
+            pd -= U * p.ds;
+            pg -= static_cast<int64_t>(U) * p.D;
+            const T *qd = pd, *qg = pg;
+            ssm_load_rows<T, U, false>(qd, p.ds, off, cnt, dr);
+            ssm_load_rows<T, U, false>(qg, p.D, off, cnt, gr);
+            if constexpr (Z) {
+                pz -= U * p.zs;
+                const T* qz = pz;
+                ssm_load_rows<T, U, false>(qz, p.zs, off, cnt, zr);
+            }
+            rows.template load<false>(t, cnt, rv);
+            Rows::store(lds, lane, rv);
+            ssm_wave_sync();
+            float dt[U], dy[U];
+            ssm_steps<T, U>(dr, bias, p.softplus, cnt, dt);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                dy[i] = IO<T>::ld(gr[i]);
+                if constexpr (Z) {
+                    const float z = IO<T>::ld(zr[i]);
+                    dy[i] *= z * sigmoid_hw(z);
+                }
+            }
+            ssm_mask<U>(cnt, dy);
+#pragma unroll
+            for (int i = U - 1; i >= 0; --i) {
+#pragma unroll
+                for (int n = 0; n < NS; n += 4) {
+                    float Cv[4];
+                    ssm_lds4(lds + i * Rows::VALS + NS + n, Cv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        G[n + e] = ssm_exp2(dt[i] * A[n + e]) * fmaf(Cv[e], dy[i], G[n + e]);
+                    ssm_done4(G, n);
+                }
+            }
+            ssm_wave_sync();
+        }
+    }
     if (!valid) return;
     if (n0 == 0) f.part_s[row * p.D + c] = S;
 #pragma unroll

@@ -2876,7 +2876,9 @@ def ssm_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
     within [0, L]) marks the padding of a ragged batch: steps past a length are
     not read and leave the state as it is; their outputs and gradients are zero.
     Differentiable in every tensor but ``lengths``, through both outputs; the
-    gradients do not change from run to run.  ``A`` must be finite.  The backward's
+    gradients do not change from run to run.  ``A`` must be finite, of either
+    sign: states and gradients are in range as far as fp32 is, whatever they grow
+    by over a sequence (one step's ``exp(dt A)`` is an fp32 number).  The backward's
     workspace holds a state every 4 steps (B L D N bytes)."""
     if x.ndim != 3:
         raise ValueError("ssm_scan: x must be [B, L, D]")

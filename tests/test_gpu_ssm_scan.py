@@ -416,3 +416,53 @@ def test_one_tensor_in_several_places(gpu):
     for got, parts in ((shared[0], g[:3]), (shared[1], g[3:])):
         want, mag = sum(p.double() for p in parts), sum(p.double().abs() for p in parts)
         assert bool(((got.double() - want).abs() <= 2 * 2.0 ** -24 * mag + 1e-30).all())
+
+
+def growing(L, zero_rows, N=4, D=66, quiet=None, seed=30, init=None):
+    """A of 1, 0.5, 0 and -1, steps of 1: zero input rows first, then 30 with
+    values; output gradients in the first rows up to ``quiet`` only."""
+    t, kw = make(1, L, D, N, 1, F32, z=False, softplus=False, bias=False, init=init is not None, seed=seed)
+    t["delta"].fill_(1.0)
+    t["A"][:] = torch.tensor([1.0, 0.5, 0.0, -1.0], device="cuda")[:N]
+    t["x"][:, :zero_rows] = 0.0
+    if init is not None:
+        t["initial_state"].fill_(init)
+    return t, kw
+
+
+@pytest.mark.parametrize("segment", [8, 104, 400])
+def test_growth_over_zero_rows(gpu, monkeypatch, segment):
+    """A decay above one, exp(400) in all, on a state of zero: the state stays
+    zero until the first value, and the gradient zero after the last one."""
+    from mogt_amd import ops
+    announce(f"ssm_scan growth, segments of {segment}")
+    monkeypatch.setattr(ops, "SSM_MIN_SEGMENT", segment)
+    t, kw = growing(400, 370)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None}
+    out, state = call({**{k: None for k in NAMES}, **leaves}, kw, return_state=True)
+    dout = torch.zeros_like(out)
+    dout[:, :30] = torch.randn(1, 30, 66, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    want, mag = oracle(t, kw, dout=dout, dstate=torch.zeros_like(state))
+    tol = bound(t, 26 * 60)   # 30 steps of A = 1 forward and 30 backward, undamped
+    check("out", out, want["out"], mag["out"], tol)
+    check("state", state, want["state"], mag["state"], tol)
+    for k, g in zip(leaves, torch.autograd.grad(out, list(leaves.values()), dout)):
+        check("d" + k, g, want["d" + k], mag["d" + k], tol)
+
+
+@pytest.mark.parametrize("segment", [8, 104])
+def test_growth_of_a_small_state(gpu, monkeypatch, segment):
+    """exp(104) = 1.5e45 lies beyond fp32, exp(104) 1e-30 does not; and the same
+    for the gradient on its way back."""
+    from mogt_amd import ops
+    monkeypatch.setattr(ops, "SSM_MIN_SEGMENT", segment)
+    t, kw = growing(130, 130, init=1e-30)
+    t["delta"][:, 104:] = 0.0
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None}
+    out, state = call({**{k: None for k in NAMES}, **leaves}, kw, return_state=True)
+    dout, dstate = torch.zeros_like(out), torch.full_like(state, 1e-20)
+    want, mag = oracle(t, kw, dout=dout, dstate=dstate)
+    tol = bound(t, 26 * 208)
+    check("state", state, want["state"], mag["state"], tol)
+    for k, g in zip(leaves, torch.autograd.grad([out, state], list(leaves.values()), [dout, dstate])):
+        check("d" + k, g, want["d" + k], mag["d" + k], tol)
