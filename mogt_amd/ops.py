@@ -238,12 +238,12 @@ class _Op:
         return out
 
 
-    def in_backward(self, ctx, grad: torch.Tensor, *args):
-        """The op on an incoming gradient and what ``ctx`` saved: of a plain call
-        the arguments were looked at when it was recorded."""
-        if torch.is_grad_enabled() or not getattr(ctx, "plain", False) or not _plain((grad,)):
-            return self(grad, *args)
-        return self.impl(grad, *args)
+    def in_backward(self, ctx, grads: tuple, *args):
+        """The op on incoming gradients and what ``ctx`` saved: of a plain call
+        the other arguments were looked at when it was recorded."""
+        if torch.is_grad_enabled() or not getattr(ctx, "plain", False) or not _plain(grads):
+            return self(*grads, *args)
+        return self.impl(*grads, *args)
 
 
 def _op(qualname: str, mutates: tuple = ()):
@@ -2588,8 +2588,8 @@ def _short_conv_backward(ctx, dy, dlast):
     if dy is None:
         dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
     need = ctx.needs_input_grad
-    dx, dw, db, dinit = _short_conv_grad_op.in_backward(ctx, dy, dlast, x, weight, bias, initial_state, lengths,
-                                                        ctx.silu, need[0], need[3])
+    dx, dw, db, dinit = _short_conv_grad_op.in_backward(ctx, (dy, dlast), x, weight, bias, initial_state,
+                                                        lengths, ctx.silu, need[0], need[3])
     return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dinit if need[3] else None,
             None, None, None)
 
@@ -2810,8 +2810,8 @@ def _ssm_scan_backward(ctx, dout, dfinal, dcarries):
     if dout is None:
         dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
     need = list(ctx.needs_input_grad[:9])
-    grads = _ssm_scan_grad_op.in_backward(ctx, dout, dfinal, x, delta, A, B, C, D, z, delta_bias, lengths, carries,
-                                          ctx.softplus, need)
+    grads = _ssm_scan_grad_op.in_backward(ctx, (dout, dfinal), x, delta, A, B, C, D, z, delta_bias, lengths,
+                                          carries, ctx.softplus, need)
     return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 4
 
 

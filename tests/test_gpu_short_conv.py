@@ -248,3 +248,17 @@ def test_layer_for_prompts_and_tokens(gpu):
         # more sums of up to 29 steps and 16 states
         err = (torch.cat(got[i]) - want).abs().max()
         assert float(err) <= 64 * 29 * 2.0 ** -24 * float(want.abs().max())
+
+
+def test_negated_gradient_of_the_state(gpu):
+    """A gradient of the final state that is a lazily negated view."""
+    t, _ = make(2, 20, 64, 4, F32, seed=11)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    g = torch.Generator(device="cuda").manual_seed(4)
+    dy, ds = torch.randn(2, 20, 64, generator=g, device="cuda"), torch.randn(2, 3, 64, generator=g, device="cuda")
+    for a, b in ((dy, torch._neg_view(ds)), (torch._neg_view(dy), ds)):
+        assert a.is_neg() or b.is_neg()
+        got, want = (torch.autograd.grad(list(call(leaves, None, True, return_state=True)), list(leaves.values()),
+                                         list(d)) for d in ((a, b), (a.resolve_neg(), b.resolve_neg())))
+        for k, u, v in zip(leaves, got, want):
+            assert torch.equal(u, v), k

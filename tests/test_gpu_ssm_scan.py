@@ -466,3 +466,18 @@ def test_growth_of_a_small_state(gpu, monkeypatch, segment):
     check("state", state, want["state"], mag["state"], tol)
     for k, g in zip(leaves, torch.autograd.grad([out, state], list(leaves.values()), [dout, dstate])):
         check("d" + k, g, want["d" + k], mag["d" + k], tol)
+
+
+def test_negated_gradient_of_the_state(gpu):
+    """A gradient of the final state that is a lazily negated view."""
+    t, kw = make(1, 20, 64, 16, 1, F32, seed=31)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    g = torch.Generator(device="cuda").manual_seed(4)
+    dout = torch.randn(1, 20, 64, generator=g, device="cuda")
+    dstate = torch.randn(1, 64, 16, generator=g, device="cuda")
+    for a, b in ((dout, torch._neg_view(dstate)), (torch._neg_view(dout), dstate)):
+        assert a.is_neg() or b.is_neg()
+        got, want = (torch.autograd.grad(list(call(leaves, kw, return_state=True)), list(leaves.values()), list(d))
+                     for d in ((a, b), (a.resolve_neg(), b.resolve_neg())))
+        for k, u, v in zip(leaves, got, want):
+            assert torch.equal(u, v), k
