@@ -115,6 +115,7 @@ __device__ __forceinline__ float wave_sums4(const float (&u)[4]) {
 // of 16 states have no room for it.
 constexpr bool grad_via_lds(int NS, int OWN) { return NS == 8 || OWN > 1; }
 constexpr int grad_row(int NS) { return 2 * NS + 4; }
+constexpr int GRAD_ROWS = 65;   // of a buffer of products: a lane's each, and one for all idle lanes
 
 template <typename T, typename TB, int NS, bool Z, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
@@ -305,7 +306,9 @@ __global__ __launch_bounds__(64 * SSM_CARRY_WAVES) void ssm_carry_back_kernel(Ss
 // dB and dC are summed over the 64 channels through LDS: each lane leaves its 2 NS
 // products in a row (padded to 16-byte accesses without bank conflicts) and adds 4
 // values of NS / 2 rows, which leaves 4 values instead of 2 NS to exchange between
-// lanes.  KEEP: the decays of a block's last steps stay in registers beside its
+// lanes.  Idle lanes write to a row that is not read, and their own stay zero (their
+// states repeat the last channel's, and zero times an infinity there would be NaN).
+// KEEP: the decays of a block's last steps stay in registers beside its
 // states; 16 states leave room for two steps of them, the others form them again
 // on the way back.
 template <typename T, typename TB, int NS, int OWN, bool Z, bool SPLIT, bool WHOLE>
@@ -327,7 +330,7 @@ void ssm_grad_kernel(SsmBwd f) {
     float* s_chan = smem;
     float* s_part = s_chan + 2 * R * 3 * 64;
     float* s_rows = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + nb * Rows::ALL;
-    float* s_prod = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + NB * Rows::ALL + nb * (64 * ROW);
+    float* s_prod = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + NB * Rows::ALL + nb * (GRAD_ROWS * ROW);
     // a step's products are summed while the next ones are formed (331 us instead of
     // 354, one card): two buffers, for which only a work-group of one wave has the room
     constexpr bool BEHIND = VIA_LDS && !SPLIT;
@@ -342,16 +345,14 @@ void ssm_grad_kernel(SsmBwd f) {
     const int te = min(t1, len);
     const int64_t row = static_cast<int64_t>(b) * p.nseg + seg;
 
-    // gradient arriving at the segment's end.  Idle lanes repeat the last
-    // channel's step sizes and states on inputs and gradients of zero, so they add
-    // nothing to the sums over channels.
+    // gradient arriving at the segment's end
     float A[NS], gc[NS], dA[NS];
     const int64_t cn = (static_cast<int64_t>(b) * p.D + c) * p.N + n0;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const bool in = WHOLE || n < left;
         A[n] = in ? p.A[static_cast<int64_t>(c) * p.N + n0 + n] * SSM_LOG2E : 0.0f;
-        gc[n] = in && valid ? f.part_g[(row * p.N + n0 + n) * p.D + c] : 0.0f;
+        gc[n] = in ? f.part_g[(row * p.N + n0 + n) * p.D + c] : 0.0f;
         dA[n] = 0.0f;
     }
     const float bias = p.bias ? p.bias[c] : 0.0f;
@@ -410,7 +411,13 @@ void ssm_grad_kernel(SsmBwd f) {
         else
             load_as(std::false_type(), t);
     };
-    const float on = valid ? 1.0f : 0.0f;
+    float* s_own = s_prod + (valid ? lane : 64) * ROW;   // this lane's products
+    const bool idle = !__all(valid);
+    if (VIA_LDS && !valid) {
+#pragma unroll
+        for (int q = 0; q < (BEHIND ? 2 : 1); ++q)
+            for (int k = 0; k < ROW; ++k) s_prod[(q * GRAD_ROWS + lane) * ROW + k] = 0.0f;
+    }
     const int64_t bc_row = static_cast<int64_t>(blockIdx.x) * f.batch * p.L + bl;
     float* pbc = f.part_bc + (bc_row + t) * 2 * p.N;
     uint32_t bc_mine = bc_off + (VIA_LDS ? slot * 2 * p.N * 4u : 0u);
@@ -428,8 +435,8 @@ void ssm_grad_kernel(SsmBwd f) {
 #pragma unroll
         for (int k = 0; k < OWN; ++k) {
             const int i = nb + k * NB;
-            x[k] = IO<T>::ld(xr[k]) * on;
-            go[k] = IO<T>::ld(gr[k]) * on;
+            x[k] = IO<T>::ld(xr[k]);
+            go[k] = IO<T>::ld(gr[k]);
             raw[k] = IO<T>::ld(dr[k]) + bias;
             dt_own[k] = p.softplus ? ssm_softplus(raw[k]) : raw[k];
             z[k] = Z ? IO<T>::ld(zr[k]) : 0.0f;
@@ -492,7 +499,7 @@ void ssm_grad_kernel(SsmBwd f) {
         // LDS; BEHIND: while the step before it in time is computed
         float kept = 0.0f, u[4];
         auto read_rows = [&](int i, int k, float (&r0)[4], float (&r1)[4]) {   // k and k + 1 of step i
-            const float* q = s_mine + ((BEHIND ? i % 2 * 64 : 0) + k) * ROW;
+            const float* q = s_mine + ((BEHIND ? i % 2 * GRAD_ROWS : 0) + k) * ROW;
             ssm_lds4(q, r0);
             ssm_lds4(q + ROW, r1);
         };
@@ -540,7 +547,7 @@ void ssm_grad_kernel(SsmBwd f) {
                     dA[n] = fmaf(q, dt[i], dA[n]);
                 }
                 if constexpr (VIA_LDS) {
-                    float* q = s_prod + ((BEHIND ? i % 2 * 64 : 0) + lane) * ROW + m;
+                    float* q = s_own + (BEHIND ? i % 2 * GRAD_ROWS : 0) * ROW + m;
                     *reinterpret_cast<ssm_f4*>(q) = qb;
                     *reinterpret_cast<ssm_f4*>(q + NS) = qc;
                 } else {
@@ -574,6 +581,10 @@ void ssm_grad_kernel(SsmBwd f) {
                         put_sums(i);
                     }
                 } else {
+                    if (idle) {
+#pragma unroll
+                        for (int k = 0; k < 2 * NS; ++k) v[k] = valid ? v[k] : 0.0f;
+                    }
                     const float s = wave_sums32(v, lane);
                     if (held && i < cnt) ssm_st<float>(pbc + i * 2 * p.N, bc_mine, s);
                 }
@@ -716,7 +727,7 @@ void grad_launch_as(const SsmBwd& f, hipStream_t st) {
     const int waves = grad_waves(a.N);
     const dim3 grid(a.D / a.per * a.nbk, a.nseg, f.batch);
     const size_t lds = sizeof(float) * ((SPLIT ? (2 + waves) * SSM_R * 3 * 64 : 0) + waves * SSM_R * 2 * NS +
-                                        (grad_via_lds(NS, OWN) ? (SPLIT ? waves : 2) * 64 * grad_row(NS) : 0));
+                                        (grad_via_lds(NS, OWN) ? (SPLIT ? waves : 2) * GRAD_ROWS * grad_row(NS) : 0));
     const bool whole = a.N % NS == 0;
     if (a.z && whole)
         ssm_grad_kernel<T, TB, NS, OWN, true, SPLIT, true><<<grid, 64 * waves, lds, st>>>(f);

@@ -481,3 +481,21 @@ def test_negated_gradient_of_the_state(gpu):
                      for d in ((a, b), (a.resolve_neg(), b.resolve_neg())))
         for k, u, v in zip(leaves, got, want):
             assert torch.equal(u, v), k
+
+
+@pytest.mark.parametrize("N", [8, 16, 24, 64])
+def test_infinity_in_a_channel_block_that_is_not_full(gpu, N):
+    """An infinite input of the last channel makes infinities of the sums over
+    the channels, as in the definition: idle lanes add nothing to them."""
+    t, kw = make(1, 10, 65, N, 1, F32, z=False, seed=33)
+    t["x"][0, 6, 64] = float("inf")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    dout = torch.randn(1, 10, 65, generator=g, device="cuda")
+    want, _ = oracle(t, kw, dout=dout)
+    leaves = {k: t[k].detach().requires_grad_(True) for k in ("B", "C")}
+    got = torch.autograd.grad(call({**t, **leaves}, kw), list(leaves.values()), dout)
+    for k, v in zip(leaves, got):
+        v, w = v.double().cpu(), want["d" + k]
+        assert bool(w[0, 6].isinf().all()) and not w.isnan().any()
+        assert torch.equal(v.isnan(), w.isnan()) and torch.equal(v.isinf(), w.isinf()), k
+        assert torch.equal(v[v.isinf()].sign(), w[w.isinf()].sign()), k
