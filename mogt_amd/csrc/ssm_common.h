@@ -200,21 +200,16 @@ __device__ __forceinline__ void ssm_steps(const T (&raw)[U], float bias, int sof
 
 __device__ __forceinline__ float ssm_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// 2^x as m 2^k with m in [1, 2].  A segment's decay is 2^(A S) with a sum of step
-// sizes: it may lie far outside fp32 (a growing state, A S > 128) where the state
-// that it scales is zero or small and the product is in range.
-struct SsmDecay {
-    float m;
-    int k;
-};
-__device__ __forceinline__ SsmDecay ssm_decay(float x) {
-    const float c = __builtin_amdgcn_fmed3f(x, -1000.0f, 1000.0f), f = floorf(c);
-    return {ssm_exp2(c - f), static_cast<int>(f)};
+// The square root of 2^x.  A segment's decay is 2^(A S) with a sum of step sizes: it
+// may lie far outside fp32 (a growing state, A S > 128) where the state that it
+// scales is zero or small and the product is in range.  Its root is kept within
+// [2^-126, 2^127] and applied twice: zero stays zero and infinity infinity, and
+// what a normal number times a decay beyond that gives is infinite or below 2^-124.
+__device__ __forceinline__ float ssm_root(float x) {
+    return ssm_exp2(__builtin_amdgcn_fmed3f(0.5f * x, -126.0f, 127.0f));
 }
-// d h + v, in range wherever the result is
-__device__ __forceinline__ float ssm_fold(const SsmDecay& d, float h, float v) {
-    return fmaf(d.m, __builtin_ldexpf(h, d.k), v);
-}
+// r^2 h + v
+__device__ __forceinline__ float ssm_fold(float r, float h, float v) { return fmaf(r, r * h, v); }
 
 // What enters each segment, of one state of 64 channels: out[k] = h, then
 // h = 2^(A S[k]) h + part[k], over the segments in order (BACK: from the last
@@ -232,8 +227,7 @@ template <bool BACK>
 __device__ __forceinline__ void ssm_carry(float A, float h, const float* S, int64_t S_stride, const float* part,
                                           float* out, int64_t stride, int nseg, int formed, bool valid) {
     constexpr int U = SSM_CARRY_U;
-    __shared__ SsmDecay s_decay[2][SSM_CARRY_WAVES][64];
-    __shared__ float s_fold[2][SSM_CARRY_WAVES][64];
+    __shared__ float s_fold[2][SSM_CARRY_WAVES][2][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int W = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
     float Sv[U], e[U];
@@ -252,23 +246,22 @@ __device__ __forceinline__ void ssm_carry(float A, float h, const float* S, int6
     load(w * U);
     for (int j0 = 0, buf = 0; j0 < nseg; j0 += W * U, buf ^= 1) {
         const int j = j0 + w * U;
-        SsmDecay a[U];
-        float v[U], sum = 0.0f, f = 0.0f;
+        float a[U], v[U], sum = 0.0f, f = 0.0f;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            a[i] = ssm_decay(Sv[i] * A);
+            a[i] = ssm_root(Sv[i] * A);
             v[i] = e[i];
             sum += Sv[i];
             f = ssm_fold(a[i], f, v[i]);
         }
         if (j0 + W * U < nseg) load(j + W * U);
-        s_decay[buf][w][lane] = ssm_decay(sum * A);
-        s_fold[buf][w][lane] = f;
+        s_fold[buf][w][0][lane] = ssm_root(sum * A);
+        s_fold[buf][w][1][lane] = f;
         __syncthreads();   // a buffer is written again past the next one, when its readers are done
         float g = h;
         for (int m = 0; m < W; ++m) {
             if (m == w) g = h;
-            h = ssm_fold(s_decay[buf][m][lane], h, s_fold[buf][m][lane]);
+            h = ssm_fold(s_fold[buf][m][0][lane], h, s_fold[buf][m][1][lane]);
         }
         if (!valid) continue;
 #pragma unroll
