@@ -514,6 +514,15 @@ void ssm_grad_kernel(SsmBwd f) {
         };
 #pragma unroll
         for (int i = R - 1; i >= 0; --i) {
+            if (i < R - 1 && i == cnt - 1) {
+                // The sequence's last step (its block is the first one here): the steps
+                // behind it added their step size of zero times the end's state, which
+                // may be infinite.
+#pragma unroll
+                for (int n = 0; n < NS; ++n) dA[n] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NS; n += 4) ssm_done4(dA, n);
+            }
             float v[2 * NS];
             float sig = 0.0f;
             const float dy = SPLIT ? chan[(i * 3 + 2) * 64] : grad_y(SPLIT ? 0 : i, sig);

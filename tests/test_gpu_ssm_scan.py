@@ -499,3 +499,19 @@ def test_infinity_in_a_channel_block_that_is_not_full(gpu, N):
         assert bool(w[0, 6].isinf().all()) and not w.isnan().any()
         assert torch.equal(v.isnan(), w.isnan()) and torch.equal(v.isinf(), w.isinf()), k
         assert torch.equal(v[v.isinf()].sign(), w[w.isinf()].sign()), k
+
+
+@pytest.mark.parametrize("N", [8, 16, 24, 64])
+@pytest.mark.parametrize("L", [5, 6, 7, 8])
+def test_infinity_in_the_last_step(gpu, N, L):
+    """An infinite last input reaches the last output only: no gradient of A goes
+    through its state."""
+    t, kw = make(1, L, 64, N, 1, F32, z=False, seed=34)
+    t["x"][0, L - 1, 3] = float("inf")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    dout = torch.randn(1, L, 64, generator=g, device="cuda")
+    want, mag = oracle(t, kw, dout=dout)
+    A = t["A"].detach().requires_grad_(True)
+    (dA,) = torch.autograd.grad(call({**t, "A": A}, kw), [A], dout)
+    assert bool(want["dA"].isfinite().all())
+    check("dA", dA, want["dA"], mag["dA"], bound(t))
