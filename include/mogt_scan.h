@@ -638,7 +638,9 @@ int mogt_split_ce_bwd(const void* A, int64_t lda, int64_t plane_a, int pieces_a,
  *   contiguous), dB, dC (bc_dtype, contiguous [batch, length, groups, states]),
  *   dA, dD, ddelta_bias and dinitial_state (fp32, their tensors' layouts).  Sums
  *   run in a fixed order: results do not change from run to run.  Takes batch x
- *   length x states below 2^31 and channels x states below 2^28.
+ *   length x states below 2^31 and channels x states below 2^28.  Its workspace is
+ *   4 batch (ceil(length / 4) states 64 ceil(channels / 64) + 2 length states groups
+ *   ceil(channels / groups / 64) + ceil(length / segment) channels (2 states + 3)) bytes.
  * mogt_ssm_step: one token per sequence (length 1; rows are addressed by the
  *   batch strides), `state` [batch, channels, states] updated in place.
  * No counterpart in the reference.                                          */

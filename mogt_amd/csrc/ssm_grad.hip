@@ -42,13 +42,20 @@ struct SsmBwd {
     const float* carries;      // [B, nseg, N, D]
     void *dx, *ddelta, *dz;    // [B, L, D], each may be null
     float* dh0;                // [B, D, N] or null
-    float* marks;              // [B, ceil(L / SSM_R), G nbk, N, 64]: of a 64-channel block, idle lanes too
+    float* marks;              // [B, ceil(L / SSM_R), ceil(D / 64), N, 64]: channel c at [c / 64][n][c % 64]
     float* part_g;             // [B, nseg, N, D]
     float* part_s;             // [B, nseg, D]
     float* part_bc;            // [G nbk][B][L][2][N]: dB, dC of a 64-channel block
     float* part_a;             // [B nseg][N + 2][D]: dA, dD, gradient of the bias
     int batch, nblk;
 };
+
+// Byte offset of a channel's first state in a row of marks.  The blocks go by the
+// channel's number, not by the wave: a group of few channels takes no more room.
+__device__ __forceinline__ uint32_t mark_offset(int c, int N) {
+    return (static_cast<uint32_t>(c >> 6) * static_cast<uint32_t>(N) * 64u + static_cast<uint32_t>(c & 63)) * 4u;
+}
+__host__ __device__ inline int64_t mark_row(int64_t D, int64_t N) { return (D + 63) / 64 * 64 * N; }
 
 // Sum of each of 32 values over the wave's lanes by halving steps; a lane gets
 // value 2 * (lane / 4) + lane % 2.
@@ -153,11 +160,10 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
     const TB* pB = static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0;
     const TB* pC = static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N + n0;
     const Rows rows(pB, p.Bs, pC, p.Cs, lane, left);
-    const int64_t block_marks = static_cast<int64_t>(gridDim.x) * p.N * 64;
-    float* pm = f.marks + (static_cast<int64_t>(b) * f.nblk + t0 / SSM_R) * block_marks +
-                (static_cast<int64_t>(blockIdx.x) * p.N + n0) * 64;
+    const int64_t row_marks = mark_row(p.D, p.N);
+    float* pm = f.marks + (static_cast<int64_t>(b) * f.nblk + t0 / SSM_R) * row_marks + n0 * 64;
     float* lds = s_rows + nb * Rows::ALL;
-    uint32_t lane4 = lane * 4u;
+    uint32_t mark = mark_offset(c, p.N);
     T xr[U], dr[U], zr[U], gr[U];
     float rv[Rows::E], S = 0.0f;
     auto load = [&](int t) {   // the rows of the block at t
@@ -196,11 +202,11 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_marks_kernel(SsmBwd f) {
         Rows::store(lds, lane, rv);
         ssm_wave_sync();
         load(t + U);
-        ssm_offset(lane4);
+        ssm_offset(mark);
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-            if (WHOLE || n < left) ssm_st<float>(pm + n * 64, lane4, h[n]);
-        pm += block_marks;
+        for (int n = 0; n < NS; ++n)   // idle lanes write the last channel's once more
+            if (WHOLE || n < left) ssm_st<float>(pm + n * 64, mark, h[n]);
+        pm += row_marks;
         float Bn[4], Cn[4];   // the next four values of B and C, read ahead
         ssm_lds4(lds, Bn);
         ssm_lds4(lds + NS, Cn);
@@ -338,7 +344,7 @@ void ssm_grad_kernel(SsmBwd f) {
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;
     const bool valid = ci < p.per;
     const int c = g * p.per + (valid ? ci : p.per - 1);
-    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)), lane4 = lane * 4u;
+    uint32_t off = static_cast<uint32_t>(c) * static_cast<uint32_t>(sizeof(T)), mark = mark_offset(c, p.N);
     const int seg = blockIdx.y, b = blockIdx.z;
     const int len = ssm_length(p, b);
     const int t0 = seg * p.seg, t1 = min(t0 + p.seg, p.L);
@@ -366,7 +372,8 @@ void ssm_grad_kernel(SsmBwd f) {
     const T* pz = static_cast<const T*>(p.z) + b * p.zb + t * p.zs;
     int64_t pg = (bl + t) * p.D;   // of dx, ddelta and dz
     const T* pdo = static_cast<const T*>(f.dout) + pg;
-    const float* pm = f.marks + (((static_cast<int64_t>(b) * f.nblk + t / R) * gridDim.x + blockIdx.x) * p.N + n0) * 64;
+    const int64_t row_marks = mark_row(p.D, p.N);
+    const float* pm = f.marks + (static_cast<int64_t>(b) * f.nblk + t / R) * row_marks + n0 * 64;
     const Rows rows(static_cast<const TB*>(p.B) + b * p.Bb + static_cast<int64_t>(g) * p.N + n0, p.Bs,
                     static_cast<const TB*>(p.C) + b * p.Cb + static_cast<int64_t>(g) * p.N + n0, p.Cs, lane, left);
     // dB, dC rows of this 64-channel block: a lane ends with value `mine` of
@@ -387,7 +394,7 @@ void ssm_grad_kernel(SsmBwd f) {
         constexpr bool FULL = decltype(full)::value;
         const int cnt = te - t;
         ssm_offset(off);
-        ssm_offset(lane4);
+        ssm_offset(mark);
 #pragma unroll
         for (int k = 0; k < OWN; ++k) {
             const int i = nb + k * NB, at = FULL && !SPLIT ? i : min(i, min(cnt, R) - 1);
@@ -398,12 +405,12 @@ void ssm_grad_kernel(SsmBwd f) {
         }
         rows.template load<FULL>(t, cnt, rv);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) hm[n] = WHOLE || n < left ? ssm_ld(pm + n * 64, lane4) : 0.0f;
+        for (int n = 0; n < NS; ++n) hm[n] = WHOLE || n < left ? ssm_ld(pm + n * 64, mark) : 0.0f;
         px -= R * p.xs;
         pd -= R * p.ds;
         pz -= R * p.zs;
         pdo -= static_cast<int64_t>(R) * p.D;
-        pm -= static_cast<int64_t>(gridDim.x) * p.N * 64;
+        pm -= row_marks;
     };
     auto load = [&](int t) {
         if (te - t >= R)
@@ -787,7 +794,7 @@ BwdSizes bwd_sizes(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G, int64_
     const int64_t nseg = L > 0 ? (L + segment - 1) / segment : 1;
     BwdSizes z;
     const int64_t ncb = G * ((D / G + 63) / 64);
-    z.marks = static_cast<size_t>(B * ((L + SSM_R - 1) / SSM_R) * N * ncb * 64);
+    z.marks = static_cast<size_t>(B * ((L + SSM_R - 1) / SSM_R) * mark_row(D, N));
     z.g = static_cast<size_t>(B * nseg * N * D);
     z.s = static_cast<size_t>(B * nseg * D);
     z.bc = static_cast<size_t>(2 * ncb * B * L * N);

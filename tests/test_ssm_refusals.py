@@ -219,3 +219,16 @@ def test_scan_refuses_what_its_backward_cannot_take(L, D, N, word):
             ops.ssm_scan(*a)
         with torch.no_grad():
             assert ops.ssm_scan(*a).shape == (1, L, D)
+
+
+@pytest.mark.parametrize("B,L,D,N,G,segment", [(1, 2048, 2048, 16, 1, 24), (1, 2048, 2048, 16, 256, 24),
+                                               (1, 2048, 2048, 16, 2048, 24), (2, 513, 768, 8, 1, 8),
+                                               (3, 7, 70, 17, 7, 8), (1, 0, 5, 3, 1, 8)])
+def test_gradient_workspace_goes_by_the_channels(B, L, D, N, G, segment):
+    """As documented: the states by the channels, however few a group has; sums by
+    the 64-channel blocks of the groups."""
+    states = -(-L // 4) * N * 64 * -(-D // 64)
+    sums = 2 * L * N * G * -(-(D // G) // 64)
+    segments = max(1, -(-L // segment)) * D * (2 * N + 3)
+    got = _lib.load().mogt_ssm_scan_bwd_workspace_bytes(B, L, D, N, G, segment)
+    assert got == 4 * B * (states + sums + segments)
