@@ -673,22 +673,30 @@ void ssm_grad_kernel(SsmBwd f) {
     }
 }
 
+// Work-groups in two dimensions: a launch takes fewer than 2^32 threads along x.
+inline dim3 wide_grid(int64_t groups, unsigned z = 1) {
+    const int64_t x = groups < (1 << 20) ? groups : 1 << 20;
+    return dim3(static_cast<unsigned>(x), static_cast<unsigned>((groups + x - 1) / x), z);
+}
+__device__ __forceinline__ int64_t wide_block() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // dB, dC [B, L, G, N]: the sums over the 64-channel blocks of a group, in order.
 template <typename TB>
 __global__ __launch_bounds__(256) void ssm_bc_kernel(const float* part, TB* dB, TB* dC, int64_t rows, int G, int nbk,
                                                      int N) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;   // (row, dB or dC, n) of one group
+    const int64_t i = wide_block() * 256 + threadIdx.x;   // (row, dB or dC, n) of one group
     const int64_t all = rows * 2 * N;
     if (i >= all) return;
-    const int g = blockIdx.y;
     const int64_t r = i / (2 * N);
     const int k = static_cast<int>(i - r * (2 * N));
     TB* out = k < N ? dB : dC;
     if (!out) return;
-    const float* q = part + static_cast<int64_t>(g) * nbk * all + i;
-    float s = 0.0f;
-    for (int m = 0; m < nbk; ++m) s += q[m * all];
-    out[(r * G + g) * N + (k < N ? k : k - N)] = IO<TB>::st(s);
+    for (int g = blockIdx.z; g < G; g += gridDim.z) {
+        const float* q = part + static_cast<int64_t>(g) * nbk * all + i;
+        float s = 0.0f;
+        for (int m = 0; m < nbk; ++m) s += q[m * all];
+        out[(r * G + g) * N + (k < N ? k : k - N)] = IO<TB>::st(s);
+    }
 }
 
 // Column sums over rows of [rows][K][D], in a fixed order: a work-group takes 64
@@ -698,7 +706,7 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* part, fl
                                                            int64_t cols, int64_t D, int64_t N) {
     __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    const int64_t i = wide_block() * 64 + lane;
     float v = 0.0f;
     if (i < cols)
         for (int64_t r = w; r < rows; r += 16) v += part[r * cols + i];
@@ -720,7 +728,7 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* part, fl
 int column_sums(const float* part, float* a, float* b, float* c, int64_t rows, int64_t K, int64_t D, int64_t N,
                 hipStream_t st) {
     const int64_t cols = K * D;
-    column_sums_kernel<<<static_cast<unsigned>((cols + 63) / 64), 1024, 0, st>>>(part, a, b, c, rows, cols, D, N);
+    column_sums_kernel<<<wide_grid((cols + 63) / 64), 1024, 0, st>>>(part, a, b, c, rows, cols, D, N);
     return check_launch("column sums");
 }
 
@@ -825,7 +833,7 @@ extern "C" int mogt_ssm_scan_bwd(const mogt_ssm_problem* q, const void* dout, co
     if (q->batch == 0 || q->channels == 0) return MOGT_OK;
     if (!carries || !q->A || (q->length > 0 && !dout)) return set_error(MOGT_E_INVALID, "null input pointer");
     if (out->dz && !q->z) return set_error(MOGT_E_INVALID, "a gradient of z without z");
-    // one-dimensional grids of the sums
+    // a row of marks has 32-bit offsets
     if (q->batch * q->length * q->states >= (1ll << 31) || q->channels * q->states >= (1ll << 28))
         return set_error(MOGT_E_INVALID, "batch x length x states below 2^31 and channels x states below 2^28 expected");
     const BwdSizes n = bwd_sizes(q->batch, q->length, q->channels, q->states, q->groups, q->segment);
@@ -857,7 +865,8 @@ extern "C" int mogt_ssm_scan_bwd(const mogt_ssm_problem* q, const void* dout, co
     if (const int rc = check_launch("mogt_ssm_scan_bwd")) return rc;
     const int64_t rows = q->batch * q->length;
     if (f.part_bc && rows > 0) {
-        const dim3 grid(static_cast<unsigned>((rows * 2 * q->states + 255) / 256), static_cast<unsigned>(q->groups));
+        const dim3 grid = wide_grid((rows * 2 * q->states + 255) / 256,
+                                    static_cast<unsigned>(q->groups < 65535 ? q->groups : 65535));
         if (q->bc_dtype == MOGT_F32)
             ssm_bc_kernel<float><<<grid, 256, 0, st>>>(bc, static_cast<float*>(out->dB), static_cast<float*>(out->dC),
                                                        rows, static_cast<int>(q->groups), f.a.nbk, f.a.N);

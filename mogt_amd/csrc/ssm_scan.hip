@@ -392,6 +392,12 @@ int ssm_args(const mogt_ssm_problem* q, bool step, SsmArgs& a) {
     // 32-bit steps and channels in the kernels; batch and segments are grid dimensions
     if (q->length >= (1ll << 30) || q->channels >= (1ll << 24) || q->batch > 65535)
         return set_error(MOGT_E_INVALID, "batch up to 65535, length below 2^30, channels below 2^24 expected");
+    // fewer than 2^32 threads along x; the gradient's work-groups have up to 5 waves for 17 to 40 states
+    const int64_t blocks = q->groups * ((q->channels / q->groups + 63) / 64);
+    const int64_t waves = q->states <= 16 ? 1 : q->states <= 40 ? (q->states + 7) / 8 : (q->states + 15) / 16;
+    if (!step && blocks * 64 * waves >= (1ll << 32))
+        return set_error(MOGT_E_INVALID, "%lld blocks of a group's 64 channels with %lld states: too many for a launch",
+                         (long long)blocks, (long long)q->states);
     if (q->batch == 0 || q->channels == 0) return MOGT_OK;
     if (q->length > 0) {
         if (!q->x || !q->delta || !q->A || !q->B || !q->C) return set_error(MOGT_E_INVALID, "null input pointer");

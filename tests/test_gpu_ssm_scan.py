@@ -515,3 +515,34 @@ def test_infinity_in_the_last_step(gpu, N, L):
     (dA,) = torch.autograd.grad(call({**t, "A": A}, kw), [A], dout)
     assert bool(want["dA"].isfinite().all())
     check("dA", dA, want["dA"], mag["dA"], bound(t))
+
+
+def test_a_group_for_every_channel(gpu):
+    """More groups than a grid's second dimension holds."""
+    announce("ssm_scan 65600 groups")
+    t, kw = make(1, 3, 65600, 2, 65600, F32, seed=35)
+    run_both(t, kw, tol=(64 + 4 * (3 + 2 + 1)) * U)
+
+
+def test_the_most_channels(gpu):
+    """Sums of more columns than one dimension of a launch takes: the channels'
+    gradients are those of a call on a part of them."""
+    announce("ssm_scan 16700032 channels")
+    D, N, part = 16_700_032, 15, 64_000
+    g = torch.Generator(device="cuda").manual_seed(36)
+    x, delta, dout = (torch.randn(1, 1, D, generator=g, device="cuda") for _ in range(3))
+    A = torch.rand(D, N, generator=g, device="cuda").neg_()
+    B, C = (torch.randn(1, 1, N, generator=g, device="cuda") for _ in range(2))
+    skip, bias = (torch.randn(D, generator=g, device="cuda") for _ in range(2))
+
+    def grads(at):
+        from mogt_amd import ops
+        leaves = [v[at].detach().requires_grad_(True) for v in (A, skip, bias)]
+        out = ops.ssm_scan(x[..., at], delta[..., at], leaves[0], B, C, D=leaves[1], delta_bias=leaves[2],
+                           delta_softplus=True, initial_state=torch.ones_like(leaves[0])[None])
+        return torch.autograd.grad(out, leaves, dout[..., at])
+
+    whole = grads(slice(None))
+    for at in (slice(0, part), slice(D - part, D)):
+        for a, b in zip(whole, grads(at)):
+            assert torch.equal(a[at], b)

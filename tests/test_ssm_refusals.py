@@ -232,3 +232,10 @@ def test_gradient_workspace_goes_by_the_channels(B, L, D, N, G, segment):
     segments = max(1, -(-L // segment)) * D * (2 * N + 3)
     got = _lib.load().mogt_ssm_scan_bwd_workspace_bytes(B, L, D, N, G, segment)
     assert got == 4 * B * (states + sums + segments)
+
+
+def test_scan_entry_refuses_more_blocks_than_a_launch_takes():
+    lib = _lib.load()
+    p = scan_problem(channels=(1 << 24) - 1, groups=(1 << 24) - 1, states=128)
+    assert lib.mogt_ssm_scan_fwd(ctypes.byref(p), 64, None, None, None, 0, None) == -1
+    assert b"launch" in lib.mogt_last_error()
