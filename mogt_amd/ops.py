@@ -2485,6 +2485,14 @@ def _check_lengths(what: str, lengths: torch.Tensor, B: int) -> None:
         raise ValueError(f"{what}: lengths must be int32 or int64, got {lengths.dtype}")
 
 
+def _check_real(what: str, **params) -> None:
+    """Parameters are taken in float32; the cast of a complex one would drop its
+    imaginary part."""
+    for name, t in params.items():
+        if t is not None and not t.is_floating_point():
+            raise ValueError(f"{what}: {name} must be real floating point, got {t.dtype}")
+
+
 def _float32(t: torch.Tensor | None) -> torch.Tensor | None:
     return t if t is None or t.dtype == torch.float32 else t.float()
 
@@ -2607,6 +2615,7 @@ def _check_conv(what: str, x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     if not 1 <= weight.shape[1] <= CONV_MAX_TAPS:
         raise ValueError(f"{what}: {weight.shape[1]} taps not supported (1 to {CONV_MAX_TAPS})")
     _check_shape(what, "bias", bias, (D,))
+    _check_real(what, weight=weight, bias=bias)
     if activation not in (None, "silu"):
         raise ValueError(f"{what}: activation {activation!r} not supported (None or 'silu')")
     if state is not None:
@@ -2838,6 +2847,7 @@ def _check_ssm(what: str, x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor,
                 raise ValueError(f"{what}: {name} must have x's dtype {dtype}, got {t.dtype}")
     _check_shape(what, "D", D, (ch,))
     _check_shape(what, "delta_bias", delta_bias, (ch,))
+    _check_real(what, A=A, D=D, delta_bias=delta_bias)
     if state is not None:
         _check_shape(what, "state", state, (rows[0], ch, N))
         if state.dtype != torch.float32:

@@ -239,3 +239,31 @@ def test_scan_entry_refuses_more_blocks_than_a_launch_takes():
     p = scan_problem(channels=(1 << 24) - 1, groups=(1 << 24) - 1, states=128)
     assert lib.mogt_ssm_scan_fwd(ctypes.byref(p), 64, None, None, None, 0, None) == -1
     assert b"launch" in lib.mogt_last_error()
+
+
+@pytest.mark.parametrize("name", ["A", "D", "delta_bias"])
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.int32, torch.bool])
+def test_scan_refuses_parameters_that_are_not_real(name, dtype):
+    """A complex spectrum among them: a cast would run without its imaginary part."""
+    with FakeTensorMode():
+        shape = (8, 4) if name == "A" else (8,)
+        a = scan_args(**{name: lambda e: e(*shape, dtype=dtype)})
+        args = [a.pop(k) for k in ("x", "delta", "A", "B", "C")]
+        with pytest.raises(ValueError, match=f"{name} must be real"):
+            ops.ssm_scan(*args, **a)
+        one = dict(x=args[0][:, 0], delta=args[1][:, 0], A=args[2], B=args[3][:, 0], C=args[4][:, 0], D=a["D"],
+                   delta_bias=a["delta_bias"], state=a["initial_state"])
+        with pytest.raises(ValueError, match=f"{name} must be real"):
+            ops.ssm_step(**one)
+
+
+@pytest.mark.parametrize("name", ["weight", "bias"])
+def test_conv_refuses_parameters_that_are_not_real(name):
+    with FakeTensorMode():
+        e = lambda *s, dtype=torch.float32: torch.empty(*s, device="cuda", dtype=dtype)  # noqa: E731
+        p = dict(weight=e(8, 4), bias=e(8))
+        p[name] = p[name].to(torch.complex64)
+        with pytest.raises(ValueError, match=f"{name} must be real"):
+            ops.short_conv(e(2, 5, 8), **p)
+        with pytest.raises(ValueError, match=f"{name} must be real"):
+            ops.short_conv_step(e(2, 8), e(2, 3, 8), **p)
