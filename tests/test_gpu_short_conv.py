@@ -262,3 +262,37 @@ def test_negated_gradient_of_the_state(gpu):
                                          list(d)) for d in ((a, b), (a.resolve_neg(), b.resolve_neg())))
         for k, u, v in zip(leaves, got, want):
             assert torch.equal(u, v), k
+
+
+def test_lengths_of_four_bytes(gpu):
+    t, n = make(3, 40, 32, 4, lengths=[40, 13, 0], seed=12)
+    assert n.dtype == torch.int64
+    wide, narrow = run_both(t, n, True), run_both(t, n.int(), True)
+    for a, b in zip((*wide[:2], *wide[2].values()), (*narrow[:2], *narrow[2].values())):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("K", [2, 3, 4, 5, 8])
+@pytest.mark.parametrize("B,L,D,dtype", [(32, 347, 130, F32), (32, 701, 130, BF16), (32, 517, 260, F32),
+                                         (16, 1029, 520, BF16)])
+def test_walks_of_several_blocks(gpu, B, L, D, K, dtype):
+    """Enough waves for walks of 16 and 32 steps (two and four blocks), of single
+    channels and of 16-byte vectors, with a last vector block that is not full
+    and sequences that end inside a walk; in the backward more than the 128
+    steps of a work-group.  Bounds as above, with the steps' term for the sums
+    over steps only."""
+    announce(f"short_conv walks B={B} L={L} D={D} K={K} {dtype}")
+    lengths = [L, 0, 1, K, 31, 33, 128, 129, L - 1] + [L - 7 * i for i in range(1, B - 8)]
+    t, n = make(B, L, D, K, dtype, lengths=lengths, seed=K)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    dy = torch.randn(B, L, D, generator=g, device="cuda").to(dtype)
+    ds = torch.randn(B, K - 1, D, generator=g, device="cuda").to(dtype)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    y, state = call(leaves, n, True, return_state=True)
+    grads = torch.autograd.grad([y, state], list(leaves.values()), [dy, ds])
+    kw = dict(silu=True, initial_state=t["initial_state"], lengths=n, dy=dy, dstate=ds)
+    want, mag = (so.short_conv(t["x"], t["weight"], t["bias"], **kw, mag=m) for m in (False, True))
+    assert torch.equal(state.double().cpu(), want["state"])
+    for k, v in {"y": y, **{"d" + k: v for k, v in zip(leaves, grads)}}.items():
+        steps = B * L if k in ("dweight", "dbias") else 0
+        check(k, v, want[k], mag[k], (32 * (K + 1) + 8 + steps) * 2.0 ** -24)

@@ -546,3 +546,65 @@ def test_the_most_channels(gpu):
     for at in (slice(0, part), slice(D - part, D)):
         for a, b in zip(whole, grads(at)):
             assert torch.equal(a[at], b)
+
+
+@pytest.mark.parametrize("N", [8, 16, 24, 64])
+def test_float32_rows_of_b_and_c_beside_bf16(gpu, N):
+    """Gradients and steps with B and C in fp32 and the other rows in bf16."""
+    from mogt_amd import ops
+    announce(f"ssm_scan fp32 B and C beside bf16, N={N}")
+    t, kw = make(2, 21, 66, N, 1, BF16, seed=N + 1)
+    g = torch.Generator(device="cuda").manual_seed(N)
+    t["B"], t["C"] = (torch.randn(2, 21, 1, N, generator=g, device="cuda") for _ in range(2))
+    run_both(t, kw)
+    state = t["initial_state"].clone()
+    one = {k: t[k][:, 0] for k in ("x", "delta", "B", "C", "z")}
+    out = ops.ssm_step(one["x"], state, one["delta"], t["A"], one["B"], one["C"], D=t["D"], z=one["z"],
+                       delta_bias=t["delta_bias"], delta_softplus=True)
+    first = {k: v[:, :1] if k in one else v for k, v in t.items()}
+    want, mag = oracle(first, kw)
+    check("out", out[:, None], want["out"], mag["out"], bound(first))
+    check("state", state, want["state"], mag["state"], bound(first))
+
+
+def test_lengths_of_eight_bytes(gpu):
+    t, kw = make(3, 30, 64, 16, 1, F32, lengths=[30, 0, 13], seed=32)
+    wide = dict(kw, lengths=kw["lengths"].long())
+    for a, b in zip(run_once_all(t, wide), run_once_all(t, kw)):
+        assert torch.equal(a, b)
+    run_both(t, wide)
+
+
+def roundings(name, t):
+    """The sums an output really runs over: states for all, channels for dB and
+    dC, the batch's steps for what channels share, and twice the steps for the
+    product of decays that every state and gradient of a state carries."""
+    B, L, D = t["x"].shape
+    n = 64 + 4 * t["A"].shape[1] + 2 * L
+    return (n + (4 * D if name in ("dB", "dC") else 4 * B * L if name in ("dA", "dD", "ddelta_bias") else 0)) * U
+
+
+@pytest.mark.parametrize("segment", [24, 56, 304])
+@pytest.mark.parametrize("N,G,dtype", [(8, 1, F32), (16, 1, BF16), (12, 2, F32), (24, 1, BF16), (40, 1, F32),
+                                       (64, 1, BF16), (128, 2, F32)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_segments_of_several_blocks(gpu, monkeypatch, segment, N, G, dtype, ragged):
+    """Long calls walk many blocks of steps a segment, short ones a single one:
+    here 3, 7 and all of them, with a last block that is not full, a channel
+    block that is not full, and sequences that end inside a later block, at a
+    segment's end and one step past it."""
+    from mogt_amd import ops
+    announce(f"ssm_scan segments of {segment} N={N} G={G} {dtype} ragged={ragged}")
+    monkeypatch.setattr(ops, "SSM_MIN_SEGMENT", segment)
+    lengths = [151, 93, 56, 25] if ragged else None
+    t, kw = make(4 if ragged else 1, 151, 70, N, G, dtype, lengths=lengths, seed=segment + N)
+    assert ops._ssm_segment(*t["x"].shape, N, G) == segment
+    g = torch.Generator(device="cuda").manual_seed(1)
+    dout = torch.randn(t["x"].shape, generator=g, device="cuda").to(dtype)
+    dstate = torch.randn(t["initial_state"].shape, generator=g, device="cuda")
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    out, state = call(leaves, kw, return_state=True)
+    grads = torch.autograd.grad([out, state], list(leaves.values()), [dout, dstate])
+    want, mag = oracle(t, kw, dout=dout, dstate=dstate)
+    for k, v in {"out": out, "state": state, **{"d" + k: v for k, v in zip(leaves, grads)}}.items():
+        check(k, v, want[k], mag[k], roundings(k, t))
