@@ -2770,6 +2770,9 @@ def _ssm_scan_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, x: torch.
     b, L, ch = x.shape
     N, G = A.shape[1], B.shape[2]
     segment = _ssm_segment(b, L, ch, N, G)
+    if carries.shape != (b, max(1, -(-L // segment)), N, ch):
+        raise ValueError(f"ssm_scan_grad: carries {list(carries.shape)} are not those of a forward over segments of "
+                         f"{segment} steps")
     dout = _dense(dout if dout.dtype == x.dtype else dout.to(x.dtype))
     dfinal = None if dfinal is None else dfinal.to(torch.float32).contiguous()
     p, held = _ssm_problem(x, delta, A, B, C, D, z, delta_bias, None, lengths, softplus, segment)

@@ -267,3 +267,13 @@ def test_conv_refuses_parameters_that_are_not_real(name):
             ops.short_conv(e(2, 5, 8), **p)
         with pytest.raises(ValueError, match=f"{name} must be real"):
             ops.short_conv_step(e(2, 8), e(2, 3, 8), **p)
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 4, 8), (1, 4, 4, 8), (0,), (1, 3, 8, 4)])
+def test_gradient_refuses_the_carries_of_other_segments(shape):
+    """17 steps are three segments of 8: the kernels would read past fewer."""
+    e = torch.zeros
+    assert ops._ssm_segment(1, 17, 8, 4, 1) == 8
+    with pytest.raises(ValueError, match="carries"):
+        ops._ssm_scan_grad_op.impl(e(1, 17, 8), None, e(1, 17, 8), e(1, 17, 8), e(8, 4), e(1, 17, 1, 4), e(1, 17, 1, 4),
+                                   None, None, None, None, e(*shape), False, [True] * 5 + [False] * 3 + [True])
