@@ -608,3 +608,35 @@ def test_segments_of_several_blocks(gpu, monkeypatch, segment, N, G, dtype, ragg
     want, mag = oracle(t, kw, dout=dout, dstate=dstate)
     for k, v in {"out": out, "state": state, **{"d" + k: v for k, v in zip(leaves, grads)}}.items():
         check(k, v, want[k], mag[k], roundings(k, t))
+
+
+@pytest.mark.parametrize("z,softplus", [(True, True), (False, False)])
+def test_gradients_are_the_definitions_differences(gpu, z, softplus):
+    """Each gradient along a random direction against the four-point quotient of
+    the float64 definition, to the kernel's roundings, 1e-5 of the magnitudes, and a
+    twentieth of them for the quotient.  Its steps of 1e-5 leave 1e-20 / 30 of the
+    fifth derivative: a decay's exponent changes by at most |A way| <= 16 a step, 384
+    over 24 steps, whose fifth power is 8e12: 3e-9 of the magnitudes, which the
+    slopes of softplus and gate, of order one, change little.  Its own roundings are
+    (24 + 16 + 768) 2^-53 of the loss's magnitudes, over 1e-5: 1e-8 of them."""
+    t, kw = make(1, 24, 32, 16, z=z, softplus=softplus, seed=37)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    dout = torch.randn(1, 24, 32, generator=g, device="cuda")
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None}
+    grads = torch.autograd.grad(call({**t, **leaves}, kw), list(leaves.values()), dout)
+    _, mag = oracle(t, kw, dout=dout)
+    wide = {k: None if v is None else v.double().cpu() for k, v in t.items()}
+
+    def value(k, s, way):
+        u = {**wide, k: wide[k] + s * way}
+        r = so.ssm_scan(*(u[n] for n in ("x", "delta", "A", "B", "C")),
+                        **{n: u[n] for n in ("D", "z", "delta_bias", "initial_state")}, **kw)
+        return float((r["out"] * dout.double().cpu()).sum())
+
+    for k, v in zip(leaves, grads):
+        way = torch.randn(v.shape, generator=g, device="cuda").double().cpu().clamp(-4, 4)
+        s = 1e-5
+        quotient = (8 * (value(k, s, way) - value(k, -s, way)) - (value(k, 2 * s, way) - value(k, -2 * s, way))) / (12 * s)
+        along = float((v.double().cpu() * way).sum())
+        limit = 1.05 * roundings("d" + k, t) * float((mag["d" + k] * way.abs()).sum())
+        assert abs(along - quotient) <= limit, (k, along, quotient, limit)
