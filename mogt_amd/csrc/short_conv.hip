@@ -14,9 +14,10 @@
 // The backward forms s again instead of keeping it.
 // Measured, bf16, 4 taps: 32768 steps of 2048 channels 57 us (4.7 TB/s of the
 // 5.2 that a large copy reaches here), 200 of 768 fp32 4.1; 4 x 4095 of 1280
-// forward 21 us, backward 36 (3.5 TB/s: its arithmetic, 4 taps three times and
-// the gate's slope, is near as long) and 3.8 for the sums; one token of 256
-// sequences of 2048 channels 5.0 us, of one 3.0.
+// forward 23 us, backward 38 (3.3 TB/s; its vector instructions, 4 taps three
+// times and the gate's slope, take 53 % of the cycles at 1.6 waves a SIMD, so
+// neither memory nor the vector unit is full) and 3.8 for the sums; one token of
+// 256 sequences of 2048 channels 5.3 us, of one 2.8.
 #include <initializer_list>
 
 #include "common.h"
@@ -317,8 +318,9 @@ namespace {
 int conv_steps(int64_t B, int64_t L, int64_t D, int vec) {
     // steps a wave walks: at most 32 (rows in front are read again), fewer
     // where the GPU would otherwise hold under 8 waves per CU.  Of 8, 16 and 32
-    // steps, 200 of 768 channels take 3.9, 5.2 and 7.4 us, 2048 of 2048 8.0, 11
-    // and 14, 4 x 4095 of 1280 24, 20.4 and 22, 32768 of 2048 56, 60 and 49.
+    // steps, 200 of 768 channels fp32 take 4.2, 5.5 and 8.0 us, in bf16 2048 of 2048
+    // 9.2, 12.8 and 16.4, 4 x 4095 of 1280 26.5, 23.7 and 25.3, 32768 of 2048 64.4,
+    // 65 and 59.9 (one card, contiguous rows that rotate through 1.5 GB).
     const int64_t waves = B * ((D + 64 * vec - 1) / (64 * vec));
     int64_t s = 32;
     while (s > 8 && waves * ((L + s - 1) / s) < 2048) s /= 2;

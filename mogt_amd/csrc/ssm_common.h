@@ -177,8 +177,9 @@ typedef float ssm_f4 __attribute__((ext_vector_type(4)));
 
 // softplus(v) = max(v, 0) + log(1 + e) with e = exp(-|v|) <= 1: for the rounded
 // u = 1 + e the part that u lost, e - (u - 1), is added to log(u), which keeps
-// small results (v far below zero) exact to a few ulp.  No selects: infinities
-// and NaN pass as in the definition.
+// small results (v far below zero) as exact as e is: |v| + 2 half steps, one per
+// unit of the rounded product |v| log2(e).  No selects: infinities and NaN pass as
+// in the definition.
 __device__ __forceinline__ float ssm_softplus(float v) {
     const float e = __builtin_amdgcn_exp2f(fabsf(v) * -SSM_LOG2E);
     const float u = 1.0f + e;

@@ -17,11 +17,11 @@
 //           runs through it.
 //   sums    over the 64-channel blocks of a group (dB, dC) and over segments
 //           and sequences (dA, dD, bias), in a fixed order.
-// 2 x 8192 steps of 1280 channels with 16 states, bf16: marks 124 us (4.1 TB/s:
-// near the 5.2 of a large copy), carry 16, grad 302 (2.2 TB/s), sums 12 and 10.
-// Bound of grad: the vector unit at two waves a SIMD, which is what a block's
-// states leave room for: 21 vector instructions per state and step, 14 of them the
-// formulas' and 3 the sums over channels.  Marks every 8 steps, 8 states a wave (85
+// 2 x 8192 steps of 1280 channels with 16 states, bf16: marks 123 us (4.1 TB/s:
+// near the 5.2 of a large copy), carry 16, grad 305 (2.2 TB/s), sums 12 and 10.
+// Bound of grad: the vector unit (69 % of the cycles) at two waves a SIMD, which is
+// what a block's states leave room for: 21 vector instructions per state and step,
+// 14 of them the formulas' and 3 the sums over channels.  Marks every 8 steps, 8 states a wave (85
 // instead of 62 us at 4096 x 1024) and three waves a SIMD with a part of the states
 // in scratch memory were slower; forming all decays twice to load the next block
 // earlier changed nothing.
@@ -337,8 +337,9 @@ void ssm_grad_kernel(SsmBwd f) {
     float* s_part = s_chan + 2 * R * 3 * 64;
     float* s_rows = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + nb * Rows::ALL;
     float* s_prod = smem + (SPLIT ? (2 + NB) * R * 3 * 64 : 0) + NB * Rows::ALL + nb * (GRAD_ROWS * ROW);
-    // a step's products are summed while the next ones are formed (331 us instead of
-    // 354, one card): two buffers, for which only a work-group of one wave has the room
+    // a step's products are summed while the next ones are formed (2 x 8192 x 1280: 324
+    // us instead of 334, one card): two buffers, for which only a work-group of one wave
+    // has the room
     constexpr bool BEHIND = VIA_LDS && !SPLIT;
     const int g = blockIdx.x / p.nbk;
     const int ci = (blockIdx.x - g * p.nbk) * 64 + lane;

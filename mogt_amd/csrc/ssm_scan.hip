@@ -16,10 +16,10 @@
 // an exponential, a product and a multiply-add, and one more multiply-add for the
 // output; the two launches form the exponentials twice (holding them, N fp32
 // values per element of x, would cost N/4 times the bytes of every input
-// together).  32768 steps of 2048 channels with 16 states, bf16: sums 196 us,
-// carry 13, out 261, with 5.0 and 6.8 vector instructions per state and step (4
-// and 5 of them the above) and an instruction issued in over 90 % of the cycles;
-// the bytes alone would take 103.  B and C as scalar operands, two channels a
+// together).  32768 steps of 2048 channels with 16 states, bf16: sums 194 us,
+// carry 13, out 257, with 5.0 and 6.8 vector instructions per state and step (4
+// and 5 of them the above), which at 4 cycles each and 8 an exponential add up to
+// 94 % of the cycles; the bytes alone would take 103.  B and C as scalar operands, two channels a
 // lane, the matrix unit for w B, and one launch of longer work-groups for short
 // sequences were all slower.
 #include <type_traits>
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 64) void ssm_out_kernel(SsmFwd f) {
 // single token: four lanes per channel, each four consecutive states of every
 // sixteen (VEC: states in whole aligned quads) or every fourth state.  Bound by
 // reading and writing the states (a server's batch) or by latency (one sequence):
-// 256 sequences of 2048 channels with 16 states 16.3 us (4.3 TB/s), one 3.3.  By
+// 256 sequences of 2048 channels with 16 states 16.6 us (4.3 TB/s), one 3.1.  By
 // single states the 256 take 33.6 us.  Four sequences a thread, which share A, were no
 // faster at any batch (19.0 us for the 256, 5.1 against 3.7 for 16).
 // ---------------------------------------------------------------------------

@@ -2687,7 +2687,8 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
 # GPU (1024 SIMDs) with more waves and end closer together, but leave more states
 # to carry: kernels over 32768 steps of 2048 channels with 16 states take 526, 438,
 # 437 and 428 us with segments for 2048, 4096, 6144 and 8192 waves, forward and
-# gradients of 2 x 8192 steps of 1280 channels 617, 599, 573 and 587.
+# gradients of 2 x 8192 steps of 1280 channels 617, 599, 573 and 587.  Measured at
+# 8 and 16 states; more states carry more bytes per segment.
 SSM_WAVES = 6144
 # Shorter segments than that asks for where a call has few waves: 200 steps of
 # 1280 channels take 15.0 us in segments of 8, 18.9 of 16 and 28.4 of 32.
@@ -2695,7 +2696,7 @@ SSM_MIN_SEGMENT = 8
 
 
 def _ssm_segment(B: int, L: int, D: int, N: int, G: int) -> int:
-    """Steps of a segment (a multiple of 8)."""
+    """Steps of a segment (a multiple of 8); waves counted as of 16 states."""
     waves = max(1, B * G * -(-(D // G) // 64) * (-(-N // 16) if N > 16 else 1))
     return max(SSM_MIN_SEGMENT, 8 * -(-L // (8 * max(1, SSM_WAVES // waves))))
 
