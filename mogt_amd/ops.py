@@ -2892,11 +2892,13 @@ def ssm_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
     Differentiable in every tensor but ``lengths``, through both outputs; the
     gradients do not change from run to run.  ``A`` must be finite, of either
     sign: states and gradients are in range as far as fp32 is, whatever they grow
-    by over a sequence (one step's ``exp(dt A)`` is an fp32 number).  The backward's
-    workspace holds a state every 4 steps (B L D N bytes, D rounded up to 64),
-    8 B L N bytes of sums for every 64 channels of a group (or part of them) and
-    8 N + 12 bytes per channel and segment, a multiple of 8 steps that grows with
-    the call; the states entering the segments (4 N bytes per channel) are kept
+    by over a sequence (one step's ``exp(dt A)`` is an fp32 number); what an
+    infinite input reaches is infinite or NaN, nothing else changes by it.
+    Parameters are real and taken in float32.  The backward's workspace holds a
+    state every 4 steps (B L D N bytes, D rounded up to 64), 8 B L N bytes of sums
+    for every 64 channels of a group (or part of them) and 8 N + 12 bytes per
+    channel and segment, a multiple of 8 steps that grows with the call; the
+    states entering the segments (4 N bytes per channel and segment) are kept
     from the forward to the backward."""
     if x.ndim != 3:
         raise ValueError("ssm_scan: x must be [B, L, D]")
