@@ -699,6 +699,60 @@ int mogt_short_conv_bwd(const mogt_short_conv_problem* problem, const void* dy, 
                         size_t workspace_bytes, void* stream);
 int mogt_short_conv_step(const mogt_short_conv_problem* problem, void* state, void* y, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Linear attention with a decay for each head: per sequence and head h
+ *   S_t = exp(g_t[h]) S_{t-1} + k_t v_t^T,  S_{-1} = initial_state,  o_t = scale S_t^T q_t
+ * with an fp32 state [key_dim, value_dim] and fp32 sums; o is rounded once.  q and k
+ * (io_dtype) are [batch, length, groups, key_dim], v [batch, length, heads, value_dim],
+ * with unit stride in a head's row and the given row, batch and head strides in
+ * elements; heads / groups consecutive heads share a group's q and k.  log_decay g is
+ * fp32 at its own strides (g_row 0: one for all steps).  initial_state and lengths may
+ * be null; states [batch, heads, key_dim, value_dim] are contiguous fp32.  lengths
+ * [batch] (4- or 8-byte integers, clamped to [0, length]): steps past a sequence's
+ * length are not read, leave the state as it is and write zero.  Outputs and the
+ * workspace must not overlap each other or the inputs.  Widths 1 to
+ * MOGT_LINEAR_ATTN_MAX_DIM, batch at most 21845, heads at most 65535.
+ *
+ * `segment` (a multiple of 64 for bf16, of 32 for fp32): steps of one work-group.
+ * Workspaces are scratch (no initial content, free again once the call's work has
+ * run); their size is 0 for a problem that the call refuses.
+ * mogt_linear_attn_fwd: out [batch, length, heads, value_dim] contiguous;
+ *   final_state may be null; `carries` (may be null) [batch, heads, segments + 1,
+ *   key_dim, value_dim] receives the states entering the segments and the final
+ *   one, which the backward takes.
+ * mogt_linear_attn_bwd: from the same problem (and segment), the forward's carries,
+ *   dout (io_dtype, contiguous) and dfinal_state (may be null) the gradients, each
+ *   of which may be null: dq, dk [batch, length, groups, key_dim], dv [batch,
+ *   length, heads, value_dim] (io_dtype, contiguous), dlog_decay (fp32, [batch,
+ *   length, heads], or [heads] where decay_per_head is set) and dinitial_state.
+ *   Sums run in a fixed order: results do not change from run to run.
+ * mogt_linear_attn_step: one token per sequence (length 1; row strides are not
+ *   used), `state` updated in place, out [batch, heads, value_dim].
+ * No counterpart in the reference.                                          */
+#define MOGT_LINEAR_ATTN_MAX_DIM 128
+typedef struct mogt_linear_attn_problem {
+    int64_t batch, length, heads, groups, key_dim, value_dim, segment;
+    int io_dtype, lengths_bytes, decay_per_head;
+    float scale;
+    const void *q, *k, *v;
+    const float *log_decay, *initial_state;
+    const void* lengths;
+    int64_t q_row, q_batch, q_head, k_row, k_batch, k_head, v_row, v_batch, v_head;
+    int64_t g_row, g_batch, g_head;
+} mogt_linear_attn_problem;
+typedef struct mogt_linear_attn_gradients {
+    void *dq, *dk, *dv;
+    float *dlog_decay, *dinitial_state;
+} mogt_linear_attn_gradients;
+size_t mogt_linear_attn_workspace_bytes(const mogt_linear_attn_problem* problem);
+int mogt_linear_attn_fwd(const mogt_linear_attn_problem* problem, void* out, float* final_state, float* carries,
+                         void* workspace, size_t workspace_bytes, void* stream);
+size_t mogt_linear_attn_bwd_workspace_bytes(const mogt_linear_attn_problem* problem);
+int mogt_linear_attn_bwd(const mogt_linear_attn_problem* problem, const void* dout, const float* dfinal_state,
+                         const float* carries, const mogt_linear_attn_gradients* gradients, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

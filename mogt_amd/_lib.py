@@ -19,7 +19,7 @@ MOGT_F64 = 2
 MOGT_F16 = 3
 MOGT_CONN_EXP = 0
 MOGT_CONN_CAYLEY = 1
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _c_void_p = ctypes.c_void_p
 _c_i64 = ctypes.c_int64
@@ -44,12 +44,28 @@ class SsmProblem(ctypes.Structure):
 SSM_PROBLEM = struct.Struct("@6q4i10P10q")
 SSM_GRADIENTS = struct.Struct("@9P")
 SHORT_CONV_PROBLEM = struct.Struct("@4q3i5P2q")
+LINEAR_ATTN_PROBLEM = struct.Struct("@7q3if6P12q")
+LINEAR_ATTN_GRADIENTS = struct.Struct("@5P")
 
 
 class SsmGradients(ctypes.Structure):
     """``mogt_ssm_gradients`` of include/mogt_scan.h."""
     _fields_ = [(n, _c_void_p) for n in ("dx", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias",
                                          "dinitial_state")]
+
+
+class LinearAttnProblem(ctypes.Structure):
+    """``mogt_linear_attn_problem`` of include/mogt_scan.h."""
+    _fields_ = ([(n, _c_i64) for n in ("batch", "length", "heads", "groups", "key_dim", "value_dim", "segment")]
+                + [(n, _c_int) for n in ("io_dtype", "lengths_bytes", "decay_per_head")] + [("scale", _c_float)]
+                + [(n, _c_void_p) for n in ("q", "k", "v", "log_decay", "initial_state", "lengths")]
+                + [(n, _c_i64) for n in ("q_row", "q_batch", "q_head", "k_row", "k_batch", "k_head", "v_row", "v_batch",
+                                         "v_head", "g_row", "g_batch", "g_head")])
+
+
+class LinearAttnGradients(ctypes.Structure):
+    """``mogt_linear_attn_gradients`` of include/mogt_scan.h."""
+    _fields_ = [(n, _c_void_p) for n in ("dq", "dk", "dv", "dlog_decay", "dinitial_state")]
 
 
 class ShortConvProblem(ctypes.Structure):
@@ -255,6 +271,13 @@ SIGNATURES: dict[str, tuple] = {
         _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size,
                  _c_void_p]),
     "mogt_short_conv_step": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "mogt_linear_attn_workspace_bytes": (_c_size, [_c_void_p]),
+    "mogt_linear_attn_fwd": (
+        _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
+    "mogt_linear_attn_bwd_workspace_bytes": (_c_size, [_c_void_p]),
+    "mogt_linear_attn_bwd": (
+        _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
+    "mogt_linear_attn_step": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

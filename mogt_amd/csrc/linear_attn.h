@@ -1,0 +1,87 @@
+// Linear attention with a decay for each head, per sequence and head
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T   (dk x dv, fp32),   o_t = scale S_t^T q_t
+// and its gradients.  One pass of the form
+//   out_t = sum_{s <= t} exp(c_t - c_s) (q_t . k_s) v_s,   c_t = g_1 + ... + g_t,
+// serves the forward and, with the roles of the rows exchanged, every gradient:
+//   o   query q,  key k,  value v,  forwards
+//   dq  query do, key v,  value k,  forwards, on the same states transposed
+//   dk  query v,  key do, value q,  backwards in time
+//   dv  query k,  key q,  value do, backwards, dk's states transposed
+// Backwards the decay between neighbours is the later one's, and none lies
+// before the last step.  The gradient of g follows from the rows' products
+// (la_decay_kernel).
+//
+// Chunked form: inside a chunk of LA_T steps, with c from its start and S the
+// state before it,
+//   out_t = exp(c_t) S^T q_t + sum_{s <= t} exp(c_t - c_s) (q_t . k_s) v_s
+//   S'    = exp(c_T) S + sum_s k_s (exp(c_T - c_s) v_s)^T
+// all of them matrix products.  Sequences are cut into segments of whole chunks:
+// sums (each segment's S' from zero), carry (the states entering the segments,
+// in order), out (each segment from its state, chunk by chunk).
+#pragma once
+
+#include <type_traits>
+
+#include "common.h"
+
+namespace mogt {
+
+constexpr int LA_NV = 64;                  // value columns of a work-group, 16 a wave
+constexpr int LA_THREADS = 256;
+constexpr float LA_LOG2E = 1.4426950408889634f;
+// log2 of the least decay: exp(g) is zero in fp32 far above it, and sums over a
+// chunk stay exact to 2^-33 in 64 bits (g = -inf is this and not NaN)
+constexpr double LA_LOG2_MIN = -16384.0;
+// exp(g) is zero in fp32 at and below this g (2^-150 rounds to zero)
+constexpr float LA_G_ZERO = -103.972084f;
+
+template <typename TI> struct LaChunk;
+// Steps of a chunk, the contraction of one operand fragment (a lane holds KS / 4
+// consecutive elements), elements of padding of an LDS row, and the bf16 pieces
+// that hold an fp32 operand: two are 16 bits of it (error 2^-17), so that states,
+// gradients of decays and the sums of pairs keep what bf16 rows give them.
+template <> struct LaChunk<bf16_t> { static constexpr int T = 64, KS = 32, PAD = 8, NP = 2; };
+template <> struct LaChunk<float> { static constexpr int T = 32, KS = 16, PAD = 4, NP = 1; };
+
+struct LaRows {      // rows of one role: element strides, and the heads that share them
+    const void* p;
+    int64_t row, batch, head;
+    int div;         // head h reads h / div
+    int vec;         // 16-byte loads: aligned, strides and width whole vectors
+};
+
+struct LaPass {
+    LaRows q, k, v, x;          // x: rows multiplied with the outputs for `dot`
+    const float* init;          // state entering the first segment [B, H, dk, dv], or null: zero
+    float* states;              // [B, H, nseg + 1, dk, dv]: states entering the segments in pass order, the last after all
+    float* ctot;                // [B, H, nseg]: log2 of the segments' decays
+    float* last;                // final state [B, H, dk, dv], or null
+    void* out;                  // [B, L, H, dn], or null
+    float* dot;                 // [nvb, B, H, L] sums over the block's columns of x_t * out_t, or null
+    float qs, ps, ws;           // factors of the query's part, the pairs and the writes
+    int dc, dn;                 // width of q and k, of v
+    int nvb;                    // ceil(dn / LA_NV)
+    int rs, cs;                 // strides of a state's rows (dc) and columns (dn)
+    int reverse, out_f32, keep; // keep: this pass leaves the first and last of `states`
+};
+
+struct LaArgs {
+    LaPass pass[3];
+    const float* g;
+    const void* lengths;
+    int64_t g_row, g_batch, g_head;
+    int B, L, H, seg, nseg, len64;
+    int state;                  // dk * dv
+};
+
+__device__ __forceinline__ int la_length(const LaArgs& a, int b) {
+    if (!a.lengths) return a.L;
+    int64_t n = a.len64 ? static_cast<const int64_t*>(a.lengths)[b] : static_cast<const int32_t*>(a.lengths)[b];
+    n = n < 0 ? 0 : n > a.L ? a.L : n;
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(n));
+}
+
+// padded contraction width of a pass, which its kernel is built for
+inline int la_width(int dc) { return dc <= 32 ? 32 : dc <= 64 ? 64 : 128; }
+
+}  // namespace mogt

@@ -2945,3 +2945,226 @@ def ssm_step(x: torch.Tensor, state: torch.Tensor, delta: torch.Tensor, A: torch
     _check_step_state("ssm_step", state)
     return _ssm_step_op(x, state, delta, _float32(A), B, C, _float32(D), z, _float32(delta_bias),
                         bool(delta_softplus))
+
+
+# ---------------------------------------------------------------------------
+# linear attention with a decay for each head
+# ---------------------------------------------------------------------------
+LINEAR_ATTN_MAX_DIM = 128
+LINEAR_ATTN_CHUNK = {torch.bfloat16: 64, torch.float32: 32}   # steps of a chunk; a segment is whole chunks
+# Work-groups that a call is cut into segments for, and the least steps of one.
+LINEAR_ATTN_GROUPS = 1024
+LINEAR_ATTN_MIN_SEGMENT = 256
+
+
+def _linear_attn_segment(B: int, L: int, H: int, dv: int, dtype: torch.dtype) -> int:
+    """Steps of a segment, whole chunks."""
+    chunk = LINEAR_ATTN_CHUNK[dtype]
+    want = -(-LINEAR_ATTN_GROUPS // max(1, B * H * -(-dv // 64)))
+    steps = max(LINEAR_ATTN_MIN_SEGMENT, -(-L // want), -(-L // (1 << 20)))
+    return chunk * -(-steps // chunk)
+
+
+def _linear_attn_problem(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                         initial_state: torch.Tensor | None, lengths: torch.Tensor | None, scale: float, segment: int):
+    """The C problem and the tensors it points into; rows ``[B, L, heads, d]``,
+    or ``[B, heads, d]`` for a step."""
+    q, k, v, initial_state, lengths = (_unit_channels(q), _unit_channels(k), _unit_channels(v), _dense(initial_state),
+                                       _dense(lengths))
+    qs, ks, vs, gs = q.stride(), k.stride(), v.stride(), log_decay.stride()
+    per_head = log_decay.ndim == 1
+    step = q.ndim == 3
+    # (row, batch, head) strides; a step's rows have none
+    strides = tuple(n for s in (qs, ks, vs) for n in ((0 if step else s[1]), s[0], s[-2]))
+    g = (0, 0, gs[0]) if per_head else ((0 if step else gs[1]), gs[0], gs[-1])
+    p = _lib.LINEAR_ATTN_PROBLEM.pack(v.shape[0], 1 if step else v.shape[1], v.shape[-2], q.shape[-2], q.shape[-1],
+                                      v.shape[-1], segment, _DTYPE_CODE[q.dtype],
+                                      0 if lengths is None else lengths.element_size(), per_head, scale, q.data_ptr(),
+                                      k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(initial_state),
+                                      _ptr(lengths), *strides, *g)
+    return p, (q, k, v, log_decay, initial_state, lengths)
+
+
+@_op("mogt::linear_attention")
+def _linear_attn_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                    initial_state: torch.Tensor | None, lengths: torch.Tensor | None, scale: float, want_state: bool,
+                    want_carries: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    lib = _lib.load()
+    B, L, H, dv = v.shape
+    dk = q.shape[-1]
+    segment = _linear_attn_segment(B, L, H, dv, v.dtype)
+    f32 = dict(dtype=torch.float32, device=v.device)
+    out = torch.empty((B, L, H, dv), dtype=v.dtype, device=v.device)
+    state = torch.empty((B, H, dk, dv) if want_state else (0,), **f32)
+    carries = torch.empty((B, H, max(1, -(-L // segment)) + 1, dk, dv) if want_carries else (0,), **f32)
+    p, held = _linear_attn_problem(q, k, v, log_decay, initial_state, lengths, scale, segment)
+    nbytes = lib.mogt_linear_attn_workspace_bytes(p)
+    ws = scratch(nbytes, v.device) if nbytes else None
+    with _on_device(v.device):
+        rc = lib.mogt_linear_attn_fwd(p, out.data_ptr(), state.data_ptr() if want_state else None,
+                                      carries.data_ptr() if want_carries else None, _ptr(ws), nbytes,
+                                      _stream_handle(v.device))
+    _lib.check(rc, "mogt_linear_attn_fwd")
+    return out, state, carries
+
+
+@_linear_attn_op.register_fake
+def _(q, k, v, log_decay, initial_state, lengths, scale, want_state, want_carries):
+    B, L, H, dv = v.shape
+    dk = q.shape[-1]
+    segment = _linear_attn_segment(B, L, H, dv, v.dtype)
+    return (v.new_empty((B, L, H, dv)), log_decay.new_empty((B, H, dk, dv) if want_state else (0,)),
+            log_decay.new_empty((B, H, max(1, -(-L // segment)) + 1, dk, dv) if want_carries else (0,)))
+
+
+@_op("mogt::linear_attention_grad")
+def _linear_attn_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor,
+                         v: torch.Tensor, log_decay: torch.Tensor, initial_state: torch.Tensor | None,
+                         lengths: torch.Tensor | None, carries: torch.Tensor, scale: float,
+                         need: list[bool]) -> list[torch.Tensor]:
+    """Gradients of (q, k, v, log_decay, initial_state); empty where ``need`` is
+    false."""
+    lib = _lib.load()
+    B, L, H, dv = v.shape
+    G, dk = q.shape[-2:]
+    segment = _linear_attn_segment(B, L, H, dv, v.dtype)
+    if carries.shape != (B, H, max(1, -(-L // segment)) + 1, dk, dv):
+        raise ValueError(f"linear_attention_grad: carries {list(carries.shape)} are not those of a forward over "
+                         f"segments of {segment} steps")
+    dout = _dense(dout if dout.dtype == v.dtype else dout.to(v.dtype))
+    dfinal = None if dfinal is None else dfinal.to(torch.float32).contiguous()
+    p, held = _linear_attn_problem(q, k, v, log_decay, initial_state, lengths, scale, segment)
+    f32 = torch.float32
+    shapes = (((B, L, G, dk), q.dtype), ((B, L, G, dk), q.dtype), ((B, L, H, dv), q.dtype),
+              ((H,) if log_decay.ndim == 1 else (B, L, H), f32), ((B, H, dk, dv), f32))
+    make = torch.empty if B > 0 and H > 0 else torch.zeros
+    grads = [make(s if n else (0,), dtype=t, device=v.device) for (s, t), n in zip(shapes, need)]
+    nbytes = lib.mogt_linear_attn_bwd_workspace_bytes(p)
+    ws = scratch(nbytes, v.device)
+    out = _lib.LINEAR_ATTN_GRADIENTS.pack(*[t.data_ptr() if n else 0 for t, n in zip(grads, need)])
+    with _on_device(v.device):
+        rc = lib.mogt_linear_attn_bwd(p, dout.data_ptr(), _ptr(dfinal), carries.data_ptr(), out, ws.data_ptr(),
+                                      nbytes, _stream_handle(v.device))
+    _lib.check(rc, "mogt_linear_attn_bwd")
+    return grads
+
+
+@_linear_attn_grad_op.register_fake
+def _(dout, dfinal, q, k, v, log_decay, initial_state, lengths, carries, scale, need):
+    shapes = ((q, q.shape), (q, k.shape), (q, v.shape), (log_decay, log_decay.shape),
+              (log_decay, (v.shape[0], v.shape[2], q.shape[-1], v.shape[-1])))
+    return [t.new_empty(s if n else (0,)) for (t, s), n in zip(shapes, need)]
+
+
+def _linear_attn_setup(ctx, inputs, output):
+    q, k, v, log_decay, initial_state, lengths, scale, want_state, want_carries = inputs
+    ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths, output[2])
+    ctx.scale = scale
+    ctx.want_state = want_state
+    ctx.want_carries = want_carries
+    # the carries are saved for the backward, not differentiated
+    ctx.set_materialize_grads(False)
+
+
+def _linear_attn_backward(ctx, dout, dfinal, dcarries):
+    q, k, v, log_decay, initial_state, lengths, carries = ctx.saved_tensors
+    if not ctx.want_state:
+        dfinal = None
+    if dout is None and dfinal is None:
+        return (None,) * 9
+    if not ctx.want_carries:
+        raise RuntimeError("linear_attention: the forward kept no carries for this backward")
+    if dout is None:
+        dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
+    need = list(ctx.needs_input_grad[:5])
+    grads = _linear_attn_grad_op.in_backward(ctx, (dout, dfinal), q, k, v, log_decay, initial_state, lengths, carries,
+                                             ctx.scale, need)
+    return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 4
+
+
+_linear_attn_op.register_autograd(_linear_attn_backward, _linear_attn_setup)
+
+
+def _check_linear_attn(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                       state: torch.Tensor | None) -> None:
+    _same_device(what, q, (k, v, log_decay, state))
+    dtype_code(q.dtype, what)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what}: q, k and v must have one dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if k.shape != q.shape:
+        raise ValueError(f"{what}: q {list(q.shape)} and k {list(k.shape)} must have the same shape")
+    if v.ndim != q.ndim or v.shape[:-2] != q.shape[:-2]:
+        raise ValueError(f"{what}: v must be {list(q.shape[:-2])} + [heads, dv], got {list(v.shape)}")
+    (G, dk), (H, dv) = q.shape[-2:], v.shape[-2:]
+    if G < 1 or H % G != 0:
+        raise ValueError(f"{what}: {H} heads do not divide into {G} groups")
+    if not (1 <= dk <= LINEAR_ATTN_MAX_DIM and 1 <= dv <= LINEAR_ATTN_MAX_DIM):
+        raise ValueError(f"{what}: widths {dk} and {dv} not supported (1 to {LINEAR_ATTN_MAX_DIM})")
+    if log_decay.shape != v.shape[:-1] and log_decay.shape != (H,):
+        raise ValueError(f"{what}: log_decay must be {list(v.shape[:-1])} or [{H}], got {list(log_decay.shape)}")
+    _check_real(what, log_decay=log_decay)
+    if state is not None:
+        _check_shape(what, "state", state, (v.shape[0], H, dk, dv))
+        if state.dtype != torch.float32:
+            raise ValueError(f"{what}: the state must be float32, got {state.dtype}")
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *,
+                     scale: float | None = None, initial_state: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Linear attention with a decay for each head, over a whole sequence.
+
+    ``S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T``, ``o_t = scale S_t^T q_t`` per
+    head, for ``q``, ``k`` ``[B, L, G, dk]`` and ``v [B, L, H, dv]`` of one dtype
+    (float32 or bfloat16, any strides), each group's q and k shared by H / G
+    consecutive heads, widths up to 128; ``scale`` defaults to ``dk ** -0.5``.
+    ``log_decay`` is ``[B, L, H]``, or ``[H]`` for one decay a head (real, taken in
+    float32, at most 0 as a rule; -inf empties the state).  fp32 state and sums, the
+    output in v's dtype.  ``initial_state [B, H, dk, dv]`` (float32, zero without
+    it); ``return_state`` also returns the final one, from which
+    ``linear_attention`` and ``linear_attention_step`` continue.  ``lengths [B]``
+    (int32 or int64 on the GPU, taken within [0, L]) marks the padding of a ragged
+    batch: steps past a length are not read and leave the state as it is; their
+    outputs and gradients are zero.  Differentiable in every tensor but
+    ``lengths``, through both outputs; results do not change from run to run."""
+    if q.ndim != 4:
+        raise ValueError("linear_attention: q must be [B, L, G, dk]")
+    _check_linear_attn("linear_attention", q, k, v, log_decay, initial_state)
+    if lengths is not None:
+        _same_device("linear_attention", q, (lengths,))
+        _check_lengths("linear_attention", lengths, q.shape[0])
+    want_carries = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state))
+    out, state, _ = _linear_attn_op(q, k, v, _float32(log_decay), initial_state, lengths,
+                                    float(q.shape[-1] ** -0.5 if scale is None else scale), bool(return_state),
+                                    want_carries)
+    return (out, state) if return_state else out
+
+
+@_op("mogt::linear_attention_step_", mutates=("state",))
+def _linear_attn_step_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: torch.Tensor,
+                         log_decay: torch.Tensor, scale: float) -> torch.Tensor:
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    p, held = _linear_attn_problem(q, k, v, log_decay, None, None, scale, 0)
+    with _on_device(v.device):
+        rc = _lib.load().mogt_linear_attn_step(p, state.data_ptr(), out.data_ptr(), _stream_handle(v.device))
+    _lib.check(rc, "mogt_linear_attn_step")
+    return out
+
+
+@_linear_attn_step_op.register_fake
+def _(q, k, v, state, log_decay, scale):
+    return v.new_empty(v.shape)
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: torch.Tensor,
+                          log_decay: torch.Tensor, *, scale: float | None = None) -> torch.Tensor:
+    """One token of ``linear_attention`` for every sequence: ``q``, ``k``
+    ``[B, G, dk]``, ``v [B, H, dv]``, ``log_decay [B, H]`` or ``[H]``; ``state
+    [B, H, dk, dv]`` (float32, contiguous) is updated in place.  No autograd."""
+    if q.ndim != 3:
+        raise ValueError("linear_attention_step: q must be [B, G, dk]")
+    _check_linear_attn("linear_attention_step", q, k, v, log_decay, state)
+    _check_step_state("linear_attention_step", state)
+    return _linear_attn_step_op(q, k, v, state, _float32(log_decay),
+                                float(q.shape[-1] ** -0.5 if scale is None else scale))
