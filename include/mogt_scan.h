@@ -753,6 +753,32 @@ int mogt_linear_attn_bwd(const mogt_linear_attn_problem* problem, const void* do
                          size_t workspace_bytes, void* stream);
 int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state, void* out, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Rows and weights in e4m3 (OCP, largest value 448) with fp32 scales, each for a
+ * block of 128 values of one row, or of 128 rows by 128 values:
+ *   scale = max(largest |x| / 448, 2^-126),  q = e4m3(x / scale), nearest even
+ * A row of `dim` values has ceil(dim / 128) scales; the last block may be short.
+ * mogt_add_rmsnorm_fp8_fwd: x_out = x + (scale * z) [the product rounded to z's
+ *   dtype], as mogt_add_rmsnorm_fwd, and the rows rmsnorm(x_out) * weight in 8 bits
+ *   (statistics in fp32, no rounding before the 8 bits); x, x_out fp32, rows of
+ *   `dim` contiguous elements, dim a multiple of 4 and <= 4096.
+ * mogt_quantize_fp8: the rows of x (row stride ld, a multiple of 4) in 8 bits, with
+ *   block_rows 1 (dim <= 4096) or 128 (weights); dim a multiple of 4.
+ * mogt_linear_fp8: y[m][n] = sum_k x[m][k] w[n][k] of the values both stand for: x
+ *   [rows, width] with x_scale [rows, ceil(width / 128)], w [outputs, width]
+ *   contiguous with w_scale [ceil(outputs / 128), ceil(width / 128)]; y [rows,
+ *   outputs] contiguous, fp32 or bf16, rounded once.  width and ldx multiples of 16.
+ *   Blocks' sums are scaled and added in fp32; within a block bf16 outputs take the
+ *   8-bit matrix instruction, whose sums are within 1.4e-5 (as 2-norms, on normal
+ *   rows) and fp32 outputs the bf16 one on the same values, which adds in fp32.
+ * No workspace.  No counterpart in the reference.                           */
+int mogt_add_rmsnorm_fp8_fwd(const float* x, const void* z, float scale, const float* weight, float* x_out, void* q,
+                             float* q_scale, int64_t rows, int64_t dim, float eps, int z_dtype, void* stream);
+int mogt_quantize_fp8(const void* x, int64_t ld, void* q, float* q_scale, int64_t rows, int64_t dim, int dtype,
+                      int block_rows, void* stream);
+int mogt_linear_fp8(const void* x, int64_t ldx, const float* x_scale, const void* w, const float* w_scale, void* y,
+                    int64_t rows, int64_t outputs, int64_t width, int out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,13 +34,14 @@ HIPCC_FLAGS = [
     "-Wno-unused-function",
 ]
 
-# Per-file extras.  The rank-1 and linear attention kernels rescale MFMA
-# accumulators between chains; keeping accumulators in ordinary VGPRs avoids a copy to and from the
+# Per-file extras.  The rank-1, linear attention and 8-bit product kernels
+# rescale MFMA accumulators between chains; keeping accumulators in ordinary VGPRs avoids a copy to and from the
 # accumulation registers around every such rescale.
 FILE_FLAGS = {
     "rank1_scan.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "linear_attn_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "linear_attn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "fp8_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -278,6 +278,14 @@ SIGNATURES: dict[str, tuple] = {
     "mogt_linear_attn_bwd": (
         _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size, _c_void_p]),
     "mogt_linear_attn_step": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "mogt_add_rmsnorm_fp8_fwd": (
+        _c_int, [_c_void_p, _c_void_p, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_float,
+                 _c_int, _c_void_p]),
+    "mogt_quantize_fp8": (
+        _c_int, [_c_void_p, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_int, _c_int, _c_void_p]),
+    "mogt_linear_fp8": (
+        _c_int, [_c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_i64, _c_i64, _c_int,
+                 _c_void_p]),
 }
 
 _lock = threading.Lock()

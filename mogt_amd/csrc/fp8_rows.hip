@@ -1,0 +1,200 @@
+// Rows and weights in e4m3 (OCP, 3 fraction bits, largest value 448) with a scale
+// for each block of 128 values of a row, or of 128 rows by 128 values:
+//   scale = max(largest |x| of the block / 448, 2^-126),   q = e4m3(x / scale)
+// rounded to nearest even, so x is q * scale within half a step of the block's
+// largest value, and a block of zeros is zeros.  A NaN stays one in its place; an
+// infinity makes its block's scale infinite.
+//   add_rmsnorm_fp8  x' = x + round(s * z), n = rmsnorm(x') * w, the rows n in 8 bits:
+//                    the residual update as in add_rmsnorm, statistics in fp32
+//   quantize_rows    the rows of a matrix
+//   quantize_blocks  128 x 128 blocks (weights, laid out once)
+// Rows: one wave a row, four consecutive values a lane, so half a wave is a block
+// and its maximum five lane exchanges; bound by HBM.
+#include "common.h"
+
+namespace mogt {
+namespace {
+
+constexpr int F8_BLOCK = 128;
+constexpr float F8_MAX = 448.0f;
+constexpr int F8_WAVES = 4;   // rows per work-group
+
+__device__ __forceinline__ float f8_scale(float amax) { return fmaxf(amax / F8_MAX, 0x1p-126f); }
+
+// four values as e4m3, nearest even; magnitudes are at most 448 (1 + 2^-23), which rounds to 448
+__device__ __forceinline__ uint32_t f8_pack(const float (&v)[4], float scale) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] / scale, v[1] / scale, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2] / scale, v[3] / scale, w, true));
+}
+
+__device__ __forceinline__ float f8_max4(const float (&v)[4]) {
+    return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+}
+
+struct F8Rows {
+    const void *x, *z;
+    const float* w;
+    float* x_out;
+    uint32_t* q;       // [rows, D] bytes
+    float* scale;      // [rows, blocks]
+    int64_t rows, ldx;
+    int D, blocks;
+    float zs, eps;
+};
+
+// VPL: vectors of four values a lane (D <= 256 VPL)
+template <typename TX, typename TZ, int VPL, bool NORM>
+__global__ __launch_bounds__(64 * F8_WAVES) void f8_rows_kernel(F8Rows p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * F8_WAVES + (threadIdx.x >> 6);
+    if (row >= p.rows) return;
+    const TX* xr = static_cast<const TX*>(p.x) + row * p.ldx;
+    const TZ* zr = static_cast<const TZ*>(p.z) + row * p.D;
+    float v[VPL][4], ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+        const int c = (k * 64 + lane) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][e] = 0.0f;
+        if (c < p.D) {
+            load_vec<TX, 4>(xr + c, v[k]);
+            if constexpr (NORM) {
+                float zz[4];
+                load_vec<TZ, 4>(zr + c, zz);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[k][e] += IO<TZ>::ld(IO<TZ>::st(p.zs * zz[e]));
+                    ss = fmaf(v[k][e], v[k][e], ss);
+                }
+                store_vec<float, 4>(p.x_out + row * p.D + c, v[k]);
+            }
+        }
+    }
+    if constexpr (NORM) {
+        for (int m = 32; m > 0; m >>= 1) ss += __shfl_xor(ss, m);
+        const float inv = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
+#pragma unroll
+        for (int k = 0; k < VPL; ++k) {
+            const int c = (k * 64 + lane) * 4;
+            if (c < p.D) {
+                float w[4];
+                load_vec<float, 4>(p.w + c, w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k][e] = v[k][e] * inv * w[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+        const int c = (k * 64 + lane) * 4;
+        float m = f8_max4(v[k]);
+        for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+        const float s = f8_scale(m);
+        if (c < p.D) {
+            p.q[(row * p.D + c) >> 2] = f8_pack(v[k], s);
+            if ((lane & 31) == 0) p.scale[row * p.blocks + c / F8_BLOCK] = s;
+        }
+    }
+}
+
+// A work-group per 128 x 128 block: its maximum, then its values (read again from
+// the caches).
+template <typename T>
+__global__ __launch_bounds__(256) void f8_blocks_kernel(const T* x, int64_t ldx, uint32_t* q, float* scale, int64_t rows,
+                                                        int D) {
+    __shared__ float s_max[4];
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * F8_BLOCK;
+    const int c = blockIdx.x * F8_BLOCK + (threadIdx.x & 31) * 4, nr = static_cast<int>(min(rows - r0, static_cast<int64_t>(F8_BLOCK)));
+    float m = 0.0f;
+    for (int r = threadIdx.x >> 5; r < nr; r += 8)
+        if (c < D) {
+            float v[4];
+            load_vec<T, 4>(x + (r0 + r) * ldx + c, v);
+            m = fmaxf(m, f8_max4(v));
+        }
+    for (int i = 32; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const float s = f8_scale(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])));
+    for (int r = threadIdx.x >> 5; r < nr; r += 8)
+        if (c < D) {
+            float v[4];
+            load_vec<T, 4>(x + (r0 + r) * ldx + c, v);
+            q[((r0 + r) * D + c) >> 2] = f8_pack(v, s);
+        }
+    if (threadIdx.x == 0) scale[blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x] = s;
+}
+
+template <typename TX, typename TZ, bool NORM>
+int f8_rows_launch(const F8Rows& p, const char* what, hipStream_t st) {
+    const int64_t blocks = (p.rows + F8_WAVES - 1) / F8_WAVES;
+    if (blocks > 0x7fffffff) return set_error(MOGT_E_INVALID, "%s: %lld rows", what, (long long)p.rows);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (p.D <= 256)
+        f8_rows_kernel<TX, TZ, 1, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+    else if (p.D <= 1024)
+        f8_rows_kernel<TX, TZ, 4, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+    else if (p.D <= 2048)
+        f8_rows_kernel<TX, TZ, 8, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+    else
+        f8_rows_kernel<TX, TZ, 16, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+    return check_launch(what);
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+}  // namespace mogt
+
+using namespace mogt;
+
+extern "C" int mogt_add_rmsnorm_fp8_fwd(const float* x, const void* z, float scale, const float* weight, float* x_out,
+                                        void* q, float* q_scale, int64_t rows, int64_t dim, float eps, int z_dtype,
+                                        void* stream) {
+    clear_error();
+    if (rows < 0 || dim < 4 || dim > 4096 || dim % 4 != 0)
+        return set_error(MOGT_E_INVALID, "rows %lld of %lld: a length that is a multiple of 4 up to 4096 expected",
+                         (long long)rows, (long long)dim);
+    if (z_dtype != MOGT_F32 && z_dtype != MOGT_BF16) return set_error(MOGT_E_INVALID, "z dtype %d not supported", z_dtype);
+    if (rows == 0) return MOGT_OK;
+    if (!x || !z || !weight || !x_out || !q || !q_scale) return set_error(MOGT_E_INVALID, "null pointer");
+    if (!aligned(x, 16) || !aligned(x_out, 16) || !aligned(weight, 16) || !aligned(z, z_dtype == MOGT_BF16 ? 8 : 16) || !aligned(q, 4))
+        return set_error(MOGT_E_INVALID, "rows of four values must be aligned");
+    F8Rows p{x, z, weight, x_out, static_cast<uint32_t*>(q), q_scale, rows, dim, static_cast<int>(dim),
+             static_cast<int>((dim + F8_BLOCK - 1) / F8_BLOCK), scale, eps};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (z_dtype == MOGT_BF16) return f8_rows_launch<float, bf16_t, true>(p, "mogt_add_rmsnorm_fp8_fwd", st);
+    return f8_rows_launch<float, float, true>(p, "mogt_add_rmsnorm_fp8_fwd", st);
+}
+
+extern "C" int mogt_quantize_fp8(const void* x, int64_t ld, void* q, float* q_scale, int64_t rows, int64_t dim, int dtype,
+                                 int block_rows, void* stream) {
+    clear_error();
+    if (rows < 0 || dim < 4 || dim % 4 != 0 || dim > (1 << 30) || ld < dim)
+        return set_error(MOGT_E_INVALID, "rows %lld of %lld (stride %lld): a length that is a multiple of 4 expected",
+                         (long long)rows, (long long)dim, (long long)ld);
+    if (dtype != MOGT_F32 && dtype != MOGT_BF16) return set_error(MOGT_E_INVALID, "dtype %d not supported", dtype);
+    if (block_rows != 1 && block_rows != F8_BLOCK)
+        return set_error(MOGT_E_INVALID, "blocks of %d rows: 1 or %d expected", block_rows, F8_BLOCK);
+    if (block_rows == 1 && dim > 4096)
+        return set_error(MOGT_E_INVALID, "rows of %lld: at most 4096 values with a scale for each row", (long long)dim);
+    if (rows == 0) return MOGT_OK;
+    const size_t each = dtype == MOGT_BF16 ? 8 : 16;
+    if (!x || !q || !q_scale) return set_error(MOGT_E_INVALID, "null pointer");
+    if (!aligned(x, each) || ld % 4 != 0 || !aligned(q, 4)) return set_error(MOGT_E_INVALID, "rows of four values must be aligned");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int blocks = static_cast<int>((dim + F8_BLOCK - 1) / F8_BLOCK);
+    if (block_rows == 1) {
+        F8Rows p{x, nullptr, nullptr, nullptr, static_cast<uint32_t*>(q), q_scale, rows, ld, static_cast<int>(dim), blocks, 0.0f, 0.0f};
+        if (dtype == MOGT_BF16) return f8_rows_launch<bf16_t, float, false>(p, "mogt_quantize_fp8", st);
+        return f8_rows_launch<float, float, false>(p, "mogt_quantize_fp8", st);
+    }
+    const int64_t by = (rows + F8_BLOCK - 1) / F8_BLOCK;
+    if (by > 65535) return set_error(MOGT_E_INVALID, "%lld rows: at most %d", (long long)rows, 65535 * F8_BLOCK);
+    const dim3 grid(blocks, static_cast<unsigned>(by));
+    if (dtype == MOGT_BF16)
+        f8_blocks_kernel<bf16_t><<<grid, 256, 0, st>>>(static_cast<const bf16_t*>(x), ld, static_cast<uint32_t*>(q), q_scale, rows, static_cast<int>(dim));
+    else
+        f8_blocks_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(x), ld, static_cast<uint32_t*>(q), q_scale, rows, static_cast<int>(dim));
+    return check_launch("mogt_quantize_fp8");
+}

@@ -3168,3 +3168,162 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sta
     _check_step_state("linear_attention_step", state)
     return _linear_attn_step_op(q, k, v, state, _float32(log_decay),
                                 float(q.shape[-1] ** -0.5 if scale is None else scale))
+
+
+# ---------------------------------------------------------------------------
+# 8-bit rows and weights, and their matrix product
+# ---------------------------------------------------------------------------
+FP8_BLOCK = 128
+FP8_MAX_ROW = 4096     # values of a row with scales of its own
+_FP8 = torch.float8_e4m3fn
+
+
+def _fp8_blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+@_op("mogt::add_rmsnorm_fp8")
+def _add_rmsnorm_fp8_op(x: torch.Tensor, z: torch.Tensor, scale: float, weight: torch.Tensor, eps: float
+                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    x, z, w = x.contiguous(), z.contiguous(), weight.contiguous()
+    D = x.shape[-1]
+    x_out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    q = torch.empty(x.shape, dtype=_FP8, device=x.device)
+    q_scale = torch.empty((*x.shape[:-1], _fp8_blocks(D)), dtype=torch.float32, device=x.device)
+    with _on_device(x.device):
+        rc = _lib.load().mogt_add_rmsnorm_fp8_fwd(x.data_ptr(), z.data_ptr(), scale, w.data_ptr(), x_out.data_ptr(),
+                                                  q.data_ptr(), q_scale.data_ptr(), x.numel() // D, D, eps,
+                                                  _DTYPE_CODE[z.dtype], _stream_handle(x.device))
+    _lib.check(rc, "mogt_add_rmsnorm_fp8_fwd")
+    return x_out, q, q_scale
+
+
+@_add_rmsnorm_fp8_op.register_fake
+def _(x, z, scale, weight, eps):
+    return (x.new_empty(x.shape), x.new_empty(x.shape, dtype=_FP8),
+            x.new_empty((*x.shape[:-1], _fp8_blocks(x.shape[-1]))))
+
+
+def add_rmsnorm_fp8(x: torch.Tensor, z: torch.Tensor, scale: float, weight: torch.Tensor, eps: float = 1e-6):
+    """``add_rmsnorm`` with the normalised rows in 8 bits: ``x' = x + scale * z``
+    (fp32 residual stream), and ``rmsnorm(x') * weight`` as ``(q, q_scale)``, e4m3
+    values with a float32 scale for every 128 of a row, which ``linear_fp8`` takes.
+
+    A block's scale is its largest magnitude / 448 (2^-126 at least), the values
+    ``n / scale`` rounded to nearest even; statistics and the norm are fp32, with
+    no rounding between.  Returns ``(x', q, q_scale)``.  Rows of a multiple of 4
+    values, up to 4096.  No autograd."""
+    _same_device("add_rmsnorm_fp8", x, (z, weight))
+    if x.dtype != torch.float32:
+        raise ValueError("add_rmsnorm_fp8 keeps the residual stream in float32")
+    if x.ndim < 1 or x.shape != z.shape:
+        raise ValueError("add_rmsnorm_fp8: x and z must have the same shape")
+    dtype_code(z.dtype, "add_rmsnorm_fp8")
+    D = x.shape[-1]
+    if D < 4 or D % 4 != 0 or D > FP8_MAX_ROW:
+        raise ValueError(f"add_rmsnorm_fp8: rows of {D} values not supported (a multiple of 4 up to {FP8_MAX_ROW})")
+    _check_shape("add_rmsnorm_fp8", "weight", weight, (D,))
+    _check_real("add_rmsnorm_fp8", weight=weight)
+    return _add_rmsnorm_fp8_op(x, z, float(scale), _float32(weight), float(eps))
+
+
+@_op("mogt::quantize_fp8")
+def _quantize_fp8_op(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    D = x.shape[-1]
+    rows = _fp8_rows(x, 4)
+    q = torch.empty(x.shape, dtype=_FP8, device=x.device)
+    lead = x.shape[:-1] if block_rows == 1 else (_fp8_blocks(x.shape[0]),)
+    q_scale = torch.empty((*lead, _fp8_blocks(D)), dtype=torch.float32, device=x.device)
+    with _on_device(x.device):
+        rc = _lib.load().mogt_quantize_fp8(rows.data_ptr(), rows.stride(0), q.data_ptr(), q_scale.data_ptr(),
+                                           rows.shape[0], D, _DTYPE_CODE[x.dtype], block_rows,
+                                           _stream_handle(x.device))
+    _lib.check(rc, "mogt_quantize_fp8")
+    return q, q_scale
+
+
+@_quantize_fp8_op.register_fake
+def _(x, block_rows):
+    lead = x.shape[:-1] if block_rows == 1 else (_fp8_blocks(x.shape[0]),)
+    return (x.new_empty(x.shape, dtype=_FP8),
+            x.new_empty((*lead, _fp8_blocks(x.shape[-1])), dtype=torch.float32))
+
+
+def _fp8_rows(x: torch.Tensor, each: int) -> torch.Tensor:
+    """x as [rows, D] with unit stride in a row, aligned for vectors of ``each``
+    elements (a copy where it is not)."""
+    D = x.shape[-1]
+    rows = x.reshape(-1, D)
+    if (rows.stride(-1) != 1 or rows.stride(0) < D or rows.stride(0) % each != 0
+            or rows.data_ptr() % (each * x.element_size()) != 0):
+        rows = torch.empty(rows.shape, dtype=x.dtype, device=x.device).copy_(rows)
+    return rows
+
+
+def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
+    """``x`` (float32 or bfloat16, ``[..., D]``) in 8 bits for ``linear_fp8``: ``(q,
+    q_scale)``, e4m3 values and float32 scales of blocks of 128 values of a row
+    (``block_rows`` 1: ``q_scale [..., ceil(D / 128)]``, D up to 4096), or of 128
+    rows by 128 values of a weight ``[N, D]`` (128: ``q_scale [ceil(N / 128),
+    ceil(D / 128)]``).  A block's scale is its largest magnitude / 448 (2^-126 at
+    least), values are rounded to nearest even.  D a multiple of 4.  No autograd."""
+    require_cuda("quantize_fp8", x)
+    dtype_code(x.dtype, "quantize_fp8")
+    if block_rows not in (1, FP8_BLOCK):
+        raise ValueError(f"quantize_fp8: blocks of {block_rows} rows not supported (1 or {FP8_BLOCK})")
+    if x.ndim < 1 or (block_rows != 1 and x.ndim != 2):
+        raise ValueError("quantize_fp8: x must be [..., D], or [N, D] in blocks of rows")
+    D = x.shape[-1]
+    if D < 4 or D % 4 != 0 or (block_rows == 1 and D > FP8_MAX_ROW):
+        raise ValueError(f"quantize_fp8: rows of {D} values not supported (a multiple of 4, up to {FP8_MAX_ROW} with "
+                         "scales of their own)")
+    return _quantize_fp8_op(x, int(block_rows))
+
+
+@_op("mogt::linear_fp8")
+def _linear_fp8_op(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                   out_dtype: torch.dtype) -> torch.Tensor:
+    N, K = w.shape
+    rows = _fp8_rows(x, 16)
+    if not w.is_contiguous() or w.data_ptr() % 16 != 0:
+        w = torch.empty(w.shape, dtype=w.dtype, device=w.device).copy_(w)
+    x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
+    y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+    with _on_device(x.device):
+        rc = _lib.load().mogt_linear_fp8(rows.data_ptr(), rows.stride(0), x_scale.data_ptr(), w.data_ptr(),
+                                         w_scale.data_ptr(), y.data_ptr(), rows.shape[0], N, K, _DTYPE_CODE[out_dtype],
+                                         _stream_handle(x.device))
+    _lib.check(rc, "mogt_linear_fp8")
+    return y
+
+
+@_linear_fp8_op.register_fake
+def _(x, x_scale, w, w_scale, out_dtype):
+    return x.new_empty((*x.shape[:-1], w.shape[0]), dtype=out_dtype)
+
+
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``x w^T`` of 8-bit operands: ``x [..., K]`` in e4m3 with ``x_scale [...,
+    ceil(K / 128)]`` and ``w [N, K]`` with ``w_scale [ceil(N / 128), ceil(K /
+    128)]`` (``add_rmsnorm_fp8``, ``quantize_fp8``), K a multiple of 16.
+
+    Each block's products are added on the matrix cores, scaled and added in
+    float32, and rounded once to ``out_dtype`` (bfloat16 or float32).  bfloat16
+    outputs take the 8-bit instruction, whose sums of 128 are within about 1.4e-5
+    of their size; float32 outputs the bfloat16 one on the same values, at half
+    its rate.  No autograd."""
+    _same_device("linear_fp8", x, (x_scale, w, w_scale))
+    if x.dtype != _FP8 or w.dtype != _FP8:
+        raise ValueError(f"linear_fp8: x and w must be {_FP8}, got {x.dtype} and {w.dtype}")
+    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+        raise ValueError(f"linear_fp8: scales must be float32, got {x_scale.dtype} and {w_scale.dtype}")
+    dtype_code(out_dtype, "linear_fp8")
+    if w.ndim != 2 or x.ndim < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"linear_fp8: x must be [..., K] and w [N, K], got {list(x.shape)} and {list(w.shape)}")
+    N, K = w.shape
+    if K < 16 or K % 16 != 0:
+        raise ValueError(f"linear_fp8: rows of {K} values not supported (a multiple of 16)")
+    _check_shape("linear_fp8", "x_scale", x_scale, (*x.shape[:-1], _fp8_blocks(K)))
+    _check_shape("linear_fp8", "w_scale", w_scale, (_fp8_blocks(N), _fp8_blocks(K)))
+    return _linear_fp8_op(x, x_scale, w, w_scale, out_dtype)

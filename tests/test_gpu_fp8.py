@@ -1,0 +1,172 @@
+"""8-bit rows and weights (``ops.add_rmsnorm_fp8``, ``ops.quantize_fp8``) and
+their product (``ops.linear_fp8``) against the definitions in 64 bits.
+
+Tolerances, derived: a scale is a quotient of an fp32 value, one rounding, 2^-24
+of it, and in the norm that value's own: the residual's 1, the statistics' D / 2 + 4
+(a squared sum of D terms under a root, the reciprocal root's 2 ulp) and 2
+products: (D / 2 + 8) 2^-24.  A value x / scale carries those and its quotient's,
+and is rounded to e4m3: half a step, 2^-4 of it, or 2^-10 where steps are 2^-9; where
+the 64-bit value lies within its own error of a border the other neighbour is as
+right, so a value may be off by half a step and twice that error.  A product in
+fp32 adds K + 4 roundings of the sum S of its terms' absolute values, and with the
+8-bit instruction 2^-13 S: an instruction aligns the products that it adds to the
+largest and drops what lies below 2^-14 or so of it, from each of them at most."""
+import pytest
+import torch
+
+from conftest import announce
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F8 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+U = 2.0 ** -24
+
+
+def rnd(*s, seed=0, dtype=F32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*s, generator=g, device="cuda").to(dtype)
+
+
+def check_eight(n, q, scale, rows, rel):
+    """q, scale against the float64 values n [M, D], known to `rel`, in blocks of
+    `rows` by 128."""
+    M, D = n.shape
+    q, scale = q.double().cpu(), scale.double().cpu()
+    for i, r in enumerate(n.split(rows)):
+        for j, b in enumerate(r.split(128, 1)):
+            s = max(float(b.abs().max()) / 448, 2.0 ** -126)
+            got = float(scale[i, j])
+            assert abs(got - s) <= (rel + U) * s
+            u = b / got
+            v = q[i * rows:i * rows + b.shape[0], j * 128:j * 128 + b.shape[1]]
+            half = torch.maximum(u.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10, dtype=torch.float64))
+            assert bool(((v - u).abs() <= half + 2 * (rel + 2 * U) * u.abs()).all())
+
+
+@pytest.mark.parametrize("M,D", [(1, 4), (3, 128), (5, 132), (7, 256), (2, 260), (65, 768), (4, 1028), (9, 2048),
+                                 (2, 2052), (3, 4096)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm(gpu, M, D, dtype):
+    from mogt_amd import ops
+    announce(f"add_rmsnorm_fp8 {M} {D} {dtype}")
+    x, z, w = rnd(M, D, seed=1) * 3, rnd(M, D, seed=2, dtype=dtype), 1 + 0.2 * rnd(D, seed=3)
+    x_out, q, s = ops.add_rmsnorm_fp8(x, z, 0.3, w, 1e-5)
+    assert q.dtype == F8 and s.shape == (M, -(-D // 128))
+    assert torch.equal(x_out, ops.add_rmsnorm(x, z, 0.3, w, 1e-5)[0])
+    xd = x_out.double().cpu()
+    n = xd / torch.sqrt((xd * xd).mean(1, keepdim=True) + 1e-5) * w.double().cpu()
+    check_eight(n, q, s, 1, (D / 2 + 8) * U)
+
+
+@pytest.mark.parametrize("shape", [(1, 4), (3, 5, 128), (7, 132), (130, 4096)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_quantize_rows(gpu, shape, dtype):
+    from mogt_amd import ops
+    announce(f"quantize_fp8 rows {shape} {dtype}")
+    x = rnd(*shape, seed=4, dtype=dtype) * 50
+    q, s = ops.quantize_fp8(x)
+    assert q.shape == x.shape and s.shape == (*shape[:-1], -(-shape[-1] // 128))
+    check_eight(x.double().cpu().reshape(-1, shape[-1]), q.reshape(-1, shape[-1]), s.reshape(-1, s.shape[-1]), 1, 0.0)
+    wide = rnd(shape[0], shape[-1] + 3, seed=5, dtype=dtype)[:, 1:shape[-1] + 1]   # unaligned rows
+    a, b = ops.quantize_fp8(wide), ops.quantize_fp8(wide.contiguous())
+    assert torch.equal(a[0].float(), b[0].float()) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("M,D", [(1, 4), (127, 128), (129, 132), (300, 768), (128, 5120)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_quantize_blocks(gpu, M, D, dtype):
+    from mogt_amd import ops
+    announce(f"quantize_fp8 blocks {M} {D} {dtype}")
+    x = rnd(M, D, seed=6, dtype=dtype) * torch.exp(rnd(M, 1, seed=7)).to(dtype)
+    q, s = ops.quantize_fp8(x, block_rows=128)
+    assert s.shape == (-(-M // 128), -(-D // 128))
+    check_eight(x.double().cpu(), q, s, 128, 0.0)
+
+
+def test_zeros_and_tiny_rows(gpu):
+    """A block of zeros is zeros at the least scale, values below it do not divide
+    by zero; what is not finite stays in its block."""
+    from mogt_amd import ops
+    x = torch.zeros(4, 256, device="cuda")
+    x[1, :128] = 1e-38
+    x[2, 5] = float("nan")
+    x[3, 200] = float("inf")
+    for rows in (1, 128):
+        announce(f"quantize_fp8 special values, blocks of {rows}")
+        q, s = ops.quantize_fp8(x, block_rows=rows)
+        q = q.float()
+        assert not q[0].any() and float(s[0, 0]) > 0
+        assert bool(torch.isnan(q[2, 5])) and bool(torch.isnan(q[3, 200]))
+        assert int(torch.isnan(q).sum()) == 2
+    q, s = ops.quantize_fp8(x)
+    assert float(s[1, 0]) == 2.0 ** -126 and bool((q[1, :128].float() - 1e-38 * 2.0 ** 126).abs().max() <= 2.0 ** -10 + 0.06)
+
+
+def product(M, N, K, seed=0):
+    from mogt_amd import ops
+    x, xs = ops.quantize_fp8(rnd(M, K, seed=seed) * torch.exp(rnd(M, 1, seed=seed + 1)))
+    w, ws = ops.quantize_fp8(rnd(N, K, seed=seed + 2) / K ** 0.5, block_rows=128)
+    return x, xs, w, ws
+
+
+def check_product(y, x, xs, w, ws):
+    K, N = x.shape[-1], w.shape[0]
+    xd = x.double() * xs.double().repeat_interleave(128, -1)[..., :K]
+    wd = w.double() * ws.double().repeat_interleave(128, 1)[:, :K].repeat_interleave(128, 0)[:N]
+    want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    lim = (K + 4) * U * mag
+    if y.dtype == BF16:
+        lim = lim + 2.0 ** -13 * mag
+        lim = lim + 2.0 ** -8 * (want.abs() + lim)
+    err = (y.double() - want).abs()
+    assert bool((err <= lim + 1e-30).all()), f"{float((err / (lim + 1e-30)).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("M,N,K", [
+    (1, 1, 16), (1, 17, 128), (2, 130, 144), (15, 64, 768), (16, 129, 1024), (17, 16, 2048), (33, 300, 112),
+    (64, 128, 640), (65, 128, 128), (66, 1, 16), (100, 131, 272), (129, 257, 384), (501, 300, 768), (1000, 5, 1040),
+])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_product(gpu, M, N, K, out):
+    from mogt_amd import ops
+    announce(f"linear_fp8 {M} {N} {K} {out}")
+    p = product(M, N, K)
+    y = ops.linear_fp8(*p, out_dtype=out)
+    assert y.dtype == out and y.shape == (M, N)
+    check_product(y, *p)
+
+
+@pytest.mark.parametrize("M,N,K", [(4100, 3500, 400), (3841, 4097, 256)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_product_of_many_tiles(gpu, M, N, K, out):
+    from mogt_amd import ops
+    announce(f"linear_fp8 {M} {N} {K} {out}")
+    p = product(M, N, K, seed=9)
+    check_product(ops.linear_fp8(*p, out_dtype=out), *p)
+
+
+def test_product_layouts(gpu):
+    """Leading dimensions, rows of a wider matrix, unaligned and transposed operands."""
+    from mogt_amd import ops
+    announce("linear_fp8 layouts")
+    x, xs, w, ws = product(70, 96, 160)
+    want = ops.linear_fp8(x, xs, w, ws)
+    got = ops.linear_fp8(x.view(7, 10, 160), xs.view(7, 10, 2), w, ws)
+    assert got.shape == (7, 10, 96) and torch.equal(got.view(70, 96), want)
+    for pad in (16, 3):
+        wide = torch.zeros(70, 160 + 2 * pad, device="cuda").to(F8)
+        wide[:, pad:pad + 160] = x
+        assert torch.equal(ops.linear_fp8(wide[:, pad:pad + 160], xs, w, ws), want)
+    wt = torch.empty(160, 96, device="cuda", dtype=F8).copy_(w.t()).t()
+    assert torch.equal(ops.linear_fp8(x, xs, wt, ws), want)
+    assert ops.linear_fp8(x[:0], xs[:0], w, ws).shape == (0, 96)
+
+
+def test_norm_feeds_the_product(gpu):
+    """A projection after a residual norm, for a batch and for one token."""
+    from mogt_amd import ops
+    for M in (1, 200):
+        announce(f"add_rmsnorm_fp8 into linear_fp8, {M} rows")
+        x, z, weight = rnd(M, 768, seed=1), rnd(M, 768, seed=2, dtype=BF16), 1 + 0.1 * rnd(768, seed=3)
+        w, ws = ops.quantize_fp8(rnd(320, 768, seed=4) / 768 ** 0.5, block_rows=128)
+        _, q, s = ops.add_rmsnorm_fp8(x, z, 0.5, weight)
+        check_product(ops.linear_fp8(q, s, w, ws), q, s, w, ws)
