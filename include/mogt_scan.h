@@ -718,7 +718,7 @@ int mogt_short_conv_step(const mogt_short_conv_problem* problem, void* state, vo
  * run); their size is 0 for a problem that the call refuses.
  * mogt_linear_attn_fwd: out [batch, length, heads, value_dim] contiguous;
  *   final_state may be null; `carries` (may be null) [batch, heads, segments + 1,
- *   key_dim, value_dim] receives the states entering the segments and the final
+ *   value_dim, key_dim] receives the states entering the segments and the final
  *   one, which the backward takes.
  * mogt_linear_attn_bwd: from the same problem (and segment), the forward's carries,
  *   dout (io_dtype, contiguous) and dfinal_state (may be null) the gradients, each

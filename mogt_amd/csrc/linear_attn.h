@@ -26,9 +26,6 @@
 
 namespace mogt {
 
-constexpr int LA_NV = 64;                  // value columns of a work-group, 16 a wave
-constexpr int LA_THREADS = 256;
-constexpr float LA_LOG2E = 1.4426950408889634f;
 // log2 of the least decay: exp(g) is zero in fp32 far above it, and sums over a
 // chunk stay exact to 2^-33 in 64 bits (g = -inf is this and not NaN)
 constexpr double LA_LOG2_MIN = -16384.0;
@@ -36,12 +33,10 @@ constexpr double LA_LOG2_MIN = -16384.0;
 constexpr float LA_G_ZERO = -103.972084f;
 
 template <typename TI> struct LaChunk;
-// Steps of a chunk, the contraction of one operand fragment (a lane holds KS / 4
-// consecutive elements), elements of padding of an LDS row, and the bf16 pieces
-// that hold an fp32 operand: two are 16 bits of it (error 2^-17), so that states,
-// gradients of decays and the sums of pairs keep what bf16 rows give them.
-template <> struct LaChunk<bf16_t> { static constexpr int T = 64, KS = 32, PAD = 8, NP = 2; };
-template <> struct LaChunk<float> { static constexpr int T = 32, KS = 16, PAD = 4, NP = 1; };
+// Steps of a chunk and the contraction of one operand fragment (a lane holds KS /
+// 4 consecutive elements).
+template <> struct LaChunk<bf16_t> { static constexpr int T = 64, KS = 32; };
+template <> struct LaChunk<float> { static constexpr int T = 32, KS = 16; };
 
 struct LaRows {      // rows of one role: element strides, and the heads that share them
     const void* p;
@@ -53,15 +48,15 @@ struct LaRows {      // rows of one role: element strides, and the heads that sh
 struct LaPass {
     LaRows q, k, v, x;          // x: rows multiplied with the outputs for `dot`
     const float* init;          // state entering the first segment [B, H, dk, dv], or null: zero
-    float* states;              // [B, H, nseg + 1, dk, dv]: states entering the segments in pass order, the last after all
+    float* states;              // [B, H, nseg + 1, dv, dk]: states entering the segments in pass order, the last after all
     float* ctot;                // [B, H, nseg]: log2 of the segments' decays
     float* last;                // final state [B, H, dk, dv], or null
     void* out;                  // [B, L, H, dn], or null
-    float* dot;                 // [nvb, B, H, L] sums over the block's columns of x_t * out_t, or null
+    float* dot;                 // [B, H, L] sums over the columns of x_t * out_t, or null
     float qs, ps, ws;           // factors of the query's part, the pairs and the writes
     int dc, dn;                 // width of q and k, of v
-    int nvb;                    // ceil(dn / LA_NV)
-    int rs, cs;                 // strides of a state's rows (dc) and columns (dn)
+    int rs, cs;                 // strides of the rows (dc) and columns (dn) of one of `states`
+    int user_rs, user_cs;       // ... of `init` and `last`, [dk, dv]
     int reverse, out_f32, keep; // keep: this pass leaves the first and last of `states`
 };
 
@@ -81,7 +76,15 @@ __device__ __forceinline__ int la_length(const LaArgs& a, int b) {
     return __builtin_amdgcn_readfirstlane(static_cast<int>(n));
 }
 
-// padded contraction width of a pass, which its kernel is built for
+// Padded contraction width and tiles of 16 value columns a wave of a pass, which
+// its kernel is built for, and the waves of a SIMD that its registers are held to.
 inline int la_width(int dc) { return dc <= 32 ? 32 : dc <= 64 ? 64 : 128; }
+inline int la_tiles(int dn) { return dn <= 64 ? 1 : 2; }
+constexpr int la_waves_per_simd(int width, int tiles) { return tiles == 2 || width > 64 ? 2 : 3; }
+constexpr int LA_THREADS = 256;
+
+inline bool la_one_kind(const LaPass& a, const LaPass& b) {
+    return la_width(a.dc) == la_width(b.dc) && la_tiles(a.dn) == la_tiles(b.dn) && !a.dot == !b.dot && a.out_f32 == b.out_f32;
+}
 
 }  // namespace mogt

@@ -1,6 +1,8 @@
 // Linear attention with a decay for each head: the states between segments, the
 // gradient of the decays, shared heads' sums, the single-token form and the entry
 // points (linear_attn.h has the mathematics, linear_attn_kernel.h the passes).
+#include <initializer_list>
+
 #include "linear_attn.h"
 
 namespace mogt {
@@ -14,16 +16,17 @@ namespace {
 
 // The states entering the segments, in place: slot 0 is the initial state, slot
 // j + 1 = exp(c_j) slot j + what segment j wrote from zero.  A thread owns one
-// element and reads eight segments ahead.
+// element and reads 32 segments at once; `init` is [dk, dv], the segments' [dv, dk].
 __global__ __launch_bounds__(256) void la_carry_kernel(float* states, const float* ctot, const float* init, int nseg,
-                                                       int state) {
-    constexpr int U = 8;
+                                                       int dk, int dv) {
+    constexpr int U = 32;
     const int e = blockIdx.x * 256 + threadIdx.x;
+    const int state = dk * dv;
     const int64_t seq = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
     if (e >= state) return;
     float* q = states + seq * (nseg + 1) * state + e;
     const float* c = ctot + seq * nseg;
-    float h = init ? init[seq * state + e] : 0.0f;
+    float h = init ? init[seq * state + e % dk * dv + e / dk] : 0.0f;
     q[0] = h;
     for (int j = 0; j < nseg - 1; j += U) {
         float w[U];
@@ -41,11 +44,12 @@ __global__ __launch_bounds__(256) void la_carry_kernel(float* states, const floa
 
 struct LaDecay {
     const float *states, *rstates;   // [B, H, nseg + 1, state], in time order and in reverse
-    const float *dot_q, *dot_k;      // [parts, B, H, L]
+    const float *dot_q, *dot_k;      // [B, H, L]
     float* dg;                       // [B, L, H], or null
     double* part;                    // [H, B, nseg] sums of the segments, or null
     float* dinit;                    // [B, H, state], or null
-    int parts, have_last;            // have_last: a gradient of the final state came in
+    int dk;
+    int have_last;                   // a gradient of the final state came in
 };
 
 // dg_s = sum_{t >= s} (q_t . dq_t - k_t . dk_t) within the segment, plus the
@@ -69,7 +73,9 @@ __global__ __launch_bounds__(256) void la_decay_kernel(LaArgs a, LaDecay d) {
     if (j == 0 && d.dinit) {   // its gradient, before the first step's decay (an empty sequence has none)
         const float* X = d.rstates + (seq * (a.nseg + 1) + a.nseg) * a.state;
         const float e = n > 0 ? __expf(gb[0]) : 1.0f;
-        for (int i = threadIdx.x; i < a.state; i += 256) d.dinit[seq * a.state + i] = e == 0.0f ? 0.0f : e * X[i];
+        const int dv = a.state / d.dk;
+        for (int i = threadIdx.x; i < a.state; i += 256)
+            d.dinit[seq * a.state + i] = e == 0.0f ? 0.0f : e * X[i % dv * d.dk + i / dv];
     }
     if (!d.dg && !d.part) return;
     double carry = 0.0, total = 0.0;
@@ -88,13 +94,8 @@ __global__ __launch_bounds__(256) void la_decay_kernel(LaArgs a, LaDecay d) {
         const int t = hi - 1 - static_cast<int>(threadIdx.x);
         double x = 0.0;
         if (t >= t0) {
-            float q = 0.0f, k = 0.0f;
-            for (int i = 0; i < d.parts; ++i) {
-                const int64_t at = (static_cast<int64_t>(i) * a.B * a.H + seq) * a.L + t;
-                q += d.dot_q[at];
-                k += d.dot_k[at];
-            }
-            x = static_cast<double>(q) - static_cast<double>(k);
+            const int64_t at = seq * a.L + t;
+            x = static_cast<double>(d.dot_q[at]) - static_cast<double>(d.dot_k[at]);
         }
         for (int m = 1; m < 64; m <<= 1) {   // inclusive sums over the lanes
             const double y = __shfl_up(x, m);
@@ -216,6 +217,20 @@ int64_t la_segments(const mogt_linear_attn_problem* q) {
     return n > 0 ? n : 1;
 }
 
+// Rows of a segment are addressed by 32-bit byte offsets.
+int la_check_rows(const mogt_linear_attn_problem* q) {
+    const int64_t es = q->io_dtype == MOGT_BF16 ? 2 : 4, most = 0x7fffffff;
+    const int64_t steps = q->segment < q->length ? q->segment : q->length;
+    if (q->q_row < 0 || q->k_row < 0 || q->v_row < 0 || q->g_row < 0)
+        return set_error(MOGT_E_INVALID, "negative row strides");
+    int64_t row = q->heads * (q->key_dim > q->value_dim ? q->key_dim : q->value_dim) * 4 / es;   // of fp32 outputs
+    for (const int64_t r : {q->q_row, q->k_row, q->v_row, q->g_row * 4 / es}) row = r > row ? r : row;
+    if (row > most / es || row * es * (steps > 0 ? steps : 1) > most - 1024)
+        return set_error(MOGT_E_INVALID, "segment of %lld rows %lld elements apart: below 2^31 bytes expected",
+                         (long long)steps, (long long)row);
+    return MOGT_OK;
+}
+
 int la_args(const mogt_linear_attn_problem* q, LaArgs& a) {
     if (const int rc = la_check(q)) return rc;
     const int chunk = q->io_dtype == MOGT_BF16 ? LaChunk<bf16_t>::T : LaChunk<float>::T;
@@ -223,6 +238,7 @@ int la_args(const mogt_linear_attn_problem* q, LaArgs& a) {
         return set_error(MOGT_E_INVALID, "segment of %lld steps: a multiple of %d expected", (long long)q->segment, chunk);
     const int64_t nseg = la_segments(q);
     if (nseg > (1 << 20)) return set_error(MOGT_E_INVALID, "%lld segments: at most 2^20", (long long)nseg);
+    if (const int rc = la_check_rows(q)) return rc;
     a.g = q->log_decay;
     a.g_row = q->g_row; a.g_batch = q->g_batch; a.g_head = q->g_head;
     a.lengths = q->lengths;
@@ -271,9 +287,10 @@ LaPass la_pass(const mogt_linear_attn_problem* q, const LaRows& query, const LaR
     p.q = query; p.k = key; p.v = value; p.x = value;
     p.dc = keys ? dk : dv;
     p.dn = keys ? dv : dk;
-    p.nvb = (p.dn + LA_NV - 1) / LA_NV;
-    p.rs = keys ? dv : 1;
-    p.cs = keys ? 1 : dv;
+    p.rs = keys ? 1 : dk;
+    p.cs = keys ? dk : 1;
+    p.user_rs = keys ? dv : 1;
+    p.user_cs = keys ? 1 : dv;
     p.qs = p.ps = p.ws = 1.0f;
     return p;
 }
@@ -285,8 +302,8 @@ void la_launch(const mogt_linear_attn_problem* q, const LaArgs& a, int count, bo
         la_launch_passes<float>(a, count, out, st);
 }
 
-void la_carry(const LaArgs& a, float* states, const float* ctot, const float* init, hipStream_t st) {
-    la_carry_kernel<<<dim3((a.state + 255) / 256, a.H, a.B), 256, 0, st>>>(states, ctot, init, a.nseg, a.state);
+void la_carry(const LaArgs& a, int dk, float* states, const float* ctot, const float* init, hipStream_t st) {
+    la_carry_kernel<<<dim3((a.state + 255) / 256, a.H, a.B), 256, 0, st>>>(states, ctot, init, a.nseg, dk, a.state / dk);
 }
 
 size_t al(size_t x) { return round_up(x, 256); }
@@ -331,7 +348,7 @@ extern "C" int mogt_linear_attn_fwd(const mogt_linear_attn_problem* q, void* out
     p.out = out;
     if (a.nseg > 1) {
         la_launch(q, a, 1, false, st);
-        la_carry(a, p.states, p.ctot, p.init, st);
+        la_carry(a, static_cast<int>(q->key_dim), p.states, p.ctot, p.init, st);
     }
     p.qs = p.ps = q->scale;
     la_launch(q, a, 1, true, st);
@@ -341,8 +358,8 @@ extern "C" int mogt_linear_attn_fwd(const mogt_linear_attn_problem* q, void* out
 extern "C" size_t mogt_linear_attn_bwd_workspace_bytes(const mogt_linear_attn_problem* q) {
     LaArgs a{};
     if (la_args(q, a) != MOGT_OK) return 0;
-    const size_t rows = static_cast<size_t>(q->batch) * q->length * q->heads, parts = (q->key_dim + LA_NV - 1) / LA_NV;
-    return la_states_bytes(q) + la_ctot_bytes(q) + 2 * al(parts * rows * 4) +
+    const size_t rows = static_cast<size_t>(q->batch) * q->length * q->heads;
+    return la_states_bytes(q) + la_ctot_bytes(q) + 2 * al(rows * 4) +
            al(static_cast<size_t>(q->batch * q->heads * a.nseg) * 8) +
            (q->heads > q->groups ? 2 * al(rows * q->key_dim * 4) : 0);
 }
@@ -361,7 +378,6 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
         return set_error(MOGT_E_WORKSPACE, "workspace of %zu bytes expected, got %zu", need, workspace ? workspace_bytes : 0);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const size_t rows = static_cast<size_t>(q->batch) * q->length * q->heads;
-    const int parts = static_cast<int>((q->key_dim + LA_NV - 1) / LA_NV);
     char* w = static_cast<char*>(workspace);
     auto take = [&](size_t bytes) {
         char* p = w;
@@ -370,8 +386,8 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
     };
     float* rstates = reinterpret_cast<float*>(take(la_states_bytes(q)));
     float* rctot = reinterpret_cast<float*>(take(la_ctot_bytes(q)));
-    float* dot_q = reinterpret_cast<float*>(take(al(parts * rows * 4)));
-    float* dot_k = reinterpret_cast<float*>(take(al(parts * rows * 4)));
+    float* dot_q = reinterpret_cast<float*>(take(al(rows * 4)));
+    float* dot_k = reinterpret_cast<float*>(take(al(rows * 4)));
     double* part = reinterpret_cast<double*>(take(al(static_cast<size_t>(q->batch * q->heads * a.nseg) * 8)));
     const bool shared = q->heads > q->groups;
     float* share_q = shared ? reinterpret_cast<float*>(take(al(rows * q->key_dim * 4))) : nullptr;
@@ -404,7 +420,7 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
     if (a.nseg > 1) {
         a.pass[0] = dv;
         la_launch(q, a, 1, false, st);
-        la_carry(a, rstates, rctot, dfinal_state, st);
+        la_carry(a, static_cast<int>(q->key_dim), rstates, rctot, dfinal_state, st);
     }
     // every pass that is asked for; the decays' gradient takes the products of
     // dq and dk, it and the initial state's the gradients of the states
@@ -413,10 +429,11 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
     if (g->dv || need_g || g->dinitial_state) todo[count++] = dv;
     if (g->dk || need_g) todo[count++] = dk;
     if (g->dq || need_g) todo[count++] = dq;
-    for (int i = 0; i < count;) {   // those of one padded width in one launch
+    for (int i = 0; i < count;) {   // those of one kind in one launch
         int m = 0;
-        const int width = la_width(todo[i].dc);
-        while (i < count && la_width(todo[i].dc) == width) a.pass[m++] = todo[i++];
+        do
+            a.pass[m++] = todo[i++];
+        while (i < count && la_one_kind(a.pass[0], todo[i]));
         la_launch(q, a, m, true, st);
     }
     if (need_g || g->dinitial_state) {
@@ -425,7 +442,7 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
         d.rstates = rstates;
         d.dot_q = dot_q;
         d.dot_k = dot_k;
-        d.parts = parts;
+            d.dk = static_cast<int>(q->key_dim);
         d.have_last = dfinal_state != nullptr;
         d.dinit = g->dinitial_state;
         if (need_g) {

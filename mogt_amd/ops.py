@@ -2952,25 +2952,41 @@ def ssm_step(x: torch.Tensor, state: torch.Tensor, delta: torch.Tensor, A: torch
 # ---------------------------------------------------------------------------
 LINEAR_ATTN_MAX_DIM = 128
 LINEAR_ATTN_CHUNK = {torch.bfloat16: 64, torch.float32: 32}   # steps of a chunk; a segment is whole chunks
-# Work-groups that a call is cut into segments for, and the least steps of one.
+# Work-groups that a call is cut into segments for: three or four a compute unit,
+# two where states are wider than 64 (their kernels fill one with two, and a state is
+# 64 KB to carry).  Forward passes: 2 x 8192 steps of 12 heads of 64 take 60 us with
+# 768 groups, 66 with 512 and 80 with 256; 32768 steps of 16 heads of 128 take 331 us
+# with 1024, 319 with 512 and 350 with 384.
 LINEAR_ATTN_GROUPS = 1024
-LINEAR_ATTN_MIN_SEGMENT = 256
+LINEAR_ATTN_WIDE_GROUPS = 512
+LINEAR_ATTN_MIN_SEGMENT = 256   # the least steps of a segment
+LINEAR_ATTN_SEGMENT_BYTES = 0x7fffffff - 1024   # of a segment's rows, addressed by 32-bit offsets
 
 
-def _linear_attn_segment(B: int, L: int, H: int, dv: int, dtype: torch.dtype) -> int:
+def _linear_attn_segment(B: int, L: int, H: int, dk: int, dv: int, dtype: torch.dtype) -> int:
     """Steps of a segment, whole chunks."""
     chunk = LINEAR_ATTN_CHUNK[dtype]
-    want = -(-LINEAR_ATTN_GROUPS // max(1, B * H * -(-dv // 64)))
+    want = -(-(LINEAR_ATTN_GROUPS if max(dk, dv) <= 64 else LINEAR_ATTN_WIDE_GROUPS) // max(1, B * H))
     steps = max(LINEAR_ATTN_MIN_SEGMENT, -(-L // want), -(-L // (1 << 20)))
-    return chunk * -(-steps // chunk)
+    most = LINEAR_ATTN_SEGMENT_BYTES // (4 * max(1, H) * max(dk, dv))
+    return chunk * max(1, min(-(-steps // chunk), most // chunk))
+
+
+def _linear_attn_rows(t: torch.Tensor, steps: int) -> torch.Tensor:
+    """Rows with unit stride in a head, near enough for a segment's offsets."""
+    t = _unit_channels(t)
+    return t if t.ndim < 4 or t.stride(1) * t.element_size() * steps <= LINEAR_ATTN_SEGMENT_BYTES else t.contiguous()
 
 
 def _linear_attn_problem(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
                          initial_state: torch.Tensor | None, lengths: torch.Tensor | None, scale: float, segment: int):
     """The C problem and the tensors it points into; rows ``[B, L, heads, d]``,
     or ``[B, heads, d]`` for a step."""
-    q, k, v, initial_state, lengths = (_unit_channels(q), _unit_channels(k), _unit_channels(v), _dense(initial_state),
-                                       _dense(lengths))
+    steps = min(segment, v.shape[1])
+    q, k, v, initial_state, lengths = (_linear_attn_rows(q, steps), _linear_attn_rows(k, steps),
+                                       _linear_attn_rows(v, steps), _dense(initial_state), _dense(lengths))
+    if log_decay.ndim == 3 and log_decay.stride(1) * 4 * steps > LINEAR_ATTN_SEGMENT_BYTES:
+        log_decay = log_decay.contiguous()
     qs, ks, vs, gs = q.stride(), k.stride(), v.stride(), log_decay.stride()
     per_head = log_decay.ndim == 1
     step = q.ndim == 3
@@ -2992,11 +3008,11 @@ def _linear_attn_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     lib = _lib.load()
     B, L, H, dv = v.shape
     dk = q.shape[-1]
-    segment = _linear_attn_segment(B, L, H, dv, v.dtype)
+    segment = _linear_attn_segment(B, L, H, dk, dv, v.dtype)
     f32 = dict(dtype=torch.float32, device=v.device)
     out = torch.empty((B, L, H, dv), dtype=v.dtype, device=v.device)
     state = torch.empty((B, H, dk, dv) if want_state else (0,), **f32)
-    carries = torch.empty((B, H, max(1, -(-L // segment)) + 1, dk, dv) if want_carries else (0,), **f32)
+    carries = torch.empty((B, H, max(1, -(-L // segment)) + 1, dv, dk) if want_carries else (0,), **f32)
     p, held = _linear_attn_problem(q, k, v, log_decay, initial_state, lengths, scale, segment)
     nbytes = lib.mogt_linear_attn_workspace_bytes(p)
     ws = scratch(nbytes, v.device) if nbytes else None
@@ -3012,9 +3028,9 @@ def _linear_attn_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
 def _(q, k, v, log_decay, initial_state, lengths, scale, want_state, want_carries):
     B, L, H, dv = v.shape
     dk = q.shape[-1]
-    segment = _linear_attn_segment(B, L, H, dv, v.dtype)
+    segment = _linear_attn_segment(B, L, H, dk, dv, v.dtype)
     return (v.new_empty((B, L, H, dv)), log_decay.new_empty((B, H, dk, dv) if want_state else (0,)),
-            log_decay.new_empty((B, H, max(1, -(-L // segment)) + 1, dk, dv) if want_carries else (0,)))
+            log_decay.new_empty((B, H, max(1, -(-L // segment)) + 1, dv, dk) if want_carries else (0,)))
 
 
 @_op("mogt::linear_attention_grad")
@@ -3027,8 +3043,8 @@ def _linear_attn_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, q: tor
     lib = _lib.load()
     B, L, H, dv = v.shape
     G, dk = q.shape[-2:]
-    segment = _linear_attn_segment(B, L, H, dv, v.dtype)
-    if carries.shape != (B, H, max(1, -(-L // segment)) + 1, dk, dv):
+    segment = _linear_attn_segment(B, L, H, dk, dv, v.dtype)
+    if carries.shape != (B, H, max(1, -(-L // segment)) + 1, dv, dk):
         raise ValueError(f"linear_attention_grad: carries {list(carries.shape)} are not those of a forward over "
                          f"segments of {segment} steps")
     dout = _dense(dout if dout.dtype == v.dtype else dout.to(v.dtype))

@@ -64,7 +64,7 @@ def run_both(t, kw, seed=1, **more):
     leaves = {n: x.detach().requires_grad_(True) for n, x in t.items() if x is not None}
     out, state = call(leaves, kw, return_state=True, **more)
     grads = dict(zip(leaves, torch.autograd.grad([out, state], list(leaves.values()), [dout, dstate])))
-    segment = ops._linear_attn_segment(B, L, H, dv, t["v"].dtype)
+    segment = ops._linear_attn_segment(B, L, H, t["q"].shape[-1], dv, t["v"].dtype)
     want, mag = [lo.linear_attention(t["q"], t["k"], t["v"], t["log_decay"], initial_state=t["initial_state"],
                                      dout=dout, dstate=dstate, mag=m, segment=segment, **kw, **more) for m in (0, 1)]
     tol = bound(t)
