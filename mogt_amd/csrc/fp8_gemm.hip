@@ -13,8 +13,8 @@
 // Tiles: a work-group of MW x NW waves, a wave 16 MT rows of x by 16 NT rows of w.
 // D[row of w][row of x]: a lane's results are four consecutive outputs of one row,
 // its row's scale one factor.  Stages of one block of K, two in LDS, filled by
-// direct loads: 128-byte rows, 16-byte chunk c of row r at place c ^ r % 8 (no bank
-// conflicts).  A lane's 32 values of an operand are chunks g and g + 4 (g = lane /
+// direct loads: 128-byte rows, their 16-byte chunks at places that give no bank
+// conflicts (f8_twist).  A lane's 32 values of an operand are chunks g and g + 4 (g = lane /
 // 16), the same of both operands, which is an order of the sum only.  Rows past the
 // end and chunks past K load zeros.
 //
@@ -40,31 +40,47 @@ struct F8Gemm {
     int nm, nn;          // tiles
 };
 
-// the block's product of 16 rows of w by 16 rows of x
-template <bool EXACT>
-__device__ __forceinline__ f8_f4 f8_block(f8_i8 w, f8_i8 x) {
-    f8_f4 d = {0, 0, 0, 0};
-    if constexpr (!EXACT) {
-        // scales of one (2^(127 - 127))
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, d, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-    } else {
+// An operand's 32 values of a lane as the matrix instruction takes them.
+template <bool EXACT> struct F8Operand;
+template <> struct F8Operand<false> {
+    f8_i8 v;
+    __device__ __forceinline__ F8Operand() {}
+    __device__ __forceinline__ F8Operand(f8_i4 lo, f8_i4 hi) : v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]} {}
+};
+template <> struct F8Operand<true> {
+    f8_b8 v[4];
+    __device__ __forceinline__ F8Operand() {}
+    __device__ __forceinline__ F8Operand(f8_i4 lo, f8_i4 hi) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f8_b8 a, b;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const f8_b2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * i + j], 1.0f, false);
-                const f8_b2 a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * i + j], 1.0f, true);
-                const f8_b2 b0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * i + j], 1.0f, false);
-                const f8_b2 b1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * i + j], 1.0f, true);
-                a[4 * j] = a0[0]; a[4 * j + 1] = a0[1]; a[4 * j + 2] = a1[0]; a[4 * j + 3] = a1[1];
-                b[4 * j] = b0[0]; b[4 * j + 1] = b0[1]; b[4 * j + 2] = b1[0]; b[4 * j + 3] = b1[1];
+                const int u = i < 2 ? lo[2 * i + j] : hi[2 * i - 4 + j];
+                const f8_b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, 1.0f, false);
+                const f8_b2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, 1.0f, true);
+                v[i][4 * j] = a[0];
+                v[i][4 * j + 1] = a[1];
+                v[i][4 * j + 2] = b[0];
+                v[i][4 * j + 3] = b[1];
             }
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, d, 0, 0, 0);
-        }
-        return d;
     }
+};
+
+// the block's product of 16 rows of w by 16 rows of x
+__device__ __forceinline__ f8_f4 f8_block(const F8Operand<false>& w, const F8Operand<false>& x) {
+    // scales of one (2^(127 - 127))
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f8_f4{0, 0, 0, 0}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
 }
+__device__ __forceinline__ f8_f4 f8_block(const F8Operand<true>& w, const F8Operand<true>& x) {
+    f8_f4 d = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], d, 0, 0, 0);
+    return d;
+}
+
+// Chunk c of row r lies at place c ^ f8_twist(r): the 16 rows of a fragment's reads, two
+// rows to the banks' width, fall into distinct banks.
+__device__ __forceinline__ int f8_twist(int row) { return (row >> 1) & 7; }
 
 template <bool EXACT>
 __device__ __forceinline__ void f8_store(const F8Gemm& p, int64_t m, int n, f8_f4 v) {
@@ -88,6 +104,7 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
     constexpr int LOADS = ROWS / 8 / WAVES;   // 1 KB loads of a wave and stage
     static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && NT * 16 <= 128 && 128 % (NT * 16) == 0, "tile");
     __shared__ __attribute__((aligned(1024))) char smem[2 * ROWS * 128];
+    __shared__ float s_xs[2][BM];   // scales of the rows of x
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 4;
     const int wm = wave / NW, wn = wave % NW;
     // an XCD takes a run of tiles, eight row blocks at a time (its L2 keeps their rows)
@@ -105,19 +122,24 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
     const lds_i32x4 rx = lds_rsrc(p.x + m0 * p.ldx, static_cast<uint32_t>((mrows - 1) * p.ldx + p.K));
     const lds_i32x4 rw = lds_rsrc(p.w + static_cast<int64_t>(n0) * p.K, static_cast<uint32_t>(nrows) * p.K);
     const uint32_t lds0 = lds_addr(smem);
-    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;   // of the row, where LDS place lane % 8 is filled
+    // lane's place lane % 8 of row 8 i + lane / 8 takes the chunk that the twist puts there
+    int chunk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) chunk[i] = ((lane & 7) ^ f8_twist(8 * i + (lane >> 3))) * 16;
     constexpr int OUTSIDE = 0x7ffffff0;
+    static_assert(WAVES % 2 == 0, "rows of one parity of eight a wave");
+    const int ch = chunk[0] * (1 - (wave & 1)) + chunk[1] * (wave & 1);   // 8 (i WAVES + wave) rows on: the wave's parity
     int off[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
         const int r = (i * WAVES + wave) * 8 + (lane >> 3);   // rows of x, then of w
         if (i < BM / 8 / WAVES)
-            off[i] = r < mrows ? static_cast<int>(r * p.ldx) + chunk : OUTSIDE;
+            off[i] = r < mrows ? static_cast<int>(r * p.ldx) + ch : OUTSIDE;
         else
-            off[i] = r - BM < nrows ? (r - BM) * p.K + chunk : OUTSIDE;
+            off[i] = r - BM < nrows ? (r - BM) * p.K + ch : OUTSIDE;
     }
     auto issue = [&](int s) {
-        const bool in = s * 128 + chunk < p.K;
+        const bool in = s * 128 + ch < p.K;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
             lds_dma16(i < BM / 8 / WAVES ? rx : rw, in && off[i] != OUTSIDE ? off[i] + s * 128 : OUTSIDE, 0,
@@ -128,47 +150,52 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f8_f4{0, 0, 0, 0};
-    // scales of the lane's rows of x and of the wave's rows of w
-    const float* xs[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-        xs[i] = p.xs + min(m0 + (wm * MT + i) * 16 + (lane & 15), p.M - 1) * p.kb;
+    // scales: a thread's row of x, and the wave's rows of w
+    const float* xs = p.xs + min(m0 + tid % BM, p.M - 1) * p.kb;
     const float* ws = p.ws + static_cast<int64_t>(min(n0 + wn * NT * 16, p.N - 1) / 128) * p.kb;
-    float sx[MT], sw = ws[0];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sx[i] = xs[i][0];
+    float sx = xs[0], sw = ws[0];
     issue(0);
+    const int twist = f8_twist(lane & 15);   // of every row the lane reads: they are 16 apart
     for (int s = 0; s < p.kb; ++s) {
+        if (BM == 64 * WAVES || tid < BM) s_xs[s & 1][tid % BM] = sx;
         lds_wait_vm<0>();
         __syncthreads();
-        float f[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) f[i] = sx[i] * sw;
+        const float wscale = sw;
         if (s + 1 < p.kb) {
             issue(s + 1);
             sw = ws[s + 1];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) sx[i] = xs[i][s + 1];
+            sx = xs[s + 1];
         }
         const char* st = smem + (s & 1) * (ROWS * 128);
         auto frag = [&](int r) {
-            const char* q = st + r * 128;
-            const f8_i4 lo = *reinterpret_cast<const f8_i4*>(q + ((grp ^ (r & 7)) << 4));
-            const f8_i4 hi = *reinterpret_cast<const f8_i4*>(q + (((grp + 4) ^ (r & 7)) << 4));
-            return f8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            const char* q = st + (r + (lane & 15)) * 128;
+            return F8Operand<EXACT>(*reinterpret_cast<const f8_i4*>(q + ((grp ^ twist) << 4)),
+                                    *reinterpret_cast<const f8_i4*>(q + (((grp + 4) ^ twist) << 4)));
         };
-        f8_i8 w[NT];
+        float f[MT];
+        F8Operand<EXACT> w[NT], x[2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j] = frag(BM + (wn * NT + j) * 16 + (lane & 15));
+        for (int j = 0; j < NT; ++j) w[j] = frag(BM + (wn * NT + j) * 16);
+        x[0] = frag(wm * MT * 16);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const f8_i8 x = frag((wm * MT + i) * 16 + (lane & 15));
+        for (int i = 0; i < MT; ++i) f[i] = s_xs[s & 1][(wm * MT + i) * 16 + (lane & 15)] * wscale;
+        // A product's result is there some 12 cycles after the next one has begun: it is
+        // scaled three products later.  The order is held, or each would be waited for.
+        constexpr int LAG = 3;
+        f8_f4 d[LAG + 1];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const f8_f4 d = f8_block<EXACT>(w[j], x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], f[i], acc[i][j][e]);
+        for (int t = 0; t < MT * NT + LAG; ++t) {
+            if (t < MT * NT) {
+                const int i = t / NT, j = t % NT;
+                if (j == 0 && i + 1 < MT) x[(i + 1) & 1] = frag((wm * MT + i + 1) * 16);
+                d[t % (LAG + 1)] = f8_block(w[j], x[i & 1]);
             }
+            if (t >= LAG) {
+                const int u = t - LAG, i = u / NT, j = u % NT;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[u % (LAG + 1)][e], f[i], acc[i][j][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 #pragma unroll
@@ -206,14 +233,14 @@ __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
         f8_i4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
         if (k < p.K) lo = *reinterpret_cast<const f8_i4*>(row + k);
         if (k + 64 < p.K) hi = *reinterpret_cast<const f8_i4*>(row + k + 64);
-        return f8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        return F8Operand<EXACT>(lo, hi);
     };
 #pragma unroll 4
     for (int s = wave; s < p.kb; s += 4) {
-        const f8_i8 w = frag(wr, s);
+        const F8Operand<EXACT> w = frag(wr, s);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const f8_f4 d = f8_block<EXACT>(w, frag(xr[i], s));
+            const f8_f4 d = f8_block(w, frag(xr[i], s));
             const float f = xs[i][s] * ws[s];
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(d[e], f, acc[i][e]);
@@ -247,9 +274,16 @@ void f8_launch(F8Gemm& p, hipStream_t st) {
         p.nn = (p.N + bn - 1) / bn;
         return p.nm * p.nn;
     };
-    if (tiles(256, 256) >= 200)
+    if constexpr (EXACT) {
+        if (tiles(128, 256) >= 200) {
+            f8_gemm_kernel<2, 4, 4, 4, EXACT><<<p.nm * p.nn, 512, 0, st>>>(p);
+            return;
+        }
+    } else if (tiles(256, 256) >= 200) {
         f8_gemm_kernel<2, 4, 8, 4, EXACT><<<p.nm * p.nn, 512, 0, st>>>(p);
-    else {
+        return;
+    }
+    {
         tiles(64, 128);
         f8_gemm_kernel<2, 2, 2, 4, EXACT><<<p.nm * p.nn, 256, 0, st>>>(p);
     }
