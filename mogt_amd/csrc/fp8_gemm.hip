@@ -38,6 +38,7 @@ struct F8Gemm {
     int64_t M, ldx, ldy;
     int N, K, kb;
     int nm, nn;          // tiles
+    int whole;           // rows of y are whole 16 bytes, a tile's within 2^31 bytes
 };
 
 // An operand's 32 values of a lane as the matrix instruction takes them.
@@ -78,6 +79,13 @@ __device__ __forceinline__ f8_f4 f8_block(const F8Operand<true>& w, const F8Oper
     return d;
 }
 
+// x, which the compiler takes for a new value: what follows from it is formed again
+// where it is needed, not held in registers from tile to tile.
+__device__ __forceinline__ int f8_again(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // Chunk c of row r lies at place c ^ f8_twist(r): the 16 rows of a fragment's reads, two
 // rows to the banks' width, fall into distinct banks.
 __device__ __forceinline__ int f8_twist(int row) { return (row >> 1) & 7; }
@@ -98,115 +106,185 @@ __device__ __forceinline__ void f8_store(const F8Gemm& p, int64_t m, int n, f8_f
     }
 }
 
+// Tiles of work-group `bid` of `grid` (a multiple of 8, or all of n): its XCD (ids
+// mod 8) takes a run of them, dealt to the XCD's work-groups in turn.
+struct F8Walk {
+    int next, step, end;
+};
+__device__ __forceinline__ F8Walk f8_walk(int n, int grid, int bid) {
+    const int xcd = bid % 8, q = n / 8, rem = n % 8;
+    const int first = xcd * q + min(xcd, rem);
+    return F8Walk{first + bid / 8, (grid - xcd + 7) / 8, first + q + (xcd < rem ? 1 : 0)};
+}
+
 template <int MW, int NW, int MT, int NT, bool EXACT>
 __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
+    typedef typename std::conditional<EXACT, float, bf16_t>::type TO;
     constexpr int BM = MW * MT * 16, BN = NW * NT * 16, WAVES = MW * NW, ROWS = BM + BN;
     constexpr int LOADS = ROWS / 8 / WAVES;   // 1 KB loads of a wave and stage
+    constexpr int STAGE = ROWS * 128, OUTSIDE = 0x7ffffff0;
     static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && NT * 16 <= 128 && 128 % (NT * 16) == 0, "tile");
-    __shared__ __attribute__((aligned(1024))) char smem[2 * ROWS * 128];
+    static_assert(WAVES % 2 == 0, "a wave's loads fill rows of one parity of eights");
+    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
     __shared__ float s_xs[2][BM];   // scales of the rows of x
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 4;
     const int wm = wave / NW, wn = wave % NW;
-    // an XCD takes a run of tiles, eight row blocks at a time (its L2 keeps their rows)
-    int mb, nb;
-    {
-        const int n = p.nm * p.nn, xcd = blockIdx.x % 8, loc = blockIdx.x / 8, q = n / 8, rem = n % 8;
-        const int v = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + loc;
-        const int group = 8 * p.nn, g = v / group, gm = min(p.nm - 8 * g, 8), in = v - g * group;
-        mb = 8 * g + in % gm;
-        nb = in / gm;
-    }
-    const int64_t m0 = static_cast<int64_t>(mb) * BM;
-    const int n0 = nb * BN;
-    const int mrows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(BM))), nrows = min(p.N - n0, BN);
-    const lds_i32x4 rx = lds_rsrc(p.x + m0 * p.ldx, static_cast<uint32_t>((mrows - 1) * p.ldx + p.K));
-    const lds_i32x4 rw = lds_rsrc(p.w + static_cast<int64_t>(n0) * p.K, static_cast<uint32_t>(nrows) * p.K);
     const uint32_t lds0 = lds_addr(smem);
-    // lane's place lane % 8 of row 8 i + lane / 8 takes the chunk that the twist puts there
-    int chunk[2];
+    const int twist = f8_twist(lane & 15);   // of every row the lane reads: they are 16 apart
+    // place lane % 8 of row lane / 8 of a load takes the chunk that the twist puts there
+    const int ch = ((lane & 7) ^ f8_twist((wave & 1) * 8 + (lane >> 3))) * 16;
+
+    // the tile whose stages are being loaded
+    int64_t m0;
+    int n0, off[LOADS];
+    lds_i32x4 rx, rw;
+    const float *xs, *ws;
+    auto enter = [&](int v) __attribute__((always_inline)) {
+        // eight row blocks at a time (an XCD's L2 keeps their rows)
+        const int group = 8 * p.nn, g = v / group, gm = min(p.nm - 8 * g, 8), in = v - g * group;
+        const int mb = __builtin_amdgcn_readfirstlane(8 * g + in % gm), nb = __builtin_amdgcn_readfirstlane(in / gm);
+        m0 = static_cast<int64_t>(mb) * BM;
+        n0 = nb * BN;
+        const int mrows = static_cast<int>(min(p.M - m0, static_cast<int64_t>(BM))), nrows = min(p.N - n0, BN), l = f8_again(lane);
+        rx = lds_rsrc(p.x + m0 * p.ldx, static_cast<uint32_t>((mrows - 1) * p.ldx + p.K));
+        rw = lds_rsrc(p.w + static_cast<int64_t>(n0) * p.K, static_cast<uint32_t>(nrows) * p.K);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) chunk[i] = ((lane & 7) ^ f8_twist(8 * i + (lane >> 3))) * 16;
-    constexpr int OUTSIDE = 0x7ffffff0;
-    static_assert(WAVES % 2 == 0, "rows of one parity of eight a wave");
-    const int ch = chunk[0] * (1 - (wave & 1)) + chunk[1] * (wave & 1);   // 8 (i WAVES + wave) rows on: the wave's parity
-    int off[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int r = (i * WAVES + wave) * 8 + (lane >> 3);   // rows of x, then of w
-        if (i < BM / 8 / WAVES)
-            off[i] = r < mrows ? static_cast<int>(r * p.ldx) + ch : OUTSIDE;
-        else
-            off[i] = r - BM < nrows ? (r - BM) * p.K + ch : OUTSIDE;
-    }
-    auto issue = [&](int s) {
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = (i * WAVES + wave) * 8 + (l >> 3);   // rows of x, then of w
+            if (i < BM / 8 / WAVES)
+                off[i] = r < mrows ? static_cast<int>(r * p.ldx) + ch : OUTSIDE;
+            else
+                off[i] = r - BM < nrows ? (r - BM) * p.K + ch : OUTSIDE;
+        }
+        // scales: a thread's row of x, and the wave's rows of w
+        xs = p.xs + min(m0 + tid % BM, p.M - 1) * p.kb;
+        ws = p.ws + static_cast<int64_t>(min(n0 + wn * NT * 16, p.N - 1) / 128) * p.kb;
+    };
+    float sx, sw;
+    auto issue = [&](int s, int buf) __attribute__((always_inline)) {
         const bool in = s * 128 + ch < p.K;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
             lds_dma16(i < BM / 8 / WAVES ? rx : rw, in && off[i] != OUTSIDE ? off[i] + s * 128 : OUTSIDE, 0,
-                      lds0 + (s & 1) * (ROWS * 128) + (i * WAVES + wave) * 1024);
+                      lds0 + buf * STAGE + (i * WAVES + wave) * 1024);
+        sw = ws[s];
+        sx = xs[s];
     };
-    f8_f4 acc[MT][NT];
+
+    F8Walk walk = f8_walk(p.nm * p.nn, gridDim.x, blockIdx.x);
+    if (walk.next >= walk.end) return;
+    enter(walk.next);
+    issue(0, 0);
+    // stores of the tile before, issued after this one's first loads
+    constexpr int OUT_ROW = NT * 16 * sizeof(TO), CH = OUT_ROW / 16, STORES = MT * 16 * OUT_ROW / 1024;
+    bool stored = false;
+    int buf = 0;
+    while (true) {
+        const int64_t m1 = m0;   // the tile being multiplied
+        const int n1 = n0;
+        const bool more = walk.next + walk.step < walk.end;
+        f8_f4 acc[MT][NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f8_f4{0, 0, 0, 0};
-    // scales: a thread's row of x, and the wave's rows of w
-    const float* xs = p.xs + min(m0 + tid % BM, p.M - 1) * p.kb;
-    const float* ws = p.ws + static_cast<int64_t>(min(n0 + wn * NT * 16, p.N - 1) / 128) * p.kb;
-    float sx = xs[0], sw = ws[0];
-    issue(0);
-    const int twist = f8_twist(lane & 15);   // of every row the lane reads: they are 16 apart
-    for (int s = 0; s < p.kb; ++s) {
-        if (BM == 64 * WAVES || tid < BM) s_xs[s & 1][tid % BM] = sx;
-        lds_wait_vm<0>();
-        __syncthreads();
-        const float wscale = sw;
-        if (s + 1 < p.kb) {
-            issue(s + 1);
-            sw = ws[s + 1];
-            sx = xs[s + 1];
-        }
-        const char* st = smem + (s & 1) * (ROWS * 128);
-        auto frag = [&](int r) {
-            const char* q = st + (r + (lane & 15)) * 128;
-            return F8Operand<EXACT>(*reinterpret_cast<const f8_i4*>(q + ((grp ^ twist) << 4)),
-                                    *reinterpret_cast<const f8_i4*>(q + (((grp + 4) ^ twist) << 4)));
-        };
-        float f[MT];
-        F8Operand<EXACT> w[NT], x[2];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) w[j] = frag(BM + (wn * NT + j) * 16);
-        x[0] = frag(wm * MT * 16);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) f[i] = s_xs[s & 1][(wm * MT + i) * 16 + (lane & 15)] * wscale;
-        // A product's result is there some 12 cycles after the next one has begun: it is
-        // scaled three products later.  The order is held, or each would be waited for.
-        constexpr int LAG = 3;
-        f8_f4 d[LAG + 1];
-#pragma unroll
-        for (int t = 0; t < MT * NT + LAG; ++t) {
-            if (t < MT * NT) {
-                const int i = t / NT, j = t % NT;
-                if (j == 0 && i + 1 < MT) x[(i + 1) & 1] = frag((wm * MT + i + 1) * 16);
-                d[t % (LAG + 1)] = f8_block(w[j], x[i & 1]);
+            for (int j = 0; j < NT; ++j) acc[i][j] = f8_f4{0, 0, 0, 0};
+        for (int s = 0; s < p.kb; ++s, buf ^= 1) {
+            if (BM == 64 * WAVES || tid < BM) s_xs[buf][tid % BM] = sx;
+            const float wscale = sw;
+            if (s == 0 && stored)
+                lds_wait_vm<STORES>();
+            else
+                lds_wait_vm<0>();
+            __syncthreads();
+            if (s + 1 < p.kb) {
+                issue(s + 1, buf ^ 1);
+            } else if (more) {   // the next tile's first stage loads while this one's last is multiplied
+                walk.next += walk.step;
+                enter(walk.next);
+                issue(0, buf ^ 1);
             }
-            if (t >= LAG) {
-                const int u = t - LAG, i = u / NT, j = u % NT;
+            // the lane's two chunks of a row, which lie 64 bytes apart (bit 2 of the place)
+            const char* lo = smem + buf * STAGE + (lane & 15) * 128 + ((grp ^ twist) << 4);
+            const char* hi = smem + buf * STAGE + (lane & 15) * 128 + (((grp ^ twist) << 4) ^ 64);
+            auto frag = [&](int r) __attribute__((always_inline)) {
+                return F8Operand<EXACT>(*reinterpret_cast<const f8_i4*>(lo + r * 128), *reinterpret_cast<const f8_i4*>(hi + r * 128));
+            };
+            float f[MT];
+            F8Operand<EXACT> w[NT], x[2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[u % (LAG + 1)][e], f[i], acc[i][j][e]);
+            for (int j = 0; j < NT; ++j) w[j] = frag(BM + (wn * NT + j) * 16);
+            x[0] = frag(wm * MT * 16);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) f[i] = s_xs[buf][(wm * MT + i) * 16 + (lane & 15)] * wscale;
+            // A product's result is there some 12 cycles after the next one has begun: it is
+            // scaled three products later.  The order is held, or each would be waited for.
+            constexpr int LAG = 3;
+            f8_f4 d[LAG + 1];
+#pragma unroll
+            for (int t = 0; t < MT * NT + LAG; ++t) {
+                if (t < MT * NT) {
+                    const int i = t / NT, j = t % NT;
+                    if (j == 0 && i + 1 < MT) x[(i + 1) & 1] = frag((wm * MT + i + 1) * 16);
+                    d[t % (LAG + 1)] = f8_block(w[j], x[i & 1]);
+                }
+                if (t >= LAG) {
+                    const int u = t - LAG, i = u / NT, j = u % NT;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[u % (LAG + 1)][e], f[i], acc[i][j][e]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
-    }
+        if (p.whole) {
+            // Through the last stage's LDS (no wave reads it any more), so that a row of the
+            // wave's leaves in whole lines: straight from the registers 16 rows' 32 bytes a
+            // store took 33 us a tile, more than its sixteen stages.
+            constexpr int ROOM = STAGE / WAVES / (16 * OUT_ROW), G = ROOM >= MT ? MT : ROOM >= 4 ? 4 : ROOM >= 2 ? 2 : 1;
+            static_assert(ROOM >= 1 && MT % G == 0, "a tile's rows fit");
+            __syncthreads();
+            const int l = f8_again(lane);
+            char* const mine = smem + (buf ^ 1) * STAGE + wave * (STAGE / WAVES / 16 * 16);
+            const int left = static_cast<int>(min(p.M - m1, static_cast<int64_t>(BM))) - wm * MT * 16, nw = p.N - n1 - wn * NT * 16;
+            const int ldy = static_cast<int>(p.ldy);
+            const auto ry = __builtin_amdgcn_make_buffer_rsrc(
+                static_cast<char*>(p.y) + (m1 * p.ldy + n1) * static_cast<int64_t>(sizeof(TO)), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t m = m0 + (wm * MT + i) * 16 + (lane & 15);
-        if (m >= p.M) continue;
+            for (int i0 = 0; i0 < MT; i0 += G) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int n = n0 + (wn * NT + j) * 16 + 4 * grp;
-            if (n < p.N) f8_store<EXACT>(p, m, n, acc[i][j]);
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const int r = 16 * i + (l & 15), byte = (16 * j + 4 * (l >> 4)) * static_cast<int>(sizeof(TO));
+                        Pack<TO, 4> v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v.v[e] = IO<TO>::st(acc[i0 + i][j][e]);
+                        *reinterpret_cast<Pack<TO, 4>*>(mine + r * OUT_ROW + ((byte >> 4 ^ (r & (CH - 1))) << 4) + (byte & 15)) = v;
+                    }
+                // only the wave's own rows: its reads wait for its writes
+#pragma unroll
+                for (int k = 0; k < G * 16 * OUT_ROW / 1024; ++k) {
+                    const int id = 64 * k + l, r = id / CH, c = id % CH;
+                    const f8_i4 v = *reinterpret_cast<const f8_i4*>(mine + r * OUT_ROW + ((c ^ (r & (CH - 1))) << 4));
+                    const int m = 16 * i0 + r, n = c * (16 / static_cast<int>(sizeof(TO)));
+                    const uint32_t at = static_cast<uint32_t>((wm * MT * 16 + m) * ldy + wn * NT * 16 + n) * static_cast<uint32_t>(sizeof(TO));
+                    const bool in = (m < left) & (n < nw);
+                    __builtin_amdgcn_raw_buffer_store_b128(v, ry, in ? at : 0xffffff00u, 0, 0);
+                }
+            }
+            stored = true;
+        } else {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int64_t m = m1 + (wm * MT + i) * 16 + (lane & 15);
+                if (m >= p.M) continue;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int n = n1 + (wn * NT + j) * 16 + 4 * grp;
+                    if (n < p.N) f8_store<EXACT>(p, m, n, acc[i][j]);
+                }
+            }
         }
+        if (!more) return;
     }
 }
 
@@ -258,7 +336,7 @@ __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
 }
 
 template <bool EXACT>
-void f8_launch(F8Gemm& p, hipStream_t st) {
+void f8_launch(F8Gemm& p, int cus, hipStream_t st) {
     if (p.M <= 64) {
         const unsigned grid = (p.N + 15) / 16;
         if (p.M <= 16)
@@ -274,18 +352,15 @@ void f8_launch(F8Gemm& p, hipStream_t st) {
         p.nn = (p.N + bn - 1) / bn;
         return p.nm * p.nn;
     };
-    if constexpr (EXACT) {
-        if (tiles(128, 256) >= 200) {
-            f8_gemm_kernel<2, 4, 4, 4, EXACT><<<p.nm * p.nn, 512, 0, st>>>(p);
-            return;
-        }
-    } else if (tiles(256, 256) >= 200) {
-        f8_gemm_kernel<2, 4, 8, 4, EXACT><<<p.nm * p.nn, 512, 0, st>>>(p);
-        return;
-    }
-    {
-        tiles(64, 128);
-        f8_gemm_kernel<2, 2, 2, 4, EXACT><<<p.nm * p.nn, 256, 0, st>>>(p);
+    const int each = EXACT ? 4 : 2;
+    p.whole = p.N * each % 16 == 0 && p.ldy * each * 256 < 0x7fffff00;
+    constexpr int BM = EXACT ? 128 : 256;
+    if (tiles(BM, 256) >= 200) {
+        const int n = tiles(BM, 256);
+        f8_gemm_kernel<2, 4, BM / 32, 4, EXACT><<<n < cus ? n : cus, 512, 0, st>>>(p);
+    } else {
+        const int n = tiles(64, 128);
+        f8_gemm_kernel<2, 2, 2, 4, EXACT><<<n < 3 * cus ? n : 3 * cus, 256, 0, st>>>(p);
     }
 }
 
@@ -312,11 +387,13 @@ extern "C" int mogt_linear_fp8(const void* x, int64_t ldx, const float* x_scale,
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(y)) & 15)
         return set_error(MOGT_E_INVALID, "operands and output must be 16-byte aligned");
     F8Gemm p{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(w), x_scale, w_scale, y, rows, ldx, outputs,
-             static_cast<int>(outputs), static_cast<int>(width), static_cast<int>((width + 127) / 128), 0, 0};
+             static_cast<int>(outputs), static_cast<int>(width), static_cast<int>((width + 127) / 128), 0, 0, 0};
+    int cus = 0;
+    if (const int rc = device_cu_count(cus)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (out_dtype == MOGT_F32)
-        f8_launch<true>(p, st);
+        f8_launch<true>(p, cus, st);
     else
-        f8_launch<false>(p, st);
+        f8_launch<false>(p, cus, st);
     return check_launch("mogt_linear_fp8");
 }
