@@ -124,6 +124,7 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
     constexpr int LOADS = ROWS / 8 / WAVES;   // 1 KB loads of a wave and stage
     constexpr int STAGE = ROWS * 128, OUTSIDE = 0x7ffffff0;
     static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && NT * 16 <= 128 && 128 % (NT * 16) == 0, "tile");
+    static_assert(LOADS <= MT * NT, "a load beside each product");
     static_assert(WAVES % 2 == 0, "a wave's loads fill rows of one parity of eights");
     __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
     __shared__ float s_xs[2][BM];   // scales of the rows of x
@@ -161,20 +162,20 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
         ws = p.ws + static_cast<int64_t>(min(n0 + wn * NT * 16, p.N - 1) / 128) * p.kb;
     };
     float sx, sw;
-    auto issue = [&](int s, int buf) __attribute__((always_inline)) {
-        const bool in = s * 128 + ch < p.K;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            lds_dma16(i < BM / 8 / WAVES ? rx : rw, in && off[i] != OUTSIDE ? off[i] + s * 128 : OUTSIDE, 0,
-                      lds0 + buf * STAGE + (i * WAVES + wave) * 1024);
-        sw = ws[s];
-        sx = xs[s];
+    // load i of stage s of the tile into buffer `buf` (s < 0: none left, nothing is read)
+    auto issue = [&](int i, int s, int buf) __attribute__((always_inline)) {
+        const bool in = (s >= 0) & (s * 128 + ch < p.K) & (off[i] != OUTSIDE);
+        lds_dma16(i < BM / 8 / WAVES ? rx : rw, in ? off[i] + s * 128 : OUTSIDE, 0,
+                  lds0 + buf * STAGE + (i * WAVES + wave) * 1024);
     };
 
     F8Walk walk = f8_walk(p.nm * p.nn, gridDim.x, blockIdx.x);
     if (walk.next >= walk.end) return;
     enter(walk.next);
-    issue(0, 0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) issue(i, 0, 0);
+    sw = ws[0];
+    sx = xs[0];
     // stores of the tile before, issued after this one's first loads
     constexpr int OUT_ROW = NT * 16 * sizeof(TO), CH = OUT_ROW / 16, STORES = MT * 16 * OUT_ROW / 1024;
     bool stored = false;
@@ -196,13 +197,6 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
             else
                 lds_wait_vm<0>();
             __syncthreads();
-            if (s + 1 < p.kb) {
-                issue(s + 1, buf ^ 1);
-            } else if (more) {   // the next tile's first stage loads while this one's last is multiplied
-                walk.next += walk.step;
-                enter(walk.next);
-                issue(0, buf ^ 1);
-            }
             // the lane's two chunks of a row, which lie 64 bytes apart (bit 2 of the place)
             const char* lo = smem + buf * STAGE + (lane & 15) * 128 + ((grp ^ twist) << 4);
             const char* hi = smem + buf * STAGE + (lane & 15) * 128 + (((grp ^ twist) << 4) ^ 64);
@@ -216,6 +210,20 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
             x[0] = frag(wm * MT * 16);
 #pragma unroll
             for (int i = 0; i < MT; ++i) f[i] = s_xs[buf][(wm * MT + i) * 16 + (lane & 15)] * wscale;
+            // the stage that loads meanwhile: this tile's next, or the next tile's first
+            int stage = s + 1;
+            if (stage == p.kb) {
+                stage = more ? 0 : -1;
+                if (more) {
+                    walk.next += walk.step;
+                    enter(walk.next);
+                }
+            }
+            if (stage >= 0) {
+                sw = ws[stage];
+                sx = xs[stage];
+            }
+            __builtin_amdgcn_sched_barrier(0);
             // A product's result is there some 12 cycles after the next one has begun: it is
             // scaled three products later.  The order is held, or each would be waited for.
             constexpr int LAG = 3;
@@ -227,6 +235,7 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
                     if (j == 0 && i + 1 < MT) x[(i + 1) & 1] = frag((wm * MT + i + 1) * 16);
                     d[t % (LAG + 1)] = f8_block(w[j], x[i & 1]);
                 }
+                if (t < LOADS) issue(t, stage, buf ^ 1);
                 if (t >= LAG) {
                     const int u = t - LAG, i = u / NT, j = u % NT;
 #pragma unroll
