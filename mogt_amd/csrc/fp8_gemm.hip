@@ -346,14 +346,12 @@ __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
 
 template <bool EXACT>
 void f8_launch(F8Gemm& p, int cus, hipStream_t st) {
-    if (p.M <= 64) {
+    if (p.M <= 32) {
         const unsigned grid = (p.N + 15) / 16;
         if (p.M <= 16)
             f8_gemv_kernel<1, EXACT><<<grid, 256, 0, st>>>(p);
-        else if (p.M <= 32)
-            f8_gemv_kernel<2, EXACT><<<grid, 256, 0, st>>>(p);
         else
-            f8_gemv_kernel<4, EXACT><<<grid, 256, 0, st>>>(p);
+            f8_gemv_kernel<2, EXACT><<<grid, 256, 0, st>>>(p);
         return;
     }
     auto tiles = [&](int bm, int bn) {
@@ -364,9 +362,12 @@ void f8_launch(F8Gemm& p, int cus, hipStream_t st) {
     const int each = EXACT ? 4 : 2;
     p.whole = p.N * each % 16 == 0 && p.ldy * each * 256 < 0x7fffff00;
     constexpr int BM = EXACT ? 128 : 256;
-    if (tiles(BM, 256) >= 200) {
+    if (tiles(BM, 256) >= (EXACT ? 2 * cus : cus * 3 / 4)) {
         const int n = tiles(BM, 256);
         f8_gemm_kernel<2, 4, BM / 32, 4, EXACT><<<n < cus ? n : cus, 512, 0, st>>>(p);
+    } else if (tiles(128, 128) >= cus) {
+        const int n = tiles(128, 128);
+        f8_gemm_kernel<2, 2, 4, 4, EXACT><<<n < 2 * cus ? n : 2 * cus, 256, 0, st>>>(p);
     } else {
         const int n = tiles(64, 128);
         f8_gemm_kernel<2, 2, 2, 4, EXACT><<<n < 3 * cus ? n : 3 * cus, 256, 0, st>>>(p);

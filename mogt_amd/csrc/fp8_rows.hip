@@ -8,8 +8,10 @@
 //                    the residual update as in add_rmsnorm, statistics in fp32
 //   quantize_rows    the rows of a matrix
 //   quantize_blocks  128 x 128 blocks (weights, laid out once)
-// Rows: one wave a row, four consecutive values a lane, so half a wave is a block
-// and its maximum five lane exchanges; bound by HBM.
+// Four consecutive values a lane: half a wave is a block and its maximum five lane
+// exchanges.  The norm takes one wave a row, which it holds in registers; its sum of
+// squares is added in 64 bits, so that values at a border of the 8 bits fall where the
+// definition's do.  Bound by HBM.
 #include "common.h"
 
 namespace mogt {
@@ -27,73 +29,89 @@ __device__ __forceinline__ uint32_t f8_pack(const float (&v)[4], float scale) {
     return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2] / scale, v[3] / scale, w, true));
 }
 
+// the largest of the 32 lanes of a half wave
+__device__ __forceinline__ float f8_block_max(float m) {
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+    return m;
+}
+
 __device__ __forceinline__ float f8_max4(const float (&v)[4]) {
     return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 }
 
-struct F8Rows {
-    const void *x, *z;
+struct F8Norm {
+    const float* x;
+    const void* z;
     const float* w;
     float* x_out;
     uint32_t* q;       // [rows, D] bytes
     float* scale;      // [rows, blocks]
-    int64_t rows, ldx;
+    int64_t rows;
     int D, blocks;
     float zs, eps;
 };
 
 // VPL: vectors of four values a lane (D <= 256 VPL)
-template <typename TX, typename TZ, int VPL, bool NORM>
-__global__ __launch_bounds__(64 * F8_WAVES) void f8_rows_kernel(F8Rows p) {
+template <typename TZ, int VPL>
+__global__ __launch_bounds__(64 * F8_WAVES) void f8_norm_kernel(F8Norm p) {
     const int lane = threadIdx.x & 63;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * F8_WAVES + (threadIdx.x >> 6);
     if (row >= p.rows) return;
-    const TX* xr = static_cast<const TX*>(p.x) + row * p.ldx;
+    const float* xr = p.x + row * p.D;
     const TZ* zr = static_cast<const TZ*>(p.z) + row * p.D;
-    float v[VPL][4], ss = 0.0f;
+    float v[VPL][4];
+    double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
         const int c = (k * 64 + lane) * 4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[k][e] = 0.0f;
         if (c < p.D) {
-            load_vec<TX, 4>(xr + c, v[k]);
-            if constexpr (NORM) {
-                float zz[4];
-                load_vec<TZ, 4>(zr + c, zz);
+            float zz[4];
+            load_vec<float, 4>(xr + c, v[k]);
+            load_vec<TZ, 4>(zr + c, zz);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[k][e] += IO<TZ>::ld(IO<TZ>::st(p.zs * zz[e]));
-                    ss = fmaf(v[k][e], v[k][e], ss);
-                }
-                store_vec<float, 4>(p.x_out + row * p.D + c, v[k]);
+            for (int e = 0; e < 4; ++e) {
+                v[k][e] += IO<TZ>::ld(IO<TZ>::st(p.zs * zz[e]));
+                ss = fma(static_cast<double>(v[k][e]), static_cast<double>(v[k][e]), ss);
             }
+            store_vec<float, 4>(p.x_out + row * p.D + c, v[k]);
         }
     }
-    if constexpr (NORM) {
-        for (int m = 32; m > 0; m >>= 1) ss += __shfl_xor(ss, m);
-        const float inv = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-            const int c = (k * 64 + lane) * 4;
-            if (c < p.D) {
-                float w[4];
-                load_vec<float, 4>(p.w + c, w);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[k][e] = v[k][e] * inv * w[e];
-            }
-        }
-    }
+    for (int m = 32; m > 0; m >>= 1) ss += __shfl_xor(ss, m);
+    const float inv = static_cast<float>(1.0 / sqrt(ss / p.D + static_cast<double>(p.eps)));
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
         const int c = (k * 64 + lane) * 4;
-        float m = f8_max4(v[k]);
-        for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-        const float s = f8_scale(m);
+        if (c < p.D) {
+            float w[4];
+            load_vec<float, 4>(p.w + c, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][e] = v[k][e] * inv * w[e];
+        }
+        const float s = f8_scale(f8_block_max(f8_max4(v[k])));
         if (c < p.D) {
             p.q[(row * p.D + c) >> 2] = f8_pack(v[k], s);
             if ((lane & 31) == 0) p.scale[row * p.blocks + c / F8_BLOCK] = s;
         }
+    }
+}
+
+// Half a wave per block of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void f8_rows_kernel(const T* x, int64_t ldx, uint32_t* q, float* scale, int64_t total,
+                                                      int D, int blocks) {
+    const int64_t id = blockIdx.x * 8ll + (threadIdx.x >> 5);
+    const int64_t row = id / blocks;
+    const int block = static_cast<int>(id - row * blocks), c = block * F8_BLOCK + (threadIdx.x & 31) * 4;
+    const bool in = id < total && c < D;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (in) load_vec<T, 4>(x + row * ldx + c, v);
+    const float s = f8_scale(f8_block_max(f8_max4(v)));
+    if (in) {
+        q[(row * D + c) >> 2] = f8_pack(v, s);
+        if ((threadIdx.x & 31) == 0) scale[id] = s;
     }
 }
 
@@ -125,20 +143,39 @@ __global__ __launch_bounds__(256) void f8_blocks_kernel(const T* x, int64_t ldx,
     if (threadIdx.x == 0) scale[blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x] = s;
 }
 
-template <typename TX, typename TZ, bool NORM>
-int f8_rows_launch(const F8Rows& p, const char* what, hipStream_t st) {
+template <typename TZ>
+int f8_norm_launch(const F8Norm& p, hipStream_t st) {
     const int64_t blocks = (p.rows + F8_WAVES - 1) / F8_WAVES;
-    if (blocks > 0x7fffffff) return set_error(MOGT_E_INVALID, "%s: %lld rows", what, (long long)p.rows);
+    if (blocks > 0x7fffffff) return set_error(MOGT_E_INVALID, "%lld rows are too many", (long long)p.rows);
     const dim3 grid(static_cast<unsigned>(blocks));
     if (p.D <= 256)
-        f8_rows_kernel<TX, TZ, 1, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+        f8_norm_kernel<TZ, 1><<<grid, 64 * F8_WAVES, 0, st>>>(p);
     else if (p.D <= 1024)
-        f8_rows_kernel<TX, TZ, 4, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+        f8_norm_kernel<TZ, 4><<<grid, 64 * F8_WAVES, 0, st>>>(p);
     else if (p.D <= 2048)
-        f8_rows_kernel<TX, TZ, 8, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+        f8_norm_kernel<TZ, 8><<<grid, 64 * F8_WAVES, 0, st>>>(p);
     else
-        f8_rows_kernel<TX, TZ, 16, NORM><<<grid, 64 * F8_WAVES, 0, st>>>(p);
-    return check_launch(what);
+        f8_norm_kernel<TZ, 16><<<grid, 64 * F8_WAVES, 0, st>>>(p);
+    return check_launch("mogt_add_rmsnorm_fp8_fwd");
+}
+
+template <typename T>
+int f8_quantize_launch(const void* x, int64_t ld, void* q, float* scale, int64_t rows, int64_t dim, int block_rows,
+                       hipStream_t st) {
+    const int blocks = static_cast<int>((dim + F8_BLOCK - 1) / F8_BLOCK), D = static_cast<int>(dim);
+    const T* xt = static_cast<const T*>(x);
+    uint32_t* qt = static_cast<uint32_t*>(q);
+    if (block_rows == 1) {
+        const int64_t groups = (rows * blocks + 7) / 8;
+        if (rows > (1ll << 40) || groups > 0x7fffffff)
+            return set_error(MOGT_E_INVALID, "%lld rows of %lld are too many", (long long)rows, (long long)dim);
+        f8_rows_kernel<T><<<static_cast<unsigned>(groups), 256, 0, st>>>(xt, ld, qt, scale, rows * blocks, D, blocks);
+    } else {
+        const int64_t by = (rows + F8_BLOCK - 1) / F8_BLOCK;
+        if (by > 65535) return set_error(MOGT_E_INVALID, "%lld rows: at most %d", (long long)rows, 65535 * F8_BLOCK);
+        f8_blocks_kernel<T><<<dim3(blocks, static_cast<unsigned>(by)), 256, 0, st>>>(xt, ld, qt, scale, rows, D);
+    }
+    return check_launch("mogt_quantize_fp8");
 }
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -160,11 +197,11 @@ extern "C" int mogt_add_rmsnorm_fp8_fwd(const float* x, const void* z, float sca
     if (!x || !z || !weight || !x_out || !q || !q_scale) return set_error(MOGT_E_INVALID, "null pointer");
     if (!aligned(x, 16) || !aligned(x_out, 16) || !aligned(weight, 16) || !aligned(z, z_dtype == MOGT_BF16 ? 8 : 16) || !aligned(q, 4))
         return set_error(MOGT_E_INVALID, "rows of four values must be aligned");
-    F8Rows p{x, z, weight, x_out, static_cast<uint32_t*>(q), q_scale, rows, dim, static_cast<int>(dim),
+    F8Norm p{x, z, weight, x_out, static_cast<uint32_t*>(q), q_scale, rows, static_cast<int>(dim),
              static_cast<int>((dim + F8_BLOCK - 1) / F8_BLOCK), scale, eps};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (z_dtype == MOGT_BF16) return f8_rows_launch<float, bf16_t, true>(p, "mogt_add_rmsnorm_fp8_fwd", st);
-    return f8_rows_launch<float, float, true>(p, "mogt_add_rmsnorm_fp8_fwd", st);
+    if (z_dtype == MOGT_BF16) return f8_norm_launch<bf16_t>(p, st);
+    return f8_norm_launch<float>(p, st);
 }
 
 extern "C" int mogt_quantize_fp8(const void* x, int64_t ld, void* q, float* q_scale, int64_t rows, int64_t dim, int dtype,
@@ -176,25 +213,11 @@ extern "C" int mogt_quantize_fp8(const void* x, int64_t ld, void* q, float* q_sc
     if (dtype != MOGT_F32 && dtype != MOGT_BF16) return set_error(MOGT_E_INVALID, "dtype %d not supported", dtype);
     if (block_rows != 1 && block_rows != F8_BLOCK)
         return set_error(MOGT_E_INVALID, "blocks of %d rows: 1 or %d expected", block_rows, F8_BLOCK);
-    if (block_rows == 1 && dim > 4096)
-        return set_error(MOGT_E_INVALID, "rows of %lld: at most 4096 values with a scale for each row", (long long)dim);
     if (rows == 0) return MOGT_OK;
     const size_t each = dtype == MOGT_BF16 ? 8 : 16;
     if (!x || !q || !q_scale) return set_error(MOGT_E_INVALID, "null pointer");
     if (!aligned(x, each) || ld % 4 != 0 || !aligned(q, 4)) return set_error(MOGT_E_INVALID, "rows of four values must be aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int blocks = static_cast<int>((dim + F8_BLOCK - 1) / F8_BLOCK);
-    if (block_rows == 1) {
-        F8Rows p{x, nullptr, nullptr, nullptr, static_cast<uint32_t*>(q), q_scale, rows, ld, static_cast<int>(dim), blocks, 0.0f, 0.0f};
-        if (dtype == MOGT_BF16) return f8_rows_launch<bf16_t, float, false>(p, "mogt_quantize_fp8", st);
-        return f8_rows_launch<float, float, false>(p, "mogt_quantize_fp8", st);
-    }
-    const int64_t by = (rows + F8_BLOCK - 1) / F8_BLOCK;
-    if (by > 65535) return set_error(MOGT_E_INVALID, "%lld rows: at most %d", (long long)rows, 65535 * F8_BLOCK);
-    const dim3 grid(blocks, static_cast<unsigned>(by));
-    if (dtype == MOGT_BF16)
-        f8_blocks_kernel<bf16_t><<<grid, 256, 0, st>>>(static_cast<const bf16_t*>(x), ld, static_cast<uint32_t*>(q), q_scale, rows, static_cast<int>(dim));
-    else
-        f8_blocks_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(x), ld, static_cast<uint32_t*>(q), q_scale, rows, static_cast<int>(dim));
-    return check_launch("mogt_quantize_fp8");
+    if (dtype == MOGT_BF16) return f8_quantize_launch<bf16_t>(x, ld, q, q_scale, rows, dim, block_rows, st);
+    return f8_quantize_launch<float>(x, ld, q, q_scale, rows, dim, block_rows, st);
 }

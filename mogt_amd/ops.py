@@ -3190,7 +3190,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sta
 # 8-bit rows and weights, and their matrix product
 # ---------------------------------------------------------------------------
 FP8_BLOCK = 128
-FP8_MAX_ROW = 4096     # values of a row with scales of its own
+FP8_MAX_ROW = 4096     # values of a row of the norm
 _FP8 = torch.float8_e4m3fn
 
 
@@ -3226,8 +3226,8 @@ def add_rmsnorm_fp8(x: torch.Tensor, z: torch.Tensor, scale: float, weight: torc
     values with a float32 scale for every 128 of a row, which ``linear_fp8`` takes.
 
     A block's scale is its largest magnitude / 448 (2^-126 at least), the values
-    ``n / scale`` rounded to nearest even; statistics and the norm are fp32, with
-    no rounding between.  Returns ``(x', q, q_scale)``.  Rows of a multiple of 4
+    ``n / scale`` rounded to nearest even; the norm is fp32, its sum of squares in
+    64 bits.  Returns ``(x', q, q_scale)``.  Rows of a multiple of 4
     values, up to 4096.  No autograd."""
     _same_device("add_rmsnorm_fp8", x, (z, weight))
     if x.dtype != torch.float32:
@@ -3279,9 +3279,8 @@ def _fp8_rows(x: torch.Tensor, each: int) -> torch.Tensor:
 def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
     """``x`` (float32 or bfloat16, ``[..., D]``) in 8 bits for ``linear_fp8``: ``(q,
     q_scale)``, e4m3 values and float32 scales of blocks of 128 values of a row
-    (``block_rows`` 1: ``q_scale [..., ceil(D / 128)]``, D up to 4096), or of 128
-    rows by 128 values of a weight ``[N, D]`` (128: ``q_scale [ceil(N / 128),
-    ceil(D / 128)]``).  A block's scale is its largest magnitude / 448 (2^-126 at
+    (``block_rows`` 1: ``q_scale [..., ceil(D / 128)]``), or of 128 rows by 128
+    values of a weight ``[N, D]`` (128: ``q_scale [ceil(N / 128), ceil(D / 128)]``).  A block's scale is its largest magnitude / 448 (2^-126 at
     least), values are rounded to nearest even.  D a multiple of 4.  No autograd."""
     require_cuda("quantize_fp8", x)
     dtype_code(x.dtype, "quantize_fp8")
@@ -3290,9 +3289,8 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
     if x.ndim < 1 or (block_rows != 1 and x.ndim != 2):
         raise ValueError("quantize_fp8: x must be [..., D], or [N, D] in blocks of rows")
     D = x.shape[-1]
-    if D < 4 or D % 4 != 0 or (block_rows == 1 and D > FP8_MAX_ROW):
-        raise ValueError(f"quantize_fp8: rows of {D} values not supported (a multiple of 4, up to {FP8_MAX_ROW} with "
-                         "scales of their own)")
+    if D < 4 or D % 4 != 0:
+        raise ValueError(f"quantize_fp8: rows of {D} values not supported (a multiple of 4)")
     return _quantize_fp8_op(x, int(block_rows))
 
 

@@ -57,7 +57,7 @@ def test_norm(gpu, M, D, dtype):
     check_eight(n, q, s, 1, (D / 2 + 8) * U)
 
 
-@pytest.mark.parametrize("shape", [(1, 4), (3, 5, 128), (7, 132), (130, 4096)])
+@pytest.mark.parametrize("shape", [(1, 4), (3, 5, 128), (7, 132), (130, 4096), (3, 5124)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_quantize_rows(gpu, shape, dtype):
     from mogt_amd import ops
