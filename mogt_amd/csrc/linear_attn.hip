@@ -132,11 +132,13 @@ __global__ __launch_bounds__(64) void la_decay_sum_kernel(const double* part, in
 
 // gradients of rows that `share` heads read: [rows, groups, share, d] fp32 to [rows, groups, d]
 template <typename TI>
-__global__ __launch_bounds__(256) void la_group_kernel(const float* from, TI* to, int64_t total, int d, int share) {
+__global__ __launch_bounds__(256) void la_group_kernel(const float* dq, const float* dk, TI* to_q, TI* to_k, int64_t total,
+                                                       int d, int share) {
     const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-    if (i >= total) return;
+    TI* to = blockIdx.y ? to_k : to_q;
+    if (i >= total || !to) return;
     const int64_t row = i / d;
-    const float* p = from + row * share * d + (i - row * d);
+    const float* p = (blockIdx.y ? dk : dq) + row * share * d + (i - row * d);
     float x = 0.0f;
     for (int j = 0; j < share; ++j) x += p[static_cast<int64_t>(j) * d];
     to[i] = IO<TI>::st(x);
@@ -458,16 +460,15 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
     if (shared) {
         const int share = static_cast<int>(q->heads / q->groups), d = static_cast<int>(q->key_dim);
         const int64_t total = q->batch * q->length * q->groups * q->key_dim;
-        auto sum = [&](const float* from, void* to) {
-            if (!to || total == 0) return;
-            const unsigned blocks = static_cast<unsigned>((total + 255) / 256);
+        if (total > 0 && (g->dq || g->dk)) {
+            const dim3 grid(static_cast<unsigned>((total + 255) / 256), 2);
             if (q->io_dtype == MOGT_BF16)
-                la_group_kernel<bf16_t><<<blocks, 256, 0, st>>>(from, static_cast<bf16_t*>(to), total, d, share);
+                la_group_kernel<bf16_t><<<grid, 256, 0, st>>>(share_q, share_k, static_cast<bf16_t*>(g->dq),
+                                                              static_cast<bf16_t*>(g->dk), total, d, share);
             else
-                la_group_kernel<float><<<blocks, 256, 0, st>>>(from, static_cast<float*>(to), total, d, share);
-        };
-        sum(share_q, g->dq);
-        sum(share_k, g->dk);
+                la_group_kernel<float><<<grid, 256, 0, st>>>(share_q, share_k, static_cast<float*>(g->dq),
+                                                             static_cast<float*>(g->dk), total, d, share);
+        }
     }
     return check_launch("mogt_linear_attn_bwd");
 }

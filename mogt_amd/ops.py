@@ -2959,7 +2959,12 @@ LINEAR_ATTN_CHUNK = {torch.bfloat16: 64, torch.float32: 32}   # steps of a chunk
 # with 1024, 319 with 512 and 350 with 384.
 LINEAR_ATTN_GROUPS = 1024
 LINEAR_ATTN_WIDE_GROUPS = 512
-LINEAR_ATTN_MIN_SEGMENT = 256   # the least steps of a segment
+# The least steps of a segment, and the length up to which one work-group runs through
+# (a segment's sums, the carry and another launch cost what they save): kernels over
+# 2 x 513 steps of 6 heads with gradients, fp32, take 75 us in segments of 64, 95 of 128
+# and 139 of 256; 200 steps of 12 heads 16.3 us in one and 16.8 in segments of 64.
+LINEAR_ATTN_MIN_SEGMENT = 64
+LINEAR_ATTN_ONE_SEGMENT = 256
 LINEAR_ATTN_SEGMENT_BYTES = 0x7fffffff - 1024   # of a segment's rows, addressed by 32-bit offsets
 
 
@@ -2967,7 +2972,7 @@ def _linear_attn_segment(B: int, L: int, H: int, dk: int, dv: int, dtype: torch.
     """Steps of a segment, whole chunks."""
     chunk = LINEAR_ATTN_CHUNK[dtype]
     want = -(-(LINEAR_ATTN_GROUPS if max(dk, dv) <= 64 else LINEAR_ATTN_WIDE_GROUPS) // max(1, B * H))
-    steps = max(LINEAR_ATTN_MIN_SEGMENT, -(-L // want), -(-L // (1 << 20)))
+    steps = L if L <= LINEAR_ATTN_ONE_SEGMENT else max(LINEAR_ATTN_MIN_SEGMENT, -(-L // want), -(-L // (1 << 20)))
     most = LINEAR_ATTN_SEGMENT_BYTES // (4 * max(1, H) * max(dk, dv))
     return chunk * max(1, min(-(-steps // chunk), most // chunk))
 
@@ -2987,17 +2992,16 @@ def _linear_attn_problem(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
                                        _linear_attn_rows(v, steps), _dense(initial_state), _dense(lengths))
     if log_decay.ndim == 3 and log_decay.stride(1) * 4 * steps > LINEAR_ATTN_SEGMENT_BYTES:
         log_decay = log_decay.contiguous()
-    qs, ks, vs, gs = q.stride(), k.stride(), v.stride(), log_decay.stride()
-    per_head = log_decay.ndim == 1
-    step = q.ndim == 3
-    # (row, batch, head) strides; a step's rows have none
-    strides = tuple(n for s in (qs, ks, vs) for n in ((0 if step else s[1]), s[0], s[-2]))
-    g = (0, 0, gs[0]) if per_head else ((0 if step else gs[1]), gs[0], gs[-1])
-    p = _lib.LINEAR_ATTN_PROBLEM.pack(v.shape[0], 1 if step else v.shape[1], v.shape[-2], q.shape[-2], q.shape[-1],
-                                      v.shape[-1], segment, _DTYPE_CODE[q.dtype],
+    shape, qs, ks, vs, gs = v.shape, q.stride(), k.stride(), v.stride(), log_decay.stride()
+    # row strides; a step's rows have none
+    L, qr, kr, vr, gr = (1, 0, 0, 0, 0) if len(shape) == 3 else (shape[1], qs[1], ks[1], vs[1], gs[-2] if len(gs) > 1
+                                                                 else 0)
+    per_head = len(gs) == 1
+    p = _lib.LINEAR_ATTN_PROBLEM.pack(shape[0], L, shape[-2], *q.shape[-2:], shape[-1], segment, _DTYPE_CODE[q.dtype],
                                       0 if lengths is None else lengths.element_size(), per_head, scale, q.data_ptr(),
                                       k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(initial_state),
-                                      _ptr(lengths), *strides, *g)
+                                      _ptr(lengths), qr, qs[0], qs[-2], kr, ks[0], ks[-2], vr, vs[0], vs[-2], gr,
+                                      0 if per_head else gs[0], gs[-1])
     return p, (q, k, v, log_decay, initial_state, lengths)
 
 
