@@ -17,6 +17,8 @@ namespace {
 // The states entering the segments, in place: slot 0 is the initial state, slot
 // j + 1 = exp(c_j) slot j + what segment j wrote from zero.  A thread owns one
 // element and reads 32 segments at once; `init` is [dk, dv], the segments' [dv, dk].
+// A decay is its root applied twice, each finite: a state of a segment that grows
+// is in range wherever the definition's is, and one of zeros stays zero.
 __global__ __launch_bounds__(256) void la_carry_kernel(float* states, const float* ctot, const float* init, int nseg,
                                                        int dk, int dv) {
     constexpr int U = 32;
@@ -36,7 +38,8 @@ __global__ __launch_bounds__(256) void la_carry_kernel(float* states, const floa
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (j + i < nseg - 1) {
-                h = fmaf(__builtin_amdgcn_exp2f(c[j + i]), h, w[i]);
+                const float root = __builtin_amdgcn_exp2f(fminf(0.5f * c[j + i], 127.0f));
+                h = fmaf(root, root * h, w[i]);
                 q[static_cast<int64_t>(j + i + 1) * state] = h;
             }
     }
@@ -415,10 +418,9 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
     dq.qs = dq.ps = q->scale;
     dq.out = shared && g->dq ? share_q : g->dq;
     dq.out_f32 = shared;
-    if (need_g) {
-        dk.dot = dot_k;
-        dq.dot = dot_q;
-    }
+    // formed in any case: a row's gradient does not depend on which others are asked for
+    dk.dot = dot_k;
+    dq.dot = dot_q;
     if (a.nseg > 1) {
         a.pass[0] = dv;
         la_launch(q, a, 1, false, st);

@@ -187,7 +187,7 @@ struct LaTile {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int u = row(me) + i * STEP;
-            const uint32_t at = static_cast<uint32_t>(first + u * step + c * static_cast<int>(sizeof(TI)));
+            const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(u) * static_cast<uint32_t>(step) + c * static_cast<uint32_t>(sizeof(TI));
             if constexpr (VEC) {
                 r[i] = __builtin_amdgcn_raw_buffer_load_b128(b, ((u < left) & (c < d)) ? at : LA_OUTSIDE, 0, 0);
             } else if constexpr (sizeof(TI) == 4) {
@@ -363,13 +363,15 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
         const double g2 = static_cast<double>(g) * 1.4426950408889634;
         const double c = la_wave_sums(g2 < LA_LOG2_MIN ? LA_LOG2_MIN : g2), end = la_lane(c, 63);
         const float hi = static_cast<float>(c);
+        // finite factors: growth keeps a state of zeros, or rows of zeros, what they are
+        auto factor = [](double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x > 127.0 ? 127.0 : x)); };
         if (lane < T) {
             s.hi[buf][lane] = hi;
             s.lo[buf][lane] = static_cast<float>(c - hi);
-            s.in[buf][lane] = p.qs * __builtin_amdgcn_exp2f(hi);
-            s.w[buf][lane] = p.ws * __builtin_amdgcn_exp2f(static_cast<float>(end - c));
+            s.in[buf][lane] = p.qs * factor(c);
+            s.w[buf][lane] = p.ws * factor(end - c);
         }
-        if (lane == 0) s.end[buf] = __builtin_amdgcn_exp2f(static_cast<float>(end));
+        if (lane == 0) s.end[buf] = factor(end);
         total += end;
     };
     auto load = [&](int u0, int me) {
@@ -422,7 +424,7 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) {
                     const int u = 16 * tt + (lane & 15), cc = c0 + 16 * c;
-                    const uint32_t at = static_cast<uint32_t>((first + u) * sx + cc * ES);
+                    const uint32_t at = static_cast<uint32_t>(first + u) * static_cast<uint32_t>(sx) + cc * ES;
                     if constexpr (VEC) {
                         const uint32_t o = ((u0 + u < cnt) & (cc < dn)) ? at : LA_OUTSIDE;
                         if constexpr (ES == 2)
@@ -548,7 +550,7 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
                     const int cc = c0 + 16 * c;
-                    const uint32_t at = static_cast<uint32_t>((first + u) * so + cc * OS);
+                    const uint32_t at = static_cast<uint32_t>(first + u) * static_cast<uint32_t>(so) + cc * OS;
                     if constexpr (VEC) {
                         const uint32_t o = (in & (cc < dn)) ? at : LA_OUTSIDE;
                         if constexpr (F32) {
@@ -673,8 +675,6 @@ void la_launch_passes(const LaArgs& a, int count, bool out, hipStream_t st) {
             la_pass_kernel<TI, W, N, true, true, V, true><<<grid, LA_THREADS, 0, st>>>(a);
         else if (dot)
             la_pass_kernel<TI, W, N, true, true, V, F><<<grid, LA_THREADS, 0, st>>>(a);
-        else if (f32)
-            la_pass_kernel<TI, W, N, true, false, V, true><<<grid, LA_THREADS, 0, st>>>(a);
         else
             la_pass_kernel<TI, W, N, true, false, V, F><<<grid, LA_THREADS, 0, st>>>(a);
     };

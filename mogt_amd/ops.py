@@ -3139,14 +3139,19 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     (float32 or bfloat16, any strides), each group's q and k shared by H / G
     consecutive heads, widths up to 128; ``scale`` defaults to ``dk ** -0.5``.
     ``log_decay`` is ``[B, L, H]``, or ``[H]`` for one decay a head (real, taken in
-    float32, at most 0 as a rule; -inf empties the state).  fp32 state and sums, the
-    output in v's dtype.  ``initial_state [B, H, dk, dv]`` (float32, zero without
+    float32, at most 0 as a rule; -inf empties the state; over 64 steps it may grow by
+    up to exp(88)).  fp32 state and sums, the output in v's dtype.  ``initial_state [B, H, dk, dv]`` (float32, zero without
     it); ``return_state`` also returns the final one, from which
     ``linear_attention`` and ``linear_attention_step`` continue.  ``lengths [B]``
     (int32 or int64 on the GPU, taken within [0, L]) marks the padding of a ragged
     batch: steps past a length are not read and leave the state as it is; their
     outputs and gradients are zero.  Differentiable in every tensor but
-    ``lengths``, through both outputs; results do not change from run to run."""
+    ``lengths``, through both outputs; results do not change from run to run.  What an
+    input that is not finite reaches is infinite or NaN: later outputs, earlier
+    gradients, and the decays' gradients of its segment (up to ``ceil(L / 1024 B H)``
+    steps rounded up to whole chunks of 64, or 32 in float32, and 64 at least; all of
+    256 steps or fewer).  The backward keeps a state for every segment and takes as
+    many again, and 8 bytes a row and head, as workspace."""
     if q.ndim != 4:
         raise ValueError("linear_attention: q must be [B, L, G, dk]")
     _check_linear_attn("linear_attention", q, k, v, log_decay, initial_state)

@@ -170,3 +170,122 @@ def test_norm_feeds_the_product(gpu):
         w, ws = ops.quantize_fp8(rnd(320, 768, seed=4) / 768 ** 0.5, block_rows=128)
         _, q, s = ops.add_rmsnorm_fp8(x, z, 0.5, weight)
         check_product(ops.linear_fp8(q, s, w, ws), q, s, w, ws)
+
+
+@pytest.mark.parametrize("M,N,K", [(4100, 3520, 400), (700, 2304, 272), (2600, 1032, 144), (33, 64, 1040), (16, 40, 16)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_product_of_whole_rows(gpu, M, N, K, out):
+    """Outputs whose rows are whole 16 bytes leave through LDS: several tiles a
+    work-group, edges inside a tile, blocks of K that are not full."""
+    from mogt_amd import ops
+    announce(f"linear_fp8 {M} {N} {K} {out}")
+    p = product(M, N, K, seed=5)
+    check_product(ops.linear_fp8(*p, out_dtype=out), *p)
+
+
+@pytest.mark.parametrize("M,N,K", [(9000, 8200, 128), (20000, 4096, 256)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_product_of_several_tiles_a_work_group(gpu, M, N, K, out):
+    """Against the same product of its rows in pieces small enough for one tile a
+    work-group, whose blocks are added in the same order."""
+    from mogt_amd import ops
+    announce(f"linear_fp8 {M} {N} {K} {out}")
+    x, xs, w, ws = product(M, N, K, seed=6)
+    y = ops.linear_fp8(x, xs, w, ws, out_dtype=out)
+    for lo in range(0, M, 4000):
+        part = ops.linear_fp8(x[lo:lo + 100], xs[lo:lo + 100], w, ws, out_dtype=out)
+        check_product(part, x[lo:lo + 100], xs[lo:lo + 100], w, ws)
+        assert torch.equal(part, y[lo:lo + 100])
+    check_product(y[-300:], x[-300:], xs[-300:], w, ws)
+
+
+def test_product_neighbours_are_left_alone(gpu):
+    """Rows behind the last and columns past the end of the output's memory."""
+    from mogt_amd import _lib
+    from mogt_amd import ops
+    for M, N, K, out in ((70, 130, 144, BF16), (300, 520, 128, BF16), (129, 132, 128, F32), (5, 24, 32, F32), (4000, 3500, 128, BF16)):
+        announce(f"mogt_linear_fp8 {M} {N} {K} {out}")
+        x, xs, w, ws = product(M, N, K, seed=7)
+        y = torch.full((M + 3, N), 7.0, device="cuda", dtype=out)
+        rc = _lib.load().mogt_linear_fp8(x.data_ptr(), K, xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), M, N, K,
+                                         1 if out == BF16 else 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert torch.equal(y[:M], ops.linear_fp8(x, xs, w, ws, out_dtype=out)) and bool((y[M:] == 7).all())
+
+
+def test_what_is_not_finite_stays_in_its_row(gpu):
+    from mogt_amd import ops
+    announce("linear_fp8 special values")
+    for M in (5, 200):
+        x, xs, w, ws = product(M, 96, 272, seed=8)
+        want = ops.linear_fp8(x, xs, w, ws)
+        bad = x.float()
+        bad[3, 7] = float("nan")
+        s = xs.clone()
+        s[2, 1] = float("inf")
+        got = ops.linear_fp8(bad.to(F8), s, w, ws)
+        rest = [i for i in range(M) if i not in (2, 3)]
+        assert torch.equal(got[rest], want[rest]) and not got[2:4].isfinite().any()
+
+
+def test_empty(gpu):
+    from mogt_amd import ops
+    announce("8-bit operators, empty")
+    w, ws = ops.quantize_fp8(torch.randn(40, 32, device="cuda"), block_rows=128)
+    z = torch.zeros(0, 32, device="cuda")
+    x, q, s = ops.add_rmsnorm_fp8(z, z, 1.0, torch.ones(32, device="cuda"))
+    assert x.shape == q.shape == (0, 32) and s.shape == (0, 1)
+    assert ops.linear_fp8(q, s, w, ws).shape == (0, 40)
+    assert ops.linear_fp8(q, s, w[:0], ws[:0]).shape == (0, 0)
+    assert [t.shape for t in ops.quantize_fp8(z, block_rows=128)] == [(0, 32), (0, 1)]
+    assert [t.shape for t in ops.quantize_fp8(z.view(0, 4, 8))] == [(0, 4, 8), (0, 4, 1)]
+
+
+def test_strides_of_the_norm_and_one_row(gpu):
+    from mogt_amd import ops
+    announce("add_rmsnorm_fp8 strides")
+    x, z, w = rnd(4, 6, 256, seed=1), rnd(4, 6, 256, seed=2, dtype=BF16), rnd(256, seed=3)
+    want = ops.add_rmsnorm_fp8(x, z, 0.7, w)
+    far = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (x, z)]
+    wide = torch.zeros(4, 6, 513, device="cuda", dtype=BF16)
+    wide[..., 1:257] = z
+    for a in (ops.add_rmsnorm_fp8(*far, 0.7, w), ops.add_rmsnorm_fp8(x, wide[..., 1:257], 0.7, w.double())):
+        assert all(torch.equal(p.float(), r.float()) for p, r in zip(a, want))
+    one = ops.add_rmsnorm_fp8(x[1, 2], z[1, 2], 0.7, w)
+    assert one[2].shape == (2,) and all(torch.equal(p.float(), r[1, 2].float()) for p, r in zip(one, want))
+
+
+def test_streams_and_captured_graphs(gpu):
+    """Two streams at once, and a norm and its products captured and replayed on
+    changing inputs with eager work between."""
+    from mogt_amd import ops
+    announce("8-bit operators captured")
+    shapes = [(1, 768), (300, 768), (4200, 768)]
+    w, ws = ops.quantize_fp8(rnd(3504, 768, seed=1) / 28, block_rows=128)
+    weight = rnd(768, seed=2)
+
+    def work(x, z):
+        res, q, s = ops.add_rmsnorm_fp8(x, z, 0.5, weight)
+        return res, q, s, ops.linear_fp8(q, s, w, ws), ops.linear_fp8(q, s, w, ws, out_dtype=F32)
+
+    held = [(rnd(*s, seed=3), rnd(*s, seed=4, dtype=BF16)) for s in shapes]
+    want = [work(*h) for h in held]
+    streams = [torch.cuda.Stream() for _ in held]
+    torch.cuda.synchronize()
+    got = []
+    for s, h in zip(streams, held):
+        with torch.cuda.stream(s):
+            got.append(work(*h))
+    torch.cuda.synchronize()
+    same = lambda a, b: all(torch.equal(p.float(), r.float()) for p, r in zip(a, b))  # noqa: E731
+    assert all(same(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [work(*h) for h in held]
+    for seed in range(10, 13):
+        for x, z in held:
+            x.copy_(rnd(*x.shape, seed=seed))
+            z.copy_(rnd(*x.shape, seed=seed + 50, dtype=BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(same(a, work(*h)) for a, h in zip(out, held))
