@@ -274,7 +274,7 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
     constexpr int T = LaChunk<TI>::T, KS = LaChunk<TI>::KS, NP = la_pieces<TI, DOT>();
     constexpr int NW = la_pieces_write<TI>(), TT = T / 16, RT = DK / 16, NV = 64 * CT;
     constexpr int E = KS / 4, ES = static_cast<int>(sizeof(TI));
-    constexpr bool LATE = OUT && CT == 2;   // rows of the next chunk are loaded once the outputs' registers are free
+    constexpr bool LATE = DOT && CT == 2;   // rows of the next chunk are loaded once the outputs' registers are free
     __shared__ __align__(16) LaLds<TI, DK, CT, OUT, NP> s;
 
     const int which = __builtin_amdgcn_readfirstlane(blockIdx.z / a.B), b = blockIdx.z - which * a.B, h = blockIdx.y;
@@ -349,6 +349,10 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
         if (a.nseg == 1 && p.keep && slot) write_state(slot, p.rs, p.cs);
     }
 
+    // A state that only feeds this pass's outputs takes two pieces of its writes; one
+    // that is handed on (a segment's, the last) or whose products are wanted three.
+    // (The last's whether it is asked for or not: outputs do not depend on that.)
+    const bool exact = seg == a.nseg - 1;
     LaTile<TI, DK, VEC> tq, tk;
     LaTile<TI, NV, VEC> tv;
     // One wave forms a chunk's decays while the others work on the chunk before.
@@ -592,30 +596,39 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
             for (int r = 0; r < RT; ++r) S[c][r] *= end;
 #pragma unroll
         for (int k = 0; k < T / KS; ++k) {
-            Frag wv[CT][NW];
             float w[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) w[e] = s.w[buf][KS * k + 4 * grp + Op::order(e)];
+            auto write = [&](auto pieces, int from) __attribute__((always_inline)) {
+                constexpr int N = decltype(pieces)::value;
+                Frag wv[CT][N];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                float x[E];
+                for (int c = 0; c < CT; ++c) {
+                    float x[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = Op::value(vf[c][k], e) * w[e];
-                Op::template split<NW>(x, wv[c]);
-            }
-            // products of one tile lie apart: the next waits for the last's result
-            constexpr int G = RT * CT < 4 ? RT : 4 / CT;
+                    for (int e = 0; e < E; ++e) x[e] = Op::value(vf[c][k], e) * w[e];
+                    Op::template split<N>(x, wv[c]);
+                }
+                // products of one tile lie apart: the next waits for the last's result
+                constexpr int G = RT * CT < 4 ? RT : 4 / CT;
 #pragma unroll
-            for (int r0 = 0; r0 < RT; r0 += G) {
-                Frag kf[G];
+                for (int r0 = 0; r0 < RT; r0 += G) {
+                    Frag kf[G];
 #pragma unroll
-                for (int r = 0; r < G; ++r) kf[r] = Op::template column<DK>(s.k, KS * k, r0 + r, lane);
+                    for (int r = 0; r < G; ++r) kf[r] = Op::template column<DK>(s.k, KS * k, r0 + r, lane);
 #pragma unroll
-                for (int piece = 0; piece < NW; ++piece)
+                    for (int piece = from; piece < N; ++piece)
 #pragma unroll
-                    for (int r = 0; r < G; ++r)
+                        for (int r = 0; r < G; ++r)
 #pragma unroll
-                        for (int c = 0; c < CT; ++c) S[c][r0 + r] = Op::mma(kf[r], wv[c][piece], S[c][r0 + r]);
+                            for (int c = 0; c < CT; ++c) S[c][r0 + r] = Op::mma(kf[r], wv[c][piece], S[c][r0 + r]);
+                }
+            };
+            if constexpr (OUT && !DOT && NW == 3) {
+                write(std::integral_constant<int, 2>(), 0);
+                if (exact) write(std::integral_constant<int, 3>(), 2);
+            } else {
+                write(std::integral_constant<int, NW>(), 0);
             }
         }
         if constexpr (OUT && DOT) {

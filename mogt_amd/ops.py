@@ -2952,12 +2952,12 @@ def ssm_step(x: torch.Tensor, state: torch.Tensor, delta: torch.Tensor, A: torch
 # ---------------------------------------------------------------------------
 LINEAR_ATTN_MAX_DIM = 128
 LINEAR_ATTN_CHUNK = {torch.bfloat16: 64, torch.float32: 32}   # steps of a chunk; a segment is whole chunks
-# Work-groups that a call is cut into segments for: three or four a compute unit,
-# two where states are wider than 64 (their kernels fill one with two, and a state is
-# 64 KB to carry).  Forward passes: 2 x 8192 steps of 12 heads of 64 take 60 us with
-# 768 groups, 66 with 512 and 80 with 256; 32768 steps of 16 heads of 128 take 331 us
-# with 1024, 319 with 512 and 350 with 384.
-LINEAR_ATTN_GROUPS = 1024
+# Work-groups that a call is cut into segments for: three a compute unit, two where
+# states are wider than 64 (their kernels fill one with two, and a state is 64 KB to
+# carry).  Kernels of 2 x 8192 steps of 12 heads of 64, forward and gradients, take
+# 199 us with 768 groups, 223 with 1024 and 224 with 512; 32768 steps of 16 heads of 128,
+# forward, 319 us with 512, 331 with 1024 and 350 with 384.
+LINEAR_ATTN_GROUPS = 768
 LINEAR_ATTN_WIDE_GROUPS = 512
 # The least steps of a segment, and the length up to which one work-group runs through
 # (a segment's sums, the carry and another launch cost what they save): kernels over
@@ -3148,10 +3148,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     outputs and gradients are zero.  Differentiable in every tensor but
     ``lengths``, through both outputs; results do not change from run to run.  What an
     input that is not finite reaches is infinite or NaN: later outputs, earlier
-    gradients, and the decays' gradients of its segment (up to ``ceil(L / 1024 B H)``
-    steps rounded up to whole chunks of 64, or 32 in float32, and 64 at least; all of
-    256 steps or fewer).  The backward keeps a state for every segment and takes as
-    many again, and 8 bytes a row and head, as workspace."""
+    gradients, and the decays' gradients of its segment: a stretch of whole chunks (64
+    steps, 32 in float32) that grows with the call, all of 256 steps or fewer.  The
+    forward keeps a state for every segment (none of it without gradients); the
+    backward's workspace takes as many again and 8 bytes a row and head, and fp32
+    gradients of q and k for every head where heads share them."""
     if q.ndim != 4:
         raise ValueError("linear_attention: q must be [B, L, G, dk]")
     _check_linear_attn("linear_attention", q, k, v, log_decay, initial_state)
