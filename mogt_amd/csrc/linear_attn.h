@@ -80,8 +80,7 @@ __device__ __forceinline__ int la_length(const LaArgs& a, int b) {
 // its kernel is built for, and the waves of a SIMD that its registers are held to.
 inline int la_width(int dc) { return dc <= 32 ? 32 : dc <= 64 ? 64 : 128; }
 inline int la_tiles(int dn) { return dn <= 64 ? 1 : 2; }
-constexpr int la_waves_per_simd(int width, int tiles) { return tiles == 2 || width > 64 ? 2 : 3; }
-constexpr int LA_THREADS = 256;
+constexpr int la_waves_per_simd(int width, int tiles, int waves) { return waves == 8 ? 4 : tiles == 2 || width > 64 ? 2 : 3; }
 
 inline bool la_one_kind(const LaPass& a, const LaPass& b) {
     return la_width(a.dc) == la_width(b.dc) && la_tiles(a.dn) == la_tiles(b.dn) && !a.dot == !b.dot && a.out_f32 == b.out_f32;

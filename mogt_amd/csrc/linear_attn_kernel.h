@@ -1,5 +1,9 @@
 // The chunked pass of linear attention (linear_attn.h has the mathematics), one
-// work-group of four waves per segment and head, a wave for CT times 16 value columns.
+// work-group per segment and head, a wave for CT times 16 value columns: four waves
+// up to 64 columns; for 128 eight of 16, with a wave's registers halved and four
+// waves a SIMD (32768 steps of 16 heads of 128, bf16, outputs: 157 us, with four
+// waves of 32 columns 169), but where loads are of single elements, which take more
+// registers: those are four of 32.
 //
 // Tiles (16x16 matrix instructions, D[row][column]: a lane holds column lane % 16
 // and rows 4 (lane / 16) .. + 3):
@@ -23,20 +27,24 @@ typedef uint32_t la_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t la_u2 __attribute__((ext_vector_type(2)));
 typedef float la_f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 la_b2 __attribute__((ext_vector_type(2)));
+typedef uint16_t la_h2 __attribute__((ext_vector_type(2)));
 
 template <typename TI> struct LaOp;
 
 // LDS rows of W elements.  bf16: 16-byte chunk c of row r lies at place c ^ f(r),
 // f a bit permutation of r % 16: 16 rows' pieces of one column fall into distinct
-// banks, and so do the 8 rows by 32 bytes of a transposing read.  fp32: 16 bytes
-// of padding a row do the same.
+// banks, and so do the 8 rows by 32 bytes of a transposing read.  16 bytes after
+// every 16 rows keep reads of rows 16 apart from being joined into one of two
+// addresses, which takes twice the time of both (measured: 16 cycles against 8;
+// the passes took 3 to 6 % longer).  fp32: 16 bytes of padding a row do it all.
 //
 // A fragment's contraction of KS elements is held 4 by 4: lane group g (lane / 16)
 // has elements 4 g .. 4 g + 3 of every 16, which is an accumulator tile's row
 // order, so that a state's tiles are operands as they are.
 template <> struct LaOp<bf16_t> {
     typedef la_b8 frag;
-    template <int W> static constexpr int stride() { return W; }
+    static constexpr int PAD = 8;   // after 16 rows
+    template <int W> static constexpr int size(int rows) { return rows * W + rows / 16 * PAD; }
     template <int W>
     static __device__ __forceinline__ int twist(int row) {
         constexpr int N = W / 8;   // chunks of a row
@@ -44,7 +52,7 @@ template <> struct LaOp<bf16_t> {
         return (i & (N / 2 - 1)) << 1 | i / (N / 2);
     }
     template <int W>
-    static __device__ __forceinline__ int at(int row, int col) { return row * W + ((((col >> 3) ^ twist<W>(row)) << 3) | (col & 7)); }
+    static __device__ __forceinline__ int at(int row, int col) { return row * W + (row >> 4) * PAD + ((((col >> 3) ^ twist<W>(row)) << 3) | (col & 7)); }
     static __device__ __forceinline__ la_f4 mma(frag a, frag b, la_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -67,7 +75,7 @@ template <> struct LaOp<bf16_t> {
         const bf16_t* q = p + at<W>(s + 4 * (lane >> 4) + ((lane & 15) >> 2), 16 * tile + 4 * (lane & 3));
         typedef __attribute__((address_space(3))) la_s4* lds;
         const la_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(q));
-        const la_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(q + 16 * W));
+        const la_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(q + 16 * W + PAD));
         return __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     // element e of the lane's is number order(e) + 4 g of the fragment's
@@ -95,7 +103,7 @@ template <> struct LaOp<bf16_t> {
 
 template <> struct LaOp<float> {
     typedef la_f4 frag;
-    template <int W> static constexpr int stride() { return W + 4; }
+    template <int W> static constexpr int size(int rows) { return rows * (W + 4); }
     template <int W>
     static __device__ __forceinline__ int at(int row, int col) { return row * (W + 4) + col; }
     static __device__ __forceinline__ la_f4 mma(frag a, frag b, la_f4 c) {
@@ -170,11 +178,11 @@ __device__ __forceinline__ int la_again(int x) {
 // The rows of a chunk on their way from memory to LDS: W elements wide, 16 bytes
 // at a time over the work-group's threads.  VEC: whole aligned vectors, else one
 // element at a time.
-template <typename TI, int W, bool VEC>
+template <typename TI, int W, int THREADS, bool VEC>
 struct LaTile {
     static constexpr int T = LaChunk<TI>::T, EPC = 16 / sizeof(TI), CPR = W / EPC;
-    static constexpr int N = (T * CPR + LA_THREADS - 1) / LA_THREADS;
-    static constexpr int STEP = LA_THREADS / CPR;   // rows between a thread's loads
+    static constexpr int N = (T * CPR + THREADS - 1) / THREADS;
+    static constexpr int STEP = THREADS / CPR;   // rows between a thread's loads
     la_u4 r[N];
 
     static __device__ __forceinline__ int row(int me) { return me / CPR; }
@@ -212,16 +220,12 @@ struct LaTile {
     }
     // whether any element is infinite or NaN
     __device__ __forceinline__ bool wild() const {
-        bool any = false;
+        la_h2 m = {0, 0};   // the greatest magnitudes' upper halves (bf16: of each half)
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w = r[i][j];
-                if (sizeof(TI) == 2) any |= (w & 0x7f80u) == 0x7f80u;
-                any |= (w & 0x7f800000u) == 0x7f800000u;
-            }
-        return any;
+            for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(la_h2, r[i][j] & 0x7fff7fffu));
+        return (m[1] >= 0x7f80) | (sizeof(TI) == 2 && m[0] >= 0x7f80);
     }
 };
 
@@ -230,21 +234,21 @@ struct LaTile {
 template <typename TI> constexpr int la_pieces_write() { return sizeof(TI) == 2 ? 3 : 1; }
 template <typename TI, bool DOT> constexpr int la_pieces() { return sizeof(TI) == 2 ? (DOT ? 3 : 2) : 1; }
 
-template <typename TI, int DK, int CT, bool OUT, int NP>
+template <typename TI, int DK, int CT, int WAVES, bool OUT, int NP>
 struct LaLds {
     static constexpr int T = LaChunk<TI>::T;
     typedef LaOp<TI> Op;
-    TI q[OUT ? T * Op::template stride<DK>() : 8];
-    TI k[T * Op::template stride<DK>()];
-    TI v[T * Op::template stride<64 * CT>()];
-    TI p[OUT ? NP : 1][OUT ? T * Op::template stride<T>() : 8];
+    TI q[OUT ? Op::template size<DK>(T) : 8];
+    TI k[Op::template size<DK>(T)];
+    TI v[Op::template size<16 * CT * WAVES>(T)];
+    TI p[OUT ? NP : 1][OUT ? Op::template size<T>(T) : 8];
     // of this chunk and the next, in turn:
     float hi[2][T], lo[2][T];   // c_t in two parts: differences are as exact as their size
     float in[2][T], w[2][T];    // factors of the query's part and of the writes
     float end[2];               // exp(c_T)
     float g[64];
     int wild;                 // 1 + the last chunk with an infinite or NaN value
-    float dot[OUT ? 4 * T : 4];
+    float dot[OUT ? WAVES * T : 4];
 };
 
 // Four fp32 values rounded to TI, and what is left of them.
@@ -267,15 +271,15 @@ __device__ __forceinline__ void la_pack4(float (&x)[4], Pack<bf16_t, 4>& w, bool
 
 // OUT: the outputs (else a segment's state from zero); DOT: with their rows'
 // products; VEC: every role's rows in whole aligned vectors; F32: fp32 outputs.
-template <typename TI, int DK, int CT, bool OUT, bool DOT, bool VEC, bool F32>
-__global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass_kernel(LaArgs a) {
+template <typename TI, int DK, int CT, int WAVES, bool OUT, bool DOT, bool VEC, bool F32>
+__global__ __launch_bounds__(64 * WAVES, la_waves_per_simd(DK, CT, WAVES)) void la_pass_kernel(LaArgs a) {
     typedef LaOp<TI> Op;
     typedef typename Op::frag Frag;
     constexpr int T = LaChunk<TI>::T, KS = LaChunk<TI>::KS, NP = la_pieces<TI, DOT>();
-    constexpr int NW = la_pieces_write<TI>(), TT = T / 16, RT = DK / 16, NV = 64 * CT;
+    constexpr int NW = la_pieces_write<TI>(), TT = T / 16, RT = DK / 16, NV = 16 * CT * WAVES, THREADS = 64 * WAVES;
     constexpr int E = KS / 4, ES = static_cast<int>(sizeof(TI));
-    constexpr bool LATE = DOT && CT == 2;   // rows of the next chunk are loaded once the outputs' registers are free
-    __shared__ __align__(16) LaLds<TI, DK, CT, OUT, NP> s;
+    constexpr bool LATE = DOT && NV > 64;   // rows of the next chunk are loaded once the outputs' registers are free
+    __shared__ __align__(16) LaLds<TI, DK, CT, WAVES, OUT, NP> s;
 
     const int which = __builtin_amdgcn_readfirstlane(blockIdx.z / a.B), b = blockIdx.z - which * a.B, h = blockIdx.y;
     const LaPass p = a.pass[which];   // a copy: its fields are read once
@@ -353,10 +357,10 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
     // that is handed on (a segment's, the last) or whose products are wanted three.
     // (The last's whether it is asked for or not: outputs do not depend on that.)
     const bool exact = seg == a.nseg - 1;
-    LaTile<TI, DK, VEC> tq, tk;
-    LaTile<TI, NV, VEC> tv;
+    LaTile<TI, DK, THREADS, VEC> tq, tk;
+    LaTile<TI, NV, THREADS, VEC> tv;
     // One wave forms a chunk's decays while the others work on the chunk before.
-    constexpr int DW = 3;
+    constexpr int DW = WAVES - 1;
     double total = 0.0;
     auto load_decay = [&](int u0, int lane) {   // g of the lane's step
         const int u = reverse ? cnt - u0 - lane : u0 + lane;
@@ -390,7 +394,7 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
 #pragma unroll
         for (int piece = 0; piece < NP; ++piece)
             for (int tt = 0; tt < TT; tt += 2)
-                s.p[piece][Op::template at<T>(16 * tt + (threadIdx.x >> 4), 16 * (tt + 1) + (threadIdx.x & 15))] = 0;
+                if (threadIdx.x < 256) s.p[piece][Op::template at<T>(16 * tt + (threadIdx.x >> 4), 16 * (tt + 1) + (threadIdx.x & 15))] = 0;
     }
     constexpr int OS = F32 ? 4 : ES;
     const bool writes = p.out != nullptr;
@@ -450,12 +454,13 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
 
         la_f4 acc[CT][OUT ? TT : 1];
         if constexpr (OUT) {
-            // pairs: the waves take the tiles of the lower triangle in turn (waves with
-            // none left form the last one again: no branch between the tiles)
+            // pairs: the waves take the tiles of the lower triangle in turn; the last wave,
+            // which formed the decays, has the fewest
             constexpr int TILES = TT * (TT + 1) / 2;
 #pragma unroll
-            for (int j = 0; j < (TILES + 3) / 4; ++j) {
-                const int idx = min(wave + 4 * j, TILES - 1);
+            for (int j = 0; j < (TILES + WAVES - 1) / WAVES; ++j) {
+                if (wave + WAVES * j >= TILES) break;
+                const int idx = wave + WAVES * j;
                 const int tt = idx < 1 ? 0 : idx < 3 ? 1 : idx < 6 ? 2 : 3, ts = idx - tt * (tt + 1) / 2;
                 la_f4 d = {0, 0, 0, 0};
 #pragma unroll
@@ -637,7 +642,7 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
             if (threadIdx.x < T && u < cnt) {
                 float x = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) x += s.dot[w * T + threadIdx.x];
+                for (int w = 0; w < WAVES; ++w) x += s.dot[w * T + threadIdx.x];
                 dot[reverse ? cnt - 1 - u : u] = x;
             }
         }
@@ -647,7 +652,7 @@ __global__ __launch_bounds__(LA_THREADS, la_waves_per_simd(DK, CT)) void la_pass
         // rows past the sequence's length
         if (p.out) {
             const int from = max(t0, n), to = min(t0 + a.seg, a.L);
-            for (int i = threadIdx.x; i < (to - from) * dn; i += LA_THREADS) {
+            for (int i = threadIdx.x; i < (to - from) * dn; i += THREADS) {
                 const int64_t t = from + i / dn;
                 const int64_t at = (b * static_cast<int64_t>(a.L) + t) * out_row + static_cast<int64_t>(h) * dn + i % dn;
                 if constexpr (F32)
@@ -679,29 +684,33 @@ void la_launch_passes(const LaArgs& a, int count, bool out, hipStream_t st) {
     }
     const bool dot = out && a.pass[0].dot, f32 = out && a.pass[0].out_f32;
     const dim3 grid(out ? a.nseg : a.nseg - 1, a.H, static_cast<unsigned>(a.B) * count);
-    auto with = [&](auto width, auto tiles, auto whole) {
-        constexpr int W = decltype(width)::value, N = decltype(tiles)::value;
+    auto with = [&](auto width, auto tiles, auto waves, auto whole) {
+        constexpr int W = decltype(width)::value, N = decltype(tiles)::value, G = decltype(waves)::value;
         constexpr bool V = decltype(whole)::value, F = sizeof(TI) == 4;
         if (!out)
-            la_pass_kernel<TI, W, N, false, false, V, F><<<grid, LA_THREADS, 0, st>>>(a);
+            la_pass_kernel<TI, W, N, G, false, false, V, F><<<grid, 64 * G, 0, st>>>(a);
         else if (dot && f32)
-            la_pass_kernel<TI, W, N, true, true, V, true><<<grid, LA_THREADS, 0, st>>>(a);
+            la_pass_kernel<TI, W, N, G, true, true, V, true><<<grid, 64 * G, 0, st>>>(a);
         else if (dot)
-            la_pass_kernel<TI, W, N, true, true, V, F><<<grid, LA_THREADS, 0, st>>>(a);
+            la_pass_kernel<TI, W, N, G, true, true, V, F><<<grid, 64 * G, 0, st>>>(a);
         else
-            la_pass_kernel<TI, W, N, true, false, V, F><<<grid, LA_THREADS, 0, st>>>(a);
+            la_pass_kernel<TI, W, N, G, true, false, V, F><<<grid, 64 * G, 0, st>>>(a);
     };
+    typedef std::integral_constant<int, 1> one;
+    typedef std::integral_constant<int, 2> two;
+    typedef std::integral_constant<int, 4> four;
+    typedef std::integral_constant<int, 8> eight;
     auto pick = [&](auto width) {
-        if (la_tiles(a.pass[0].dn) == 2) {
+        if (a.pass[0].dn <= 64) {
             if (vec)
-                with(width, std::integral_constant<int, 2>(), std::true_type());
+                with(width, one(), four(), std::true_type());
             else
-                with(width, std::integral_constant<int, 2>(), std::false_type());
+                with(width, one(), four(), std::false_type());
         } else {
             if (vec)
-                with(width, std::integral_constant<int, 1>(), std::true_type());
+                with(width, one(), eight(), std::true_type());
             else
-                with(width, std::integral_constant<int, 1>(), std::false_type());
+                with(width, two(), four(), std::false_type());
         }
     };
     switch (la_width(a.pass[0].dc)) {
