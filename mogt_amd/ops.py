@@ -3236,8 +3236,8 @@ def add_rmsnorm_fp8(x: torch.Tensor, z: torch.Tensor, scale: float, weight: torc
     values with a float32 scale for every 128 of a row, which ``linear_fp8`` takes.
 
     A block's scale is its largest magnitude / 448 (2^-126 at least), the values
-    ``n / scale`` rounded to nearest even; the norm is fp32, its sum of squares in
-    64 bits.  Returns ``(x', q, q_scale)``.  Rows of a multiple of 4
+    ``n / scale`` rounded to nearest even; the norm is in 64 bits, of ``x'`` before it
+    is rounded.  Returns ``(x', q, q_scale)``.  Rows of a multiple of 4
     values, up to 4096.  No autograd."""
     _same_device("add_rmsnorm_fp8", x, (z, weight))
     if x.dtype != torch.float32:
