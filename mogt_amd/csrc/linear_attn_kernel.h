@@ -15,6 +15,12 @@
 //   writes   S = exp(c_T) S + K^T (w V): D[row of S][v]
 // Operands that contract over steps are read transposed from LDS (bf16: the
 // transposing LDS read).  S never leaves registers inside a segment.
+//
+// 32768 steps of 16 heads of 128, bf16: sums 74 us (268 MB; without its products
+// as long: 4.4 TB/s while it runs), outputs 157 us (537 MB; 148 without loads: the
+// vector unit is busy for 51 % of the cycles, the matrix unit 25 %, LDS 29 %, what
+// is left are the waits between the steps above).  2 x 8192 steps of 12 heads of 64:
+// sums 17 us, outputs 30, two gradients with their products 66 (100 MB each).
 #include "linear_attn.h"
 
 namespace mogt {
