@@ -2977,6 +2977,11 @@ def _linear_attn_segment(B: int, L: int, H: int, dk: int, dv: int, dtype: torch.
     return chunk * max(1, min(-(-steps // chunk), most // chunk))
 
 
+def _empty_rows(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape (``empty_like`` takes half the time)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _linear_attn_rows(t: torch.Tensor, steps: int) -> torch.Tensor:
     """Rows with unit stride in a head, near enough for a segment's offsets."""
     t = _unit_channels(t)
@@ -3013,10 +3018,9 @@ def _linear_attn_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     B, L, H, dv = v.shape
     dk = q.shape[-1]
     segment = _linear_attn_segment(B, L, H, dk, dv, v.dtype)
-    f32 = dict(dtype=torch.float32, device=v.device)
-    out = torch.empty((B, L, H, dv), dtype=v.dtype, device=v.device)
-    state = torch.empty((B, H, dk, dv) if want_state else (0,), **f32)
-    carries = torch.empty((B, H, max(1, -(-L // segment)) + 1, dv, dk) if want_carries else (0,), **f32)
+    out = _empty_rows(v)
+    state = log_decay.new_empty((B, H, dk, dv) if want_state else 0)
+    carries = log_decay.new_empty((B, H, max(1, -(-L // segment)) + 1, dv, dk) if want_carries else 0)
     p, held = _linear_attn_problem(q, k, v, log_decay, initial_state, lengths, scale, segment)
     nbytes = lib.mogt_linear_attn_workspace_bytes(p)
     ws = scratch(nbytes, v.device) if nbytes else None
@@ -3054,11 +3058,10 @@ def _linear_attn_grad_op(dout: torch.Tensor, dfinal: torch.Tensor | None, q: tor
     dout = _dense(dout if dout.dtype == v.dtype else dout.to(v.dtype))
     dfinal = None if dfinal is None else dfinal.to(torch.float32).contiguous()
     p, held = _linear_attn_problem(q, k, v, log_decay, initial_state, lengths, scale, segment)
-    f32 = torch.float32
-    shapes = (((B, L, G, dk), q.dtype), ((B, L, G, dk), q.dtype), ((B, L, H, dv), q.dtype),
-              ((H,) if log_decay.ndim == 1 else (B, L, H), f32), ((B, H, dk, dv), f32))
-    make = torch.empty if B > 0 and H > 0 else torch.zeros
-    grads = [make(s if n else (0,), dtype=t, device=v.device) for (s, t), n in zip(shapes, need)]
+    shapes = ((q, (B, L, G, dk)), (q, (B, L, G, dk)), (q, (B, L, H, dv)), (log_decay, log_decay.shape),
+              (log_decay, (B, H, dk, dv)))
+    grads = [(t.new_empty(s) if B > 0 and H > 0 else t.new_zeros(s)) if n else t.new_empty(0)
+             for (t, s), n in zip(shapes, need)]
     nbytes = lib.mogt_linear_attn_bwd_workspace_bytes(p)
     ws = scratch(nbytes, v.device)
     out = _lib.LINEAR_ATTN_GRADIENTS.pack(*[t.data_ptr() if n else 0 for t, n in zip(grads, need)])
@@ -3170,7 +3173,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 @_op("mogt::linear_attention_step_", mutates=("state",))
 def _linear_attn_step_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: torch.Tensor,
                          log_decay: torch.Tensor, scale: float) -> torch.Tensor:
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    out = _empty_rows(v)
     p, held = _linear_attn_problem(q, k, v, log_decay, None, None, scale, 0)
     with _on_device(v.device):
         rc = _lib.load().mogt_linear_attn_step(p, state.data_ptr(), out.data_ptr(), _stream_handle(v.device))
@@ -3213,9 +3216,9 @@ def _add_rmsnorm_fp8_op(x: torch.Tensor, z: torch.Tensor, scale: float, weight: 
                         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     x, z, w = x.contiguous(), z.contiguous(), weight.contiguous()
     D = x.shape[-1]
-    x_out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-    q = torch.empty(x.shape, dtype=_FP8, device=x.device)
-    q_scale = torch.empty((*x.shape[:-1], _fp8_blocks(D)), dtype=torch.float32, device=x.device)
+    x_out = torch.empty_like(x)
+    q = torch.empty_like(x, dtype=_FP8)
+    q_scale = x.new_empty((*x.shape[:-1], _fp8_blocks(D)))
     with _on_device(x.device):
         rc = _lib.load().mogt_add_rmsnorm_fp8_fwd(x.data_ptr(), z.data_ptr(), scale, w.data_ptr(), x_out.data_ptr(),
                                                   q.data_ptr(), q_scale.data_ptr(), x.numel() // D, D, eps,
@@ -3312,7 +3315,7 @@ def _linear_fp8_op(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_sc
     if not w.is_contiguous() or w.data_ptr() % 16 != 0:
         w = torch.empty(w.shape, dtype=w.dtype, device=w.device).copy_(w)
     x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
-    y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+    y = x_scale.new_empty((*x.shape[:-1], N), dtype=out_dtype)
     with _on_device(x.device):
         rc = _lib.load().mogt_linear_fp8(rows.data_ptr(), rows.stride(0), x_scale.data_ptr(), w.data_ptr(),
                                          w_scale.data_ptr(), y.data_ptr(), rows.shape[0], N, K, _DTYPE_CODE[out_dtype],
