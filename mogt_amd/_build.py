@@ -35,8 +35,9 @@ HIPCC_FLAGS = [
 ]
 
 # Per-file extras.  The rank-1, linear attention and 8-bit product kernels
-# rescale MFMA accumulators between chains; keeping accumulators in ordinary VGPRs avoids a copy to and from the
-# accumulation registers around every such rescale.
+# rescale MFMA accumulators between chains; keeping accumulators in ordinary
+# VGPRs avoids a copy to and from the accumulation registers around every such
+# rescale.
 FILE_FLAGS = {
     "rank1_scan.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "linear_attn_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
@@ -53,8 +54,11 @@ def source_manifest() -> dict[str, str]:
     against the tree, and a profile taken from one build can name the exact
     sources its kernels came from."""
     files = sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "mogt_scan.h"]
-    out = {f.name: hashlib.sha256(f.read_bytes()).hexdigest()[:12] for f in files}
-    flags = repr((HIPCC_FLAGS, sorted(FILE_FLAGS.items())))
+    # a file's extras belong to its own entry, so that profiles of other files stay
+    # valid; the rank-1 scan's are part of `flags`, which its profiles name
+    own = {name: repr(extra).encode() for name, extra in FILE_FLAGS.items() if name != "rank1_scan.hip"}
+    out = {f.name: hashlib.sha256(f.read_bytes() + own.get(f.name, b"")).hexdigest()[:12] for f in files}
+    flags = repr((HIPCC_FLAGS, sorted(item for item in FILE_FLAGS.items() if item[0] not in own)))
     out["flags"] = hashlib.sha256(flags.encode()).hexdigest()[:12]
     return out
 
