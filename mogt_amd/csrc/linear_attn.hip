@@ -454,7 +454,7 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
         d.rstates = rstates;
         d.dot_q = dot_q;
         d.dot_k = dot_k;
-            d.dk = static_cast<int>(q->key_dim);
+        d.dk = static_cast<int>(q->key_dim);
         d.have_last = dfinal_state != nullptr;
         d.dinit = g->dinitial_state;
         if (need_g) {

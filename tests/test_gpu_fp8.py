@@ -115,6 +115,32 @@ def test_zeros_and_tiny_rows(gpu):
     assert float(s[1, 0]) == 2.0 ** -126 and bool((q[1, :128].float() - 1e-38 * 2.0 ** 126).abs().max() <= 2.0 ** -10 + 0.06)
 
 
+def test_norm_special_values(gpu):
+    """Rows below the least scale, of zeros, and with what is not finite: the last
+    leave their own row only, a row with an infinity is zeros but for it (its norm is
+    over an infinite root mean square), as the definition's."""
+    from mogt_amd import ops
+    announce("add_rmsnorm_fp8 special values")
+    x, z, w = rnd(7, 516, seed=21), torch.zeros(7, 516, device="cuda"), 1 + 0.2 * rnd(516, seed=22)
+    want = ops.add_rmsnorm_fp8(x, z, 1.0, w)
+    bad = x.clone()
+    bad[1] = 0.0
+    bad[3, 130] = float("nan")
+    bad[5, 200] = float("-inf")
+    x_out, q, s = ops.add_rmsnorm_fp8(bad, z, 1.0, w)
+    q = q.float()
+    assert torch.equal(q[[0, 2, 4, 6]], want[1].float()[[0, 2, 4, 6]]) and torch.equal(s[[0, 2, 4, 6]], want[2][[0, 2, 4, 6]])
+    assert not q[1].any() and bool((s[1] == 2.0 ** -126).all())
+    assert bool(q[3].isnan().all())
+    assert bool(q[5, 200].isnan()) and not q[5, [i for i in range(516) if i != 200]].any()
+    # normalised values up to 3e-36: the scale is 2^-126 and steps are its e4m3 steps
+    xo, q, s = ops.add_rmsnorm_fp8(x, z, 1.0, w * 1e-36)
+    xd = xo.double()
+    u = xd / torch.sqrt((xd * xd).mean(1, keepdim=True) + 1e-6) * (w * 1e-36).double() * 2.0 ** 126
+    assert bool((s == 2.0 ** -126).all())
+    assert bool(((q.double() - u).abs() <= torch.clamp(u.abs() * 2.0 ** -4, min=2.0 ** -10) * (1 + 1e-6)).all())
+
+
 def product(M, N, K, seed=0):
     from mogt_amd import ops
     x, xs = ops.quantize_fp8(rnd(M, K, seed=seed) * torch.exp(rnd(M, 1, seed=seed + 1)))

@@ -204,6 +204,31 @@ def test_what_is_not_finite_reaches_no_earlier_output(gpu, dtype, name, value):
         check(n, got[n][0, rows][:, heads], want[n][0, rows][:, heads], mag[n][0, rows][:, heads], bound(t))
 
 
+@pytest.mark.parametrize("dtype,dk,dv", [(F32, 64, 128), (BF16, 32, 128), (BF16, 128, 96), (BF16, 128, 100), (F32, 128, 65)])
+def test_wide_values(gpu, dtype, dk, dv):
+    """More than 64 value columns (whole vectors and single elements): ragged, in
+    segments, a decay of zero, and an infinity that reaches no earlier step."""
+    announce(f"linear_attention wide {dk} {dv} {dtype}")
+    t, kw = make(3, 330, 2, 1, dk, dv, dtype, seed=dv)
+    t["log_decay"][1, 100] = float("-inf")
+    kw["lengths"] = torch.tensor([330, 201, 0], device="cuda", dtype=torch.int32)
+    out, state, _ = run_both(t, kw)
+    assert not out[1, 201:].any() and not out[2].any()
+    bad = dict(t, v=t["v"].clone())
+    bad["v"][0, 177, 1, dv - 1] = float("inf")
+    leaves = {n: x.detach() for n, x in bad.items() if x is not None}
+    got, got_state = call(leaves, kw, return_state=True)
+    rest = torch.ones(dv, dtype=torch.bool)
+    rest[dv - 1] = False
+    want, mag = [lo.linear_attention(t["q"], t["k"], t["v"], t["log_decay"], initial_state=t["initial_state"], mag=m,
+                                     lengths=kw["lengths"]) for m in (0, 1)]
+    for rows, heads, cols in ((slice(0, 177), slice(None), slice(None)), (slice(None), 0, slice(None)),
+                              (slice(None), slice(None), rest)):
+        check("out", got[0, rows][:, heads][..., cols], want["out"][0, rows][:, heads][..., cols],
+              mag["out"][0, rows][:, heads][..., cols], bound(t))
+    assert not got[0, 177, 1, dv - 1].isfinite() and torch.equal(got[1:], out[1:]) and torch.equal(got_state[1:], state[1:])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_decay_of_minus_infinity_and_growth(gpu, dtype):
     """A state emptied in the middle of a chunk, decays far below fp32's least,
