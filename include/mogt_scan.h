@@ -760,7 +760,7 @@ int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state,
  * A row of `dim` values has ceil(dim / 128) scales; the last block may be short.
  * mogt_add_rmsnorm_fp8_fwd: x_out = x + (scale * z) [the product rounded to z's
  *   dtype], as mogt_add_rmsnorm_fwd, and the rows rmsnorm(x_out) * weight in 8 bits
- *   (sum of squares in 64 bits, no rounding before the 8 bits); x, x_out fp32, rows of
+ *   (in 64 bits from the sum on, not rounded before the 8 bits); x, x_out fp32, rows of
  *   `dim` contiguous elements, dim a multiple of 4 and <= 4096.
  * mogt_quantize_fp8: the rows of x (row stride ld, a multiple of 4) in 8 bits, with
  *   block_rows 1 or 128 (weights); dim a multiple of 4.
