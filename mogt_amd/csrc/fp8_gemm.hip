@@ -34,6 +34,7 @@ namespace {
 
 typedef int f8_i8 __attribute__((ext_vector_type(8)));
 typedef int f8_i4 __attribute__((ext_vector_type(4)));
+typedef int f8_i2 __attribute__((ext_vector_type(2)));
 typedef float f8_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 f8_b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 f8_b2 __attribute__((ext_vector_type(2)));
@@ -45,7 +46,7 @@ struct F8Gemm {
     int64_t M, ldx, ldy;
     int N, K, kb;
     int nm, nn;          // tiles
-    int whole;           // rows of y are whole 16 bytes, a tile's within 2^31 bytes
+    int piece;           // bytes of a store: the most that rows of y are whole in, up to 16; 0: a tile's lie beyond 2^31 bytes
 };
 
 // An operand's 32 values of a lane as the matrix instruction takes them.
@@ -111,6 +112,19 @@ __device__ __forceinline__ void f8_store(const F8Gemm& p, int64_t m, int n, f8_f
         for (int i = 0; i < 4; ++i)
             if (n + i < p.N) y[i] = IO<T>::st(v[i]);
     }
+}
+
+// `B` bytes from LDS to byte `at` of the buffer (an offset out of its range writes nothing)
+template <int B>
+__device__ __forceinline__ void f8_store_piece(const char* from, __amdgpu_buffer_rsrc_t to, uint32_t at) {
+    if constexpr (B == 16)
+        __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const f8_i4*>(from), to, at, 0, 0);
+    else if constexpr (B == 8)
+        __builtin_amdgcn_raw_buffer_store_b64(*reinterpret_cast<const f8_i2*>(from), to, at, 0, 0);
+    else if constexpr (B == 4)
+        __builtin_amdgcn_raw_buffer_store_b32(*reinterpret_cast<const int*>(from), to, at, 0, 0);
+    else
+        __builtin_amdgcn_raw_buffer_store_b16(*reinterpret_cast<const int16_t*>(from), to, at, 0, 0);
 }
 
 // Tiles of work-group `bid` of `grid` (a multiple of 8, or all of n): its XCD (ids
@@ -251,10 +265,12 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (p.whole) {
+        if (p.piece) {
             // Through the last stage's LDS (no wave reads it any more), so that a row of the
             // wave's leaves in whole lines: straight from the registers 16 rows' 32 bytes a
-            // store took 33 us a tile, more than its sixteen stages.
+            // store took 33 us a tile, more than its sixteen stages.  Rows that are not whole
+            // 16 bytes leave in smaller pieces, coalesced all the same (4096 x 4098 x 2048, bf16:
+            // 71 us, straight from the registers 100; 13577 x 3919 x 864: 107, 154).
             constexpr int ROOM = STAGE / WAVES / (16 * OUT_ROW), G = ROOM >= MT ? MT : ROOM >= 4 ? 4 : ROOM >= 2 ? 2 : 1;
             static_assert(ROOM >= 1 && MT % G == 0, "a tile's rows fit");
             __syncthreads();
@@ -277,15 +293,25 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
                         *reinterpret_cast<Pack<TO, 4>*>(mine + r * OUT_ROW + ((byte >> 4 ^ (r & (CH - 1))) << 4) + (byte & 15)) = v;
                     }
                 // only the wave's own rows: its reads wait for its writes
-#pragma unroll
-                for (int k = 0; k < G * 16 * OUT_ROW / 1024; ++k) {
-                    const int id = 64 * k + l, r = id / CH, c = id % CH;
-                    const f8_i4 v = *reinterpret_cast<const f8_i4*>(mine + r * OUT_ROW + ((c ^ (r & (CH - 1))) << 4));
-                    const int m = 16 * i0 + r, n = c * (16 / static_cast<int>(sizeof(TO)));
-                    const uint32_t at = static_cast<uint32_t>((wm * MT * 16 + m) * ldy + wn * NT * 16 + n) * static_cast<uint32_t>(sizeof(TO));
-                    const bool in = (m < left) & (n < nw);
-                    __builtin_amdgcn_raw_buffer_store_b128(v, ry, in ? at : 0xffffff00u, 0, 0);
-                }
+                auto leave = [&](auto piece) __attribute__((always_inline)) {
+                    constexpr int B = decltype(piece)::value, PR = OUT_ROW / B;   // pieces of a row
+#pragma unroll 4
+                    for (int k = 0; k < G * 16 * OUT_ROW / (64 * B); ++k) {
+                        const int id = 64 * k + l, r = id / PR, byte = id % PR * B;
+                        const int m = 16 * i0 + r, n = byte / static_cast<int>(sizeof(TO));
+                        const uint32_t at = static_cast<uint32_t>((wm * MT * 16 + m) * ldy + wn * NT * 16 + n) * static_cast<uint32_t>(sizeof(TO));
+                        const bool in = (m < left) & (n < nw);
+                        f8_store_piece<B>(mine + r * OUT_ROW + ((byte >> 4 ^ (r & (CH - 1))) << 4) + (byte & 15), ry, in ? at : 0xffffff00u);
+                    }
+                };
+                if (p.piece == 16)
+                    leave(std::integral_constant<int, 16>());
+                else if (p.piece == 8)
+                    leave(std::integral_constant<int, 8>());
+                else if (EXACT || p.piece == 4)
+                    leave(std::integral_constant<int, 4>());
+                else
+                    leave(std::integral_constant<int, 2>());
             }
             stored = true;
         } else {
@@ -376,7 +402,8 @@ void f8_launch(F8Gemm& p, int cus, hipStream_t st) {
     // and up to 32 rows the form without tiles: 32 x 6144 9.9 against 10.6 and 15.4, 16 x
     // 6144 7.2 against 10.7 and 15.1.
     const int each = EXACT ? 4 : 2;
-    p.whole = p.N * each % 16 == 0 && p.ldy * each * 256 < 0x7fffff00;
+    const int64_t row = p.ldy * each;
+    p.piece = row * 256 >= 0x7fffff00 ? 0 : row % 16 == 0 ? 16 : row % 8 == 0 ? 8 : row % 4 == 0 ? 4 : 2;
     constexpr int BM = EXACT ? 128 : 256;
     if (tiles(BM, 256) >= (EXACT ? 2 * cus : cus * 3 / 4)) {
         const int n = tiles(BM, 256);

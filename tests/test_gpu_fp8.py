@@ -253,6 +253,33 @@ def test_product_neighbours_are_left_alone(gpu):
         assert torch.equal(y[:M], ops.linear_fp8(x, xs, w, ws, out_dtype=out)) and bool((y[M:] == 7).all())
 
 
+@pytest.mark.parametrize("N", [3502, 3501, 523, 262])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_product_of_rows_in_pieces(gpu, N, out):
+    """Outputs whose rows are whole 2, 4 or 8 bytes: each tile's size, and rows behind the last."""
+    from mogt_amd import _lib
+    announce(f"linear_fp8 rows of {N} {out}")
+    for M in (70, 700, 4100):
+        p = product(M, N, 272, seed=9)
+        x, xs, w, ws = p
+        y = torch.full((M + 3, N), 7.0, device="cuda", dtype=out)
+        rc = _lib.load().mogt_linear_fp8(x.data_ptr(), 272, xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), M, N, 272,
+                                         1 if out == BF16 else 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and bool((y[M:] == 7).all())
+        check_product(y[:M], *p)
+
+
+def test_product_of_very_long_rows(gpu):
+    """A tile's rows of the output more than 2^31 bytes apart in all."""
+    from mogt_amd import ops
+    announce("linear_fp8 long rows")
+    N = 1 << 22
+    x, xs, w, ws = product(40, N, 16, seed=10)
+    y = ops.linear_fp8(x, xs, w, ws)
+    for a, b in ((0, 384), (N - 384, N), (N // 2 - 128, N // 2 + 128)):
+        assert torch.equal(y[:, a:b], ops.linear_fp8(x, xs, w[a:b], ws[a // 128:b // 128]))
+
+
 def test_what_is_not_finite_stays_in_its_row(gpu):
     from mogt_amd import ops
     announce("linear_fp8 special values")
