@@ -267,13 +267,16 @@ int la_args(const mogt_linear_attn_problem* q, LaArgs& a) {
 
 LaRows la_rows(const mogt_linear_attn_problem* q, const void* p, int64_t row, int64_t batch, int64_t head, int div,
                int64_t width) {
-    const int64_t es = q->io_dtype == MOGT_BF16 ? 2 : 4, each = 16 / es;
+    const int64_t es = q->io_dtype == MOGT_BF16 ? 2 : 4;
     LaRows r;
     r.p = p;
     r.row = row; r.batch = batch; r.head = head;
     r.div = div;
-    r.vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0 && row % each == 0 && batch % each == 0 && head % each == 0 &&
-            width % each == 0;
+    auto whole = [&](int64_t n) {
+        return reinterpret_cast<uintptr_t>(p) % n == 0 && row % (n / es) == 0 && batch % (n / es) == 0 && head % (n / es) == 0 &&
+               width % (n / es) == 0;
+    };
+    r.vec = whole(16) ? LA_VECTORS : es == 2 && whole(8) ? LA_HALVES : LA_SINGLE;
     return r;
 }
 

@@ -182,9 +182,8 @@ __device__ __forceinline__ int la_again(int x) {
 }
 
 // The rows of a chunk on their way from memory to LDS: W elements wide, 16 bytes
-// at a time over the work-group's threads.  VEC: whole aligned vectors, else one
-// element at a time.
-template <typename TI, int W, int THREADS, bool VEC>
+// at a time over the work-group's threads, or by their halves or single elements.
+template <typename TI, int W, int THREADS, int VEC>
 struct LaTile {
     static constexpr int T = LaChunk<TI>::T, EPC = 16 / sizeof(TI), CPR = W / EPC;
     static constexpr int N = (T * CPR + THREADS - 1) / THREADS;
@@ -202,8 +201,15 @@ struct LaTile {
         for (int i = 0; i < N; ++i) {
             const int u = row(me) + i * STEP;
             const uint32_t at = static_cast<uint32_t>(first) + static_cast<uint32_t>(u) * static_cast<uint32_t>(step) + c * static_cast<uint32_t>(sizeof(TI));
-            if constexpr (VEC) {
+            if constexpr (VEC == LA_VECTORS) {
                 r[i] = __builtin_amdgcn_raw_buffer_load_b128(b, ((u < left) & (c < d)) ? at : LA_OUTSIDE, 0, 0);
+            } else if constexpr (VEC == LA_HALVES) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const la_u2 w = __builtin_amdgcn_raw_buffer_load_b64(b, ((u < left) & (c + 4 * e < d)) ? at + 8 * e : LA_OUTSIDE, 0, 0);
+                    r[i][2 * e] = w[0];
+                    r[i][2 * e + 1] = w[1];
+                }
             } else if constexpr (sizeof(TI) == 4) {
 #pragma unroll
                 for (int e = 0; e < EPC; ++e)
@@ -276,8 +282,8 @@ __device__ __forceinline__ void la_pack4(float (&x)[4], Pack<bf16_t, 4>& w, bool
 }
 
 // OUT: the outputs (else a segment's state from zero); DOT: with their rows'
-// products; VEC: every role's rows in whole aligned vectors; F32: fp32 outputs.
-template <typename TI, int DK, int CT, int WAVES, bool OUT, bool DOT, bool VEC, bool F32>
+// products; VEC: the least of the roles' rows; F32: fp32 outputs.
+template <typename TI, int DK, int CT, int WAVES, bool OUT, bool DOT, int VEC, bool F32>
 __global__ __launch_bounds__(64 * WAVES, la_waves_per_simd(DK, CT, WAVES)) void la_pass_kernel(LaArgs a) {
     typedef LaOp<TI> Op;
     typedef typename Op::frag Frag;
@@ -683,16 +689,19 @@ __global__ __launch_bounds__(64 * WAVES, la_waves_per_simd(DK, CT, WAVES)) void 
 // (la_one_kind).
 template <typename TI>
 void la_launch_passes(const LaArgs& a, int count, bool out, hipStream_t st) {
-    bool vec = true;
+    int vec = LA_VECTORS;
     for (int i = 0; i < count; ++i) {
         const LaPass& p = a.pass[i];
-        vec = vec && p.k.vec && p.v.vec && (!out || (p.q.vec && (!p.dot || p.x.vec)));
+        vec = min(vec, min(p.k.vec, p.v.vec));
+        if (out) vec = min(vec, min(p.q.vec, p.dot ? p.x.vec : vec));
+        if (out && reinterpret_cast<uintptr_t>(p.out) % 16 != 0) vec = LA_SINGLE;
     }
     const bool dot = out && a.pass[0].dot, f32 = out && a.pass[0].out_f32;
     const dim3 grid(out ? a.nseg : a.nseg - 1, a.H, static_cast<unsigned>(a.B) * count);
     auto with = [&](auto width, auto tiles, auto waves, auto whole) {
         constexpr int W = decltype(width)::value, N = decltype(tiles)::value, G = decltype(waves)::value;
-        constexpr bool V = decltype(whole)::value, F = sizeof(TI) == 4;
+        constexpr int V = decltype(whole)::value;
+        constexpr bool F = sizeof(TI) == 4;
         if (!out)
             la_pass_kernel<TI, W, N, G, false, false, V, F><<<grid, 64 * G, 0, st>>>(a);
         else if (dot && f32)
@@ -706,18 +715,17 @@ void la_launch_passes(const LaArgs& a, int count, bool out, hipStream_t st) {
     typedef std::integral_constant<int, 2> two;
     typedef std::integral_constant<int, 4> four;
     typedef std::integral_constant<int, 8> eight;
+    typedef std::integral_constant<int, LA_SINGLE> single;
+    typedef std::integral_constant<int, sizeof(TI) == 2 ? LA_HALVES : LA_VECTORS> halves;
+    typedef std::integral_constant<int, LA_VECTORS> vectors;
     auto pick = [&](auto width) {
-        if (a.pass[0].dn <= 64) {
-            if (vec)
-                with(width, one(), four(), std::true_type());
-            else
-                with(width, one(), four(), std::false_type());
-        } else {
-            if (vec)
-                with(width, one(), eight(), std::true_type());
-            else
-                with(width, two(), four(), std::false_type());
-        }
+        const bool narrow = a.pass[0].dn <= 64;
+        if (vec == LA_VECTORS)
+            narrow ? with(width, one(), four(), vectors()) : with(width, one(), eight(), vectors());
+        else if (vec == LA_HALVES)
+            narrow ? with(width, one(), four(), halves()) : with(width, one(), eight(), halves());
+        else
+            narrow ? with(width, one(), four(), single()) : with(width, two(), four(), single());
     };
     switch (la_width(a.pass[0].dc)) {
         case 32: pick(std::integral_constant<int, 32>()); break;

@@ -229,6 +229,40 @@ def test_wide_values(gpu, dtype, dk, dv):
     assert not got[0, 177, 1, dv - 1].isfinite() and torch.equal(got[1:], out[1:]) and torch.equal(got_state[1:], state[1:])
 
 
+@pytest.mark.parametrize("B,L,H,G,dk,dv", [(2, 300, 2, 1, 100, 100), (1, 333, 3, 3, 36, 60), (1, 130, 2, 2, 12, 124),
+                                           (2, 90, 4, 2, 4, 4)])
+def test_rows_of_half_vectors(gpu, B, L, H, G, dk, dv):
+    """bf16 rows that are whole in 8 bytes and not in 16: the same values from rows
+    that are whole in neither, to the bit."""
+    announce(f"linear_attention half vectors {B} {L} {H} {G} {dk} {dv}")
+    t, kw = make(B, L, H, G, dk, dv, BF16, seed=dk)
+    out, state, grads = run_both(t, kw)
+    dout, dstate = gradients_in(t)
+    odd = dict(t)
+    for n in ("q", "k", "v"):
+        wide = torch.zeros(*t[n].shape[:-1], t[n].shape[-1] + 3, device="cuda", dtype=BF16)
+        wide[..., 1:-2] = t[n]
+        odd[n] = wide[..., 1:-2]
+    for a, b in zip(run_all(odd, kw, dout, dstate)[:5], run_all(t, kw, dout, dstate)[:5]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_output_memory_at_any_element(gpu, dtype):
+    """Through the C entry: an output that no vector is aligned in, and the elements
+    around it."""
+    from mogt_amd import _lib, ops
+    announce(f"linear_attention output alignment {dtype}")
+    t, _ = make(1, 90, 2, 2, 32, 64, dtype, seed=3)
+    want, _ = call(t, {}, return_state=True)
+    p, held = ops._linear_attn_problem(t["q"], t["k"], t["v"], t["log_decay"], t["initial_state"], None, 32 ** -0.5, 128)
+    y = torch.full((want.numel() + 8,), 7.0, device="cuda", dtype=dtype)
+    rc = _lib.load().mogt_linear_attn_fwd(p, y.data_ptr() + 3 * y.element_size(), None, None, None, 0,
+                                          torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert torch.equal(y[3:-5].view(want.shape), want) and bool((y[:3] == 7).all()) and bool((y[-5:] == 7).all())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_decay_of_minus_infinity_and_growth(gpu, dtype):
     """A state emptied in the middle of a chunk, decays far below fp32's least,
