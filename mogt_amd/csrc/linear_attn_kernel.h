@@ -241,10 +241,8 @@ struct LaTile {
     }
 };
 
-// Pieces of an fp32 operand (LaChunk): of the writes, of pairs and reads, and of
-// those where the outputs' products with their rows are wanted (dot).
-template <typename TI> constexpr int la_pieces_write() { return sizeof(TI) == 2 ? 3 : 1; }
-template <typename TI, bool DOT> constexpr int la_pieces() { return sizeof(TI) == 2 ? (DOT ? 3 : 2) : 1; }
+// Pieces of an fp32 operand: three bf16 hold its 24 bits.
+template <typename TI> constexpr int la_pieces() { return sizeof(TI) == 2 ? 3 : 1; }
 
 template <typename TI, int DK, int CT, int WAVES, bool OUT, int NP>
 struct LaLds {
@@ -287,10 +285,12 @@ template <typename TI, int DK, int CT, int WAVES, bool OUT, bool DOT, int VEC, b
 __global__ __launch_bounds__(64 * WAVES, la_waves_per_simd(DK, CT, WAVES)) void la_pass_kernel(LaArgs a) {
     typedef LaOp<TI> Op;
     typedef typename Op::frag Frag;
-    constexpr int T = LaChunk<TI>::T, KS = LaChunk<TI>::KS, NP = la_pieces<TI, DOT>();
-    constexpr int NW = la_pieces_write<TI>(), TT = T / 16, RT = DK / 16, NV = 16 * CT * WAVES, THREADS = 64 * WAVES;
+    constexpr int T = LaChunk<TI>::T, KS = LaChunk<TI>::KS, NP = la_pieces<TI>();
+    constexpr int TT = T / 16, RT = DK / 16, NV = 16 * CT * WAVES, THREADS = 64 * WAVES;
     constexpr int E = KS / 4, ES = static_cast<int>(sizeof(TI));
-    constexpr bool LATE = DOT && NV > 64;   // rows of the next chunk are loaded once the outputs' registers are free
+    // Wide values: the next chunk's rows are loaded once the outputs' registers are free
+    // (outputs of 32768 steps of 16 heads of 128: 218 us, loaded first and spilled 239).
+    constexpr bool LATE = OUT && NV > 64 && (DOT || DK > 64);
     __shared__ __align__(16) LaLds<TI, DK, CT, WAVES, OUT, NP> s;
 
     const int which = __builtin_amdgcn_readfirstlane(blockIdx.z / a.B), b = blockIdx.z - which * a.B, h = blockIdx.y;
@@ -365,10 +365,6 @@ __global__ __launch_bounds__(64 * WAVES, la_waves_per_simd(DK, CT, WAVES)) void 
         if (a.nseg == 1 && p.keep && slot) write_state(slot, p.rs, p.cs);
     }
 
-    // A state that only feeds this pass's outputs takes two pieces of its writes; one
-    // that is handed on (a segment's, the last) or whose products are wanted three.
-    // (The last's whether it is asked for or not: outputs do not depend on that.)
-    const bool exact = seg == a.nseg - 1;
     LaTile<TI, DK, THREADS, VEC> tq, tk;
     LaTile<TI, NV, THREADS, VEC> tv;
     // One wave forms a chunk's decays while the others work on the chunk before.
@@ -616,36 +612,27 @@ __global__ __launch_bounds__(64 * WAVES, la_waves_per_simd(DK, CT, WAVES)) void 
             float w[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) w[e] = s.w[buf][KS * k + 4 * grp + Op::order(e)];
-            auto write = [&](auto pieces, int from) __attribute__((always_inline)) {
-                constexpr int N = decltype(pieces)::value;
-                Frag wv[CT][N];
+            Frag wv[CT][NP];
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    float x[E];
+            for (int c = 0; c < CT; ++c) {
+                float x[E];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] = Op::value(vf[c][k], e) * w[e];
-                    Op::template split<N>(x, wv[c]);
-                }
-                // products of one tile lie apart: the next waits for the last's result
-                constexpr int G = RT * CT < 4 ? RT : 4 / CT;
+                for (int e = 0; e < E; ++e) x[e] = Op::value(vf[c][k], e) * w[e];
+                Op::template split<NP>(x, wv[c]);
+            }
+            // products of one tile lie apart: the next waits for the last's result
+            constexpr int G = RT * CT < 4 ? RT : 4 / CT;
 #pragma unroll
-                for (int r0 = 0; r0 < RT; r0 += G) {
-                    Frag kf[G];
+            for (int r0 = 0; r0 < RT; r0 += G) {
+                Frag kf[G];
 #pragma unroll
-                    for (int r = 0; r < G; ++r) kf[r] = Op::template column<DK>(s.k, KS * k, r0 + r, lane);
+                for (int r = 0; r < G; ++r) kf[r] = Op::template column<DK>(s.k, KS * k, r0 + r, lane);
 #pragma unroll
-                    for (int piece = from; piece < N; ++piece)
+                for (int piece = 0; piece < NP; ++piece)
 #pragma unroll
-                        for (int r = 0; r < G; ++r)
+                    for (int r = 0; r < G; ++r)
 #pragma unroll
-                            for (int c = 0; c < CT; ++c) S[c][r0 + r] = Op::mma(kf[r], wv[c][piece], S[c][r0 + r]);
-                }
-            };
-            if constexpr (OUT && !DOT && NW == 3) {
-                write(std::integral_constant<int, 2>(), 0);
-                if (exact) write(std::integral_constant<int, 3>(), 2);
-            } else {
-                write(std::integral_constant<int, NW>(), 0);
+                        for (int c = 0; c < CT; ++c) S[c][r0 + r] = Op::mma(kf[r], wv[c][piece], S[c][r0 + r]);
             }
         }
         if constexpr (OUT && DOT) {
