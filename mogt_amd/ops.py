@@ -3211,10 +3211,17 @@ def _fp8_blocks(n: int) -> int:
     return -(-n // FP8_BLOCK)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor at a multiple of four of its elements (a copy where it is
+    not: a view into a flat buffer)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % (4 * t.element_size()) == 0 else t.clone()
+
+
 @_op("mogt::add_rmsnorm_fp8")
 def _add_rmsnorm_fp8_op(x: torch.Tensor, z: torch.Tensor, scale: float, weight: torch.Tensor, eps: float
                         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    x, z, w = x.contiguous(), z.contiguous(), weight.contiguous()
+    x, z, w = _aligned(x), _aligned(z), _aligned(weight)
     D = x.shape[-1]
     x_out = torch.empty_like(x)
     q = torch.empty_like(x, dtype=_FP8)
