@@ -767,7 +767,8 @@ int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state,
  * mogt_linear_fp8: y[m][n] = sum_k x[m][k] w[n][k] of the values both stand for: x
  *   [rows, width] with x_scale [rows, ceil(width / 128)], w [outputs, width]
  *   contiguous with w_scale [ceil(outputs / 128), ceil(width / 128)]; y [rows,
- *   outputs] contiguous, fp32 or bf16, rounded once.  width and ldx multiples of 16.
+ *   outputs] contiguous, fp32 or bf16, rounded once.  width and ldx multiples of 16,
+ *   ldx at most 2^22, outputs at most 2^30; x, w and y 16-byte aligned.
  *   Blocks' sums are scaled and added in fp32; within a block bf16 outputs take the
  *   8-bit matrix instruction, whose sums are within 1.4e-5 (as 2-norms, on normal
  *   rows) and fp32 outputs the bf16 one on the same values, which adds in fp32.

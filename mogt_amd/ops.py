@@ -3204,6 +3204,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sta
 # ---------------------------------------------------------------------------
 FP8_BLOCK = 128
 FP8_MAX_ROW = 4096     # values of a row of the norm
+FP8_MAX_STRIDE = 1 << 22   # of the product's rows, whose tiles are addressed by 32-bit offsets
 _FP8 = torch.float8_e4m3fn
 
 
@@ -3266,12 +3267,12 @@ def add_rmsnorm_fp8(x: torch.Tensor, z: torch.Tensor, scale: float, weight: torc
 @_op("mogt::quantize_fp8")
 def _quantize_fp8_op(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
     D = x.shape[-1]
-    rows = _fp8_rows(x, 4)
+    rows, ld = _fp8_rows(x, 4)
     q = torch.empty(x.shape, dtype=_FP8, device=x.device)
     lead = x.shape[:-1] if block_rows == 1 else (_fp8_blocks(x.shape[0]),)
     q_scale = torch.empty((*lead, _fp8_blocks(D)), dtype=torch.float32, device=x.device)
     with _on_device(x.device):
-        rc = _lib.load().mogt_quantize_fp8(rows.data_ptr(), rows.stride(0), q.data_ptr(), q_scale.data_ptr(),
+        rc = _lib.load().mogt_quantize_fp8(rows.data_ptr(), ld, q.data_ptr(), q_scale.data_ptr(),
                                            rows.shape[0], D, _DTYPE_CODE[x.dtype], block_rows,
                                            _stream_handle(x.device))
     _lib.check(rc, "mogt_quantize_fp8")
@@ -3285,15 +3286,16 @@ def _(x, block_rows):
             x.new_empty((*lead, _fp8_blocks(x.shape[-1])), dtype=torch.float32))
 
 
-def _fp8_rows(x: torch.Tensor, each: int) -> torch.Tensor:
+def _fp8_rows(x: torch.Tensor, each: int, most: int | None = None) -> tuple[torch.Tensor, int]:
     """x as [rows, D] with unit stride in a row, aligned for vectors of ``each``
-    elements (a copy where it is not)."""
+    elements, and its row stride, at most ``most`` (a copy where it is not)."""
     D = x.shape[-1]
     rows = x.reshape(-1, D)
-    if (rows.stride(-1) != 1 or rows.stride(0) < D or rows.stride(0) % each != 0
+    ld = rows.stride(0) if rows.shape[0] > 1 else D   # one row's is any number
+    if (rows.stride(-1) != 1 or ld < D or ld % each != 0 or (most is not None and ld > most)
             or rows.data_ptr() % (each * x.element_size()) != 0):
-        rows = torch.empty(rows.shape, dtype=x.dtype, device=x.device).copy_(rows)
-    return rows
+        rows, ld = torch.empty(rows.shape, dtype=x.dtype, device=x.device).copy_(rows), D
+    return rows, ld
 
 
 def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
@@ -3318,13 +3320,13 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
 def _linear_fp8_op(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                    out_dtype: torch.dtype) -> torch.Tensor:
     N, K = w.shape
-    rows = _fp8_rows(x, 16)
+    rows, ld = _fp8_rows(x, 16, FP8_MAX_STRIDE)
     if not w.is_contiguous() or w.data_ptr() % 16 != 0:
         w = torch.empty(w.shape, dtype=w.dtype, device=w.device).copy_(w)
     x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
     y = x_scale.new_empty((*x.shape[:-1], N), dtype=out_dtype)
     with _on_device(x.device):
-        rc = _lib.load().mogt_linear_fp8(rows.data_ptr(), rows.stride(0), x_scale.data_ptr(), w.data_ptr(),
+        rc = _lib.load().mogt_linear_fp8(rows.data_ptr(), ld, x_scale.data_ptr(), w.data_ptr(),
                                          w_scale.data_ptr(), y.data_ptr(), rows.shape[0], N, K, _DTYPE_CODE[out_dtype],
                                          _stream_handle(x.device))
     _lib.check(rc, "mogt_linear_fp8")
@@ -3340,7 +3342,7 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x w^T`` of 8-bit operands: ``x [..., K]`` in e4m3 with ``x_scale [...,
     ceil(K / 128)]`` and ``w [N, K]`` with ``w_scale [ceil(N / 128), ceil(K /
-    128)]`` (``add_rmsnorm_fp8``, ``quantize_fp8``), K a multiple of 16.
+    128)]`` (``add_rmsnorm_fp8``, ``quantize_fp8``), K a multiple of 16 up to 2^22.
 
     Each block's products are added on the matrix cores, scaled and added in
     float32, and rounded once to ``out_dtype`` (bfloat16 or float32).  bfloat16
