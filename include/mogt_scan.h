@@ -769,7 +769,9 @@ int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state,
  *   contiguous with w_scale [ceil(outputs / 128), ceil(width / 128)]; y [rows,
  *   outputs] contiguous, fp32 or bf16, rounded once.  width and ldx multiples of 16,
  *   ldx at most 2^22, outputs at most 2^30; x, w and y 16-byte aligned.
- *   Blocks' sums are scaled and added in fp32; within a block bf16 outputs take the
+ *   Blocks' sums are scaled and added in fp32, the scales' product over its whole range
+ *   (only where a row's scale is above 2^110 and a block's above 2^103 a sum of zero
+ *   becomes NaN, and every other infinite); within a block bf16 outputs take the
  *   8-bit matrix instruction, whose sums are within 1.4e-5 (as 2-norms, on normal
  *   rows) and fp32 outputs the bf16 one on the same values, which adds in fp32.
  * No workspace.  No counterpart in the reference.                           */

@@ -49,24 +49,45 @@ struct F8Gemm {
     int piece;           // bytes of a store: the most that rows of y are whole in, up to 16; 0: a tile's lie beyond 2^31 bytes
 };
 
-// An operand's 32 values of a lane as the matrix instruction takes them.
+// A weight block's scale as 2^h times what is left, which is in [1, 2) for h of -100 to
+// 103.  2^h goes to the operand (`power`: as the matrix instruction's 8-bit exponent, or
+// as a float for the conversion to bf16), so that the row's scale times `rest` and the
+// block's sum are normal numbers wherever the scaled sum is one: sums are 2^-18 to 2^25.
+// (Both scales in one factor were subnormal for rows of 1e-36, and infinite times a sum
+// of zero above 2^128.  Now only a row's scale above 2^110 times a block's above 2^103 is:
+// those of sums that are not zero are infinite.)
+struct F8Scale {
+    float rest;
+    int power;
+};
+template <bool EXACT> constexpr int F8_ONE = EXACT ? 127 << 23 : 127;
+template <bool EXACT>
+__device__ __forceinline__ F8Scale f8_part(float s) {
+    const int e = __builtin_amdgcn_readfirstlane(__float_as_int(s)) >> 23 & 255, h = min(max(e, 27), 230);
+    return F8Scale{__builtin_ldexpf(s, 127 - h), EXACT ? h << 23 : h};
+}
+
+// An operand's 32 values of a lane as the matrix instruction takes them, times 2^h.
 template <bool EXACT> struct F8Operand;
 template <> struct F8Operand<false> {
     f8_i8 v;
+    int power;
     __device__ __forceinline__ F8Operand() {}
-    __device__ __forceinline__ F8Operand(f8_i4 lo, f8_i4 hi) : v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]} {}
+    __device__ __forceinline__ F8Operand(f8_i4 lo, f8_i4 hi, int power)
+        : v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, power(power) {}
 };
 template <> struct F8Operand<true> {
     f8_b8 v[4];
     __device__ __forceinline__ F8Operand() {}
-    __device__ __forceinline__ F8Operand(f8_i4 lo, f8_i4 hi) {
+    __device__ __forceinline__ F8Operand(f8_i4 lo, f8_i4 hi, int power) {
+        const float scale = __int_as_float(power);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int u = i < 2 ? lo[2 * i + j] : hi[2 * i - 4 + j];
-                const f8_b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, 1.0f, false);
-                const f8_b2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, 1.0f, true);
+                const f8_b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, scale, false);
+                const f8_b2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, scale, true);
                 v[i][4 * j] = a[0];
                 v[i][4 * j + 1] = a[1];
                 v[i][4 * j + 2] = b[0];
@@ -77,8 +98,7 @@ template <> struct F8Operand<true> {
 
 // the block's product of 16 rows of w by 16 rows of x
 __device__ __forceinline__ f8_f4 f8_block(const F8Operand<false>& w, const F8Operand<false>& x) {
-    // scales of one (2^(127 - 127))
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f8_f4{0, 0, 0, 0}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f8_f4{0, 0, 0, 0}, 0, 0, 0, w.power, 0, x.power);
 }
 __device__ __forceinline__ f8_f4 f8_block(const F8Operand<true>& w, const F8Operand<true>& x) {
     f8_f4 d = {0, 0, 0, 0};
@@ -212,7 +232,7 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
             for (int j = 0; j < NT; ++j) acc[i][j] = f8_f4{0, 0, 0, 0};
         for (int s = 0; s < p.kb; ++s, buf ^= 1) {
             if (BM == 64 * WAVES || tid < BM) s_xs[buf][tid % BM] = sx;
-            const float wscale = sw;
+            const F8Scale wscale = f8_part<EXACT>(sw);
             if (s == 0 && stored)
                 lds_wait_vm<STORES>();
             else
@@ -221,16 +241,17 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
             // the lane's two chunks of a row, which lie 64 bytes apart (bit 2 of the place)
             const char* lo = smem + buf * STAGE + (lane & 15) * 128 + ((grp ^ twist) << 4);
             const char* hi = smem + buf * STAGE + (lane & 15) * 128 + (((grp ^ twist) << 4) ^ 64);
-            auto frag = [&](int r) __attribute__((always_inline)) {
-                return F8Operand<EXACT>(*reinterpret_cast<const f8_i4*>(lo + r * 128), *reinterpret_cast<const f8_i4*>(hi + r * 128));
+            auto frag = [&](int r, int power) __attribute__((always_inline)) {
+                return F8Operand<EXACT>(*reinterpret_cast<const f8_i4*>(lo + r * 128), *reinterpret_cast<const f8_i4*>(hi + r * 128), power);
             };
+            const float* const xscale = s_xs[buf] + wm * MT * 16 + (lane & 15);
             float f[MT];
             F8Operand<EXACT> w[NT], x[2];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) w[j] = frag(BM + (wn * NT + j) * 16);
-            x[0] = frag(wm * MT * 16);
+            for (int j = 0; j < NT; ++j) w[j] = frag(BM + (wn * NT + j) * 16, wscale.power);
+            x[0] = frag(wm * MT * 16, F8_ONE<EXACT>);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) f[i] = s_xs[buf][(wm * MT + i) * 16 + (lane & 15)] * wscale;
+            for (int i = 0; i < MT; ++i) f[i] = xscale[16 * i] * wscale.rest;
             // the stage that loads meanwhile: this tile's next, or the next tile's first
             int stage = s + 1;
             if (stage == p.kb) {
@@ -253,7 +274,7 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
             for (int t = 0; t < MT * NT + LAG; ++t) {
                 if (t < MT * NT) {
                     const int i = t / NT, j = t % NT;
-                    if (j == 0 && i + 1 < MT) x[(i + 1) & 1] = frag((wm * MT + i + 1) * 16);
+                    if (j == 0 && i + 1 < MT) x[(i + 1) & 1] = frag((wm * MT + i + 1) * 16, F8_ONE<EXACT>);
                     d[t % (LAG + 1)] = f8_block(w[j], x[i & 1]);
                 }
                 if (t < LOADS) issue(t, stage, buf ^ 1);
@@ -348,20 +369,21 @@ __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
         xs[i] = p.xs + m * p.kb;
         acc[i] = f8_f4{0, 0, 0, 0};
     }
-    auto frag = [&](const uint8_t* row, int s) {
+    auto frag = [&](const uint8_t* row, int s, int power) {
         const int k = s * 128 + 16 * grp;
         f8_i4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
         if (k < p.K) lo = *reinterpret_cast<const f8_i4*>(row + k);
         if (k + 64 < p.K) hi = *reinterpret_cast<const f8_i4*>(row + k + 64);
-        return F8Operand<EXACT>(lo, hi);
+        return F8Operand<EXACT>(lo, hi, power);
     };
 #pragma unroll 4
     for (int s = wave; s < p.kb; s += 4) {
-        const F8Operand<EXACT> w = frag(wr, s);
+        const F8Scale wscale = f8_part<EXACT>(ws[s]);
+        const F8Operand<EXACT> w = frag(wr, s, wscale.power);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const f8_f4 d = f8_block(w, frag(xr[i], s));
-            const float f = xs[i][s] * ws[s];
+            const f8_f4 d = f8_block(w, frag(xr[i], s, F8_ONE<EXACT>));
+            const float f = xs[i][s] * wscale.rest;
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(d[e], f, acc[i][e]);
         }

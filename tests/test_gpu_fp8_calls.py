@@ -41,3 +41,61 @@ def test_product_of_one_row_of_each_long_sequence(gpu):
         for out in (F32, BF16):
             got = ops.linear_fp8(wide[:M, -1], scales[:M, -1], w, ws, out_dtype=out)
             assert torch.equal(got, ops.linear_fp8(x[:M].contiguous(), xs[:M].contiguous(), w, ws, out_dtype=out))
+
+
+def check_whole_range(y, x, xs, w, ws):
+    """As check_product, with no more slack than the output's least step."""
+    K, N = x.shape[-1], w.shape[0]
+    xd = x.double() * xs.double().repeat_interleave(128, -1)[..., :K]
+    wd = w.double() * ws.double().repeat_interleave(128, 1)[:, :K].repeat_interleave(128, 0)[:N]
+    want, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    lim = (K + 4) * 2.0 ** -24 * mag
+    if y.dtype == BF16:
+        lim = lim + 2.0 ** -13 * mag
+        lim = lim + 2.0 ** -8 * (want.abs() + lim)
+    least = 2.0 ** -149 if y.dtype == F32 else 2.0 ** -133
+    err = (y.double() - want).abs()
+    assert bool((err <= lim + least).all()), f"{float((err / (lim + least)).max()):.3g} of the bound"
+    return want
+
+
+@pytest.mark.parametrize("M", [5, 30, 40, 700, 4100])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_scales_far_from_one(gpu, M, out):
+    """The scales' product below fp32's normal numbers, or above its largest, where
+    the result is an ordinary number."""
+    from mogt_amd import ops
+    announce(f"linear_fp8 far scales {M} {out}")
+    N, K = 1300, 400
+    x, xs, w, ws = product(M, N, K, seed=3)
+    # rows of 1e-36 (scales of 2^-126) and weights of 0.02 (4.5e-5)
+    small, small_s = ops.quantize_fp8(rnd(M, K, seed=1) * 1e-36)
+    light, light_s = ops.quantize_fp8(rnd(N, K, seed=2) * 0.02, block_rows=128)
+    assert float((small_s.max().double() * light_s.max().double()).item()) < 2.0 ** -126
+    want = check_whole_range(ops.linear_fp8(small, small_s, light, light_s, out_dtype=out), small, small_s, light, light_s)
+    assert float(want.abs().median()) > 2.0 ** -124
+    # scales up to 2^+-110 that cancel
+    g = torch.Generator(device="cuda").manual_seed(5)
+    e = torch.randint(-110, 111, (xs.shape[1],), generator=g, device="cuda")
+    r = torch.randint(-9, 10, (M, 1), generator=g, device="cuda")
+    xe, we = torch.exp2((r - e).float()), torch.exp2(e.float()).expand_as(ws)
+    check_whole_range(ops.linear_fp8(x, xe, w, we.contiguous(), out_dtype=out), x, xe, w, we)
+    # a block whose scales' product is beyond fp32 and whose sums are zero for some outputs
+    zero = w.clone().view(torch.uint8)
+    zero[::3, 128:256] = 0
+    zero = zero.view(w.dtype)
+    rest = [i for i in range(K) if not 128 <= i < 256]
+    xd = x.double() * xs.double().repeat_interleave(128, -1)[..., :K]
+    wd = zero.double() * ws.double().repeat_interleave(128, 1)[:, :K].repeat_interleave(128, 0)[:N]
+    want, mag = xd[:, rest] @ wd[::3, rest].t(), xd[:, rest].abs() @ wd[::3, rest].abs().t()
+    lim = (K + 4) * 2.0 ** -24 * mag + (2.0 ** -12 * mag + 2.0 ** -8 * want.abs() if out == BF16 else 0.0)
+    for far in (2.0 ** 20, 2.0 ** 103):
+        xl, wl = xs.clone(), ws.clone()
+        xl[:, 1], wl[:, 1] = 2.0 ** 119, far
+        y = ops.linear_fp8(x, xl, zero, wl, out_dtype=out)
+        assert bool(((y[:, ::3].double() - want).abs() <= lim + 1e-30).all())
+        wl[:, 1] = float("inf")   # as the definition: infinity times nothing
+        assert bool(ops.linear_fp8(x, xl, zero, wl, out_dtype=out)[:, ::3].isnan().all())
+    # the quantiser's largest and least scales: nothing times them is nothing
+    for a, b in ((torch.finfo(F32).max / 448, 2.0 ** 103), (2.0 ** 110, torch.finfo(F32).max / 448), (2.0 ** -126, 2.0 ** -126)):
+        assert not ops.linear_fp8(torch.zeros_like(x), torch.full_like(xs, a), w, torch.full_like(ws, b), out_dtype=out).any()
