@@ -16,6 +16,7 @@
 // q = 448 x' w / largest |x' w|.  Bound by HBM: those rows with bf16 z take 147 us,
 // 5.0 TB/s (in 32 bits 140).
 #include "common.h"
+#include "wide_grid.h"
 
 namespace mogt {
 namespace {
@@ -107,7 +108,7 @@ struct F8Norm {
 template <typename TZ, int VPL>
 __global__ __launch_bounds__(64 * F8_WAVES) void f8_norm_kernel(F8Norm p) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * F8_WAVES + (threadIdx.x >> 6);
+    const int64_t row = wide_block() * F8_WAVES + (threadIdx.x >> 6);
     if (row >= p.rows) return;
     const float* xr = p.x + row * p.D;
     const TZ* zr = static_cast<const TZ*>(p.z) + row * p.D;
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(64 * F8_WAVES) void f8_norm_kernel(F8Norm p) {
 template <typename T>
 __global__ __launch_bounds__(256) void f8_rows_kernel(const T* x, int64_t ldx, uint32_t* q, float* scale, int64_t total,
                                                       int D, int blocks) {
-    const int64_t id = blockIdx.x * 8ll + (threadIdx.x >> 5);
+    const int64_t id = wide_block() * 8 + (threadIdx.x >> 5);
     const int64_t row = id / blocks;
     const int block = static_cast<int>(id - row * blocks), c = block * F8_BLOCK + (threadIdx.x & 31) * 4;
     const bool in = id < total && c < D;
@@ -207,8 +208,8 @@ __global__ __launch_bounds__(256) void f8_blocks_kernel(const T* x, int64_t ldx,
 template <typename TZ>
 int f8_norm_launch(const F8Norm& p, hipStream_t st) {
     const int64_t blocks = (p.rows + F8_WAVES - 1) / F8_WAVES;
-    if (blocks > 0x7fffffff) return set_error(MOGT_E_INVALID, "%lld rows are too many", (long long)p.rows);
-    const dim3 grid(static_cast<unsigned>(blocks));
+    if (blocks > WIDE_GRID_MAX) return set_error(MOGT_E_INVALID, "%lld rows are too many", (long long)p.rows);
+    const dim3 grid = wide_grid(blocks);
     if (p.D <= 256)
         f8_norm_kernel<TZ, 1><<<grid, 64 * F8_WAVES, 0, st>>>(p);
     else if (p.D <= 1024)
@@ -228,9 +229,9 @@ int f8_quantize_launch(const void* x, int64_t ld, void* q, float* scale, int64_t
     uint32_t* qt = static_cast<uint32_t*>(q);
     if (block_rows == 1) {
         const int64_t groups = (rows * blocks + 7) / 8;
-        if (rows > (1ll << 40) || groups > 0x7fffffff)
+        if (rows > (1ll << 40) || groups > WIDE_GRID_MAX)
             return set_error(MOGT_E_INVALID, "%lld rows of %lld are too many", (long long)rows, (long long)dim);
-        f8_rows_kernel<T><<<static_cast<unsigned>(groups), 256, 0, st>>>(xt, ld, qt, scale, rows * blocks, D, blocks);
+        f8_rows_kernel<T><<<wide_grid(groups), 256, 0, st>>>(xt, ld, qt, scale, rows * blocks, D, blocks);
     } else {
         const int64_t by = (rows + F8_BLOCK - 1) / F8_BLOCK;
         if (by > 65535) return set_error(MOGT_E_INVALID, "%lld rows: at most %d", (long long)rows, 65535 * F8_BLOCK);

@@ -28,6 +28,7 @@
 #include <type_traits>
 
 #include "ssm_common.h"
+#include "wide_grid.h"
 
 namespace mogt {
 
@@ -673,13 +674,6 @@ void ssm_grad_kernel(SsmBwd f) {
         pa[static_cast<int64_t>(p.N + 1) * p.D] = d_bias;
     }
 }
-
-// Work-groups in two dimensions: a launch takes fewer than 2^32 threads along x.
-inline dim3 wide_grid(int64_t groups, unsigned z = 1) {
-    const int64_t x = groups < (1 << 20) ? groups : 1 << 20;
-    return dim3(static_cast<unsigned>(x), static_cast<unsigned>((groups + x - 1) / x), z);
-}
-__device__ __forceinline__ int64_t wide_block() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
 
 // dB, dC [B, L, G, N]: the sums over the 64-channel blocks of a group, in order.
 template <typename TB>

@@ -99,3 +99,17 @@ def test_scales_far_from_one(gpu, M, out):
     # the quantiser's largest and least scales: nothing times them is nothing
     for a, b in ((torch.finfo(F32).max / 448, 2.0 ** 103), (2.0 ** 110, torch.finfo(F32).max / 448), (2.0 ** -126, 2.0 ** -126)):
         assert not ops.linear_fp8(torch.zeros_like(x), torch.full_like(xs, a), w, torch.full_like(ws, b), out_dtype=out).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_rows_than_a_launch_has_threads_along_x(gpu, dtype):
+    from mogt_amd import ops
+    for rows in ((1 << 26) + 5, (1 << 27) + 19):
+        announce(f"8 bits, {rows} rows of 4 {dtype}")
+        x, z, w = rnd(rows, 4, seed=1), rnd(rows, 4, seed=2, dtype=dtype), 1 + 0.1 * rnd(4, seed=3)
+        for got, want in ((ops.add_rmsnorm_fp8(x, z, 0.5, w), lambda at: ops.add_rmsnorm_fp8(x[at], z[at], 0.5, w)),
+                          (ops.quantize_fp8(z), lambda at: ops.quantize_fp8(z[at]))):
+            for at in (slice(0, 300), slice(rows // 2, rows // 2 + 300), slice(rows - 300, rows)):
+                assert all(torch.equal(a[at].float(), b.float()) for a, b in zip(got, want(at)))
+        del x, z, got
+        torch.cuda.empty_cache()
