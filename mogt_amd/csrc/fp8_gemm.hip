@@ -28,6 +28,7 @@
 // 24 %; no order of loads, reads and products that was tried changes the time by
 // more than 2 %.
 #include "lds_dma.h"
+#include "wide_grid.h"
 
 namespace mogt {
 namespace {
@@ -356,7 +357,8 @@ template <int MT, bool EXACT>
 __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
     __shared__ f8_f4 s_d[4][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = lane >> 4;
-    const int n0 = blockIdx.x * 16;
+    if (wide_block() * 16 >= p.N) return;
+    const int n0 = static_cast<int>(wide_block()) * 16;
     const uint8_t* wr = p.w + static_cast<int64_t>(min(n0 + (lane & 15), p.N - 1)) * p.K;
     const float* ws = p.ws + static_cast<int64_t>(n0 / 128) * p.kb;
     const uint8_t* xr[MT];
@@ -402,7 +404,7 @@ __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
 template <bool EXACT>
 void f8_launch(F8Gemm& p, int cus, hipStream_t st) {
     if (p.M <= 32) {
-        const unsigned grid = (p.N + 15) / 16;
+        const dim3 grid = wide_grid((p.N + 15) / 16);
         if (p.M <= 16)
             f8_gemv_kernel<1, EXACT><<<grid, 256, 0, st>>>(p);
         else

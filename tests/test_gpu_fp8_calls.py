@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from conftest import announce
-from test_gpu_fp8 import BF16, F32, product, rnd
+from test_gpu_fp8 import BF16, F32, F8, product, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +113,18 @@ def test_more_rows_than_a_launch_has_threads_along_x(gpu, dtype):
                 assert all(torch.equal(a[at].float(), b.float()) for a, b in zip(got, want(at)))
         del x, z, got
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M", [1, 17])
+def test_more_outputs_than_a_launch_has_threads_along_x(gpu, M):
+    from mogt_amd import ops
+    N, K = (1 << 28) + 272, 16
+    announce(f"linear_fp8 {M} rows by {N} outputs")
+    x, xs = ops.quantize_fp8(rnd(M, K, seed=1))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randint(0, 0x70, (N, K), generator=g, device="cuda", dtype=torch.uint8).view(F8)
+    ws = torch.rand(-(-N // 128), 1, generator=g, device="cuda") + 0.5
+    y = ops.linear_fp8(x, xs, w, ws)
+    for a in (0, N // 256 * 128, N - 272):
+        b = min(a + 384, N)
+        assert torch.equal(y[:, a:b], ops.linear_fp8(x, xs, w[a:b], ws[a // 128:-(-b // 128)]))
