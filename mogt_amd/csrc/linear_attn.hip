@@ -4,6 +4,7 @@
 #include <initializer_list>
 
 #include "linear_attn.h"
+#include "wide_grid.h"
 
 namespace mogt {
 
@@ -144,11 +145,11 @@ __global__ __launch_bounds__(64) void la_decay_sum_kernel(const double* part, in
 template <typename TI>
 __global__ __launch_bounds__(256) void la_group_kernel(const float* dq, const float* dk, TI* to_q, TI* to_k, int64_t total,
                                                        int d, int share) {
-    const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-    TI* to = blockIdx.y ? to_k : to_q;
+    const int64_t i = wide_block() * 256 + threadIdx.x;
+    TI* to = blockIdx.z ? to_k : to_q;
     if (i >= total || !to) return;
     const int64_t row = i / d;
-    const float* p = (blockIdx.y ? dk : dq) + row * share * d + (i - row * d);
+    const float* p = (blockIdx.z ? dk : dq) + row * share * d + (i - row * d);
     float x = 0.0f;
     for (int j = 0; j < share; ++j) x += p[static_cast<int64_t>(j) * d];
     to[i] = IO<TI>::st(x);
@@ -474,7 +475,7 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
         const int share = static_cast<int>(q->heads / q->groups), d = static_cast<int>(q->key_dim);
         const int64_t total = q->batch * q->length * q->groups * q->key_dim;
         if (total > 0 && (g->dq || g->dk)) {
-            const dim3 grid(static_cast<unsigned>((total + 255) / 256), 2);
+            const dim3 grid = wide_grid((total + 255) / 256, 2);
             if (q->io_dtype == MOGT_BF16)
                 la_group_kernel<bf16_t><<<grid, 256, 0, st>>>(share_q, share_k, static_cast<bf16_t*>(g->dq),
                                                               static_cast<bf16_t*>(g->dk), total, d, share);

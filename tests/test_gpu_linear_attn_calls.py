@@ -1,0 +1,36 @@
+"""Calls of linear attention at the edges of what it takes."""
+import pytest
+import torch
+
+from conftest import announce
+from test_gpu_linear_attn import BF16
+
+pytestmark = pytest.mark.gpu
+
+
+def test_shared_rows_past_a_launch_of_2_32_threads(gpu, monkeypatch):
+    """2^32 values of q and of k, each shared by two heads (104 GB in all): their
+    gradients against a call on the first and the last group of the last sequence."""
+    from mogt_amd import ops
+    if torch.cuda.mem_get_info()[0] < 130 << 30:
+        pytest.skip("needs 130 GB of free memory")
+    B, L, G, dk, segment = 4, 65536, 128, 128, 8192
+    announce(f"linear_attention gradients of {B} x {L} x {G} x {dk} shared rows")
+    monkeypatch.setattr(ops, "_linear_attn_segment", lambda *a: segment)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k = (torch.empty(B, L, G, dk, device="cuda", dtype=BF16).normal_(generator=g) for _ in "qk")
+    v, dout = (torch.empty(B, L, 2 * G, 1, device="cuda", dtype=BF16).normal_(generator=g) for _ in "vo")
+    decay = torch.rand(B, L, 2 * G, generator=g, device="cuda") * -0.1
+
+    def gradients(*t, dout):
+        leaves = [x.detach().requires_grad_(True) for x in t[:2]]
+        return torch.autograd.grad(ops.linear_attention(*leaves, *t[2:]), leaves, dout)
+
+    got = gradients(q, k, v, decay, dout=dout)
+    for at in (0, G - 1):
+        heads = slice(2 * at, 2 * at + 2)
+        want = gradients(q[3:, :, at:at + 1], k[3:, :, at:at + 1], v[3:, :, heads], decay[3:, :, heads], dout=dout[3:, :, heads])
+        for a, b in zip(got, want):
+            assert bool(b.any()) and torch.equal(a[3:, :, at:at + 1], b)
+    del q, k, v, dout, decay, got, want
+    torch.cuda.empty_cache()
