@@ -719,7 +719,8 @@ int mogt_short_conv_step(const mogt_short_conv_problem* problem, void* state, vo
  * mogt_linear_attn_fwd: out [batch, length, heads, value_dim] contiguous;
  *   final_state may be null; `carries` (may be null) [batch, heads, segments + 1,
  *   value_dim, key_dim] receives the states entering the segments and the final
- *   one, which the backward takes.
+ *   one, which the backward takes; the workspace is then 4 bytes for each sequence,
+ *   head and segment (rounded up to 256), of several segments.
  * mogt_linear_attn_bwd: from the same problem (and segment), the forward's carries,
  *   dout (io_dtype, contiguous) and dfinal_state (may be null) the gradients, each
  *   of which may be null: dq, dk [batch, length, groups, key_dim], dv [batch,

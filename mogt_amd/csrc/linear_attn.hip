@@ -350,7 +350,7 @@ extern "C" int mogt_linear_attn_fwd(const mogt_linear_attn_problem* q, void* out
     if (const int rc = la_args(q, a)) return rc;
     if (q->batch == 0 || q->heads == 0) return MOGT_OK;
     if (q->length > 0 && !out) return set_error(MOGT_E_INVALID, "null output pointer");
-    const size_t need = a.nseg > 1 ? la_states_bytes(q) + la_ctot_bytes(q) : 0;
+    const size_t need = a.nseg > 1 ? (carries ? 0 : la_states_bytes(q)) + la_ctot_bytes(q) : 0;
     if (need > 0 && (!workspace || workspace_bytes < need))
         return set_error(MOGT_E_WORKSPACE, "workspace of %zu bytes expected, got %zu", need, workspace ? workspace_bytes : 0);
     hipStream_t st = static_cast<hipStream_t>(stream);

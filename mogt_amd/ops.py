@@ -3020,9 +3020,13 @@ def _linear_attn_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     segment = _linear_attn_segment(B, L, H, dk, dv, v.dtype)
     out = _empty_rows(v)
     state = log_decay.new_empty((B, H, dk, dv) if want_state else 0)
-    carries = log_decay.new_empty((B, H, max(1, -(-L // segment)) + 1, dv, dk) if want_carries else 0)
+    segments = max(1, -(-L // segment))
+    carries = log_decay.new_empty((B, H, segments + 1, dv, dk) if want_carries else 0)
     p, held = _linear_attn_problem(q, k, v, log_decay, initial_state, lengths, scale, segment)
-    nbytes = lib.mogt_linear_attn_workspace_bytes(p)
+    if want_carries:   # the states are the carries
+        nbytes = -(-4 * B * H * segments // 256) * 256 if segments > 1 else 0
+    else:
+        nbytes = lib.mogt_linear_attn_workspace_bytes(p)
     ws = scratch(nbytes, v.device) if nbytes else None
     with _on_device(v.device):
         rc = lib.mogt_linear_attn_fwd(p, out.data_ptr(), state.data_ptr() if want_state else None,

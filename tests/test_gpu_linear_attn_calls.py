@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from conftest import announce
-from test_gpu_linear_attn import BF16
+from test_gpu_linear_attn import BF16, F32, call, gradients_in, make, run_all
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,19 @@ def test_shared_rows_past_a_launch_of_2_32_threads(gpu, monkeypatch):
             assert bool(b.any()) and torch.equal(a[3:, :, at:at + 1], b)
     del q, k, v, dout, decay, got, want
     torch.cuda.empty_cache()
+
+
+def test_a_training_forward_keeps_its_states_once(gpu):
+    from mogt_amd import ops
+    announce("linear_attention memory of a training forward")
+    t, kw = make(2, 4096, 8, 8, 128, 128, BF16, init=False)
+    leaves = {n: x.detach().requires_grad_(True) for n, x in t.items() if x is not None}
+    call(leaves, kw)
+    torch.cuda.synchronize()
+    segments = 4096 // ops._linear_attn_segment(2, 4096, 8, 128, 128, BF16)
+    states = 2 * 8 * (segments + 1) * 128 * 128 * 4
+    assert segments > 8 and states > 30 << 20
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call(leaves, kw)
+    assert torch.cuda.max_memory_allocated() - before < states + out.numel() * 2 + (4 << 20)
