@@ -433,7 +433,7 @@ extern "C" int mogt_linear_attn_bwd(const mogt_linear_attn_problem* q, const voi
     // formed in any case: a row's gradient does not depend on which others are asked for
     dk.dot = dot_k;
     dq.dot = dot_q;
-    if (a.nseg > 1) {
+    if (a.nseg > 1 && (g->dv || g->dk || need_g || g->dinitial_state)) {   // dq takes the forward's states alone
         a.pass[0] = dv;
         la_launch(q, a, 1, false, st);
         la_carry(a, static_cast<int>(q->key_dim), rstates, rctot, dfinal_state, st);

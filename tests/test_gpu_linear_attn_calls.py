@@ -50,3 +50,26 @@ def test_a_training_forward_keeps_its_states_once(gpu):
     torch.cuda.reset_peak_memory_stats()
     out = call(leaves, kw)
     assert torch.cuda.max_memory_allocated() - before < states + out.numel() * 2 + (4 << 20)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_query_gradient_alone_forms_no_reverse_states(gpu, dtype):
+    """Through the C entry, on a workspace whose first part takes the reverse states;
+    dq is the one of all."""
+    from mogt_amd import _lib, ops
+    announce(f"linear_attention dq alone {dtype}")
+    t, kw = make(2, 700, 2, 2, 32, 48, dtype, seed=3)
+    dout, dstate = gradients_in(t)
+    want = run_all(t, kw, dout, dstate)[2]
+    segment = ops._linear_attn_segment(2, 700, 2, 32, 48, dtype)
+    scale = 32 ** -0.5
+    _, _, carries = ops._linear_attn_op(t["q"], t["k"], t["v"], t["log_decay"], t["initial_state"], None, scale, True, True)
+    p, held = ops._linear_attn_problem(t["q"], t["k"], t["v"], t["log_decay"], t["initial_state"], None, scale, segment)
+    lib = _lib.load()
+    ws = torch.full((lib.mogt_linear_attn_bwd_workspace_bytes(p),), 0x5a, device="cuda", dtype=torch.uint8)
+    dq = torch.empty_like(t["q"])
+    rc = lib.mogt_linear_attn_bwd(p, dout.data_ptr(), dstate.data_ptr(), carries.data_ptr(),
+                                  _lib.LINEAR_ATTN_GRADIENTS.pack(dq.data_ptr(), 0, 0, 0, 0), ws.data_ptr(), ws.numel(),
+                                  torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(dq, want)
+    assert bool((ws[:carries.numel() * 4] == 0x5a).all())
