@@ -2998,9 +2998,9 @@ def _linear_attn_problem(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     if log_decay.ndim == 3 and log_decay.stride(1) * 4 * steps > LINEAR_ATTN_SEGMENT_BYTES:
         log_decay = log_decay.contiguous()
     shape, qs, ks, vs, gs = v.shape, q.stride(), k.stride(), v.stride(), log_decay.stride()
-    # row strides; a step's rows have none
-    L, qr, kr, vr, gr = (1, 0, 0, 0, 0) if len(shape) == 3 else (shape[1], qs[1], ks[1], vs[1], gs[-2] if len(gs) > 1
-                                                                 else 0)
+    # row strides; a step's rows have none, and a single row's are any numbers
+    L, qr, kr, vr, gr = (1, 0, 0, 0, 0) if len(shape) == 3 or shape[1] == 1 else (
+        shape[1], qs[1], ks[1], vs[1], gs[-2] if len(gs) > 1 else 0)
     per_head = len(gs) == 1
     p = _lib.LINEAR_ATTN_PROBLEM.pack(shape[0], L, shape[-2], *q.shape[-2:], shape[-1], segment, _DTYPE_CODE[q.dtype],
                                       0 if lengths is None else lengths.element_size(), per_head, scale, q.data_ptr(),

@@ -73,3 +73,13 @@ def test_the_query_gradient_alone_forms_no_reverse_states(gpu, dtype):
                                   torch.cuda.current_stream().cuda_stream)
     assert rc == 0 and torch.equal(dq, want)
     assert bool((ws[:carries.numel() * 4] == 0x5a).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_stride_of_a_single_step_is_any_number(gpu, dtype):
+    announce(f"linear_attention of one step at a stride of 2^40 {dtype}")
+    t, kw = make(3, 1, 2, 1, 32, 48, dtype, seed=4)
+    dout, dstate = gradients_in(t)
+    far = {n: x if n == "initial_state" else x.as_strided(x.shape, (x.stride(0), 1 << 40, *x.stride()[2:])) for n, x in t.items()}
+    for a, b in zip(run_all(far, kw, dout, dstate), run_all(t, kw, dout, dstate)):
+        assert torch.equal(a, b)
