@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from conftest import announce
-from test_gpu_fp8 import BF16, F32, F8, product, rnd
+from test_gpu_fp8 import BF16, F32, F8, check_product, product, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +128,51 @@ def test_more_outputs_than_a_launch_has_threads_along_x(gpu, M):
     for a in (0, N // 256 * 128, N - 272):
         b = min(a + 384, N)
         assert torch.equal(y[:, a:b], ops.linear_fp8(x, xs, w[a:b], ws[a // 128:-(-b // 128)]))
+
+
+@pytest.mark.parametrize("dtype,scale", [(F32, 0.3), (F32, 0.5), (BF16, 0.3)])
+def test_norm_and_its_scales_are_the_definition_s(gpu, dtype, scale):
+    """The norm is in 64 bits: a block's scale is off by its rounding to fp32, 2^-24 of
+    it, and no value falls on the other side of a border (one in 2^45 might).  bf16 z is
+    scaled in fp32 and rounded, fp32 z enters unrounded."""
+    from mogt_amd import ops
+    announce(f"add_rmsnorm_fp8 against 64 bits {dtype} {scale}")
+    M, D = 2048, 4096
+    x, z, w = rnd(M, D, seed=11), rnd(M, D, seed=12, dtype=dtype), 1 + 0.2 * rnd(D, seed=13)
+    _, q, s = ops.add_rmsnorm_fp8(x, z, scale, w, 1e-6)
+    factor = torch.tensor(scale, device="cuda")
+    added = factor.double() * z.double() if dtype == F32 else (factor * z.float()).bfloat16().double()
+    v = x.double() + added
+    n = (v * w.double()).view(M, 32, 128)
+    most = n.abs().amax(2)
+    want = most / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-6) / 448
+    assert bool(((s.double() - want).abs() <= 2.0 ** -24 * (1 + 1e-6) * want).all())
+    u = (448 * n / most.unsqueeze(2)).view(M, D)
+    step = torch.exp2(torch.floor(torch.log2(u.abs().clamp(min=2.0 ** -6))) - 3)
+    assert int((q.double() != torch.round(u / step) * step).sum()) == 0
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_product_of_many_tiles_and_stages(gpu, out):
+    from mogt_amd import ops
+    announce(f"linear_fp8 4100 3500 2048 {out}")
+    p = product(4100, 3500, 2048, seed=9)
+    check_product(ops.linear_fp8(*p, out_dtype=out), *p)
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_product_past_2_32_bytes(gpu, out):
+    """Operand and output of more than 2^31 elements and 2^32 bytes, against the same
+    products of a tile's rows."""
+    from mogt_amd import ops
+    M, N, K = 2_200_003, 1100, 2048
+    announce(f"linear_fp8 {M} {N} {K} {out}")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randint(0, 0x78, (M, K), generator=g, device="cuda", dtype=torch.uint8).view(F8)
+    xs = torch.rand(M, K // 128, generator=g, device="cuda") + 0.5
+    _, _, w, ws = product(1, N, K, seed=4)
+    y = ops.linear_fp8(x, xs, w, ws, out_dtype=out)
+    for a in (0, (1 << 31) // N - 50, (1 << 32) // K - 50, M - 99):
+        assert torch.equal(y[a:a + 99], ops.linear_fp8(x[a:a + 99], xs[a:a + 99], w, ws, out_dtype=out))
+    del x, xs, y
+    torch.cuda.empty_cache()

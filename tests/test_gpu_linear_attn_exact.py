@@ -7,7 +7,7 @@ import torch
 
 from conftest import announce
 from oracle import linear_attn_oracle as lo
-from test_gpu_linear_attn import BF16, F32, call
+from test_gpu_linear_attn import BF16, F32, NAMES, call, gradients_in, make, run_all
 
 pytestmark = pytest.mark.gpu
 EXACT = [(64, 64), (128, 128), (128, 100), (33, 64), (32, 17)]
@@ -96,3 +96,91 @@ def test_decayed_values_are_written_in_full_fp32(gpu, monkeypatch, dk, dv):
     got = call(dict(q=q, k=k, v=v, log_decay=g), {}, scale=1.0).double().cpu()
     assert bool((got[0, 64:128].abs() <= 12 * 2.0 ** -24 * mag[0, 64:128]).all())
     assert bool((got[0, 192:256].abs() <= 40 * 2.0 ** -24 * mag[0, 192:256]).all())   # two states, two more chunks, a carry
+
+
+@pytest.mark.parametrize("dk,dv", EXACT)
+def test_gradients_read_states_in_full_fp32(gpu, dk, dv):
+    """dq and dk: columns of the initial state, and of the final one's gradient, that
+    differ by little, read by rows e_i - e_j."""
+    announce(f"linear_attention exact gradients {dk} {dv}")
+    L = 300
+    large = whole(1, 1, dk, 1, lo=2 ** 19, hi=2 ** 20 - 1, seed=1, dtype=F32) + whole(1, 1, dk, dv, lo=-30, hi=30, seed=2, dtype=F32)
+    pick, ones, more = differences(L, dv, 3).view(1, L, 1, dv), whole(1, L, 1, dk, seed=5), whole(1, L, 1, dk, seed=6)
+    g, rows = torch.zeros(1, L, 1, device="cuda"), whole(1, L, 1, dv, seed=7)
+    for n, v, dout, init, dstate in (("q", rows, pick, large, None), ("k", pick, rows, None, large)):
+        t = dict(q=ones, k=more, v=v, log_decay=g, initial_state=init)
+        leaf = t[n].clone().requires_grad_(True)
+        out, state = call({**t, n: leaf}, {}, scale=1.0, return_state=True)
+        (got,) = torch.autograd.grad([out] if dstate is None else [out, state], [leaf], [dout] if dstate is None else [dout, dstate])
+        want = lo.linear_attention(ones, more, v, g, scale=1.0, initial_state=init, dout=dout, dstate=dstate)["d" + n]
+        assert torch.equal(got.double().cpu(), want.to(BF16).double()), n
+
+
+@pytest.mark.parametrize("L", [100, 384])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dk,dv", EXACT)
+def test_states_left_behind_are_in_full_fp32(gpu, monkeypatch, dk, dv, dtype, L):
+    """The final state, and the initial one's gradient: three rows, written 255, 254
+    and 1 times one value under one decay; the first less the others is zero, to a
+    rounding each for the product with the decay, three for its parts, and one for each
+    chunk and segment that the state goes through after that (16 are allowed for)."""
+    from mogt_amd import ops
+    announce(f"linear_attention exact states {dk} {dv} {dtype} {L}")
+    monkeypatch.setattr(ops, "LINEAR_ATTN_MIN_SEGMENT", 128)
+    monkeypatch.setattr(ops, "LINEAR_ATTN_ONE_SEGMENT", 0)
+    q, k, v, dout = (torch.zeros(1, L, 1, d, device="cuda", dtype=dtype) for d in (dk, dk, dv, dv))
+    g = -0.05 * torch.rand(1, L, 1, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    value = torch.exp2(whole(dv, lo=-3, hi=3, seed=9).float()).to(dtype)
+    for at in (20, 70) if L == 100 else (20, 150, 300):
+        g[0, at + 1:at + 3] = 0.0
+        for i, x in enumerate((255.0, 254.0, 1.0)):
+            q[0, at + i, 0, 3 * i] = k[0, at + i, 0, 3 * i] = 1.0
+            v[0, at + i, 0] = dout[0, at + i, 0] = x * value
+    init = torch.zeros(1, 1, dk, dv, device="cuda", requires_grad=True)
+    out, state = ops.linear_attention(q, k, v, g, initial_state=init, scale=1.0, return_state=True)
+    (dinit,) = torch.autograd.grad(out, init, dout)
+    for name, s in (("state", state.detach()), ("dinitial_state", dinit)):
+        s = s[0, 0].double()
+        assert bool((s[0] > 0).all()), name
+        assert bool(((s[0] - s[3] - s[6]).abs() <= 20 * 2.0 ** -24 * 2 * s[0]).all()), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (33, 20)])
+def test_the_decays_gradient_of_whole_numbers_is_exact(gpu, dk, dv, dtype):
+    """Its sums are in 64 bits and the rows' products of numbers below 2^24 exact, so
+    what is left is one rounding: for one decay a step, and for one a head."""
+    announce(f"linear_attention exact decay gradient {dk} {dv} {dtype}")
+    L, H = 700, 2
+    q, k = (whole(2, L, 1, dk, seed=s, dtype=dtype) for s in (1, 2))
+    v, dout = (whole(2, L, H, dv, seed=s, dtype=dtype) for s in (3, 4))
+    init, dstate = (whole(2, H, dk, dv, lo=-1000, hi=1000, seed=s, dtype=F32) for s in (5, 6))
+    kw = dict(lengths=torch.tensor([L, 333], device="cuda", dtype=torch.int32))
+    for g in (torch.zeros(2, L, H, device="cuda"), torch.zeros(H, device="cuda")):
+        got = run_all(dict(q=q, k=k, v=v, log_decay=g, initial_state=init), kw, dout, dstate, scale=1.0)[5]
+        want = lo.linear_attention(q, k, v, g, initial_state=init, scale=1.0, dout=dout, dstate=dstate, **kw)["dlog_decay"]
+        assert torch.equal(got.cpu(), want.float())
+
+
+@pytest.mark.parametrize("B,L,H,G,dk,dv", [(2, 700, 4, 2, 64, 64), (1, 600, 3, 3, 128, 128), (3, 330, 2, 1, 40, 100)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_errors_of_fp32_results_are_a_walk_of_roundings(gpu, B, L, H, G, dk, dv, dtype):
+    """As 2-norms: of the 390 + 2.1 L roundings that bound one result's error (see
+    test_gpu_linear_attn) each is independent of the others and of 2^-24 of a partial
+    sum, which for terms of random signs is no larger than its sum: their root times
+    2^-24.  The decays' gradient is a difference of two running sums of its segment, and
+    is held to those."""
+    from mogt_amd import ops
+    announce(f"linear_attention errors {B} {L} {H} {G} {dk} {dv} {dtype}")
+    t, kw = make(B, L, H, G, dk, dv, dtype, seed=L)
+    dout, dstate = gradients_in(t)
+    got = dict(zip(("out", "state", *("d" + n for n in NAMES)), run_all(t, kw, dout, dstate)))
+    segment = ops._linear_attn_segment(B, L, H, dk, dv, dtype)
+    want, mag = [lo.linear_attention(t["q"], t["k"], t["v"], t["log_decay"], initial_state=t["initial_state"], dout=dout,
+                                     dstate=dstate, mag=m, segment=segment) for m in (0, 1)]
+    tol = (390 + 2.1 * L) ** 0.5 * 2.0 ** -24
+    for n, x in got.items():
+        if x.dtype == F32:
+            size = (mag if n == "dlog_decay" else want)[n].norm()
+            err = float((x.double().cpu() - want[n]).norm() / size)
+            assert err <= tol, n
