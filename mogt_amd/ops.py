@@ -2954,16 +2954,31 @@ LINEAR_ATTN_MAX_DIM = 128
 LINEAR_ATTN_CHUNK = {torch.bfloat16: 64, torch.float32: 32}   # steps of a chunk; a segment is whole chunks
 # Work-groups that a call is cut into segments for: three a compute unit, two where
 # states are wider than 64 (their kernels fill one with two, and a state is 64 KB to
-# carry).  Kernels of 2 x 8192 steps of 12 heads of 64, forward and gradients, take
-# 199 us with 768 groups, 223 with 1024 and 224 with 512; 32768 steps of 16 heads of 128,
-# forward, 319 us with 512, 331 with 1024 and 350 with 384.
+# carry).  Kernels of a captured call (us), forward / with gradients:
+#   work-groups                          256        384        512        768       1024
+#   2 x 8192, 12 heads of 64, bf16                58 / 185   59 / 196   53 / 177   58 / 194
+#   2 x 8192, 12 heads of 64, fp32                    329        331        289        317
+#   8 x 1001, 12 heads of 64, fp32                  64         64         54         61
+#   1 x 32768, 16 heads of 128, bf16  279 / 945  294 / 986  264 / 926  275 / 984  276 / 994
+#   2 x 8192, 16 heads of 128, fp32       1045       1215        992       1055       1071
 LINEAR_ATTN_GROUPS = 768
 LINEAR_ATTN_WIDE_GROUPS = 512
-# The least steps of a segment, and the length up to which one work-group runs through
-# (a segment's sums, the carry and another launch cost what they save): kernels over
-# 2 x 513 steps of 6 heads with gradients, fp32, take 75 us in segments of 64, 95 of 128
-# and 139 of 256; 200 steps of 12 heads 16.3 us in one and 16.8 in segments of 64.
+# The least steps of a segment (a segment's sums, the carry and another launch cost what
+# they save).  Kernels over 2 x 513 steps of 6 heads with gradients in segments of 64,
+# 128 and 256: fp32 57, 76 and 117 us, bf16 47, 56 and 78; 1024 steps of 12 heads of 64,
+# bf16, forward: 16.9, 19.0 and 26; of 16 heads of 128 with gradients 107, 108 and 140.
 LINEAR_ATTN_MIN_SEGMENT = 64
+# The length up to which one work-group runs through: one launch, not three, which is
+# what the host takes longest over in an eager call (200 steps of 12 heads of 64, bf16:
+# 17.1 us a call, in segments of 64 24.7).  The kernels of many sequences and heads take
+# less in one too, those of few take more (256 steps, one and segments of 64, us, forward
+# / with gradients, captured):
+#                            bf16                      fp32
+#   12 heads of 64      15.5 / 54, 14.3 / 42      25 / 81, 18.4 / 52
+#   48                  15.8 / 55, 17.5 / 55      26 / 83, 22 / 67
+#   96                  15.9 / 58, 26 / 71        26 / 87, 33 / 92
+#   4 heads of 128        25 / 94, 20 / 71        51 / 173, 30 / 99
+#   64                   26 / 101, 42 / 121       54 / 182, 50 / 156
 LINEAR_ATTN_ONE_SEGMENT = 256
 LINEAR_ATTN_SEGMENT_BYTES = 0x7fffffff - 1024   # of a segment's rows, addressed by 32-bit offsets
 
