@@ -759,10 +759,11 @@ int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state,
  * block of 128 values of one row, or of 128 rows by 128 values:
  *   scale = max(largest |x| / 448, 2^-126),  q = e4m3(x / scale), nearest even
  * A row of `dim` values has ceil(dim / 128) scales; the last block may be short.
- * mogt_add_rmsnorm_fp8_fwd: x_out = x + (scale * z) [the product rounded to z's
- *   dtype], as mogt_add_rmsnorm_fwd, and the rows rmsnorm(x_out) * weight in 8 bits
- *   (in 64 bits from the sum on, not rounded before the 8 bits); x, x_out fp32, rows of
- *   `dim` contiguous elements, dim a multiple of 4 and <= 4096.
+ * mogt_add_rmsnorm_fp8_fwd: x_out = x + scale * z, as mogt_add_rmsnorm_fwd (the product
+ *   rounded to bf16 for bf16 z), and the rows rmsnorm(x') * weight in 8 bits, of the x'
+ *   that x_out is rounded from, in 64 bits and not rounded before the 8 bits: q from the
+ *   exact quotients, then the scale to fp32; x, x_out fp32, rows of `dim` contiguous
+ *   elements, dim a multiple of 4 and <= 4096.
  * mogt_quantize_fp8: the rows of x (row stride ld, a multiple of 4) in 8 bits, with
  *   block_rows 1 or 128 (weights); dim a multiple of 4.
  * mogt_linear_fp8: y[m][n] = sum_k x[m][k] w[n][k] of the values both stand for: x
@@ -772,9 +773,10 @@ int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state,
  *   ldx at most 2^22, outputs at most 2^30; x, w and y 16-byte aligned.
  *   Blocks' sums are scaled and added in fp32, the scales' product over its whole range
  *   (only where a row's scale is above 2^110 and a block's above 2^103 a sum of zero
- *   becomes NaN, and every other infinite); within a block bf16 outputs take the
- *   8-bit matrix instruction, whose sums are within 1.4e-5 (as 2-norms, on normal
- *   rows) and fp32 outputs the bf16 one on the same values, which adds in fp32.
+ *   becomes NaN, and every other infinite).  Within a block bf16 outputs take
+ *   the 8-bit matrix instruction, whose sums are off by up to 2^-13 of the sum of the
+ *   products' magnitudes (1.4e-5 on normal rows), and fp32 outputs the bf16 one on the
+ *   same values, which adds in fp32.
  * No workspace.  No counterpart in the reference.                           */
 int mogt_add_rmsnorm_fp8_fwd(const float* x, const void* z, float scale, const float* weight, float* x_out, void* q,
                              float* q_scale, int64_t rows, int64_t dim, float eps, int z_dtype, void* stream);

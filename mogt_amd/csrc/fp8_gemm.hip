@@ -4,11 +4,11 @@
 // block.  A block's products are added by one matrix instruction (16x16x128) into
 // zeros, the block's sum is scaled and added in fp32 on the vector unit.
 //
-// The 8-bit instruction aligns the products it adds: a block's sum is off by about
-// 1.4e-5 of it (measured on normal rows, the same for its form of 32 values), which
-// a bf16 output does not show.  fp32 outputs (EXACT) widen the operands to bf16, which
-// holds every e4m3 value, and add with the bf16 instruction, at half the rate, to
-// fp32's own accuracy.
+// The 8-bit instruction aligns the products it adds to the largest: a block's sum is
+// off by up to 2^-13 of the sum of their magnitudes (1.4e-5 of it on normal rows, the
+// same for the form of 32 values), which bf16 outputs take for twice the rate.  fp32
+// outputs (EXACT) widen the operands to bf16, which holds every e4m3 value, and add
+// with the bf16 instruction to fp32's own accuracy.
 //
 // Tiles: a work-group of MW x NW waves, a wave 16 MT rows of x by 16 NT rows of w.
 // D[row of w][row of x]: a lane's results are four consecutive outputs of one row,

@@ -3,9 +3,10 @@
 //   scale = max(largest |x| of the block / 448, 2^-126),   q = e4m3(x / scale)
 // rounded to nearest even, so x is q * scale within half a step of the block's
 // largest value, and a block of zeros is zeros.  A NaN stays one in its place; an
-// infinity makes its block's scale infinite.
-//   add_rmsnorm_fp8  x' = x + round(s * z), n = rmsnorm(x') * w, the rows n in 8 bits:
-//                    the residual update as in add_rmsnorm
+// infinity makes its block's scale infinite.  (The norm rounds its quotients from the
+// scale in 64 bits; the quantisers divide by the scale that they store.)
+//   add_rmsnorm_fp8  x' = x + s * z (bf16 z: the product rounded to bf16, as add_rmsnorm
+//                    does), n = rmsnorm(x') * w, the rows n in 8 bits
 //   quantize_rows    the rows of a matrix
 //   quantize_blocks  128 x 128 blocks (weights, laid out once)
 // Four consecutive values a lane: half a wave is a block and its maximum five lane

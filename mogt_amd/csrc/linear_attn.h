@@ -80,14 +80,15 @@ __device__ __forceinline__ int la_length(const LaArgs& a, int b) {
     return __builtin_amdgcn_readfirstlane(static_cast<int>(n));
 }
 
-// Padded contraction width and tiles of 16 value columns a wave of a pass, which
-// its kernel is built for, and the waves of a SIMD that its registers are held to.
+// Padded contraction width of a pass and whether its values are wide, which its kernel
+// is built for; the waves of a SIMD that the kernel's registers are held to, by its tiles
+// of 16 value columns a wave and its waves.
 inline int la_width(int dc) { return dc <= 32 ? 32 : dc <= 64 ? 64 : 128; }
-inline int la_tiles(int dn) { return dn <= 64 ? 1 : 2; }
+inline bool la_wide(int dn) { return dn > 64; }
 constexpr int la_waves_per_simd(int width, int tiles, int waves) { return waves == 8 ? 4 : tiles == 2 || width > 64 ? 2 : 3; }
 
 inline bool la_one_kind(const LaPass& a, const LaPass& b) {
-    return la_width(a.dc) == la_width(b.dc) && la_tiles(a.dn) == la_tiles(b.dn) && !a.dot == !b.dot && a.out_f32 == b.out_f32;
+    return la_width(a.dc) == la_width(b.dc) && la_wide(a.dn) == la_wide(b.dn) && !a.dot == !b.dot && a.out_f32 == b.out_f32;
 }
 
 }  // namespace mogt

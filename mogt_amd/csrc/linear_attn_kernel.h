@@ -706,7 +706,7 @@ void la_launch_passes(const LaArgs& a, int count, bool out, hipStream_t st) {
     typedef std::integral_constant<int, sizeof(TI) == 2 ? LA_HALVES : LA_VECTORS> halves;
     typedef std::integral_constant<int, LA_VECTORS> vectors;
     auto pick = [&](auto width) {
-        const bool narrow = a.pass[0].dn <= 64;
+        const bool narrow = !la_wide(a.pass[0].dn);
         if (vec == LA_VECTORS)
             narrow ? with(width, one(), four(), vectors()) : with(width, one(), eight(), vectors());
         else if (vec == LA_HALVES)
