@@ -21,12 +21,12 @@
 // Up to 32 rows (one token of a batch): the weights are read once, straight into
 // registers, by waves of 16 rows of w that share K; bound by their bytes.
 //
-// 32768 x 6144 x 2048 takes 411 us alone and 447 in a row (2.01 and 1.84 PFLOP/s;
-// torch's unscaled e4m3 product 328 and 359).  In a row the card's power bounds it:
-// of zeros the same product takes 358 us.  The matrix unit is busy for 46 % of the
-// cycles, the vector unit, which adds 4 scaled results a product, for 47 %, LDS for
-// 24 %; no order of loads, reads and products that was tried changes the time by
-// more than 2 %.
+// 32768 x 6144 x 2048 takes 438 us (1.88 PFLOP/s; torch's unscaled e4m3 product 340, its
+// bf16 product 583), to fp32 829 (995 TFLOP/s), on other cards 411 to 447.  In a row of
+// calls the card's power bounds it: of zeros the same product takes 360 us.  The matrix
+// unit is busy for 43 % of the cycles, the vector unit, which adds 4 scaled results a
+// product, for 40 %, LDS for 23 %; no order of loads, reads and products that was tried
+// changes the time by more than 2 %.  To fp32 every wave widens the operands that it reads.
 #include "lds_dma.h"
 #include "wide_grid.h"
 
@@ -418,13 +418,15 @@ void f8_launch(F8Gemm& p, int cus, hipStream_t st) {
     };
     // The largest tile that fills the card: of 2048 columns of x (us, bf16 and fp32 outputs)
     //                 256 x 256, 128 x 256     128 x 128        64 x 128
-    //   8192 x 6144   110      221             141  233         166  292
-    //   4096 x 6144    73      116              76  127          87  159
-    //   2048 x 6144    35       57              36   54          44   77
-    //   4096 x 2048                             26   44          34   52
-    //   1024 x 6144                             23   36          24   39
-    // and up to 32 rows the form without tiles: 32 x 6144 9.9 against 10.6 and 15.4, 16 x
-    // 6144 7.2 against 10.7 and 15.1.
+    //   8192 x 6144   111      214             135  219         166  276
+    //   4096 x 6144    66      108              68  109          84  141
+    //   2048 x 6144    35       66              37   55          43   72
+    //   4096 x 2048    33       38              26   39          32   46
+    //   1024 x 6144    32       37              23   37          24   38
+    //   2048 x 2048    32       34              18   26          18   26
+    //     64 x 6144    28       31              15   22          11   16
+    // and up to 32 rows the form without tiles: 32 x 6144 10.0 against 10.8 and 15.5, 16 x
+    // 6144 7.2 against 10.8 and 15.3.
     const int each = EXACT ? 4 : 2;
     const int64_t row = p.ldy * each;
     p.piece = row * 256 >= 0x7fffff00 ? 0 : row % 16 == 0 ? 16 : row % 8 == 0 ? 8 : row % 4 == 0 ? 4 : 2;

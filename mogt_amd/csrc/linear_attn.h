@@ -38,8 +38,9 @@ template <typename TI> struct LaChunk;
 template <> struct LaChunk<bf16_t> { static constexpr int T = 64, KS = 32; };
 template <> struct LaChunk<float> { static constexpr int T = 32, KS = 16; };
 
-// Loads of rows: 16 bytes, 8 bytes (bf16), an element.  2 x 8192 steps of 12 heads of
-// 100 x 100, bf16, forward: 113 us by halves, 294 by elements (128 x 128 by vectors: 113).
+// Loads of rows: 16 bytes, 8 bytes (bf16), an element.  Kernels of 2 x 8192 steps of 12
+// heads of 100 x 100, bf16, forward: 127 us by halves, 268 by elements (an instruction for
+// each, eight for 16 bytes); 128 x 128 by vectors 131.
 constexpr int LA_SINGLE = 0, LA_HALVES = 1, LA_VECTORS = 2;
 
 struct LaRows {      // rows of one role: element strides, and the heads that share them

@@ -1,9 +1,9 @@
 // The chunked pass of linear attention (linear_attn.h has the mathematics), one
 // work-group per segment and head, a wave for CT times 16 value columns: four waves
 // up to 64 columns; for 128 eight of 16, with a wave's registers halved and four
-// waves a SIMD (32768 steps of 16 heads of 128, bf16, outputs: 157 us, with four
-// waves of 32 columns 169), but where loads are of single elements, which take more
-// registers: those are four of 32.
+// waves a SIMD (kernels of 2 x 8192 steps of 16 heads of 128 with gradients, bf16: 521 us,
+// with four waves of 32 columns 533; 32768 steps, forward: 309 and 301), but where loads
+// are of single elements, which take more registers: those are four of 32.
 //
 // Tiles (16x16 matrix instructions, D[row][column]: a lane holds column lane % 16
 // and rows 4 (lane / 16) .. + 3):
@@ -16,11 +16,11 @@
 // Operands that contract over steps are read transposed from LDS (bf16: the
 // transposing LDS read).  S never leaves registers inside a segment.
 //
-// 32768 steps of 16 heads of 128, bf16: sums 74 us (268 MB; without its products
-// as long: 4.4 TB/s while it runs), outputs 157 us (537 MB; 148 without loads: the
-// vector unit is busy for 51 % of the cycles, the matrix unit 25 %, LDS 29 %, what
+// 32768 steps of 16 heads of 128, bf16: sums 75 to 82 us (268 MB; without its
+// products as long), outputs 180 to 206 us (537 MB; the vector unit, which splits the
+// fp32 operands, is busy for 57 % of the cycles, the matrix unit 32 %, LDS 28 %, what
 // is left are the waits between the steps above).  2 x 8192 steps of 12 heads of 64:
-// sums 17 us, outputs 30, two gradients with their products 66 (100 MB each).
+// sums 17 us, outputs 33, two gradients with their products 66 (100 MB each).
 #include "linear_attn.h"
 
 namespace mogt {
