@@ -64,7 +64,7 @@ struct F8Scale {
 template <bool EXACT> constexpr int F8_ONE = EXACT ? 127 << 23 : 127;
 template <bool EXACT>
 __device__ __forceinline__ F8Scale f8_part(float s) {
-    const int e = __builtin_amdgcn_readfirstlane(__float_as_int(s)) >> 23 & 255, h = min(max(e, 27), 230);
+    const int e = __float_as_int(s) >> 23 & 255, h = min(max(e, 27), 230);
     return F8Scale{__builtin_ldexpf(s, 127 - h), EXACT ? h << 23 : h};
 }
 
@@ -357,8 +357,7 @@ template <int MT, bool EXACT>
 __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
     __shared__ f8_f4 s_d[4][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = lane >> 4;
-    if (wide_block() * 16 >= p.N) return;
-    const int n0 = static_cast<int>(wide_block()) * 16;
+    const int n0 = min(static_cast<int>(wide_block()), (p.N - 1) / 16) * 16;   // work-groups too many repeat the last
     const uint8_t* wr = p.w + static_cast<int64_t>(min(n0 + (lane & 15), p.N - 1)) * p.K;
     const float* ws = p.ws + static_cast<int64_t>(n0 / 128) * p.kb;
     const uint8_t* xr[MT];

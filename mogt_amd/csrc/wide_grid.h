@@ -7,13 +7,15 @@
 
 namespace mogt {
 
-constexpr int64_t WIDE_GRID_MAX = 65535ll << 20;
+constexpr int WIDE_GRID_LOG2 = 20;
+constexpr int64_t WIDE_GRID_MAX = 65535ll << WIDE_GRID_LOG2;
 
 // `groups` work-groups (up to WIDE_GRID_MAX) or some more, numbered by wide_block()
 inline dim3 wide_grid(int64_t groups, unsigned z = 1) {
-    const int64_t x = groups < (1 << 20) ? groups : 1 << 20;
+    const int64_t x = groups < (1 << WIDE_GRID_LOG2) ? groups : 1 << WIDE_GRID_LOG2;
     return dim3(static_cast<unsigned>(x), static_cast<unsigned>((groups + x - 1) / x), z);
 }
-__device__ __forceinline__ int64_t wide_block() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+// A second row follows only rows of 2^20: the grid's size is not read.
+__device__ __forceinline__ int64_t wide_block() { return static_cast<int64_t>(blockIdx.y) << WIDE_GRID_LOG2 | blockIdx.x; }
 
 }  // namespace mogt
