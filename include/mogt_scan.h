@@ -773,10 +773,10 @@ int mogt_linear_attn_step(const mogt_linear_attn_problem* problem, float* state,
  *   ldx at most 2^22, outputs at most 2^30; x, w and y 16-byte aligned.
  *   Blocks' sums are scaled and added in fp32, the scales' product over its whole range
  *   (only where a row's scale is above 2^110 and a block's above 2^103 a sum of zero
- *   becomes NaN, and every other infinite).  Within a block bf16 outputs take
- *   the 8-bit matrix instruction, whose sums are off by up to 2^-13 of the sum of the
- *   products' magnitudes (1.4e-5 on normal rows), and fp32 outputs the bf16 one on the
- *   same values, which adds in fp32.
+ *   becomes NaN, and every other infinite).  Within a block fp32 outputs, and
+ *   bf16 ones of up to 32 rows, take the bf16 matrix instruction, which adds in fp32;
+ *   bf16 outputs of more rows the 8-bit one, whose sums are off by up to 2^-13 of the sum
+ *   of the products' magnitudes (1.4e-5 on normal rows).
  * No workspace.  No counterpart in the reference.                           */
 int mogt_add_rmsnorm_fp8_fwd(const float* x, const void* z, float scale, const float* weight, float* x_out, void* q,
                              float* q_scale, int64_t rows, int64_t dim, float eps, int z_dtype, void* stream);

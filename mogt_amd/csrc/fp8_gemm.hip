@@ -6,9 +6,9 @@
 //
 // The 8-bit instruction aligns the products it adds to the largest: a block's sum is
 // off by up to 2^-13 of the sum of their magnitudes (1.4e-5 of it on normal rows, the
-// same for the form of 32 values), which bf16 outputs take for twice the rate.  fp32
-// outputs (EXACT) widen the operands to bf16, which holds every e4m3 value, and add
-// with the bf16 instruction to fp32's own accuracy.
+// same for the form of 32 values), which bf16 outputs of many rows take for twice the
+// rate.  fp32 outputs and few rows (EXACT) widen the operands to bf16, which holds every
+// e4m3 value, and add with the bf16 instruction to fp32's own accuracy.
 //
 // Tiles: a work-group of MW x NW waves, a wave 16 MT rows of x by 16 NT rows of w.
 // D[row of w][row of x]: a lane's results are four consecutive outputs of one row,
@@ -119,9 +119,9 @@ __device__ __forceinline__ int f8_again(int x) {
 // rows to the banks' width, fall into distinct banks.
 __device__ __forceinline__ int f8_twist(int row) { return (row >> 1) & 7; }
 
-template <bool EXACT>
+template <bool F32>
 __device__ __forceinline__ void f8_store(const F8Gemm& p, int64_t m, int n, f8_f4 v) {
-    typedef typename std::conditional<EXACT, float, bf16_t>::type T;
+    typedef typename std::conditional<F32, float, bf16_t>::type T;
     T* y = static_cast<T*>(p.y) + m * p.ldy + n;
     if (n + 4 <= p.N && p.ldy % 4 == 0) {
         Pack<T, 4> w;
@@ -352,8 +352,11 @@ __global__ __launch_bounds__(64 * MW * NW) void f8_gemm_kernel(F8Gemm p) {
     }
 }
 
-// Few rows: a work-group's four waves take every fourth block of K of 16 rows of w.
-template <int MT, bool EXACT>
+// Few rows: a work-group's four waves take every fourth block of K of 16 rows of w, with
+// the bf16 instruction for both outputs: the weights' bytes bound it, not the products
+// (2048 columns by 6144, 8-bit and bf16 instruction: 16 rows 7.2 and 7.4 us, 32 rows 10.1
+// and 10.2; 4096 by 32768, one row: 28.8 and 29.9).
+template <int MT, bool F32>
 __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
     __shared__ f8_f4 s_d[4][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), grp = lane >> 4;
@@ -375,15 +378,15 @@ __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
         f8_i4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
         if (k < p.K) lo = *reinterpret_cast<const f8_i4*>(row + k);
         if (k + 64 < p.K) hi = *reinterpret_cast<const f8_i4*>(row + k + 64);
-        return F8Operand<EXACT>(lo, hi, power);
+        return F8Operand<true>(lo, hi, power);
     };
 #pragma unroll 4
     for (int s = wave; s < p.kb; s += 4) {
-        const F8Scale wscale = f8_part<EXACT>(ws[s]);
-        const F8Operand<EXACT> w = frag(wr, s, wscale.power);
+        const F8Scale wscale = f8_part<true>(ws[s]);
+        const F8Operand<true> w = frag(wr, s, wscale.power);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const f8_f4 d = f8_block(w, frag(xr[i], s, F8_ONE<EXACT>));
+            const f8_f4 d = f8_block(w, frag(xr[i], s, F8_ONE<true>));
             const float f = xs[i][s] * wscale.rest;
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(d[e], f, acc[i][e]);
@@ -396,7 +399,7 @@ __global__ __launch_bounds__(256) void f8_gemv_kernel(F8Gemm p) {
         const f8_f4 d = (s_d[0][i][lane] + s_d[1][i][lane]) + (s_d[2][i][lane] + s_d[3][i][lane]);
         const int64_t m = 16 * i + (lane & 15);
         const int n = n0 + 4 * grp;
-        if (m < p.M && n < p.N) f8_store<EXACT>(p, m, n, d);
+        if (m < p.M && n < p.N) f8_store<F32>(p, m, n, d);
     }
 }
 

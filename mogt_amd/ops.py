@@ -3365,10 +3365,10 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
 
     Each block's products are added on the matrix cores, scaled and added in
     float32, and rounded once to ``out_dtype`` (bfloat16 or float32).  bfloat16
-    outputs take the 8-bit instruction, whose sums of 128 are off by up to 2^-13 of the
-    sum of their products' magnitudes (1.4e-5 on normal rows); float32 outputs the
-    bfloat16 one on the same values, which adds in float32, at half its rate.  No
-    autograd."""
+    outputs of more than 32 rows take the 8-bit instruction, whose sums of 128 are off
+    by up to 2^-13 of the sum of their products' magnitudes (1.4e-5 on normal rows);
+    float32 outputs, and up to 32 rows, the bfloat16 one on the same values, which adds
+    in float32, at half its rate.  No autograd."""
     _same_device("linear_fp8", x, (x_scale, w, w_scale))
     if x.dtype != _FP8 or w.dtype != _FP8:
         raise ValueError(f"linear_fp8: x and w must be {_FP8}, got {x.dtype} and {w.dtype}")

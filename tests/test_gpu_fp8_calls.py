@@ -178,19 +178,19 @@ def test_product_past_2_32_bytes(gpu, out):
     torch.cuda.empty_cache()
 
 
-@pytest.mark.parametrize("M,out", [(1, F32), (17, F32), (40, F32), (700, F32), (4100, F32)])
+@pytest.mark.parametrize("M,out", [(1, F32), (1, BF16), (16, BF16), (17, F32), (32, BF16), (40, F32), (700, F32), (4100, F32)])
 def test_products_that_cancel_add_in_fp32(gpu, M, out):
     """Whole numbers whose sums stay below 2^24 are exact in fp32 in any order: 32 pairs
-    of up to 224 * 224 that cancel, and 64 small products that are left.  (The 8-bit
-    instruction drops what lies below 2^-14 of the largest product.)"""
+    of 2^16 to 448 * 448 that cancel, and between them 64 products of up to 9 that are
+    left.  (The 8-bit instruction drops what lies below 2^-14 of the largest product.)"""
     from mogt_amd import ops
     announce(f"linear_fp8 products that cancel {M} {out}")
     g = torch.Generator(device="cuda").manual_seed(6)
-    r = lambda *s: torch.randint(-7, 8, s, generator=g, device="cuda").float()  # noqa: E731
+    r = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, generator=g, device="cuda").float()  # noqa: E731
     N, K = 300, 384
-    x, w = r(M, K // 128, 128), r(N, K // 128, 128)
-    x[..., :64], w[..., :64] = 32 * x[..., :64], 32 * w[..., :64]
-    x[..., 32:64], w[..., 32:64] = x[..., :32], -w[..., :32]
+    x, w = r(-3, 3, M, K // 128, 128), r(-3, 3, N, K // 128, 128)
+    x[..., ::4], w[..., ::4] = 32 * r(8, 14, M, K // 128, 32), 32 * r(8, 14, N, K // 128, 32)
+    x[..., 1::4], w[..., 1::4] = x[..., ::4], -w[..., ::4]
     x, w = x.view(M, K).to(F8), w.view(N, K).to(F8)
     y = ops.linear_fp8(x, torch.ones(M, 3, device="cuda"), w, torch.ones(3, 3, device="cuda"), out_dtype=out)
     assert torch.equal(y.double(), (x.double() @ w.double().t()).to(out).double())
