@@ -21,9 +21,9 @@
 // Up to 32 rows (one token of a batch): the weights are read once, straight into
 // registers, by waves of 16 rows of w that share K; bound by their bytes.
 //
-// 32768 x 6144 x 2048 takes 438 us (1.88 PFLOP/s; torch's unscaled e4m3 product 340, its
-// bf16 product 583), to fp32 829 (995 TFLOP/s), on other cards 411 to 447.  In a row of
-// calls the card's power bounds it: of zeros the same product takes 360 us.  The matrix
+// 32768 x 6144 x 2048 takes 406 to 438 us on different cards (2.03 to 1.88 PFLOP/s;
+// torch's unscaled e4m3 product 340, its bf16 product 583), to fp32 794 to 829.  In a row
+// of calls the card's power bounds it: of zeros the same product takes 360 us.  The matrix
 // unit is busy for 43 % of the cycles, the vector unit, which adds 4 scaled results a
 // product, for 40 %, LDS for 23 %; no order of loads, reads and products that was tried
 // changes the time by more than 2 %.  To fp32 every wave widens the operands that it reads.
